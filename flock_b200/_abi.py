@@ -28,7 +28,8 @@ FLOCK_ATTN_EXACT, FLOCK_ATTN_FAST = 0, 1
 FLOCK_DECODE_KERNELS, FLOCK_DECODE_PERSISTENT, FLOCK_DECODE_EAGER, FLOCK_DECODE_STREAM = \
     0, 1, 2, 3
 FLOCK_PREFILL_EXACT, FLOCK_PREFILL_TENSOR = 0, 1
-FLOCK_KV_F32, FLOCK_KV_BF16, FLOCK_KV_FP8 = 0, 1, 2
+FLOCK_KV_F32, FLOCK_KV_BF16, FLOCK_KV_FP8, FLOCK_KV_Q4 = 0, 1, 2, 3
+FLOCK_WORKSPACE_BYTES = 8388608
 FLOCK_MATVEC_EXACT, FLOCK_MATVEC_FAST = 0, 1
 FLOCK_TP_NCCL, FLOCK_TP_PEER = 0, 1
 
@@ -103,6 +104,11 @@ SIGNATURES = {
     "flock_op_embed": [_vp, _vp, _i32p, _i, _fp],
     "flock_op_argmax": [_vp, _fp, _i64, _i64p, _fp],
     "flock_argmax_noalloc": [_vp, _i64, _vp, _vp, _vp],
+    "flock_kv_create": [_vp, _i, _i, _i, _i64, _vp, _vp, _vp, _vp, _vp, _pp],
+    "flock_kv_free": [_vp],
+    "flock_kv_append": [_vp, _vp, _vp, _i64, _i64, _i, _vp],
+    "flock_kv_read": [_vp, _i64, _i, _vp, _vp, _vp],
+    "flock_kv_attention": [_vp, _vp, _i64, _i, _i, _i64, _i, _i, _vp, _i64, _vp],
     "flock_layer_create": [_vp, _cfgp, _i, _ccp, _pp, _pp],
     "flock_layer_free": [_vp],
     "flock_layer_encode": [_vp, _fp, _i],

@@ -1,0 +1,292 @@
+// Caches in caller-owned memory: append, read back and attention with a
+// sliding window and sinks (include/flock_cuda.h flock_kv_*).
+#include <cuda_runtime.h>
+
+#include <new>
+
+#include "flock_internal.h"
+#include "kv.cuh"
+
+using namespace flock;
+
+struct flock_kv {
+  flock_dev* dev = nullptr;
+  int kv_dtype = 0;
+  KvView view{};
+  uint8_t* workspace = nullptr;
+  DBuf own_k, own_v, own_ks, own_vs, own_ws;  // allocated here when the caller gave none
+};
+
+namespace {
+
+constexpr int64_t KV_MAX_CAPACITY = (int64_t)1 << 30;
+
+// The handle's device made current for the call, the caller's restored after.
+struct OnDevice {
+  int before = -1, want;
+  explicit OnDevice(int ordinal) : want(ordinal) {}
+  int enter() {
+    FLOCK_CK(cudaGetDevice(&before));
+    if (before != want) FLOCK_CK(cudaSetDevice(want));
+    return FLOCK_OK;
+  }
+  ~OnDevice() {
+    if (before >= 0 && before != want) cudaSetDevice(before);
+  }
+};
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// A pointer the caller says is device memory of `dev`: asked of the runtime
+// once, when a handle is made.
+int check_device_pointer(const flock_dev* dev, const void* p, const char* what) {
+  cudaPointerAttributes at = {};
+  const cudaError_t e = cudaPointerGetAttributes(&at, p);
+  if (e != cudaSuccess || at.type == cudaMemoryTypeUnregistered || at.type == cudaMemoryTypeHost) {
+    cudaGetLastError();
+    set_error("%s is not device memory", what);
+    return FLOCK_E_ARG;
+  }
+  if (at.device != dev->ordinal) {
+    set_error("%s is on device %d, the handle on device %d", what, at.device, dev->ordinal);
+    return FLOCK_E_ARG;
+  }
+  if (!aligned16(p)) {
+    set_error("%s is not 16-byte aligned", what);
+    return FLOCK_E_ARG;
+  }
+  return FLOCK_OK;
+}
+
+int check_range(const flock_kv* c, const char* who, int64_t pos, int n) {
+  if (pos < 0 || n < 0 || pos + n > c->view.capacity) {
+    set_error("%s: positions %lld .. %lld are not inside a cache of %lld keys", who,
+              (long long)pos, (long long)pos + n - 1, (long long)c->view.capacity);
+    return FLOCK_E_STATE;
+  }
+  return FLOCK_OK;
+}
+
+size_t plane_bytes(int kv_dtype, int n_kv_heads, int64_t capacity) {
+  const size_t values = (size_t)capacity * n_kv_heads * KV_HD;
+  return kv_dtype == FLOCK_KV_Q4     ? values / 2
+         : kv_dtype == FLOCK_KV_FP8  ? values
+         : kv_dtype == FLOCK_KV_BF16 ? values * 2
+                                     : values * 4;
+}
+
+template <typename F>
+int by_dtype(int kv_dtype, F f) {
+  switch (kv_dtype) {
+    case FLOCK_KV_Q4: return f(std::integral_constant<int, FLOCK_KV_Q4>());
+    case FLOCK_KV_FP8: return f(std::integral_constant<int, FLOCK_KV_FP8>());
+    case FLOCK_KV_BF16: return f(std::integral_constant<int, FLOCK_KV_BF16>());
+    default: return f(std::integral_constant<int, FLOCK_KV_F32>());
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int flock_kv_create(flock_dev* dev, int kv_dtype, int n_kv_heads, int head_dim, int64_t capacity,
+                    void* k, void* v, void* k_scales, void* v_scales, void* workspace,
+                    flock_kv** out) {
+  if (!dev || !out) {
+    set_error("kv_create: dev and out must not be NULL");
+    return FLOCK_E_ARG;
+  }
+  if (kv_dtype != FLOCK_KV_F32 && kv_dtype != FLOCK_KV_BF16 && kv_dtype != FLOCK_KV_FP8 &&
+      kv_dtype != FLOCK_KV_Q4) {
+    set_error("kv_create: kv_dtype %d is not FLOCK_KV_F32, _BF16, _FP8 or _Q4", kv_dtype);
+    return FLOCK_E_ARG;
+  }
+  if (head_dim != KV_HD) {
+    set_error("kv_create: head_dim %d: the kernels are built for head_dim 128", head_dim);
+    return FLOCK_E_UNSUPPORTED;
+  }
+  if (n_kv_heads < 1 || n_kv_heads > 65535 || capacity < 1 || capacity > KV_MAX_CAPACITY) {
+    set_error("kv_create: n_kv_heads %d must be in 1..65535 and capacity %lld in 1..%lld",
+              n_kv_heads, (long long)capacity, (long long)KV_MAX_CAPACITY);
+    return FLOCK_E_ARG;
+  }
+  const bool q4 = kv_dtype == FLOCK_KV_Q4;
+  if (q4 && capacity % 16) {
+    set_error("kv_create: a 4-bit cache's capacity %lld must be a multiple of 16",
+              (long long)capacity);
+    return FLOCK_E_ARG;
+  }
+  if ((!k) != (!v) || (k && q4 && (!k_scales || !v_scales)) ||
+      ((k_scales || v_scales) && (!q4 || !k))) {
+    set_error("kv_create: give both planes or none, and both scale planes with a 4-bit cache's "
+              "planes only");
+    return FLOCK_E_ARG;
+  }
+  OnDevice on(dev->ordinal);
+  FLOCK_TRY(on.enter());
+  flock_kv* c = new (std::nothrow) flock_kv();
+  if (!c) {
+    set_error("kv_create: out of host memory");
+    return FLOCK_E_NOMEM;
+  }
+  auto fill = [&]() -> int {
+    const size_t bytes = plane_bytes(kv_dtype, n_kv_heads, capacity);
+    const size_t sbytes = (size_t)capacity * n_kv_heads * 4 * sizeof(uint16_t);
+    if (k) {
+      FLOCK_TRY(check_device_pointer(dev, k, "kv_create: k"));
+      FLOCK_TRY(check_device_pointer(dev, v, "kv_create: v"));
+      if (q4) {
+        FLOCK_TRY(check_device_pointer(dev, k_scales, "kv_create: k_scales"));
+        FLOCK_TRY(check_device_pointer(dev, v_scales, "kv_create: v_scales"));
+      }
+    } else {
+      FLOCK_TRY(c->own_k.alloc(bytes));
+      FLOCK_TRY(c->own_v.alloc(bytes));
+      FLOCK_CK(cudaMemset(c->own_k.p, 0, bytes));
+      FLOCK_CK(cudaMemset(c->own_v.p, 0, bytes));
+      k = c->own_k.p;
+      v = c->own_v.p;
+      if (q4) {
+        FLOCK_TRY(c->own_ks.alloc(sbytes));
+        FLOCK_TRY(c->own_vs.alloc(sbytes));
+        FLOCK_CK(cudaMemset(c->own_ks.p, 0, sbytes));
+        FLOCK_CK(cudaMemset(c->own_vs.p, 0, sbytes));
+        k_scales = c->own_ks.p;
+        v_scales = c->own_vs.p;
+      }
+    }
+    if (workspace) {
+      FLOCK_TRY(check_device_pointer(dev, workspace, "kv_create: workspace"));
+    } else {
+      FLOCK_TRY(c->own_ws.alloc(FLOCK_WORKSPACE_BYTES));
+      FLOCK_CK(cudaMemset(c->own_ws.p, 0, FLOCK_WORKSPACE_BYTES));
+      workspace = c->own_ws.p;
+    }
+    if (c->own_k.p || c->own_ws.p) FLOCK_CK(cudaStreamSynchronize(nullptr));
+    return FLOCK_OK;
+  };
+  const int rc = fill();
+  if (rc != FLOCK_OK) {
+    delete c;
+    return rc;
+  }
+  c->dev = dev_retain(dev);
+  c->kv_dtype = kv_dtype;
+  c->view.k = k;
+  c->view.v = v;
+  c->view.ks = static_cast<uint16_t*>(k_scales);
+  c->view.vs = static_cast<uint16_t*>(v_scales);
+  c->view.capacity = capacity;
+  c->view.n_kv_heads = n_kv_heads;
+  c->workspace = static_cast<uint8_t*>(workspace);
+  *out = c;
+  return FLOCK_OK;
+}
+
+int flock_kv_free(flock_kv* c) {
+  if (!c) return FLOCK_OK;
+  flock_dev* dev = c->dev;
+  {
+    OnDevice on(dev->ordinal);
+    FLOCK_TRY(on.enter());
+    delete c;
+  }
+  dev_release(dev);
+  return FLOCK_OK;
+}
+
+int flock_kv_append(flock_kv* c, const float* k, const float* v, int64_t row_stride, int64_t pos,
+                    int n, void* stream) {
+  if (!c || (n > 0 && (!k || !v))) {
+    set_error("kv_append: the cache, k and v must not be NULL");
+    return FLOCK_E_ARG;
+  }
+  FLOCK_TRY(check_range(c, "kv_append", pos, n));
+  const int64_t row = (int64_t)c->view.n_kv_heads * KV_HD;
+  if (row_stride == 0) row_stride = row;
+  if (row_stride < row || row_stride % 4 || !aligned16(k) || !aligned16(v)) {
+    set_error("kv_append: row_stride %lld must be a multiple of 4, at least %lld, and k and v "
+              "16-byte aligned", (long long)row_stride, (long long)row);
+    return FLOCK_E_ARG;
+  }
+  if (n == 0) return FLOCK_OK;
+  OnDevice on(c->dev->ordinal);
+  FLOCK_TRY(on.enter());
+  const unsigned grid = (unsigned)(((int64_t)n * c->view.n_kv_heads + 7) / 8);
+  return by_dtype(c->kv_dtype, [&](auto kv) -> int {
+    k_kv_append<decltype(kv)::value><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        c->view, k, v, row_stride, pos, n);
+    FLOCK_CK(cudaGetLastError());
+    return FLOCK_OK;
+  });
+}
+
+int flock_kv_read(flock_kv* c, int64_t pos, int n, float* k, float* v, void* stream) {
+  if (!c || (n > 0 && (!k || !v)) || !aligned16(k) || !aligned16(v)) {
+    set_error("kv_read: the cache, k and v must not be NULL, k and v 16-byte aligned");
+    return FLOCK_E_ARG;
+  }
+  FLOCK_TRY(check_range(c, "kv_read", pos, n));
+  if (n == 0) return FLOCK_OK;
+  OnDevice on(c->dev->ordinal);
+  FLOCK_TRY(on.enter());
+  const unsigned grid = (unsigned)(((int64_t)n * c->view.n_kv_heads + 7) / 8);
+  return by_dtype(c->kv_dtype, [&](auto kv) -> int {
+    k_kv_read<decltype(kv)::value><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        c->view, pos, n, k, v);
+    FLOCK_CK(cudaGetLastError());
+    return FLOCK_OK;
+  });
+}
+
+int flock_kv_attention(flock_kv* c, const float* q, int64_t q_stride, int n_heads, int n_queries,
+                       int64_t pos, int window, int sinks, float* out, int64_t out_stride,
+                       void* stream) {
+  if (!c || (n_queries > 0 && (!q || !out))) {
+    set_error("kv_attention: the cache, q and out must not be NULL");
+    return FLOCK_E_ARG;
+  }
+  if (n_heads < 1 || n_heads % c->view.n_kv_heads) {
+    set_error("kv_attention: n_heads %d must be a multiple of n_kv_heads %d", n_heads,
+              c->view.n_kv_heads);
+    return FLOCK_E_ARG;
+  }
+  if (window < 0 || sinks < 0) {
+    set_error("kv_attention: window %d and sinks %d must not be negative (window 0: no window)",
+              window, sinks);
+    return FLOCK_E_ARG;
+  }
+  FLOCK_TRY(check_range(c, "kv_attention", pos, n_queries));
+  const int64_t row = (int64_t)n_heads * KV_HD;
+  if (q_stride == 0) q_stride = row;
+  if (out_stride == 0) out_stride = row;
+  if (q_stride < row || q_stride % 4 || out_stride < row || out_stride % 4 || !aligned16(q) ||
+      !aligned16(out)) {
+    set_error("kv_attention: q_stride %lld and out_stride %lld must be multiples of 4, at least "
+              "%lld, and q and out 16-byte aligned", (long long)q_stride, (long long)out_stride,
+              (long long)row);
+    return FLOCK_E_ARG;
+  }
+  if (n_queries == 0) return FLOCK_OK;
+  OnDevice on(c->dev->ordinal);
+  FLOCK_TRY(on.enter());
+  KvAttnArgs a = {};
+  a.c = c->view;
+  a.q = q;
+  a.out = out;
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.pos = pos;
+  a.n_queries = n_queries;
+  a.n_heads = n_heads;
+  a.window = window;
+  a.sinks = sinks;
+  const unsigned grid = (unsigned)(((int64_t)n_queries * n_heads + 3) / 4);
+  return by_dtype(c->kv_dtype, [&](auto kv) -> int {
+    k_kv_attn<decltype(kv)::value><<<grid, 128, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    FLOCK_CK(cudaGetLastError());
+    return FLOCK_OK;
+  });
+}
+
+}  // extern "C"

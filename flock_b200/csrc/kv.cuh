@@ -1,0 +1,239 @@
+// A KV cache in memory the caller owns, and the kernels that fill and read it
+// (flock_kv_* in include/flock_cuda.h).
+//
+// Cached element types.  f32, bf16 and e4m3 caches hold rows
+// [key][kv head][128], the layers' own layout.  The 4-bit cache
+// (FLOCK_KV_Q4) holds per head a plane of 64-byte rows [kv head][key][64] and
+// a plane of f16 block scales [kv head][key][4]; a block is 32 values along
+// the head in the Q4_0 rule (kernels/lib.ts:64 quantRowQ4): d = m / -8 with m
+// the first value of largest magnitude, code = clamp(floor(x / d + 8.5), 0,
+// 15), value (code - 8) * f16(d), byte i of the block = code i | code i+16
+// << 4.  The head's four blocks are interleaved so that one attention lane's
+// codes are one aligned load: byte i of block b of a key lies at
+// 16 (i / 4) + 4 b + i % 4, of a value row at 8 (i / 2) + 2 b + i % 2.
+// Head-major planes keep a head's keys contiguous: its scales (8 bytes a key)
+// fill whole sectors, where [key][head] rows would use 8 bytes of each 32.
+#pragma once
+#include "common.cuh"
+#include "mbar.cuh"
+
+namespace flock {
+
+constexpr int KV_HD = 128;
+
+// What every kernel here needs of a cache.
+struct KvView {
+  void* k;
+  void* v;
+  uint16_t* ks;   // FLOCK_KV_Q4: f16 scales [kv head][capacity][4]
+  uint16_t* vs;
+  int64_t capacity;
+  int n_kv_heads;
+};
+
+// f16 magnitude a 4-bit block's scale saturates at: values past 8 * 65504 are
+// clamped before the block is coded (as e4m3 saturates at 448).
+constexpr float Q4_SCALE_MAX = 65504.0f;
+constexpr float Q4_VALUE_MAX = 8.0f * Q4_SCALE_MAX;
+
+// Index of (key, head) in rows of `row` elements: 64-bit, a long cache's
+// element offsets pass 2^31.
+FLOCK_DEV size_t kv_row(const KvView& c, int64_t key, int head) {
+  return ((size_t)key * c.n_kv_heads + head) * KV_HD;
+}
+FLOCK_DEV size_t q4_row(const KvView& c, int64_t key, int head) {
+  return ((size_t)head * c.capacity + key);
+}
+
+// Elements 4 lane .. 4 lane + 3 of a cached row, widened exactly.
+template <int KV, bool IS_K>
+FLOCK_DEV float4 kv_load4(const KvView& c, int64_t key, int head, int lane) {
+  const void* base = IS_K ? c.k : c.v;
+  if constexpr (KV == FLOCK_KV_Q4) {
+    const size_t row = q4_row(c, key, head);
+    const int b = lane >> 3, i0 = (4 * lane) & 31, byte0 = i0 & 15, sh = i0 & 16 ? 4 : 0;
+    const uint8_t* r = static_cast<const uint8_t*>(base) + row * 64;
+    uint32_t w;
+    if (IS_K) {
+      w = *reinterpret_cast<const uint32_t*>(r + 16 * (byte0 >> 2) + 4 * b);
+    } else {
+      const uint32_t lo = *reinterpret_cast<const uint16_t*>(r + 8 * (byte0 >> 1) + 2 * b);
+      const uint32_t hi = *reinterpret_cast<const uint16_t*>(r + 8 * (byte0 >> 1) + 8 + 2 * b);
+      w = lo | (hi << 16);
+    }
+    const float d = __half2float(__ushort_as_half((IS_K ? c.ks : c.vs)[row * 4 + b]));
+    w = (w >> sh) & 0x0F0F0F0Fu;
+    float x, y, z, t;
+    dec_nib4(w, x, y, z, t);
+    return make_float4(fmul(x, d), fmul(y, d), fmul(z, d), fmul(t, d));
+  } else if constexpr (KV == FLOCK_KV_FP8) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(base) +
+                                                          kv_row(c, key, head) + 4 * lane);
+    const float2 a = fp8x2_widen(w), b = fp8x2_widen(w >> 16);
+    return make_float4(a.x, a.y, b.x, b.y);
+  } else if constexpr (KV == FLOCK_KV_BF16) {
+    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) +
+                                                    kv_row(c, key, head) + 4 * lane);
+    const float2 a = bf16x2_widen(w.x), b = bf16x2_widen(w.y);
+    return make_float4(a.x, a.y, b.x, b.y);
+  } else {
+    return *reinterpret_cast<const float4*>(static_cast<const float*>(base) +
+                                            kv_row(c, key, head) + 4 * lane);
+  }
+}
+
+// One row (lane: elements 4 lane .. 4 lane + 3) into the 4-bit cache.
+//
+// The code of x is decided in f64, x * (1 / d) + 8.5 with one rounding each,
+// as flock_quant_q4 decides it: the codes of a row are the host's bytes.  A
+// block with a NaN gets a NaN scale (every value of it reads back NaN).
+template <bool IS_K>
+FLOCK_DEV void q4_store_row(const KvView& c, int64_t key, int head, float4 x4, int lane) {
+  float x[4] = {x4.x, x4.y, x4.z, x4.w};
+  bool nan = false;
+  float top = 0.0f;  // this lane's first value of largest magnitude
+  int at = 4 * (lane & 7);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    nan |= x[i] != x[i];
+    x[i] = fminf(fmaxf(x[i], -Q4_VALUE_MAX), Q4_VALUE_MAX);
+    if (fabsf(x[i]) > fabsf(top)) {
+      top = x[i];
+      at = 4 * (lane & 7) + i;
+    }
+  }
+#pragma unroll
+  for (int s = 1; s < 8; s <<= 1) {  // over the block's 8 lanes; the lower index wins a tie
+    const float o = __shfl_xor_sync(0xffffffffu, top, s);
+    const int oa = __shfl_xor_sync(0xffffffffu, at, s);
+    if (fabsf(o) > fabsf(top) || (fabsf(o) == fabsf(top) && oa < at)) {
+      top = o;
+      at = oa;
+    }
+    nan |= __shfl_xor_sync(0xffffffffu, (int)nan, s) != 0;
+  }
+  const double d = (double)top / -8.0;
+  const double inv = d == 0.0 ? 0.0 : 1.0 / d;
+  uint32_t code = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const double t = floor(__dadd_rn(__dmul_rn((double)x[i], inv), 8.5));
+    const int q = t < 0.0 ? 0 : t > 15.0 ? 15 : (int)t;
+    code |= (uint32_t)q << (8 * i);
+  }
+  // lanes 0-3 of a block hold values 0..15 (low nibbles), lanes 4-7 16..31
+  const uint32_t high = __shfl_xor_sync(0xffffffffu, code, 4);
+  const size_t row = q4_row(c, key, head);
+  const int b = lane >> 3, p = lane & 7;
+  if (p < 4) {
+    const uint32_t w = code | (high << 4);  // bytes 4 p .. 4 p + 3 of block b
+    uint8_t* r = static_cast<uint8_t*>(IS_K ? c.k : c.v) + row * 64;
+    if (IS_K) {
+      *reinterpret_cast<uint32_t*>(r + 16 * p + 4 * b) = w;
+    } else {
+      *reinterpret_cast<uint16_t*>(r + 16 * p + 2 * b) = (uint16_t)w;
+      *reinterpret_cast<uint16_t*>(r + 16 * p + 8 + 2 * b) = (uint16_t)(w >> 16);
+    }
+  }
+  if (p == 0)
+    (IS_K ? c.ks : c.vs)[row * 4 + b] =
+        nan ? (uint16_t)0x7E00u : __half_as_ushort(__float2half_rn((float)d));
+}
+
+template <int KV, bool IS_K>
+FLOCK_DEV void kv_store4(const KvView& c, int64_t key, int head, float4 x, int lane) {
+  void* base = IS_K ? c.k : c.v;
+  if constexpr (KV == FLOCK_KV_Q4) {
+    q4_store_row<IS_K>(c, key, head, x, lane);
+  } else if constexpr (KV == FLOCK_KV_FP8) {
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(base) + kv_row(c, key, head) + 4 * lane) =
+        (uint32_t)fp8_bits(x.x) | (uint32_t)fp8_bits(x.y) << 8 | (uint32_t)fp8_bits(x.z) << 16 |
+        (uint32_t)fp8_bits(x.w) << 24;
+  } else if constexpr (KV == FLOCK_KV_BF16) {
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + kv_row(c, key, head) + 4 * lane) =
+        make_uint2((uint32_t)bf16_bits(x.x) | (uint32_t)bf16_bits(x.y) << 16,
+                   (uint32_t)bf16_bits(x.z) | (uint32_t)bf16_bits(x.w) << 16);
+  } else {
+    *reinterpret_cast<float4*>(static_cast<float*>(base) + kv_row(c, key, head) + 4 * lane) = x;
+  }
+}
+
+// One warp per cached row: k and v of (token, head) rounded into the cache.
+template <int KV>
+static __global__ void __launch_bounds__(256) k_kv_append(KvView c, const float* k, const float* v,
+                                                          int64_t row_stride, int64_t pos, int n) {
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (item >= (int64_t)n * c.n_kv_heads) return;
+  const int64_t tok = item / c.n_kv_heads;
+  const int head = (int)(item % c.n_kv_heads);
+  const size_t src = (size_t)tok * row_stride + (size_t)head * KV_HD + 4 * lane;
+  const float4 kx = __ldg(reinterpret_cast<const float4*>(k + src));
+  const float4 vx = __ldg(reinterpret_cast<const float4*>(v + src));
+  kv_store4<KV, true>(c, pos + tok, head, kx, lane);
+  kv_store4<KV, false>(c, pos + tok, head, vx, lane);
+}
+
+// The cached rows [pos, pos + n) as f32 [n][kv heads][128].
+template <int KV>
+static __global__ void __launch_bounds__(256) k_kv_read(KvView c, int64_t pos, int n, float* k,
+                                                        float* v) {
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (item >= (int64_t)n * c.n_kv_heads) return;
+  const int64_t tok = item / c.n_kv_heads;
+  const int head = (int)(item % c.n_kv_heads);
+  const size_t dst = (size_t)item * KV_HD + 4 * lane;
+  *reinterpret_cast<float4*>(k + dst) = kv_load4<KV, true>(c, pos + tok, head, lane);
+  *reinterpret_cast<float4*>(v + dst) = kv_load4<KV, false>(c, pos + tok, head, lane);
+}
+
+// Queries at positions pos .. pos + n_queries - 1, row i of q [n_heads][128]
+// at q + i * q_stride.  Query position p sees key j iff j <= p and (window
+// == 0 or j > p - window or j < sinks).
+struct KvAttnArgs {
+  KvView c;
+  const float* q;
+  float* out;
+  int64_t q_stride, out_stride;
+  int64_t pos;
+  int n_queries, n_heads, window, sinks;
+};
+
+// One warp per (query, head): the running maximum and sum of a softmax over
+// the visible keys in order, one key at a time.
+template <int KV>
+static __global__ void __launch_bounds__(128) k_kv_attn(const KvAttnArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (item >= (int64_t)a.n_queries * a.n_heads) return;
+  const int query = (int)(item / a.n_heads), h = (int)(item % a.n_heads);
+  const int head = h / (a.n_heads / a.c.n_kv_heads);
+  const int64_t p = a.pos + query;
+  const int64_t lo = a.window && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
+  const int64_t sinks = a.sinks < lo ? a.sinks : lo;
+  const float scale = __double2float_rn(1.0 / sqrt(128.0));
+  const float4 q = *reinterpret_cast<const float4*>(a.q + query * a.q_stride + h * KV_HD + 4 * lane);
+  float m = -INFINITY, l = 0.0f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int64_t i = 0; i < sinks + p - lo + 1; i++) {
+    const int64_t key = i < sinks ? i : lo + (i - sinks);
+    const float4 kx = kv_load4<KV, true>(a.c, key, head, lane);
+    float s = ffma(q.w, kx.w, ffma(q.z, kx.z, ffma(q.y, kx.y, fmul(q.x, kx.x))));
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) s = fadd(s, __shfl_xor_sync(0xffffffffu, s, d));
+    s = fmul(s, scale);
+    const float mn = fmaxf(m, s);
+    const float e = expf(fsub(s, mn)), f = expf(fsub(m, mn));
+    const float4 vx = kv_load4<KV, false>(a.c, key, head, lane);
+    o = make_float4(ffma(e, vx.x, fmul(f, o.x)), ffma(e, vx.y, fmul(f, o.y)),
+                    ffma(e, vx.z, fmul(f, o.z)), ffma(e, vx.w, fmul(f, o.w)));
+    l = ffma(f, l, e);
+    m = mn;
+  }
+  const float inv = fdiv(1.0f, l);
+  *reinterpret_cast<float4*>(a.out + query * a.out_stride + h * KV_HD + 4 * lane) =
+      make_float4(fmul(o.x, inv), fmul(o.y, inv), fmul(o.z, inv), fmul(o.w, inv));
+}
+
+}  // namespace flock

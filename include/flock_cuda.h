@@ -70,6 +70,8 @@ extern "C" {
                            (ties to even, magnitudes past 448 saturate to 448, no
                            scale) once and every read widens it exactly.  Needs
                            FLOCK_ATTN_FAST and FLOCK_PREFILL_TENSOR. */
+#define FLOCK_KV_Q4 3   /* 4-bit KV cache: blocks of 32 values along the head in the Q4_0 rule
+                           (lib.ts:64), 4.5 bits a value, 0.14 of f32's bytes per key */
 
 #define FLOCK_MATVEC_EXACT 0 /* one-token matvecs in cpuMatmulQ8F32(coop(64))'s f32 order
                                 (lib.ts:213), bit-identical */
@@ -85,6 +87,7 @@ typedef struct flock_model flock_model;
 typedef struct flock_shard flock_shard;
 typedef struct flock_head flock_head;
 typedef struct flock_comm flock_comm;
+typedef struct flock_kv flock_kv;
 
 /* kernels/layer.ts:87-112 LayerConfig (+ the decode-attention choice). */
 typedef struct flock_layer_config {
@@ -259,6 +262,58 @@ FLOCK_API int flock_op_argmax(flock_dev* dev, const float* x, int64_t n, int64_t
  * them on one stream. */
 FLOCK_API int flock_argmax_noalloc(const float* x, int64_t n, int32_t* index_out, float* value_out,
                                    void* stream);
+
+/* ------------------------------------------------------------- KV caches
+ * A KV cache in device memory, with its attention, for callers that keep
+ * their own keys and queries on the device (no counterpart in the reference,
+ * whose cache lives inside Layer).  k, v, q and out are device pointers on
+ * the handle's device, f32, 16-byte aligned; strides count floats between
+ * rows, 0 meaning dense.  `stream` is a cudaStream_t (NULL: the default
+ * stream): work is enqueued there and nothing waits for it, so buffers that
+ * another stream uses must be ordered by the caller, and the calls may be
+ * captured into a graph (positions are then fixed at capture).
+ *
+ * A handle's attention uses its workspace: attention calls of one handle must
+ * not overlap on the GPU (one stream, or events between them); streams or
+ * captured graphs that may run at the same time need a handle each, which may
+ * share the planes but not the workspace.
+ *
+ * Planes.  FLOCK_KV_F32 / _BF16 / _FP8: k and v [capacity][n_kv_heads][128].
+ * FLOCK_KV_Q4: k and v are bytes [n_kv_heads][capacity][64], k_scales and
+ * v_scales f16 [n_kv_heads][capacity][4], capacity a multiple of 16: a head's
+ * four blocks of 32 values, byte i of a block = code i | code i+16 << 4, value
+ * (code - 8) * scale; byte i of block b lies at 16 (i / 4) + 4 b + i % 4 of
+ * the row in k and at 8 (i / 2) + 2 b + i % 2 in v. */
+#define FLOCK_WORKSPACE_BYTES 8388608 /* of a flock_kv or flock_verify_draft workspace */
+
+/* A cache of `capacity` keys over the caller's planes (NULL: the handle
+ * allocates them, zero-filled).  workspace: FLOCK_WORKSPACE_BYTES of device
+ * memory that were zero-filled once and that nothing else writes (NULL: the
+ * handle allocates it).  Caller-owned memory must outlive the handle.
+ * head_dim must be 128. */
+FLOCK_API int flock_kv_create(flock_dev* dev, int kv_dtype, int n_kv_heads, int head_dim,
+                              int64_t capacity, void* k, void* v, void* k_scales, void* v_scales,
+                              void* workspace, flock_kv** out);
+FLOCK_API int flock_kv_free(flock_kv* c);
+/* Round n rows of k and v [n_kv_heads][128] into the cache at positions pos ..
+ * pos + n - 1.  f32 is kept, bf16 and e4m3 round to nearest even as the layers'
+ * appends do (e4m3 saturates at 448), the 4-bit blocks take flock_quant_q4's
+ * codes (values saturate at 8 * 65504; a block with a NaN reads back NaN). */
+FLOCK_API int flock_kv_append(flock_kv* c, const float* k, const float* v, int64_t row_stride,
+                              int64_t pos, int n, void* stream);
+/* The cached rows pos .. pos + n - 1 as f32 [n][n_kv_heads][128]. */
+FLOCK_API int flock_kv_read(flock_kv* c, int64_t pos, int n, float* k, float* v, void* stream);
+/* Causal attention of n_queries queries [n_heads][128] at positions pos ..
+ * pos + n_queries - 1 over the cache, which holds every key up to them: query
+ * position p sees key j iff j <= p and (window == 0, or j > p - window, or j <
+ * sinks).  Scale 1/sqrt(128), softmax and sums in f32; query heads share the
+ * kv heads in order (n_heads a multiple of n_kv_heads).  Keys no query sees
+ * are not read into the result, whatever they hold; a NaN or infinity in a
+ * key or value that only some queries of the call see makes the others'
+ * outputs undefined. */
+FLOCK_API int flock_kv_attention(flock_kv* c, const float* q, int64_t q_stride, int n_heads,
+                                 int n_queries, int64_t pos, int window, int sinks, float* out,
+                                 int64_t out_stride, void* stream);
 
 /* ---------------------------------------------------------------- layer */
 

@@ -25,8 +25,10 @@ export const FLOCK_PREFILL_TENSOR = 1;
 export const FLOCK_KV_F32 = 0;
 export const FLOCK_KV_BF16 = 1;
 export const FLOCK_KV_FP8 = 2;
+export const FLOCK_KV_Q4 = 3;
 export const FLOCK_MATVEC_EXACT = 0;
 export const FLOCK_MATVEC_FAST = 1;
+export const FLOCK_WORKSPACE_BYTES = 8388608;
 export const FLOCK_TP_NCCL = 0;
 export const FLOCK_TP_PEER = 1;
 export const FLOCK_DECODE_KERNELS = 0;
@@ -109,6 +111,16 @@ export const symbols = {
   flock_op_argmax: { parameters: ["pointer", "buffer", "i64", "buffer", "buffer"], result: "i32" },
   // (x, n, index_out, value_out, stream)
   flock_argmax_noalloc: { parameters: ["buffer", "i64", "buffer", "buffer", "buffer"], result: "i32" },
+  // (dev, kv_dtype, n_kv_heads, head_dim, capacity, k, v, k_scales, v_scales, workspace, out)
+  flock_kv_create: { parameters: ["pointer", "i32", "i32", "i32", "i64", "buffer", "buffer", "buffer", "buffer", "buffer", "buffer"], result: "i32" },
+  // (c)
+  flock_kv_free: { parameters: ["pointer"], result: "i32" },
+  // (c, k, v, row_stride, pos, n, stream)
+  flock_kv_append: { parameters: ["pointer", "buffer", "buffer", "i64", "i64", "i32", "buffer"], result: "i32" },
+  // (c, pos, n, k, v, stream)
+  flock_kv_read: { parameters: ["pointer", "i64", "i32", "buffer", "buffer", "buffer"], result: "i32" },
+  // (c, q, q_stride, n_heads, n_queries, pos, window, sinks, out, out_stride, stream)
+  flock_kv_attention: { parameters: ["pointer", "buffer", "i64", "i32", "i32", "i64", "i32", "i32", "buffer", "i64", "buffer"], result: "i32" },
   // (dev, cfg, n_tensors, names, tensors, out)
   flock_layer_create: { parameters: ["pointer", "buffer", "i32", "buffer", "buffer", "buffer"], result: "i32" },
   // (layer)

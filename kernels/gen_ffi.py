@@ -24,7 +24,7 @@ HEADER = os.path.join(HERE, "..", "include", "flock_cuda.h")
 OUT = os.path.join(HERE, "cuda_ffi.ts")
 
 HANDLES = {"flock_dev", "flock_tensor", "flock_layer", "flock_model", "flock_shard",
-           "flock_head", "flock_comm", "flock_gguf"}
+           "flock_head", "flock_comm", "flock_gguf", "flock_kv"}
 SCALARS = {"int": "i32", "int32_t": "i32", "int64_t": "i64", "uint32_t": "u32",
            "float": "f32", "double": "f64"}
 # C scalar sizes/alignments for the struct layout
