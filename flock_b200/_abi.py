@@ -109,6 +109,8 @@ SIGNATURES = {
     "flock_kv_append": [_vp, _vp, _vp, _i64, _i64, _i, _vp],
     "flock_kv_read": [_vp, _i64, _i, _vp, _vp, _vp],
     "flock_kv_attention": [_vp, _vp, _i64, _i, _i, _i64, _i, _i, _vp, _i64, _vp],
+    "flock_verify_draft": [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i, _i, _i64,
+                           ctypes.c_double, _vp, _vp, _vp, _vp],
     "flock_layer_create": [_vp, _cfgp, _i, _ccp, _pp, _pp],
     "flock_layer_free": [_vp],
     "flock_layer_encode": [_vp, _fp, _i],

@@ -152,6 +152,48 @@ class KVCache:
             _abi.check(rc)
 
 
+class DraftVerifier:
+    """flock_verify_draft over a vocabulary: drafted tokens checked against the
+    target's logits with given uniform numbers.  ``workspace``: WORKSPACE_BYTES
+    of device uint8 that no overlapping call uses."""
+
+    def __init__(self, dev: Device, vocab: int, workspace):
+        self.dev, self.vocab = dev, vocab
+        self._keep = workspace
+        self._ws = _workspace(workspace, dev.ordinal)
+        self._verify = _abi.lib().flock_verify_draft
+
+    def _logits(self, a, what: str, n: int, rows: int) -> tuple:
+        p, shape, st = _array(a, "f32", self.dev.ordinal, what)
+        if tuple(shape) != (n, rows, self.vocab):
+            raise ValueError(f"{what} is {tuple(shape)}, want {(n, rows, self.vocab)}")
+        if st is None:
+            return p, 0
+        step = st[1] if rows > 1 else st[0]
+        if st[2] != 1 or (n > 1 and st[0] != rows * step) or step < self.vocab:
+            raise ValueError(f"{what} has strides {tuple(st)}: rows must be evenly spaced")
+        return p, step
+
+    def verify(self, target, draft, ids, u, tokens, accepted, lens=None,
+               temperature: float = 1.0, stream: int = 0) -> None:
+        """target [n][d + 1][vocab] f32, draft [n][d][vocab] f32 or None, ids
+        [n][d] i32, u [n][d + 1] f32 in [0, 1), lens [n] i32 or None; into
+        tokens [n][d + 1] and accepted [n], i32.  include/flock_cuda.h
+        flock_verify_draft has the rule."""
+        o = self.dev.ordinal
+        ip, (n, d), st = _array(ids, "i32", o, "ids")
+        if st is not None:
+            raise ValueError("ids must be dense")
+        tp, ts = self._logits(target, "target", n, d + 1)
+        dp, ds = (None, 0) if draft is None else self._logits(draft, "draft", n, d)
+        rc = self._verify(self.dev.handle, tp, ts, dp, ds, ip, _dense(u, "f32", o, "u", (n, d + 1)),
+                          None if lens is None else _dense(lens, "i32", o, "lens", (n,)), n, d,
+                          self.vocab, temperature, _dense(tokens, "i32", o, "tokens", (n, d + 1)),
+                          _dense(accepted, "i32", o, "accepted", (n,)), self._ws, stream or None)
+        if rc:
+            _abi.check(rc)
+
+
 def _workspace(a, ordinal: int) -> int:
     p, shape, strides = _array(a, "u8", ordinal, "workspace")
     if strides is not None or math.prod(shape) < WORKSPACE_BYTES:

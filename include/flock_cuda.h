@@ -315,6 +315,41 @@ FLOCK_API int flock_kv_attention(flock_kv* c, const float* q, int64_t q_stride, 
                                  int n_queries, int64_t pos, int window, int sinks, float* out,
                                  int64_t out_stride, void* stream);
 
+/* ----------------------------------------------------- draft verification
+ * Drafted tokens checked against the target model's distribution (no
+ * counterpart in the reference, which decodes greedily, one token a step).
+ * Device pointers on dev's device; `stream` as in flock_kv_*.
+ *
+ * n_seqs sequences of up to n_drafts drafted tokens ids [n_seqs][n_drafts]
+ * (lens [n_seqs]: each sequence's count, clamped to 0..n_drafts; NULL: all).
+ * target: logits [n_seqs][n_drafts + 1][vocab], row i the distribution after
+ * the tokens before draft i, rows target_stride floats apart (0: dense).
+ * draft: the logits [n_seqs][n_drafts][vocab] the drafts were drawn from at
+ * the same temperature, or NULL when each draft was certain (a lookup).
+ * u [n_seqs][n_drafts + 1]: uniform numbers in [0, 1).
+ *
+ * With p_i and q_i the softmax of the rows / temperature (q_i = 1 at ids[i]
+ * without draft logits), draft i is kept iff u_i q_i(ids[i]) < p_i(ids[i]) and
+ * every one before it was.  At the first refusal r the next token is drawn
+ * from max(p_r - q_r, 0), normalised (from p_r where nothing is left), after
+ * `lens` kept drafts from p: the lowest index whose running sum passes
+ * u_{n_drafts} of the total.  temperature 0: drafts are kept while they equal
+ * the argmax (lowest index among the maxima, NaN never one), draft and u are
+ * not read.  tokens [n_seqs][n_drafts + 1]: the kept drafts, the next token,
+ * then -1; accepted [n_seqs]: how many were kept.
+ *
+ * -inf logits are probability 0.  A row with a NaN or +inf, or with only
+ * -inf, has no distribution: the drafts end there and the next token is -1.
+ * An id outside 0..vocab-1 is refused.  Rows past a sequence's drafts are not
+ * read.  workspace: FLOCK_WORKSPACE_BYTES of device memory, 16-byte aligned,
+ * of which nothing is kept between calls; calls that may overlap on the GPU
+ * need one each.  At most 512 drafts and 65535 rows of logits a call. */
+FLOCK_API int flock_verify_draft(flock_dev* dev, const float* target, int64_t target_stride,
+                                 const float* draft, int64_t draft_stride, const int32_t* ids,
+                                 const float* u, const int32_t* lens, int n_seqs, int n_drafts,
+                                 int64_t vocab, double temperature, int32_t* tokens,
+                                 int32_t* accepted, void* workspace, void* stream);
+
 /* ---------------------------------------------------------------- layer */
 
 /* kernels/layer.ts:228 Layer.fromBuffers: `names` are the GGUF suffixes

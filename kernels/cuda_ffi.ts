@@ -121,6 +121,8 @@ export const symbols = {
   flock_kv_read: { parameters: ["pointer", "i64", "i32", "buffer", "buffer", "buffer"], result: "i32" },
   // (c, q, q_stride, n_heads, n_queries, pos, window, sinks, out, out_stride, stream)
   flock_kv_attention: { parameters: ["pointer", "buffer", "i64", "i32", "i32", "i64", "i32", "i32", "buffer", "i64", "buffer"], result: "i32" },
+  // (dev, target, target_stride, draft, draft_stride, ids, u, lens, n_seqs, n_drafts, vocab, temperature, tokens, accepted, workspace, stream)
+  flock_verify_draft: { parameters: ["pointer", "buffer", "i64", "buffer", "i64", "buffer", "buffer", "buffer", "i32", "i32", "i64", "f64", "buffer", "buffer", "buffer", "buffer"], result: "i32" },
   // (dev, cfg, n_tensors, names, tensors, out)
   flock_layer_create: { parameters: ["pointer", "buffer", "i32", "buffer", "buffer", "buffer"], result: "i32" },
   // (layer)
