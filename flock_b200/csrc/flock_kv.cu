@@ -6,6 +6,7 @@
 
 #include "flock_internal.h"
 #include "kv.cuh"
+#include "kv_rows.cuh"
 
 using namespace flock;
 
@@ -83,6 +84,33 @@ int by_dtype(int kv_dtype, F f) {
     case FLOCK_KV_BF16: return f(std::integral_constant<int, FLOCK_KV_BF16>());
     default: return f(std::integral_constant<int, FLOCK_KV_F32>());
   }
+}
+
+// A few query rows per kv head: k_kv_rows, RT rows a CTA.
+template <int KV, int RT>
+int launch_rows(const flock_kv* c, const KvAttnArgs& a, cudaStream_t st) {
+  using L = KrLayout<KV>;
+  KvRowsArgs p = {};
+  p.a = a;
+  p.group = a.n_heads / a.c.n_kv_heads;
+  p.rows = a.n_queries * p.group;
+  const int tiles = (p.rows + RT - 1) / RT;
+  const int64_t items = (int64_t)tiles * a.c.n_kv_heads;
+  // key splits: every warp a group of keys, as far as one CTA per SM allows
+  const int64_t lo = a.window && a.pos + 1 > a.window ? a.pos + 1 - a.window : 0;
+  const int64_t keys = a.pos + a.n_queries - lo + (a.sinks < lo ? a.sinks : lo);
+  const int64_t want = (keys + KR_GROUP * L::WARPS - 1) / (KR_GROUP * L::WARPS);
+  const int64_t room = c->dev->sm_count / items;
+  p.splits = (int)(want < room ? want : room);
+  if (p.splits < 1) p.splits = 1;
+  p.count = reinterpret_cast<uint32_t*>(c->workspace);
+  p.part = reinterpret_cast<float*>(c->workspace + KR_PART_OFFSET);
+  auto k = k_kv_rows<KV, RT>;
+  FLOCK_TRY(kernel_setup((const void*)k, (int)L::SMEM));
+  k<<<dim3((unsigned)p.splits, (unsigned)tiles, (unsigned)a.c.n_kv_heads), L::THREADS, L::SMEM,
+      st>>>(p);
+  FLOCK_CK(cudaGetLastError());
+  return FLOCK_OK;
 }
 
 }  // namespace
@@ -282,6 +310,13 @@ int flock_kv_attention(flock_kv* c, const float* q, int64_t q_stride, int n_head
   a.window = window;
   a.sinks = sinks;
   const unsigned grid = (unsigned)(((int64_t)n_queries * n_heads + 3) / 4);
+  const int64_t rows = (int64_t)n_queries * (n_heads / c->view.n_kv_heads);
+  if (rows <= 16)
+    return by_dtype(c->kv_dtype, [&](auto kv) -> int {
+      constexpr int KV = decltype(kv)::value;
+      return rows <= 2 ? launch_rows<KV, 2>(c, a, static_cast<cudaStream_t>(stream))
+                       : launch_rows<KV, 4>(c, a, static_cast<cudaStream_t>(stream));
+    });
   return by_dtype(c->kv_dtype, [&](auto kv) -> int {
     k_kv_attn<decltype(kv)::value><<<grid, 128, 0, static_cast<cudaStream_t>(stream)>>>(a);
     FLOCK_CK(cudaGetLastError());
