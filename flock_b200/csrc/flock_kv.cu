@@ -314,8 +314,8 @@ int flock_kv_attention(flock_kv* c, const float* q, int64_t q_stride, int n_head
   if (rows <= 16)
     return by_dtype(c->kv_dtype, [&](auto kv) -> int {
       constexpr int KV = decltype(kv)::value;
-      return rows <= 2 ? launch_rows<KV, 2>(c, a, static_cast<cudaStream_t>(stream))
-                       : launch_rows<KV, 4>(c, a, static_cast<cudaStream_t>(stream));
+      return rows <= 2 ? launch_rows<KV, kr_rows<KV>(2)>(c, a, static_cast<cudaStream_t>(stream))
+                       : launch_rows<KV, kr_rows<KV>(4)>(c, a, static_cast<cudaStream_t>(stream));
     });
   return by_dtype(c->kv_dtype, [&](auto kv) -> int {
     k_kv_attn<decltype(kv)::value><<<grid, 128, 0, static_cast<cudaStream_t>(stream)>>>(a);

@@ -6,22 +6,24 @@
 // widened once, in registers, straight into the operand of a matrix
 // instruction, for all query heads that share the kv head.
 //
-// mma.sync m16n8k16 (bf16, f32 accumulation) rather than tcgen05: with two to
-// four live rows there is nothing to amortise a pass of the operands through
-// shared memory and tensor memory over; this path takes cached bytes from
-// shared memory to the operand registers with no store in between.
+// mma.sync m16n8k16 (f32 accumulation) rather than tcgen05: with two to eight
+// live rows there is nothing to amortise a pass of the operands through shared
+// memory and tensor memory over; this path takes cached bytes from shared
+// memory to the operand registers with no store in between.
 //
-// f32 results from bf16 operands.  A code minus 8, an e4m3 and a bf16 are bf16
-// values; an f32 x is hi + mid + lo, three bf16 of 8 bits each (24 bits, f32's
-// range).  Queries and softmax weights are split that way, and the three parts
-// sit in different ROWS of the 16-row operand ("slots"), which a decode leaves
-// empty anyway: one instruction multiplies all three.  f32 caches split their
-// elements too, three instructions a step.
+// f32 results from 16-bit operands.  Codes minus 8 and e4m3 values are f16
+// values, so there queries and softmax weights are split as hi + lo, two f16
+// of 11 bits (22 bits; scaled by powers of two so that f16's range never
+// cuts a part that matters).  bf16 and f32 elements need f32's range: hi + mid
+// + lo, three bf16 of 8 bits.  The parts sit in different ROWS of the 16-row
+// operand, which a decode leaves empty anyway: one instruction multiplies all.
 //
-// 4-bit blocks.  Scores: a block's 32 products are summed exactly as integers
-// times query parts, then multiplied by the key's scale in f32 (one
-// accumulator per block).  Values: the scale joins the weight, p d_b, split
-// after the product: one weight operand per block.
+// 4-bit blocks.  Scores: a block's 32 products are summed as integers times
+// query parts, then multiplied by the key's scale in f32 (one accumulator per
+// block).  Values: the scale joins the weight before its split, so the weight
+// operand differs per block; its rows hold (block, query row), each lane
+// computes its own block's weights only, and of an output tile's rows the ones
+// of the tile's block count.
 //
 // Work split: CTA (split z, row tile, kv head), its warps taking 16-key groups
 // in turn, each with its own cp.async ring, running maximum, sum and output;
@@ -95,56 +97,83 @@ FLOCK_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "me
 template <int N>
 FLOCK_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-FLOCK_DEV void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+template <bool F16>
+FLOCK_DEV void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 FLOCK_DEV float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Two f32 -> bf16 pair (nearest even), lo in the low half.
+// Two f32 -> a pair of 16-bit values (nearest even), lo in the low half.
 FLOCK_DEV uint32_t bf2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-FLOCK_DEV float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
-FLOCK_DEV float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-// x minus the bf16 parts a slot leaves to the ones before it (exact
-// differences): part `slot` of hi + mid + lo for two values.
-FLOCK_DEV uint32_t bf_part(float x, float y, int slot) {
-  uint32_t w = bf2(x, y);
-  if (slot >= 1) {
-    x = fsub(x, bf_lo(w));
-    y = fsub(y, bf_hi(w));
-    w = bf2(x, y);
-  }
-  if (slot >= 2) {
-    x = fsub(x, bf_lo(w));
-    y = fsub(y, bf_hi(w));
-    w = bf2(x, y);
-  }
-  return w;
+FLOCK_DEV uint32_t hf2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
-// Codes at bits 0-3 and 16-19 -> (code - 8) as a bf16 pair: 0x4300 | code is
-// the bf16 128 + code, and 136 is taken off exactly.
-FLOCK_DEV uint32_t nib_bf2(uint32_t w) {
-  const uint32_t u = (w & 0x000F000Fu) | 0x43004300u;
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u),
-                                   __nv_bfloat162(__ushort_as_bfloat16(0x4308),
-                                                  __ushort_as_bfloat16(0x4308)));
-  return *reinterpret_cast<const uint32_t*>(&r);
+FLOCK_DEV float2 h2f2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+// x = hi + lo (f16), x = hi + mid + lo (bf16), for two values; every
+// difference is exact.
+FLOCK_DEV void split_f16(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = hf2(x, y);
+  const float2 f = h2f2(hi);
+  lo = hf2(fsub(x, f.x), fsub(y, f.y));
 }
-// Two e4m3 in the low half -> bf16 pair, exactly (e4m3 is a subset of both
-// f16 and bf16).
-FLOCK_DEV uint32_t fp8_bf2(uint32_t w) {
-  const float2 f = fp8x2_widen(w);
-  return bf2(f.x, f.y);
+FLOCK_DEV void split_bf16(float x, float y, uint32_t (&w)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; i++) {
+    w[i] = bf2(x, y);
+    x = fsub(x, __uint_as_float(w[i] << 16));
+    y = fsub(y, __uint_as_float(w[i] & 0xffff0000u));
+  }
+}
+// (a & b) | c in one instruction.
+FLOCK_DEV uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+FLOCK_DEV uint32_t hfma2_u(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+FLOCK_DEV uint32_t hadd2_u(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// The eight codes of a word -> (code - 8) as four f16 pairs: 0x6400 | code is
+// the f16 1024 + code, 0x6400 | 16 code is 1024 + 16 code, and the rest is
+// taken off exactly.  v[e]: bits 4 e .. 4 e + 3 of both halfwords.
+FLOCK_DEV void nib_f16(uint32_t w, uint32_t (&v)[4]) {
+  const uint32_t hi = w >> 8;
+  v[0] = hadd2_u(and_or(w, 0x000F000Fu, 0x64006400u), 0xE408E408u);                // - 1032
+  v[1] = hfma2_u(and_or(w, 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);   // / 16 - 72
+  v[2] = hadd2_u(and_or(hi, 0x000F000Fu, 0x64006400u), 0xE408E408u);
+  v[3] = hfma2_u(and_or(hi, 0x00F000F0u, 0x64006400u), 0x2C002C00u, 0xD480D480u);
+}
+// Two e4m3 in the low half -> f16 pair, exactly.
+FLOCK_DEV uint32_t fp8_f16(uint32_t w) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFFu), __NV_E4M3);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // The head dimension that element e (0-3) of lane column c meets in QK step ks
@@ -169,35 +198,28 @@ FLOCK_DEV int kr_vdim(int t, int n) {
 
 // One stage of keys key0 .. key0 + 15 of a head into shared memory; keys
 // outside [from, to) are zero-filled, so what lies there cannot reach a
-// product.
+// product.  kb, vb: the head's first rows; sb: this lane's scale plane at the
+// head's first row.
 template <int KV>
-FLOCK_DEV void kr_load(uint32_t stage, const KvView& c, int head, int64_t key0, int64_t from,
-                       int64_t to, int lane) {
+FLOCK_DEV void kr_load(uint32_t stage, const uint8_t* kb, const uint8_t* vb, const uint8_t* sb,
+                       int64_t step, int key0, int from, int to, int lane) {
   using L = KrLayout<KV>;
   constexpr int CHUNKS = L::ROW / 16;  // 16-byte chunks of a row
-  const uint8_t* kb = static_cast<const uint8_t*>(c.k);
-  const uint8_t* vb = static_cast<const uint8_t*>(c.v);
-  size_t base, step;
-  if (KV == FLOCK_KV_Q4) {
-    base = q4_row(c, 0, head) * 64;
-    step = 64;
-  } else {
-    base = (size_t)head * L::ROW;
-    step = (size_t)c.n_kv_heads * L::ROW;
-  }
+  const bool whole = key0 >= from && key0 + KR_GROUP <= to;
 #pragma unroll
   for (int i = 0; i < KR_GROUP * CHUNKS / 32; i++) {
     const int at = i * 32 + lane, r = at / CHUNKS, ch = at % CHUNKS;
-    const bool ok = key0 + r >= from && key0 + r < to;
-    const size_t off = base + (size_t)(ok ? key0 + r : from) * step + ch * 16;
+    const bool ok = whole || (key0 + r >= from && key0 + r < to);
+    // a 4-bit head's rows are contiguous: one offset for the whole group
+    const int64_t off = KV == FLOCK_KV_Q4 ? (int64_t)key0 * 64 + at * 16
+                                          : (int64_t)(ok ? key0 + r : from) * step + ch * 16;
     cp_async16(stage + r * L::K_STRIDE + ch * 16, kb + off, ok);
     cp_async16(stage + L::V_OFF + (r >> 2) * L::V_GROUP + (r & 3) * L::ROW + ch * 16, vb + off, ok);
   }
   if (KV == FLOCK_KV_Q4) {
     const int r = lane & 15;
-    const bool ok = key0 + r >= from && key0 + r < to;
-    const uint16_t* s = (lane < 16 ? c.ks : c.vs) + q4_row(c, ok ? key0 + r : from, head) * 4;
-    cp_async8(stage + L::S_OFF + lane * 8, s, ok);
+    const bool ok = whole || (key0 + r >= from && key0 + r < to);
+    cp_async8(stage + L::S_OFF + lane * 8, sb + (int64_t)(key0 + r) * 8, ok);
   }
 }
 
@@ -212,7 +234,16 @@ FLOCK_DEV uint2 lds64(uint32_t a) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
   return r;
 }
-FLOCK_DEV float2 h2f2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+
+// Rows of the operands, RT query rows per CTA.  Score operand: 4-bit RT = 2:
+// rows 0-1 hi, 2-3 lo, and again in 4-7; RT = 4: 0-3 hi, 4-7 lo.  e4m3 (RT 8):
+// 0-7 hi, 8-15 lo.  bf16, f32 (RT 4): 0-3 hi, 4-7 mid, 8-11 lo.  Weight operand:
+// as the score operand, but 4-bit RT = 2: row 2 b + j block b's hi, 8 + 2 b + j
+// its lo; RT = 4: row 4 b + j block b, hi and lo in two operands.
+template <int KV>
+constexpr int kr_rows(int rows) {
+  return KV == FLOCK_KV_FP8 ? 8 : KV == FLOCK_KV_Q4 && rows <= 2 ? 2 : 4;
+}
 
 // Keys of a stage are dealt to operand columns so that a lane's four score
 // columns are four neighbouring keys: column n of score tile t is key
@@ -220,6 +251,8 @@ FLOCK_DEV float2 h2f2(uint32_t w) { return __half22float2(*reinterpret_cast<cons
 template <int KV, int RT>
 static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(const KvRowsArgs p) {
   using L = KrLayout<KV>;
+  constexpr bool Q4 = KV == FLOCK_KV_Q4;
+  constexpr bool F16 = Q4 || KV == FLOCK_KV_FP8;
   extern __shared__ __align__(16) uint8_t kr_smem[];
   __shared__ float s_ml[L::WARPS][RT][2];
   __shared__ int s_last;
@@ -227,58 +260,93 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int z = blockIdx.x, tile = blockIdx.y, head = blockIdx.z;
-  // slot and row of this lane's operand rows: row g is (slot, j), row g + 8
-  // carries the last part of four rows and is empty for two
-  const int j = g % RT, slot = g / RT;
+  const int j = g % RT;  // this lane's query row
   const int row = tile * RT + j;
   const int first_q = tile * RT / p.group;
-  const int last_row = min(p.rows, (tile + 1) * RT) - 1;
-  const int last_q = last_row / p.group;
+  const int last_q = (min(p.rows, (tile + 1) * RT) - 1) / p.group;
   // keys that some row of the tile sees: sinks [0, sk), then [lo, hi)
-  const int64_t hi = a.pos + last_q + 1;
-  const int64_t lo = a.window && a.pos + first_q + 1 > a.window ? a.pos + first_q + 1 - a.window : 0;
-  const int64_t sk = a.sinks < lo ? a.sinks : lo;
-  const int sink_groups = (int)((sk + KR_GROUP - 1) / KR_GROUP);
-  const int64_t lo16 = lo & ~(int64_t)(KR_GROUP - 1);
-  const int groups = sink_groups + (int)((hi - lo16 + KR_GROUP - 1) / KR_GROUP);
+  const int pos = (int)a.pos;
+  const int hi = pos + last_q + 1;
+  const int lo = a.window && pos + first_q + 1 > a.window ? pos + first_q + 1 - a.window : 0;
+  const int sk = min(a.sinks, lo);
+  const int sink_groups = (sk + KR_GROUP - 1) / KR_GROUP;
+  const int lo16 = lo & ~(KR_GROUP - 1);
+  const int groups = sink_groups + (hi - lo16 + KR_GROUP - 1) / KR_GROUP;
   const int g0 = (int)((int64_t)z * groups / p.splits), g1 = (int)((int64_t)(z + 1) * groups / p.splits);
   // this row's own keys: sinks [0, row_sk), then [row_lo, row_hi)
   const int my_q = min(row, p.rows - 1) / p.group;
-  const int64_t row_hi = a.pos + my_q + 1;
-  const int64_t row_lo = a.window && row_hi > a.window ? row_hi - a.window : 0;
-  const int64_t row_sk = a.sinks < row_lo ? a.sinks : row_lo;
+  const int row_hi = pos + my_q + 1;
+  const int row_lo = a.window && row_hi > a.window ? row_hi - a.window : 0;
+  const int row_sk = min(a.sinks, row_lo);
 
   const uint32_t ring = smem_u32(kr_smem) + warp * L::STAGES * L::STAGE;
-  auto key_of = [&](int grp) -> int64_t {
-    return grp < sink_groups ? (int64_t)grp * KR_GROUP : lo16 + (int64_t)(grp - sink_groups) * KR_GROUP;
+  const size_t hbase = Q4 ? q4_row(a.c, 0, head) * 64 : (size_t)head * L::ROW;
+  const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + hbase;
+  const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + hbase;
+  const uint8_t* sb = Q4 ? reinterpret_cast<const uint8_t*>((lane < 16 ? a.c.ks : a.c.vs) +
+                                                            q4_row(a.c, 0, head) * 4)
+                         : nullptr;
+  const int64_t step = (int64_t)a.c.n_kv_heads * L::ROW;
+  auto key_of = [&](int grp) {
+    return grp < sink_groups ? grp * KR_GROUP : lo16 + (grp - sink_groups) * KR_GROUP;
   };
   auto fetch = [&](int grp, int st) {
     if (grp < g1) {
       const bool sink = grp < sink_groups;
-      kr_load<KV>(ring + st * L::STAGE, a.c, head, key_of(grp), sink ? 0 : lo, sink ? sk : hi, lane);
+      kr_load<KV>(ring + st * L::STAGE, kb, vb, sb, step, key_of(grp), sink ? 0 : lo,
+                  sink ? sk : hi, lane);
     }
     cp_async_commit();
   };
 #pragma unroll
   for (int s = 0; s < L::STAGES - 1; s++) fetch(g0 + warp + s * L::WARPS, s);
 
-  // the query operand: q * log2(e) / sqrt(128), its bf16 parts by slot
+  // The query operand: the parts of q log2(e) / sqrt(128), for f16 scaled by
+  // a power of two that brings the row's largest into [2^13, 2^14).
   uint32_t qa[8][4];
+  float unscale = 1.0f;
   {
     const float k = __double2float_rn(1.4426950408889634 / sqrt(128.0));
     const bool live = row < p.rows;
-    const float* q = a.q + my_q * a.q_stride + ((int64_t)head * p.group + min(row, p.rows - 1) % p.group) * KV_HD;
+    const float* q = a.q + my_q * a.q_stride +
+                     ((int64_t)head * p.group + min(row, p.rows - 1) % p.group) * KV_HD;
+    float x[8][4], top = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < 8; ks++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        x[ks][e] = live ? fmul(__ldg(q + kr_kdim<KV>(ks, c, e)), k) : 0.0f;
+        top = fmaxf(top, fabsf(x[ks][e]));
+      }
+    float scale = 1.0f;
+    if (F16) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int biased = (int)(__float_as_uint(top) >> 23);
+      const int e = biased == 0 ? 0 : max(-100, min(100, biased - 127 - 13));
+      scale = __uint_as_float((uint32_t)(127 - e) << 23);
+      unscale = __uint_as_float((uint32_t)(127 + e) << 23);
+    }
 #pragma unroll
     for (int ks = 0; ks < 8; ks++) {
-      float x[4];
-#pragma unroll
-      for (int e = 0; e < 4; e++) x[e] = live ? fmul(__ldg(q + kr_kdim<KV>(ks, c, e)), k) : 0.0f;
-      const bool used = slot < 3;
-      qa[ks][0] = used ? bf_part(x[0], x[1], slot) : 0;
-      qa[ks][2] = used ? bf_part(x[2], x[3], slot) : 0;
-      const bool low = RT == 4 && g < 4;  // row g + 8: part 2 of row g
-      qa[ks][1] = low ? bf_part(x[0], x[1], 2) : 0;
-      qa[ks][3] = low ? bf_part(x[2], x[3], 2) : 0;
+      if (F16) {
+        uint32_t h0, l0, h1, l1;
+        split_f16(fmul(x[ks][0], scale), fmul(x[ks][1], scale), h0, l0);
+        split_f16(fmul(x[ks][2], scale), fmul(x[ks][3], scale), h1, l1);
+        const bool low = Q4 && (RT == 2 ? (g & 2) : (g & 4));
+        qa[ks][0] = low ? l0 : h0;
+        qa[ks][2] = low ? l1 : h1;
+        qa[ks][1] = Q4 ? 0 : l0;
+        qa[ks][3] = Q4 ? 0 : l1;
+      } else {
+        uint32_t w0[3], w1[3];
+        split_bf16(x[ks][0], x[ks][1], w0);
+        split_bf16(x[ks][2], x[ks][3], w1);
+        qa[ks][0] = g < 4 ? w0[0] : w0[1];
+        qa[ks][2] = g < 4 ? w1[0] : w1[1];
+        qa[ks][1] = g < 4 ? w0[2] : 0;
+        qa[ks][3] = g < 4 ? w1[2] : 0;
+      }
     }
   }
   float o[16][4];
@@ -286,7 +354,14 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
   for (int t = 0; t < 16; t++)
 #pragma unroll
     for (int e = 0; e < 4; e++) o[t][e] = 0.0f;
-  float m = -INFINITY, l = 0.0f;
+  // Weights are 2^(s - base), base = m + dexp - 6: m a running maximum that may
+  // lag by 2^8, 2^dexp a bound on the value scales so far, so a weight times a
+  // scale is at most 2^14, inside f16, and its lo part loses nothing above
+  // 2^-31 of the largest.
+  constexpr float HEADROOM = F16 ? 6.0f : 0.0f;
+  float m = -INFINITY, l = 0.0f, base = 0.0f;
+  int dexp = Q4 ? -24 : 0;
+  float dlim = Q4 ? 5.9604645e-8f : 0.0f;  // 2^dexp
 
   int st = 0;
   for (int grp = g0 + warp; grp < g1; grp += L::WARPS) {
@@ -297,35 +372,38 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
     // ------------------------------------------------------------- scores
     float s[4];  // keys 4 c + i of this lane's row
     const uint32_t kaddr = stage + (4 * (g >> 1) + (g & 1)) * L::K_STRIDE + 16 * c;
-    uint4 sc0, sc1;
-    if (KV == FLOCK_KV_Q4) {
-      sc0 = lds128(stage + L::S_OFF + 32 * c);
-      sc1 = lds128(stage + L::S_OFF + 32 * c + 16);
-    }
+    if constexpr (Q4) {
+      const uint4 scales[2] = {lds128(stage + L::S_OFF + 32 * c),
+                               lds128(stage + L::S_OFF + 32 * c + 16)};
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
-      const uint32_t kt = kaddr + 2 * t * L::K_STRIDE;
-      if constexpr (KV == FLOCK_KV_Q4) {
-        const uint4 w4 = lds128(kt);
+      for (int t = 0; t < 2; t++) {
+        const uint4 w4 = lds128(kaddr + 2 * t * L::K_STRIDE);
         const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-        const uint4 sc = t ? sc1 : sc0;  // keys 4 c + 2 t and the next, four blocks each
-        const float2 d0[2] = {h2f2(sc.x), h2f2(sc.y)}, d1[2] = {h2f2(sc.z), h2f2(sc.w)};
-        float s0 = 0.0f, s1 = 0.0f;
+        // keys 4 c + 2 t and the next, four blocks each
+        const float2 k0[2] = {h2f2(scales[t].x), h2f2(scales[t].y)},
+                     k1[2] = {h2f2(scales[t].z), h2f2(scales[t].w)};
+        uint64_t sum = pack2(0.0f, 0.0f);
 #pragma unroll
         for (int b = 0; b < 4; b++) {
           float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_bf16(acc, qa[2 * b], nib_bf2(w[b]), nib_bf2(w[b] >> 8));
-          mma_bf16(acc, qa[2 * b + 1], nib_bf2(w[b] >> 4), nib_bf2(w[b] >> 12));
-          if (RT == 4) {
-            acc[0] = fadd(acc[0], acc[2]);
-            acc[1] = fadd(acc[1], acc[3]);
-          }
-          s0 = ffma(b & 1 ? d0[b >> 1].y : d0[b >> 1].x, acc[0], s0);
-          s1 = ffma(b & 1 ? d1[b >> 1].y : d1[b >> 1].x, acc[1], s1);
+          uint32_t v[4];
+          nib_f16(w[b], v);
+          mma16<F16>(acc, qa[2 * b], v[0], v[2]);
+          mma16<F16>(acc, qa[2 * b + 1], v[1], v[3]);
+          sum = ffma2(b & 1 ? pack2(k0[b >> 1].y, k1[b >> 1].y) : pack2(k0[b >> 1].x, k1[b >> 1].x),
+                      pack2(acc[0], acc[1]), sum);
         }
-        s[2 * t] = s0;
-        s[2 * t + 1] = s1;
-      } else {
+        const float2 r = unpack2(sum);
+        s[2 * t] = r.x;
+        s[2 * t + 1] = r.y;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++)  // hi + lo
+        s[i] = fadd(s[i], __shfl_xor_sync(0xffffffffu, s[i], RT == 2 ? 8 : 16));
+    } else {
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        const uint32_t kt = kaddr + 2 * t * L::K_STRIDE;
         float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
         if constexpr (KV == FLOCK_KV_FP8) {
 #pragma unroll
@@ -334,47 +412,41 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
             const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
             for (int i = 0; i < 4; i++)
-              mma_bf16(acc[i & 1], qa[4 * h + i], fp8_bf2(w[i]), fp8_bf2(w[i] >> 16));
+              mma16<F16>(acc[i & 1], qa[4 * h + i], fp8_f16(w[i]), fp8_f16(w[i] >> 16));
           }
         } else if constexpr (KV == FLOCK_KV_BF16) {
 #pragma unroll
           for (int h = 0; h < 4; h++) {
             const uint4 w = lds128(kt + 64 * h);
-            mma_bf16(acc[0], qa[2 * h], w.x, w.y);
-            mma_bf16(acc[1], qa[2 * h + 1], w.z, w.w);
+            mma16<F16>(acc[0], qa[2 * h], w.x, w.y);
+            mma16<F16>(acc[1], qa[2 * h + 1], w.z, w.w);
           }
         } else {
 #pragma unroll
           for (int ks = 0; ks < 8; ks++) {
             const uint4 w = lds128(kt + 64 * ks);
-            const float x0 = __uint_as_float(w.x), x1 = __uint_as_float(w.y),
-                        x2 = __uint_as_float(w.z), x3 = __uint_as_float(w.w);
+            uint32_t b0[3], b1[3];
+            split_bf16(__uint_as_float(w.x), __uint_as_float(w.y), b0);
+            split_bf16(__uint_as_float(w.z), __uint_as_float(w.w), b1);
 #pragma unroll
-            for (int part = 0; part < 3; part++)
-              mma_bf16(acc[part & 1], qa[ks], bf_part(x0, x1, part), bf_part(x2, x3, part));
+            for (int part = 0; part < 3; part++) mma16<F16>(acc[part & 1], qa[ks], b0[part], b1[part]);
           }
         }
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-          s[2 * t + i] = fadd(acc[0][i], acc[1][i]);
-          if (RT == 4) s[2 * t + i] = fadd(s[2 * t + i], fadd(acc[0][2 + i], acc[1][2 + i]));
+          s[2 * t + i] = fadd(fadd(acc[0][i], acc[1][i]), fadd(acc[0][2 + i], acc[1][2 + i]));
+          if (!F16) s[2 * t + i] = fadd(s[2 * t + i], __shfl_xor_sync(0xffffffffu, s[2 * t + i], 16));
         }
       }
     }
-    // a row's score is the sum over its slots
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      if (RT == 2) s[i] = fadd(s[i], __shfl_xor_sync(0xffffffffu, s[i], 8));
-      s[i] = fadd(s[i], __shfl_xor_sync(0xffffffffu, s[i], 16));
-    }
-    const int64_t key0 = key_of(grp);
+    const int key0 = key_of(grp);
     {  // masks, only where the group is not wholly visible to every row
       const bool sink = grp < sink_groups;
-      const int64_t from = sink ? 0 : row_lo, to = sink ? sk : row_hi;
+      const int from = sink ? 0 : row_lo, to = sink ? sk : row_hi;
       if (__any_sync(0xffffffffu, key0 < from || key0 + KR_GROUP > to)) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const int64_t key = key0 + 4 * c + i;
+          const int key = key0 + 4 * c + i;
           // every row sees the tile's sinks; a row's own may reach into the main range
           const bool seen = sink ? key < sk
                                  : key >= lo && key < row_hi && (key >= row_lo || key < row_sk);
@@ -383,90 +455,112 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
       }
     }
     // ------------------------------------------------------------ softmax
+    // this lane's value scales: its block's (RT = 4: its two blocks') of four keys
+    float d0[4], d1[4];
+    float dmax = 0.0f;
+    if constexpr (Q4) {
+      const uint4 e0 = lds128(stage + L::S_OFF + 128 + 32 * c);
+      const uint4 e1 = lds128(stage + L::S_OFF + 128 + 32 * c + 16);
+      const uint32_t es[4][2] = {{e0.x, e0.y}, {e0.z, e0.w}, {e1.x, e1.y}, {e1.z, e1.w}};
+      const uint32_t sel = RT == 2 ? 0x4410u + 0x0022u * (g >> 1) : (g & 4) ? 0x7632u : 0x5410u;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float2 d = h2f2(__byte_perm(es[i][0], es[i][1], sel));
+        d0[i] = d.x;
+        d1[i] = d.y;
+        dmax = fmaxf(dmax, fabsf(d0[i]));
+        if (RT == 4) dmax = fmaxf(dmax, fabsf(d1[i]));
+      }
+    }
     float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // The subtracted maximum may lag by up to 2^8: weights stay far inside
-    // f32's range, and the outputs are rescaled in few groups only.
-    if (__any_sync(0xffffffffu, top > fadd(m, 8.0f))) {
+    top = fmul(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)), unscale);
+    if (__any_sync(0xffffffffu, top > fadd(m, 8.0f) || (Q4 && dmax > dlim))) {
+      if (Q4) {
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) dmax = fmaxf(dmax, __shfl_xor_sync(0xffffffffu, dmax, x));
+        dexp = max(dexp, min((int)(__float_as_uint(dmax) >> 23) - 126, 16));
+        dlim = __uint_as_float((uint32_t)(127 + dexp) << 23);
+      }
       const float mn = fmaxf(m, top);
-      const float f = mn == -INFINITY ? 1.0f : exp2_approx(fsub(m, mn));
+      const float nb = mn == -INFINITY ? 0.0f : fadd(mn, (float)dexp - HEADROOM);
+      const float f = m == -INFINITY ? 0.0f : exp2_approx(fsub(base, nb));
       l = fmul(l, f);
 #pragma unroll
       for (int t = 0; t < 16; t++)
 #pragma unroll
-        for (int e = 0; e < (RT == 4 ? 4 : 2); e++)
-          o[t][e] = fmul(o[t][e], f);  // rows g and g + 8 are slots of one row
+        for (int e = 0; e < 4; e++) o[t][e] = fmul(o[t][e], f);  // rows g and g + 8: one query row
       m = mn;
+      base = nb;
     }
-    const float base = m == -INFINITY ? 0.0f : m;
     float w[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      w[i] = exp2_approx(fsub(s[i], base));
+      w[i] = exp2_approx(ffma(s[i], unscale, -base));
       l = fadd(l, w[i]);
     }
     // ------------------------------------------------------------- values
     const uint32_t vaddr = stage + L::V_OFF + c * L::V_GROUP;
-    auto weights = [&](uint32_t (&pa)[4], float x0, float x1, float x2, float x3) {
-      pa[0] = slot < 3 ? bf_part(x0, x1, slot) : 0;
-      pa[2] = slot < 3 ? bf_part(x2, x3, slot) : 0;
-      pa[1] = RT == 4 && g < 4 ? bf_part(x0, x1, 2) : 0;
-      pa[3] = RT == 4 && g < 4 ? bf_part(x2, x3, 2) : 0;
-    };
-    if constexpr (KV == FLOCK_KV_Q4) {
+    if constexpr (Q4) {
+      uint32_t pa[2][4];
+      if (RT == 2) {
+        split_f16(fmul(w[0], d0[0]), fmul(w[1], d0[1]), pa[0][0], pa[0][1]);
+        split_f16(fmul(w[2], d0[2]), fmul(w[3], d0[3]), pa[0][2], pa[0][3]);
+      } else {
+        split_f16(fmul(w[0], d0[0]), fmul(w[1], d0[1]), pa[0][0], pa[1][0]);
+        split_f16(fmul(w[2], d0[2]), fmul(w[3], d0[3]), pa[0][2], pa[1][2]);
+        split_f16(fmul(w[0], d1[0]), fmul(w[1], d1[1]), pa[0][1], pa[1][1]);
+        split_f16(fmul(w[2], d1[2]), fmul(w[3], d1[3]), pa[0][3], pa[1][3]);
+      }
       uint2 v[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) v[i] = lds64(vaddr + i * 64 + 8 * g);
-      const uint4 e0 = lds128(stage + L::S_OFF + 128 + 32 * c);
-      const uint4 e1 = lds128(stage + L::S_OFF + 128 + 32 * c + 16);
-      const uint32_t es[4][2] = {{e0.x, e0.y}, {e0.z, e0.w}, {e1.x, e1.y}, {e1.z, e1.w}};
 #pragma unroll
-      for (int hb = 0; hb < 2; hb++) {
-        float2 d[4];
+      for (int b = 0; b < 4; b++) {
+        // block b's two bytes of four keys, keys paired
+        const uint32_t sel = b & 1 ? 0x7632u : 0x5410u;
+        const uint32_t k01 = __byte_perm(b < 2 ? v[0].x : v[0].y, b < 2 ? v[1].x : v[1].y, sel);
+        const uint32_t k23 = __byte_perm(b < 2 ? v[2].x : v[2].y, b < 2 ? v[3].x : v[3].y, sel);
+        uint32_t x[4], y[4];
+        nib_f16(k01, x);
+        nib_f16(k23, y);
 #pragma unroll
-        for (int i = 0; i < 4; i++) d[i] = h2f2(es[i][hb]);
-#pragma unroll
-        for (int bb = 0; bb < 2; bb++) {
-          const int b = 2 * hb + bb;
-          // p d; a masked key's scale may be anything finite, its weight is 0
-          uint32_t pa[4];
-          weights(pa, fmul(w[0], bb ? d[0].y : d[0].x), fmul(w[1], bb ? d[1].y : d[1].x),
-                  fmul(w[2], bb ? d[2].y : d[2].x), fmul(w[3], bb ? d[3].y : d[3].x));
-          const uint32_t v0 = hb ? v[0].y : v[0].x, v1 = hb ? v[1].y : v[1].x,
-                         v2 = hb ? v[2].y : v[2].x, v3 = hb ? v[3].y : v[3].x;
-          const uint32_t k01 = __byte_perm(v0, v1, bb ? 0x7632 : 0x5410);
-          const uint32_t k23 = __byte_perm(v2, v3, bb ? 0x7632 : 0x5410);
-          // tile 4 b + e: nibble e of the halfword (low and high nibble of byte 0, then byte 1)
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            mma_bf16(o[4 * b + e], pa, nib_bf2(k01 >> (4 * e)), nib_bf2(k23 >> (4 * e)));
+        for (int e = 0; e < 4; e++) {  // tile 4 b + e: nibble e of the halfword
+          mma16<F16>(o[4 * b + e], pa[0], x[e], y[e]);
+          if (RT == 4) mma16<F16>(o[4 * b + e], pa[1], x[e], y[e]);
         }
       }
     } else {
       uint32_t pa[4];
-      weights(pa, w[0], w[1], w[2], w[3]);
+      if constexpr (F16) {
+        split_f16(w[0], w[1], pa[0], pa[1]);
+        split_f16(w[2], w[3], pa[2], pa[3]);
+      } else {
+        uint32_t w0[3], w1[3];
+        split_bf16(w[0], w[1], w0);
+        split_bf16(w[2], w[3], w1);
+        pa[0] = g < 4 ? w0[0] : w0[1];
+        pa[2] = g < 4 ? w1[0] : w1[1];
+        pa[1] = g < 4 ? w0[2] : 0;
+        pa[3] = g < 4 ? w1[2] : 0;
+      }
+      auto word = [](const uint4& v, int q) { return q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w; };
       if constexpr (KV == FLOCK_KV_FP8) {
         uint4 v[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) v[i] = lds128(vaddr + i * 128 + 16 * g);
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-          const uint32_t x[4] = {q == 0 ? v[0].x : q == 1 ? v[0].y : q == 2 ? v[0].z : v[0].w,
-                                 q == 0 ? v[1].x : q == 1 ? v[1].y : q == 2 ? v[1].z : v[1].w,
-                                 q == 0 ? v[2].x : q == 1 ? v[2].y : q == 2 ? v[2].z : v[2].w,
-                                 q == 0 ? v[3].x : q == 1 ? v[3].y : q == 2 ? v[3].z : v[3].w};
+        for (int q = 0; q < 4; q++)
 #pragma unroll
           for (int h = 0; h < 2; h++) {
             uint32_t y[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) y[i] = fp8_bf2(x[i] >> (16 * h));
-            mma_bf16(o[4 * q + 2 * h], pa, __byte_perm(y[0], y[1], 0x5410),
-                     __byte_perm(y[2], y[3], 0x5410));
-            mma_bf16(o[4 * q + 2 * h + 1], pa, __byte_perm(y[0], y[1], 0x7632),
-                     __byte_perm(y[2], y[3], 0x7632));
+            for (int i = 0; i < 4; i++) y[i] = fp8_f16(word(v[i], q) >> (16 * h));
+            mma16<F16>(o[4 * q + 2 * h], pa, __byte_perm(y[0], y[1], 0x5410),
+                       __byte_perm(y[2], y[3], 0x5410));
+            mma16<F16>(o[4 * q + 2 * h + 1], pa, __byte_perm(y[0], y[1], 0x7632),
+                       __byte_perm(y[2], y[3], 0x7632));
           }
-        }
       } else if constexpr (KV == FLOCK_KV_BF16) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -475,13 +569,11 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
           for (int i = 0; i < 4; i++) v[i] = lds128(vaddr + i * 256 + 128 * h + 16 * g);
 #pragma unroll
           for (int q = 0; q < 4; q++) {
-            uint32_t x[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = q == 0 ? v[i].x : q == 1 ? v[i].y : q == 2 ? v[i].z : v[i].w;
-            mma_bf16(o[8 * h + 2 * q], pa, __byte_perm(x[0], x[1], 0x5410),
-                     __byte_perm(x[2], x[3], 0x5410));
-            mma_bf16(o[8 * h + 2 * q + 1], pa, __byte_perm(x[0], x[1], 0x7632),
-                     __byte_perm(x[2], x[3], 0x7632));
+            const uint32_t x0 = word(v[0], q), x1 = word(v[1], q), x2 = word(v[2], q),
+                           x3 = word(v[3], q);
+            mma16<F16>(o[8 * h + 2 * q], pa, __byte_perm(x0, x1, 0x5410), __byte_perm(x2, x3, 0x5410));
+            mma16<F16>(o[8 * h + 2 * q + 1], pa, __byte_perm(x0, x1, 0x7632),
+                       __byte_perm(x2, x3, 0x7632));
           }
         }
       } else {
@@ -492,13 +584,11 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
           for (int i = 0; i < 4; i++) v[i] = lds128(vaddr + i * 512 + 128 * h + 16 * g);
 #pragma unroll
           for (int q = 0; q < 4; q++) {
-            float x[4];
+            uint32_t b0[3], b1[3];
+            split_bf16(__uint_as_float(word(v[0], q)), __uint_as_float(word(v[1], q)), b0);
+            split_bf16(__uint_as_float(word(v[2], q)), __uint_as_float(word(v[3], q)), b1);
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-              x[i] = __uint_as_float(q == 0 ? v[i].x : q == 1 ? v[i].y : q == 2 ? v[i].z : v[i].w);
-#pragma unroll
-            for (int part = 0; part < 3; part++)
-              mma_bf16(o[4 * h + q], pa, bf_part(x[0], x[1], part), bf_part(x[2], x[3], part));
+            for (int part = 0; part < 3; part++) mma16<F16>(o[4 * h + q], pa, b0[part], b1[part]);
           }
         }
       }
@@ -516,14 +606,24 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
   for (int t = 0; t < 16; t++)
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-      float x = o[t][e];
-      if (RT == 2) x = fadd(x, __shfl_xor_sync(0xffffffffu, x, 8));
-      if (RT == 4) x = fadd(x, o[t][2 + e]);
-      x = fadd(x, __shfl_xor_sync(0xffffffffu, x, 16));
-      if (g < RT) s_o[(warp * RT + j) * KV_HD + kr_vdim<KV>(t, 2 * c + e)] = x;
+      const int at = kr_vdim<KV>(t, 2 * c + e);
+      float* dst = s_o + (warp * RT + j) * KV_HD + at;
+      if constexpr (Q4) {  // the rows of the tile's block b = t / 4
+        if (RT == 2) {
+          if ((g >> 1) == (t >> 2)) *dst = fadd(o[t][e], o[t][2 + e]);
+        } else if ((g >> 2) == ((t >> 2) & 1)) {
+          *dst = t < 8 ? o[t][e] : o[t][2 + e];
+        }
+      } else if constexpr (F16) {
+        *dst = fadd(o[t][e], o[t][2 + e]);
+      } else {
+        float x = fadd(o[t][e], o[t][2 + e]);
+        x = fadd(x, __shfl_xor_sync(0xffffffffu, x, 16));
+        if (g < 4) *dst = x;
+      }
     }
   if (g < RT && c == 0) {
-    s_ml[warp][j][0] = m;
+    s_ml[warp][j][0] = l > 0.0f ? base : -INFINITY;  // weights are relative to 2^base
     s_ml[warp][j][1] = l;
   }
   __syncthreads();
