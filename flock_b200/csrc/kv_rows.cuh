@@ -21,9 +21,7 @@
 // 4-bit blocks.  Scores: a block's 32 products are summed as integers times
 // query parts, then multiplied by the key's scale in f32 (one accumulator per
 // block).  Values: the scale joins the weight before its split, so the weight
-// operand differs per block; its rows hold (block, query row), each lane
-// computes its own block's weights only, and of an output tile's rows the ones
-// of the tile's block count.
+// operand differs per block.
 //
 // Work split: CTA (split z, row tile, kv head), its warps taking 16-key groups
 // in turn, each with its own cp.async ring, running maximum, sum and output;
@@ -176,17 +174,6 @@ FLOCK_DEV uint32_t fp8_f16(uint32_t w) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The head dimension that element e (0-3) of lane column c meets in QK step ks
-// (0-7): the order in which a lane's cached bytes unpack.  k_frag and the query
-// operand agree on it, so any order is right.
-template <int KV>
-FLOCK_DEV int kr_kdim(int ks, int c, int e) {
-  if (KV == FLOCK_KV_Q4)  // block ks / 2, low or high nibbles of bytes 4 c ..; pairs two apart
-    return 32 * (ks >> 1) + 16 * (ks & 1) + 4 * c + ((e & 1) << 1 | e >> 1);
-  if (KV == FLOCK_KV_FP8) return 64 * (ks >> 2) + 16 * c + 4 * (ks & 3) + e;
-  if (KV == FLOCK_KV_BF16) return 32 * (ks >> 1) + 8 * c + 4 * (ks & 1) + e;
-  return 16 * ks + 4 * c + e;
-}
 // The head dimension of column n of output tile t (0-15).
 template <int KV>
 FLOCK_DEV int kr_vdim(int t, int n) {
@@ -235,27 +222,27 @@ FLOCK_DEV uint2 lds64(uint32_t a) {
   return r;
 }
 
-// Rows of the operands, RT query rows per CTA.  Score operand: 4-bit RT = 2:
-// rows 0-1 hi, 2-3 lo, and again in 4-7; RT = 4: 0-3 hi, 4-7 lo.  e4m3 (RT 8):
-// 0-7 hi, 8-15 lo.  bf16, f32 (RT 4): 0-3 hi, 4-7 mid, 8-11 lo.  Weight operand:
-// as the score operand, but 4-bit RT = 2: row 2 b + j block b's hi, 8 + 2 b + j
-// its lo; RT = 4: row 4 b + j block b, hi and lo in two operands.
+// Query rows per CTA.  f16 parts: operand rows 0-7 hold the rows' hi parts,
+// 8-15 their lo.  bf16 parts: 0-3 hi, 4-7 mid, 8-11 lo.
 template <int KV>
-constexpr int kr_rows(int rows) {
-  return KV == FLOCK_KV_FP8 ? 8 : KV == FLOCK_KV_Q4 && rows <= 2 ? 2 : 4;
-}
+constexpr int KR_ROWS = KV == FLOCK_KV_Q4 || KV == FLOCK_KV_FP8 ? 8 : 4;
 
 // Keys of a stage are dealt to operand columns so that a lane's four score
 // columns are four neighbouring keys: column n of score tile t is key
 // 4 (n / 2) + 2 t + n % 2, and lane column c holds keys 4 c .. 4 c + 3.
-template <int KV, int RT>
+template <int KV>
 static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(const KvRowsArgs p) {
   using L = KrLayout<KV>;
+  constexpr int RT = KR_ROWS<KV>;
   constexpr bool Q4 = KV == FLOCK_KV_Q4;
   constexpr bool F16 = Q4 || KV == FLOCK_KV_FP8;
   extern __shared__ __align__(16) uint8_t kr_smem[];
   __shared__ float s_ml[L::WARPS][RT][2];
+  __shared__ uint4 s_q[8][32];  // the query operand: [QK step][lane]
+  __shared__ float s_unscale[RT];
   __shared__ int s_last;
+  pdl_launch_dependents();
+  pdl_wait();
   const KvAttnArgs& a = p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
@@ -302,53 +289,57 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
   for (int s = 0; s < L::STAGES - 1; s++) fetch(g0 + warp + s * L::WARPS, s);
 
   // The query operand: the parts of q log2(e) / sqrt(128), for f16 scaled by
-  // a power of two that brings the row's largest into [2^13, 2^14).
-  uint32_t qa[8][4];
-  float unscale = 1.0f;
-  {
+  // a power of two that brings the row's largest into [2^13, 2^14).  A warp
+  // splits a row, four neighbouring dimensions a lane: one operand entry.
+  for (int r = warp; r < RT; r += L::WARPS) {
+    const int rr = tile * RT + r;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (rr < p.rows)
+      x = __ldg(reinterpret_cast<const float4*>(
+          a.q + (rr / p.group) * a.q_stride + ((int64_t)head * p.group + rr % p.group) * KV_HD +
+          4 * lane));
     const float k = __double2float_rn(1.4426950408889634 / sqrt(128.0));
-    const bool live = row < p.rows;
-    const float* q = a.q + my_q * a.q_stride +
-                     ((int64_t)head * p.group + min(row, p.rows - 1) % p.group) * KV_HD;
-    float x[8][4], top = 0.0f;
-#pragma unroll
-    for (int ks = 0; ks < 8; ks++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        x[ks][e] = live ? fmul(__ldg(q + kr_kdim<KV>(ks, c, e)), k) : 0.0f;
-        top = fmaxf(top, fabsf(x[ks][e]));
-      }
-    float scale = 1.0f;
+    x = make_float4(fmul(x.x, k), fmul(x.y, k), fmul(x.z, k), fmul(x.w, k));
+    const int qc = Q4 || KV == FLOCK_KV_F32 ? lane & 3 : KV == FLOCK_KV_FP8 ? (lane >> 2) & 3 : (lane >> 1) & 3;
+    const int ks = Q4 || KV == FLOCK_KV_F32 ? lane >> 2
+                   : KV == FLOCK_KV_FP8     ? (lane >> 4) * 4 + (lane & 3)
+                                            : (lane >> 3) * 2 + (lane & 1);
     if (F16) {
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      float top = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
       const int biased = (int)(__float_as_uint(top) >> 23);
       const int e = biased == 0 ? 0 : max(-100, min(100, biased - 127 - 13));
-      scale = __uint_as_float((uint32_t)(127 - e) << 23);
-      unscale = __uint_as_float((uint32_t)(127 + e) << 23);
-    }
-#pragma unroll
-    for (int ks = 0; ks < 8; ks++) {
-      if (F16) {
-        uint32_t h0, l0, h1, l1;
-        split_f16(fmul(x[ks][0], scale), fmul(x[ks][1], scale), h0, l0);
-        split_f16(fmul(x[ks][2], scale), fmul(x[ks][3], scale), h1, l1);
-        const bool low = Q4 && (RT == 2 ? (g & 2) : (g & 4));
-        qa[ks][0] = low ? l0 : h0;
-        qa[ks][2] = low ? l1 : h1;
-        qa[ks][1] = Q4 ? 0 : l0;
-        qa[ks][3] = Q4 ? 0 : l1;
-      } else {
-        uint32_t w0[3], w1[3];
-        split_bf16(x[ks][0], x[ks][1], w0);
-        split_bf16(x[ks][2], x[ks][3], w1);
-        qa[ks][0] = g < 4 ? w0[0] : w0[1];
-        qa[ks][2] = g < 4 ? w1[0] : w1[1];
-        qa[ks][1] = g < 4 ? w0[2] : 0;
-        qa[ks][3] = g < 4 ? w1[2] : 0;
+      const float scale = __uint_as_float((uint32_t)(127 - e) << 23);
+      if (lane == 0) s_unscale[r] = __uint_as_float((uint32_t)(127 + e) << 23);
+      if (Q4) {  // pairs two apart: bytes 0 and 2, 1 and 3 of a code word
+        const float y = x.y;
+        x.y = x.z;
+        x.z = y;
       }
+      uint4 w;
+      split_f16(fmul(x.x, scale), fmul(x.y, scale), w.x, w.y);
+      split_f16(fmul(x.z, scale), fmul(x.w, scale), w.z, w.w);
+      s_q[ks][4 * r + qc] = w;
+    } else {
+      uint32_t w0[3], w1[3];
+      split_bf16(x.x, x.y, w0);
+      split_bf16(x.z, x.w, w1);
+      s_q[ks][4 * r + qc] = make_uint4(w0[0], w0[2], w1[0], w1[2]);
+      s_q[ks][4 * (r + 4) + qc] = make_uint4(w0[1], 0, w1[1], 0);
     }
   }
+  __syncthreads();
+  uint32_t qa[8][4];
+#pragma unroll
+  for (int ks = 0; ks < 8; ks++) {
+    const uint4 w = s_q[ks][lane];
+    qa[ks][0] = w.x;
+    qa[ks][1] = w.y;
+    qa[ks][2] = w.z;
+    qa[ks][3] = w.w;
+  }
+  const float unscale = F16 ? s_unscale[j] : 1.0f;
   float o[16][4];
 #pragma unroll
   for (int t = 0; t < 16; t++)
@@ -390,16 +381,15 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
           nib_f16(w[b], v);
           mma16<F16>(acc, qa[2 * b], v[0], v[2]);
           mma16<F16>(acc, qa[2 * b + 1], v[1], v[3]);
-          sum = ffma2(b & 1 ? pack2(k0[b >> 1].y, k1[b >> 1].y) : pack2(k0[b >> 1].x, k1[b >> 1].x),
-                      pack2(acc[0], acc[1]), sum);
+          const uint64_t d = b & 1 ? pack2(k0[b >> 1].y, k1[b >> 1].y)
+                                   : pack2(k0[b >> 1].x, k1[b >> 1].x);
+          sum = ffma2(d, pack2(acc[0], acc[1]), sum);  // hi
+          sum = ffma2(d, pack2(acc[2], acc[3]), sum);  // lo
         }
         const float2 r = unpack2(sum);
         s[2 * t] = r.x;
         s[2 * t + 1] = r.y;
       }
-#pragma unroll
-      for (int i = 0; i < 4; i++)  // hi + lo
-        s[i] = fadd(s[i], __shfl_xor_sync(0xffffffffu, s[i], RT == 2 ? 8 : 16));
     } else {
 #pragma unroll
       for (int t = 0; t < 2; t++) {
@@ -455,22 +445,24 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
       }
     }
     // ------------------------------------------------------------ softmax
-    // this lane's value scales: its block's (RT = 4: its two blocks') of four keys
-    float d0[4], d1[4];
+    // the value scales of the lane's four keys, two blocks a word; the largest
+    // magnitude of all sixteen as a bound for the f16 weights
+    uint32_t vs[4][2];
     float dmax = 0.0f;
     if constexpr (Q4) {
       const uint4 e0 = lds128(stage + L::S_OFF + 128 + 32 * c);
       const uint4 e1 = lds128(stage + L::S_OFF + 128 + 32 * c + 16);
-      const uint32_t es[4][2] = {{e0.x, e0.y}, {e0.z, e0.w}, {e1.x, e1.y}, {e1.z, e1.w}};
-      const uint32_t sel = RT == 2 ? 0x4410u + 0x0022u * (g >> 1) : (g & 4) ? 0x7632u : 0x5410u;
+      vs[0][0] = e0.x, vs[0][1] = e0.y, vs[1][0] = e0.z, vs[1][1] = e0.w;
+      vs[2][0] = e1.x, vs[2][1] = e1.y, vs[3][0] = e1.z, vs[3][1] = e1.w;
+      auto habs = [](uint32_t x) {
+        const uint32_t u = x & 0x7FFF7FFFu;
+        return *reinterpret_cast<const __half2*>(&u);
+      };
+      __half2 h = habs(vs[0][0]);
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float2 d = h2f2(__byte_perm(es[i][0], es[i][1], sel));
-        d0[i] = d.x;
-        d1[i] = d.y;
-        dmax = fmaxf(dmax, fabsf(d0[i]));
-        if (RT == 4) dmax = fmaxf(dmax, fabsf(d1[i]));
-      }
+      for (int i = 1; i < 8; i++) h = __hmax2(h, habs(vs[i >> 1][i & 1]));
+      const float2 f = __half22float2(h);
+      dmax = fmaxf(f.x, f.y);
     }
     float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -502,32 +494,30 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
     // ------------------------------------------------------------- values
     const uint32_t vaddr = stage + L::V_OFF + c * L::V_GROUP;
     if constexpr (Q4) {
-      uint32_t pa[2][4];
-      if (RT == 2) {
-        split_f16(fmul(w[0], d0[0]), fmul(w[1], d0[1]), pa[0][0], pa[0][1]);
-        split_f16(fmul(w[2], d0[2]), fmul(w[3], d0[3]), pa[0][2], pa[0][3]);
-      } else {
-        split_f16(fmul(w[0], d0[0]), fmul(w[1], d0[1]), pa[0][0], pa[1][0]);
-        split_f16(fmul(w[2], d0[2]), fmul(w[3], d0[3]), pa[0][2], pa[1][2]);
-        split_f16(fmul(w[0], d1[0]), fmul(w[1], d1[1]), pa[0][1], pa[1][1]);
-        split_f16(fmul(w[2], d1[2]), fmul(w[3], d1[3]), pa[0][3], pa[1][3]);
-      }
       uint2 v[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) v[i] = lds64(vaddr + i * 64 + 8 * g);
 #pragma unroll
-      for (int b = 0; b < 4; b++) {
-        // block b's two bytes of four keys, keys paired
-        const uint32_t sel = b & 1 ? 0x7632u : 0x5410u;
-        const uint32_t k01 = __byte_perm(b < 2 ? v[0].x : v[0].y, b < 2 ? v[1].x : v[1].y, sel);
-        const uint32_t k23 = __byte_perm(b < 2 ? v[2].x : v[2].y, b < 2 ? v[3].x : v[3].y, sel);
-        uint32_t x[4], y[4];
-        nib_f16(k01, x);
-        nib_f16(k23, y);
+      for (int hb = 0; hb < 2; hb++) {
+        float2 d[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {  // tile 4 b + e: nibble e of the halfword
-          mma16<F16>(o[4 * b + e], pa[0], x[e], y[e]);
-          if (RT == 4) mma16<F16>(o[4 * b + e], pa[1], x[e], y[e]);
+        for (int i = 0; i < 4; i++) d[i] = h2f2(vs[i][hb]);
+#pragma unroll
+        for (int bb = 0; bb < 2; bb++) {
+          const int b = 2 * hb + bb;
+          uint32_t pa[4];
+          split_f16(fmul(w[0], bb ? d[0].y : d[0].x), fmul(w[1], bb ? d[1].y : d[1].x), pa[0], pa[1]);
+          split_f16(fmul(w[2], bb ? d[2].y : d[2].x), fmul(w[3], bb ? d[3].y : d[3].x), pa[2], pa[3]);
+          // block b's two bytes of four keys, keys paired
+          const uint32_t sel = bb ? 0x7632u : 0x5410u;
+          const uint32_t k01 = __byte_perm(hb ? v[0].y : v[0].x, hb ? v[1].y : v[1].x, sel);
+          const uint32_t k23 = __byte_perm(hb ? v[2].y : v[2].x, hb ? v[3].y : v[3].x, sel);
+          uint32_t x[4], y[4];
+          nib_f16(k01, x);
+          nib_f16(k23, y);
+#pragma unroll
+          for (int e = 0; e < 4; e++)  // tile 4 b + e: nibble e of the halfword
+            mma16<F16>(o[4 * b + e], pa, x[e], y[e]);
         }
       }
     } else {
@@ -602,25 +592,16 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
   l = fadd(l, __shfl_xor_sync(0xffffffffu, l, 2));
   __syncthreads();  // the rings are done with: their memory holds the warps' outputs
   float* s_o = reinterpret_cast<float*>(kr_smem);  // [warp][RT][128]
+  const int live = min(RT, p.rows - tile * RT);
 #pragma unroll
   for (int t = 0; t < 16; t++)
 #pragma unroll
     for (int e = 0; e < 2; e++) {
       const int at = kr_vdim<KV>(t, 2 * c + e);
       float* dst = s_o + (warp * RT + j) * KV_HD + at;
-      if constexpr (Q4) {  // the rows of the tile's block b = t / 4
-        if (RT == 2) {
-          if ((g >> 1) == (t >> 2)) *dst = fadd(o[t][e], o[t][2 + e]);
-        } else if ((g >> 2) == ((t >> 2) & 1)) {
-          *dst = t < 8 ? o[t][e] : o[t][2 + e];
-        }
-      } else if constexpr (F16) {
-        *dst = fadd(o[t][e], o[t][2 + e]);
-      } else {
-        float x = fadd(o[t][e], o[t][2 + e]);
-        x = fadd(x, __shfl_xor_sync(0xffffffffu, x, 16));
-        if (g < 4) *dst = x;
-      }
+      float x = fadd(o[t][e], o[t][2 + e]);
+      if (!F16) x = fadd(x, __shfl_xor_sync(0xffffffffu, x, 16));
+      if (g < live) *dst = x;
     }
   if (g < RT && c == 0) {
     s_ml[warp][j][0] = l > 0.0f ? base : -INFINITY;  // weights are relative to 2^base
@@ -630,7 +611,7 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
   const int item = head * gridDim.y + tile;
   const int n_items = gridDim.y * gridDim.z;
   float* part_ml = p.part + (size_t)n_items * p.splits * RT * KV_HD;
-  for (int i = threadIdx.x; i < RT * KV_HD; i += L::THREADS) {
+  for (int i = threadIdx.x; i < live * KV_HD; i += L::THREADS) {
     const int r = i / KV_HD, d = i % KV_HD;
     float mm = -INFINITY;
 #pragma unroll
@@ -645,9 +626,8 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
     }
     if (p.splits == 1) {
       const int rr = tile * RT + r;
-      if (rr < p.rows)
-        a.out[(rr / p.group) * a.out_stride + ((int64_t)head * p.group + rr % p.group) * KV_HD + d] =
-            fdiv(oo, ll);
+      a.out[(rr / p.group) * a.out_stride + ((int64_t)head * p.group + rr % p.group) * KV_HD + d] =
+          fdiv(oo, ll);
     } else {
       const size_t at = ((size_t)item * p.splits + z) * RT + r;
       p.part[at * KV_HD + d] = oo;
@@ -665,22 +645,52 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
   __syncthreads();
   if (!s_last) return;
   __threadfence();
-  for (int i = threadIdx.x; i < RT * KV_HD; i += L::THREADS) {
-    const int r = i / KV_HD, d = i % KV_HD, rr = tile * RT + r;
-    if (rr >= p.rows) break;
-    const size_t at = (size_t)item * p.splits * RT + r;
-    float mm = -INFINITY;
-    for (int s = 0; s < p.splits; s++) mm = fmaxf(mm, __ldcg(part_ml + (at + s * RT) * 2));
-    float oo = 0.0f, ll = 0.0f;
-    for (int s = 0; s < p.splits; s++) {
-      const float f = exp2_approx(fsub(__ldcg(part_ml + (at + s * RT) * 2), mm));
-      oo = ffma(f, __ldcg(p.part + (at + s * RT) * KV_HD + d), oo);
-      ll = ffma(f, __ldcg(part_ml + (at + s * RT) * 2 + 1), ll);
-    }
-    a.out[(rr / p.group) * a.out_stride + ((int64_t)head * p.group + rr % p.group) * KV_HD + d] =
-        fdiv(oo, ll);
-  }
   if (threadIdx.x == 0) p.count[item] = 0;  // ready for the next call
+  // each split's factor 2^(m_s - m) and sum, [split][RT], then their weighted outputs
+  float* s_f = reinterpret_cast<float*>(kr_smem);
+  float* s_l = s_f + p.splits * RT;
+  const size_t first = (size_t)item * p.splits * RT;
+  for (int i = threadIdx.x; i < p.splits * RT; i += L::THREADS) {
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml) + first + i);
+    s_f[i] = ml.x;
+    s_l[i] = ml.y;
+  }
+  __syncthreads();
+  for (int r = warp; r < live; r += L::WARPS) {
+    float mm = -INFINITY;
+    for (int s = lane; s < p.splits; s += 32) mm = fmaxf(mm, s_f[s * RT + r]);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+    for (int s = lane; s < p.splits; s += 32)
+      s_f[s * RT + r] = exp2_approx(fsub(s_f[s * RT + r], mm));
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < live * (KV_HD / 4); i += L::THREADS) {
+    const int r = i / (KV_HD / 4), d = 4 * (i % (KV_HD / 4)), rr = tile * RT + r;
+    float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
+    float ll = 0.0f;
+    constexpr int U = 6;  // loads in flight
+    for (int s0 = 0; s0 < p.splits; s0 += U) {
+      float4 x[U];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (s0 + u < p.splits)
+          x[u] = __ldcg(reinterpret_cast<const float4*>(
+              p.part + (first + (size_t)(s0 + u) * RT + r) * KV_HD + d));
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (s0 + u < p.splits) {
+          const float f = s_f[(s0 + u) * RT + r];
+          oo = make_float4(ffma(f, x[u].x, oo.x), ffma(f, x[u].y, oo.y), ffma(f, x[u].z, oo.z),
+                           ffma(f, x[u].w, oo.w));
+          ll = ffma(f, s_l[(s0 + u) * RT + r], ll);
+        }
+    }
+    const float inv = fdiv(1.0f, ll);
+    *reinterpret_cast<float4*>(a.out + (rr / p.group) * a.out_stride +
+                               ((int64_t)head * p.group + rr % p.group) * KV_HD + d) =
+        make_float4(fmul(oo.x, inv), fmul(oo.y, inv), fmul(oo.z, inv), fmul(oo.w, inv));
+  }
 }
 
 }  // namespace flock
