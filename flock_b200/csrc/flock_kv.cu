@@ -87,10 +87,10 @@ int by_dtype(int kv_dtype, F f) {
 }
 
 // A few query rows per kv head: k_kv_rows.
-template <int KV>
+template <int KV, int NT>
 int launch_rows(const flock_kv* c, const KvAttnArgs& a, cudaStream_t st) {
-  using L = KrLayout<KV>;
-  constexpr int RT = KR_ROWS<KV>;
+  using L = KrLayout<KV, NT>;
+  constexpr int RT = L::RT;
   KvRowsArgs p = {};
   p.a = a;
   p.group = a.n_heads / a.c.n_kv_heads;
@@ -106,8 +106,8 @@ int launch_rows(const flock_kv* c, const KvAttnArgs& a, cudaStream_t st) {
   if (p.splits < 1) p.splits = 1;
   p.count = reinterpret_cast<uint32_t*>(c->workspace);
   p.part = reinterpret_cast<float*>(c->workspace + KR_PART_OFFSET);
-  FLOCK_TRY(kernel_setup((const void*)k_kv_rows<KV>, (int)L::SMEM));
-  FLOCK_CK(launch_ex(st, k_kv_rows<KV>,
+  FLOCK_TRY(kernel_setup((const void*)k_kv_rows<KV, NT>, (int)L::SMEM));
+  FLOCK_CK(launch_ex(st, k_kv_rows<KV, NT>,
                      dim3((unsigned)p.splits, (unsigned)tiles, (unsigned)a.c.n_kv_heads),
                      dim3(L::THREADS), L::SMEM, true, p));
   return FLOCK_OK;
@@ -314,7 +314,10 @@ int flock_kv_attention(flock_kv* c, const float* q, int64_t q_stride, int n_head
   if (rows <= 16)
     return by_dtype(c->kv_dtype, [&](auto kv) -> int {
       constexpr int KV = decltype(kv)::value;
-      return launch_rows<KV>(c, a, static_cast<cudaStream_t>(stream));
+      // bf16 parts fill two column tiles with four rows; f16 parts one
+      if constexpr (KV == FLOCK_KV_Q4 || KV == FLOCK_KV_FP8)
+        if (rows <= 4) return launch_rows<KV, 1>(c, a, static_cast<cudaStream_t>(stream));
+      return launch_rows<KV, 2>(c, a, static_cast<cudaStream_t>(stream));
     });
   return by_dtype(c->kv_dtype, [&](auto kv) -> int {
     k_kv_attn<decltype(kv)::value><<<grid, 128, 0, static_cast<cudaStream_t>(stream)>>>(a);

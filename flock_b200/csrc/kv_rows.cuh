@@ -9,19 +9,23 @@
 // mma.sync m16n8k16 (f32 accumulation) rather than tcgen05: with two to eight
 // live rows there is nothing to amortise a pass of the operands through shared
 // memory and tensor memory over; this path takes cached bytes from shared
-// memory to the operand registers with no store in between.
+// memory to the operand registers with no store in between.  Keys (then head
+// dimensions) are the operand's 16 rows and query rows its 8 columns: the
+// other way round 16 rows would be mostly empty and every step twice as long.
 //
-// f32 results from 16-bit operands.  Codes minus 8 and e4m3 values are f16
-// values, so there queries and softmax weights are split as hi + lo, two f16
-// of 11 bits (22 bits; scaled by powers of two so that f16's range never
-// cuts a part that matters).  bf16 and f32 elements need f32's range: hi + mid
-// + lo, three bf16 of 8 bits.  The parts sit in different ROWS of the 16-row
-// operand, which a decode leaves empty anyway: one instruction multiplies all.
+// f32 results from 16-bit operands.  Codes and e4m3 values are f16 values, so
+// there queries and softmax weights are split as hi + lo, two f16 of 11 bits
+// (22 bits; scaled by powers of two so that f16's range never cuts a part that
+// matters).  bf16 and f32 elements need f32's range: hi + mid + lo, three bf16
+// of 8 bits.  The parts sit in neighbouring COLUMNS, which a lane's accumulator
+// holds side by side: one instruction multiplies both, an addition joins them.
 //
-// 4-bit blocks.  Scores: a block's 32 products are summed as integers times
-// query parts, then multiplied by the key's scale in f32 (one accumulator per
-// block).  Values: the scale joins the weight before its split, so the weight
-// operand differs per block.
+// 4-bit blocks.  Scores: a code c in an f16's low bits is the subnormal c
+// 2^-24, an operand for one AND; sum (c - 8) q = sum c q - 8 sum q, the second
+// term being a constant of the query that the accumulator starts from.  A
+// block's sum is multiplied by the key's scale in f32.  Values: codes minus 8
+// (over many keys the uncentred sum would cancel), the scale joins the weight,
+// so the weight operand differs per block.
 //
 // Work split: CTA (split z, row tile, kv head), its warps taking 16-key groups
 // in turn, each with its own cp.async ring, running maximum, sum and output;
@@ -45,37 +49,44 @@ struct KvRowsArgs {
   float* part;      // [item][split][RT][128], then [item][split][RT][2] (m, l)
 };
 
-// Shared-memory layout of one warp's 16-key stage, per cached type.  Key rows
-// are read 16 bytes a lane, eight lanes covering 64 bytes of two keys; value
-// rows 8 or 16 bytes a lane, eight lanes covering pieces of four keys four
-// apart.  Padding keeps both free of bank conflicts.
-template <int KV>
+#ifndef KR_W1
+#define KR_W1 16
+#define KR_S1 5
+#define KR_W2 12
+#define KR_S2 5
+#endif
+// Shared-memory layout of one warp's 16-key stage, per cached type, for NT
+// column tiles.  Key rows are read 16 bytes a lane, eight lanes covering 64
+// bytes of two keys; value rows 8 or 16 bytes a lane, eight lanes covering
+// pieces of four keys two apart.  Padding keeps both free of bank conflicts.
+template <int KV, int NT>
 struct KrTile;
-template <>
-struct KrTile<FLOCK_KV_Q4> {
-  static constexpr int ROW = 64, K_STRIDE = 64, V_GROUP = 4 * 64 + 32, WARPS = 12, STAGES = 5;
+template <int NT>
+struct KrTile<FLOCK_KV_Q4, NT> {
+  static constexpr int ROW = 64, K_STRIDE = 64, WARPS = NT == 1 ? KR_W1 : KR_W2,
+                       STAGES = NT == 1 ? KR_S1 : KR_S2;
   static constexpr int SCALES = 2 * KR_GROUP * 8;
 };
-template <>
-struct KrTile<FLOCK_KV_FP8> {
-  static constexpr int ROW = 128, K_STRIDE = 192, V_GROUP = 4 * 128 + 32, WARPS = 8, STAGES = 4;
-  static constexpr int SCALES = 0;
+template <int NT>
+struct KrTile<FLOCK_KV_FP8, NT> {
+  static constexpr int ROW = 128, K_STRIDE = 192, WARPS = 8, STAGES = 4, SCALES = 0;
 };
-template <>
-struct KrTile<FLOCK_KV_BF16> {
-  static constexpr int ROW = 256, K_STRIDE = 320, V_GROUP = 4 * 256 + 32, WARPS = 8, STAGES = 2;
-  static constexpr int SCALES = 0;
+template <int NT>
+struct KrTile<FLOCK_KV_BF16, NT> {
+  static constexpr int ROW = 256, K_STRIDE = 320, WARPS = 8, STAGES = 2, SCALES = 0;
 };
-template <>
-struct KrTile<FLOCK_KV_F32> {
-  static constexpr int ROW = 512, K_STRIDE = 576, V_GROUP = 4 * 512 + 32, WARPS = 6, STAGES = 2;
-  static constexpr int SCALES = 0;
+template <int NT>
+struct KrTile<FLOCK_KV_F32, NT> {
+  static constexpr int ROW = 512, K_STRIDE = 576, WARPS = 6, STAGES = 2, SCALES = 0;
 };
-template <int KV>
-struct KrLayout : KrTile<KV> {
-  using T = KrTile<KV>;
+template <int KV, int NT>
+struct KrLayout : KrTile<KV, NT> {
+  using T = KrTile<KV, NT>;
+  static constexpr bool F16 = KV == FLOCK_KV_Q4 || KV == FLOCK_KV_FP8;
+  static constexpr int RT = F16 ? 4 * NT : 4;  // query rows per CTA
+  static constexpr int V_PAIR = 2 * T::ROW + 32;  // two keys' value rows
   static constexpr int V_OFF = KR_GROUP * T::K_STRIDE;
-  static constexpr int S_OFF = V_OFF + KR_GROUP / 4 * T::V_GROUP;
+  static constexpr int S_OFF = V_OFF + KR_GROUP / 2 * V_PAIR;
   static constexpr int STAGE = S_OFF + T::SCALES;
   static constexpr int THREADS = 32 * T::WARPS;
   static constexpr size_t SMEM = (size_t)T::WARPS * T::STAGES * STAGE;
@@ -95,20 +106,26 @@ FLOCK_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "me
 template <int N>
 FLOCK_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// d = a b + c; not volatile, so that the compiler may order it freely.
+template <bool F16>
+FLOCK_DEV void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
+                     float c1, float c2, float c3) {
+  if (F16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2),
+          "f"(c3));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2),
+          "f"(c3));
+}
 template <bool F16>
 FLOCK_DEV void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if (F16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  mma16<F16>(d, a, b0, b1, d[0], d[1], d[2], d[3]);
 }
 FLOCK_DEV float exp2_approx(float x) {
   float y;
@@ -153,10 +170,35 @@ FLOCK_DEV uint32_t hfma2_u(uint32_t a, uint32_t b, uint32_t c) {
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
   return r;
 }
+FLOCK_DEV uint32_t hmul2_u(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+FLOCK_DEV __half2 as_h2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
 FLOCK_DEV uint32_t hadd2_u(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
+}
+FLOCK_DEV uint32_t hneg2_u(uint32_t a) {
+  const __half2 r = __hneg2(*reinterpret_cast<const __half2*>(&a));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// An 8 x 8 matrix of 16-bit values, a row's eight over four lanes, transposed.
+FLOCK_DEV uint32_t movm(uint32_t a) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+// The eight codes of a word as f16 pairs of the subnormals c 2^-24 (v[0],
+// v[2]) and 16 c 2^-24 (v[1], v[3]).  v[e]: bits 4 e .. 4 e + 3 of both halfwords.
+FLOCK_DEV void nib_sub(uint32_t w, uint32_t (&v)[4]) {
+  const uint32_t hi = w >> 8;
+  v[0] = w & 0x000F000Fu;
+  v[1] = w & 0x00F000F0u;
+  v[2] = hi & 0x000F000Fu;
+  v[3] = hi & 0x00F000F0u;
 }
 // The eight codes of a word -> (code - 8) as four f16 pairs: 0x6400 | code is
 // the f16 1024 + code, 0x6400 | 16 code is 1024 + 16 code, and the rest is
@@ -174,71 +216,71 @@ FLOCK_DEV uint32_t fp8_f16(uint32_t w) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The head dimension of column n of output tile t (0-15).
+// The head dimension of row g (half 0) or g + 8 (half 1) of output tile u (0-7).
 template <int KV>
-FLOCK_DEV int kr_vdim(int t, int n) {
-  if (KV == FLOCK_KV_Q4) return 32 * (t >> 2) + 16 * (t & 1) + 2 * n + ((t & 2) >> 1);
-  if (KV == FLOCK_KV_FP8) return 16 * n + t;
-  if (KV == FLOCK_KV_BF16) return 64 * (t >> 3) + 8 * n + (t & 7);
-  return 32 * (t >> 2) + 4 * n + (t & 3);
+FLOCK_DEV int kr_vdim(int u, int half, int g) {
+  if (KV == FLOCK_KV_Q4) {  // nibble e of the lane's two bytes of block u / 2
+    const int e = 2 * (u & 1) + half;
+    return 32 * (u >> 1) + 16 * (e & 1) + 2 * g + (e >> 1);
+  }
+  if (KV == FLOCK_KV_FP8) return 16 * g + 2 * u + half;
+  if (KV == FLOCK_KV_BF16) return 64 * (u >> 2) + 8 * g + 2 * (u & 3) + half;
+  return 32 * (u >> 1) + 4 * g + 2 * (u & 1) + half;
 }
 
 // One stage of keys key0 .. key0 + 15 of a head into shared memory; keys
 // outside [from, to) are zero-filled, so what lies there cannot reach a
 // product.  kb, vb: the head's first rows; sb: this lane's scale plane at the
 // head's first row.
-template <int KV>
+template <int KV, int NT, bool WHOLE>
 FLOCK_DEV void kr_load(uint32_t stage, const uint8_t* kb, const uint8_t* vb, const uint8_t* sb,
                        int64_t step, int key0, int from, int to, int lane) {
-  using L = KrLayout<KV>;
+  using L = KrLayout<KV, NT>;
   constexpr int CHUNKS = L::ROW / 16;  // 16-byte chunks of a row
-  const bool whole = key0 >= from && key0 + KR_GROUP <= to;
+  constexpr int ROWS = 32 / CHUNKS;    // rows a warp's 32 chunks cover (f32: one)
+  const int r0 = lane / CHUNKS, ch = lane % CHUNKS;
+  // a 4-bit head's rows are contiguous, step = 64
+  const uint8_t* ks = kb + (int64_t)(key0 + r0) * step + ch * 16;
+  const uint8_t* vs = vb + (int64_t)(key0 + r0) * step + ch * 16;
+  const uint32_t kd = stage + r0 * L::K_STRIDE + ch * 16;
+  const uint32_t vd = stage + L::V_OFF + (r0 >> 1) * L::V_PAIR + (r0 & 1) * L::ROW + ch * 16;
 #pragma unroll
-  for (int i = 0; i < KR_GROUP * CHUNKS / 32; i++) {
-    const int at = i * 32 + lane, r = at / CHUNKS, ch = at % CHUNKS;
-    const bool ok = whole || (key0 + r >= from && key0 + r < to);
-    // a 4-bit head's rows are contiguous: one offset for the whole group
-    const int64_t off = KV == FLOCK_KV_Q4 ? (int64_t)key0 * 64 + at * 16
-                                          : (int64_t)(ok ? key0 + r : from) * step + ch * 16;
-    cp_async16(stage + r * L::K_STRIDE + ch * 16, kb + off, ok);
-    cp_async16(stage + L::V_OFF + (r >> 2) * L::V_GROUP + (r & 3) * L::ROW + ch * 16, vb + off, ok);
+  for (int i = 0; i < KR_GROUP / ROWS; i++) {
+    const bool ok = WHOLE || (key0 + r0 + i * ROWS >= from && key0 + r0 + i * ROWS < to);
+    const int64_t off = ok ? (int64_t)(i * ROWS) * step : (int64_t)(from - key0 - r0) * step;
+    // value rows r0 + i ROWS: whole pairs apart, or the second of a pair
+    const uint32_t vo = ROWS >= 2 ? i * (ROWS / 2) * L::V_PAIR : (i / 2) * L::V_PAIR + (i % 2) * L::ROW;
+    cp_async16(kd + i * ROWS * L::K_STRIDE, ks + off, ok);
+    cp_async16(vd + vo, vs + off, ok);
   }
   if (KV == FLOCK_KV_Q4) {
     const int r = lane & 15;
-    const bool ok = whole || (key0 + r >= from && key0 + r < to);
+    const bool ok = WHOLE || (key0 + r >= from && key0 + r < to);
     cp_async8(stage + L::S_OFF + lane * 8, sb + (int64_t)(key0 + r) * 8, ok);
   }
 }
 
-FLOCK_DEV uint4 lds128(uint32_t a) {
-  uint4 r;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
-  return r;
-}
-FLOCK_DEV uint2 lds64(uint32_t a) {
-  uint2 r;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
-  return r;
+FLOCK_DEV uint4 ld_u4(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
+FLOCK_DEV uint2 ld_u2(const uint8_t* p) { return *reinterpret_cast<const uint2*>(p); }
+FLOCK_DEV uint32_t word_of(const uint4& v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
-// Query rows per CTA.  f16 parts: operand rows 0-7 hold the rows' hi parts,
-// 8-15 their lo.  bf16 parts: 0-3 hi, 4-7 mid, 8-11 lo.
-template <int KV>
-constexpr int KR_ROWS = KV == FLOCK_KV_Q4 || KV == FLOCK_KV_FP8 ? 8 : 4;
-
-// Keys of a stage are dealt to operand columns so that a lane's four score
-// columns are four neighbouring keys: column n of score tile t is key
-// 4 (n / 2) + 2 t + n % 2, and lane column c holds keys 4 c .. 4 c + 3.
-template <int KV>
-static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(const KvRowsArgs p) {
-  using L = KrLayout<KV>;
-  constexpr int RT = KR_ROWS<KV>;
+// Lane (g, c) = (lane / 4, lane % 4).  Scores: keys g and g + 8 of the stage,
+// query row c of each column tile (f16: tile n holds rows 4 n .. 4 n + 3 as hi,
+// lo columns; bf16: tile 0 hi, mid and tile 1 lo of rows 0-3).
+template <int KV, int NT>
+static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
+    k_kv_rows(const KvRowsArgs p) {
+  using L = KrLayout<KV, NT>;
+  constexpr int RT = L::RT;
   constexpr bool Q4 = KV == FLOCK_KV_Q4;
-  constexpr bool F16 = Q4 || KV == FLOCK_KV_FP8;
+  constexpr bool F16 = L::F16;
+  constexpr int RL = F16 ? NT : 1;  // query rows of a lane
   extern __shared__ __align__(16) uint8_t kr_smem[];
   __shared__ float s_ml[L::WARPS][RT][2];
-  __shared__ uint4 s_q[8][32];  // the query operand: [QK step][lane]
+  __shared__ uint2 s_q[NT][8][32];    // the query operand: [tile][QK step][lane]
+  __shared__ float s_corr[RT][4];     // 4-bit: -8 2^-24 sum of a block's query parts
   __shared__ float s_unscale[RT];
   __shared__ int s_last;
   pdl_launch_dependents();
@@ -247,8 +289,6 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int z = blockIdx.x, tile = blockIdx.y, head = blockIdx.z;
-  const int j = g % RT;  // this lane's query row
-  const int row = tile * RT + j;
   const int first_q = tile * RT / p.group;
   const int last_q = (min(p.rows, (tile + 1) * RT) - 1) / p.group;
   // keys that some row of the tile sees: sinks [0, sk), then [lo, hi)
@@ -260,11 +300,17 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
   const int lo16 = lo & ~(KR_GROUP - 1);
   const int groups = sink_groups + (hi - lo16 + KR_GROUP - 1) / KR_GROUP;
   const int g0 = (int)((int64_t)z * groups / p.splits), g1 = (int)((int64_t)(z + 1) * groups / p.splits);
-  // this row's own keys: sinks [0, row_sk), then [row_lo, row_hi)
-  const int my_q = min(row, p.rows - 1) / p.group;
-  const int row_hi = pos + my_q + 1;
-  const int row_lo = a.window && row_hi > a.window ? row_hi - a.window : 0;
-  const int row_sk = min(a.sinks, row_lo);
+  // a row's own keys: sinks [0, row_sk), then [row_lo, row_hi)
+  int row_lo[RL], row_hi[RL], row_sk[RL];
+  int max_lo = 0, min_hi = hi;  // a group inside [max_lo, min_hi) is visible to every row
+#pragma unroll
+  for (int n = 0; n < RL; n++) {
+    row_hi[n] = pos + min(tile * RT + 4 * n + c, p.rows - 1) / p.group + 1;
+    row_lo[n] = a.window && row_hi[n] > a.window ? row_hi[n] - a.window : 0;
+    row_sk[n] = min(a.sinks, row_lo[n]);
+  }
+  max_lo = a.window && pos + last_q + 1 > a.window ? pos + last_q + 1 - a.window : 0;
+  min_hi = pos + first_q + 1;
 
   const uint32_t ring = smem_u32(kr_smem) + warp * L::STAGES * L::STAGE;
   const size_t hbase = Q4 ? q4_row(a.c, 0, head) * 64 : (size_t)head * L::ROW;
@@ -273,15 +319,19 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
   const uint8_t* sb = Q4 ? reinterpret_cast<const uint8_t*>((lane < 16 ? a.c.ks : a.c.vs) +
                                                             q4_row(a.c, 0, head) * 4)
                          : nullptr;
-  const int64_t step = (int64_t)a.c.n_kv_heads * L::ROW;
+  const int64_t step = Q4 ? 64 : (int64_t)a.c.n_kv_heads * L::ROW;
   auto key_of = [&](int grp) {
     return grp < sink_groups ? grp * KR_GROUP : lo16 + (grp - sink_groups) * KR_GROUP;
   };
   auto fetch = [&](int grp, int st) {
     if (grp < g1) {
       const bool sink = grp < sink_groups;
-      kr_load<KV>(ring + st * L::STAGE, kb, vb, sb, step, key_of(grp), sink ? 0 : lo,
-                  sink ? sk : hi, lane);
+      const int key0 = key_of(grp), from = sink ? 0 : lo, to = sink ? sk : hi;
+      const uint32_t dst = ring + st * L::STAGE;
+      if (key0 >= from && key0 + KR_GROUP <= to)
+        kr_load<KV, NT, true>(dst, kb, vb, sb, step, key0, from, to, lane);
+      else
+        kr_load<KV, NT, false>(dst, kb, vb, sb, step, key0, from, to, lane);
     }
     cp_async_commit();
   };
@@ -290,7 +340,7 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
 
   // The query operand: the parts of q log2(e) / sqrt(128), for f16 scaled by
   // a power of two that brings the row's largest into [2^13, 2^14).  A warp
-  // splits a row, four neighbouring dimensions a lane: one operand entry.
+  // splits a row, four neighbouring dimensions a lane: one entry of each part.
   for (int r = warp; r < RT; r += L::WARPS) {
     const int rr = tile * RT + r;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -300,6 +350,7 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
           4 * lane));
     const float k = __double2float_rn(1.4426950408889634 / sqrt(128.0));
     x = make_float4(fmul(x.x, k), fmul(x.y, k), fmul(x.z, k), fmul(x.w, k));
+    // where these four dimensions meet a lane's cached bytes: step ks, lane column qc
     const int qc = Q4 || KV == FLOCK_KV_F32 ? lane & 3 : KV == FLOCK_KV_FP8 ? (lane >> 2) & 3 : (lane >> 1) & 3;
     const int ks = Q4 || KV == FLOCK_KV_F32 ? lane >> 2
                    : KV == FLOCK_KV_FP8     ? (lane >> 4) * 4 + (lane & 3)
@@ -309,276 +360,338 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
       const int biased = (int)(__float_as_uint(top) >> 23);
-      const int e = biased == 0 ? 0 : max(-100, min(100, biased - 127 - 13));
-      const float scale = __uint_as_float((uint32_t)(127 - e) << 23);
-      if (lane == 0) s_unscale[r] = __uint_as_float((uint32_t)(127 + e) << 23);
+      const int e = biased == 0 ? 0 : max(-90, min(90, biased - 127 - 13));
+      // high nibbles (4-bit, odd steps) are read as 16 c
+      const float scale = __uint_as_float((uint32_t)(127 - e - (Q4 && (ks & 1) ? 4 : 0)) << 23);
       if (Q4) {  // pairs two apart: bytes 0 and 2, 1 and 3 of a code word
         const float y = x.y;
         x.y = x.z;
         x.z = y;
       }
-      uint4 w;
-      split_f16(fmul(x.x, scale), fmul(x.y, scale), w.x, w.y);
-      split_f16(fmul(x.z, scale), fmul(x.w, scale), w.z, w.w);
-      s_q[ks][4 * r + qc] = w;
+      uint2 h, l;
+      split_f16(fmul(x.x, scale), fmul(x.y, scale), h.x, l.x);
+      split_f16(fmul(x.z, scale), fmul(x.w, scale), h.y, l.y);
+      s_q[r / 4][ks][4 * (2 * (r % 4)) + qc] = h;
+      s_q[r / 4][ks][4 * (2 * (r % 4) + 1) + qc] = l;
+      if (Q4) {
+        float sum = 0.0f;
+        const uint32_t parts[4] = {l.x, l.y, h.x, h.y};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float2 f = h2f2(parts[i]);
+          sum = fadd(sum, fadd(f.x, f.y));
+        }
+        sum = ks & 1 ? fmul(sum, 16.0f) : sum;
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) sum = fadd(sum, __shfl_xor_sync(0xffffffffu, sum, d));
+        if ((lane & 7) == 0) s_corr[r][lane >> 3] = fmul(sum, -4.76837158203125e-7f);  // -8 2^-24
+      }
+      if (lane == 0) s_unscale[r] = __uint_as_float((uint32_t)(127 + e + (Q4 ? 24 : 0)) << 23);
     } else {
       uint32_t w0[3], w1[3];
       split_bf16(x.x, x.y, w0);
       split_bf16(x.z, x.w, w1);
-      s_q[ks][4 * r + qc] = make_uint4(w0[0], w0[2], w1[0], w1[2]);
-      s_q[ks][4 * (r + 4) + qc] = make_uint4(w0[1], 0, w1[1], 0);
+      s_q[0][ks][4 * (2 * r) + qc] = make_uint2(w0[0], w1[0]);
+      s_q[0][ks][4 * (2 * r + 1) + qc] = make_uint2(w0[1], w1[1]);
+      s_q[1][ks][4 * (2 * r) + qc] = make_uint2(w0[2], w1[2]);
+      s_q[1][ks][4 * (2 * r + 1) + qc] = make_uint2(0, 0);
     }
   }
   __syncthreads();
-  uint32_t qa[8][4];
+  uint2 qb[NT][8];
+  float unscale[RL], corr[RL][4];
 #pragma unroll
-  for (int ks = 0; ks < 8; ks++) {
-    const uint4 w = s_q[ks][lane];
-    qa[ks][0] = w.x;
-    qa[ks][1] = w.y;
-    qa[ks][2] = w.z;
-    qa[ks][3] = w.w;
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int ks = 0; ks < 8; ks++) qb[n][ks] = s_q[n][ks][lane];
+#pragma unroll
+  for (int n = 0; n < RL; n++) {
+    unscale[n] = F16 ? s_unscale[4 * n + c] : 1.0f;
+#pragma unroll
+    for (int b = 0; b < 4; b++) corr[n][b] = Q4 ? s_corr[4 * n + c][b] : 0.0f;
   }
-  const float unscale = F16 ? s_unscale[j] : 1.0f;
-  float o[16][4];
+  float o[8][NT][4];
 #pragma unroll
-  for (int t = 0; t < 16; t++)
+  for (int u = 0; u < 8; u++)
 #pragma unroll
-    for (int e = 0; e < 4; e++) o[t][e] = 0.0f;
-  // Weights are 2^(s - base), base = m + dexp - 6: m a running maximum that may
-  // lag by 2^8, 2^dexp a bound on the value scales so far, so a weight times a
-  // scale is at most 2^14, inside f16, and its lo part loses nothing above
-  // 2^-31 of the largest.
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[u][n][e] = 0.0f;
+  // Weights are 2^(s - base), base = m - 6, m a running maximum that may lag by
+  // 2^8: at most 2^14, inside f16, and a lo part loses nothing above 2^-31 of
+  // the largest.  Value scales are divided by 2^dexp, a bound on those so far,
+  // which the outputs get back at the end.
   constexpr float HEADROOM = F16 ? 6.0f : 0.0f;
-  float m = -INFINITY, l = 0.0f, base = 0.0f;
-  int dexp = Q4 ? -24 : 0;
-  float dlim = Q4 ? 5.9604645e-8f : 0.0f;  // 2^dexp
+  float m[RL], l[RL], base[RL];
+#pragma unroll
+  for (int n = 0; n < RL; n++) {
+    m[n] = -INFINITY;
+    l[n] = base[n] = 0.0f;
+  }
+  int dexp = -14;
+  uint32_t dlim = 0x04000400u, dnorm = 0x74007400u;  // f16 pairs 2^dexp and 2^-dexp
 
   int st = 0;
   for (int grp = g0 + warp; grp < g1; grp += L::WARPS) {
     cp_async_wait<L::STAGES - 2>();
     __syncwarp();  // the stage has landed for every lane, and every lane is done with the last one
     fetch(grp + (L::STAGES - 1) * L::WARPS, st == 0 ? L::STAGES - 1 : st - 1);
-    const uint32_t stage = ring + st * L::STAGE;
+    const uint8_t* stage = kr_smem + (warp * L::STAGES + st) * L::STAGE;
     // ------------------------------------------------------------- scores
-    float s[4];  // keys 4 c + i of this lane's row
-    const uint32_t kaddr = stage + (4 * (g >> 1) + (g & 1)) * L::K_STRIDE + 16 * c;
+    float s[RL][2];  // keys g, g + 8
+    const uint8_t* ka = stage + g * L::K_STRIDE + 16 * c;
     if constexpr (Q4) {
-      const uint4 scales[2] = {lds128(stage + L::S_OFF + 32 * c),
-                               lds128(stage + L::S_OFF + 32 * c + 16)};
+      const uint4 w0 = ld_u4(ka), w1 = ld_u4(ka + 8 * L::K_STRIDE);
+      const uint2 e0 = ld_u2(stage + L::S_OFF + 8 * g), e1 = ld_u2(stage + L::S_OFF + 8 * g + 64);
 #pragma unroll
-      for (int t = 0; t < 2; t++) {
-        const uint4 w4 = lds128(kaddr + 2 * t * L::K_STRIDE);
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-        // keys 4 c + 2 t and the next, four blocks each
-        const float2 k0[2] = {h2f2(scales[t].x), h2f2(scales[t].y)},
-                     k1[2] = {h2f2(scales[t].z), h2f2(scales[t].w)};
-        uint64_t sum = pack2(0.0f, 0.0f);
+      for (int n = 0; n < RL; n++) s[n][0] = s[n][1] = 0.0f;
 #pragma unroll
-        for (int b = 0; b < 4; b++) {
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t v[4];
-          nib_f16(w[b], v);
-          mma16<F16>(acc, qa[2 * b], v[0], v[2]);
-          mma16<F16>(acc, qa[2 * b + 1], v[1], v[3]);
-          const uint64_t d = b & 1 ? pack2(k0[b >> 1].y, k1[b >> 1].y)
-                                   : pack2(k0[b >> 1].x, k1[b >> 1].x);
-          sum = ffma2(d, pack2(acc[0], acc[1]), sum);  // hi
-          sum = ffma2(d, pack2(acc[2], acc[3]), sum);  // lo
+      for (int b = 0; b < 4; b++) {
+        uint32_t x[4], y[4];
+        nib_sub(word_of(w0, b), x);
+        nib_sub(word_of(w1, b), y);
+        const float2 d0 = h2f2(b < 2 ? e0.x : e0.y), d1 = h2f2(b < 2 ? e1.x : e1.y);
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          float acc[4];
+          const uint32_t a0[4] = {x[0], y[0], x[2], y[2]}, a1[4] = {x[1], y[1], x[3], y[3]};
+          mma16<F16>(acc, a0, qb[n][2 * b].x, qb[n][2 * b].y, corr[n][b], 0.f, corr[n][b], 0.f);
+          mma16<F16>(acc, a1, qb[n][2 * b + 1].x, qb[n][2 * b + 1].y);
+          s[n][0] = ffma(b & 1 ? d0.y : d0.x, fadd(acc[0], acc[1]), s[n][0]);
+          s[n][1] = ffma(b & 1 ? d1.y : d1.x, fadd(acc[2], acc[3]), s[n][1]);
         }
-        const float2 r = unpack2(sum);
-        s[2 * t] = r.x;
-        s[2 * t + 1] = r.y;
       }
     } else {
+      float acc[NT][2][4];
 #pragma unroll
-      for (int t = 0; t < 2; t++) {
-        const uint32_t kt = kaddr + 2 * t * L::K_STRIDE;
-        float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        if constexpr (KV == FLOCK_KV_FP8) {
+      for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const uint4 w4 = lds128(kt + 64 * h);
-            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+        for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-              mma16<F16>(acc[i & 1], qa[4 * h + i], fp8_f16(w[i]), fp8_f16(w[i] >> 16));
-          }
-        } else if constexpr (KV == FLOCK_KV_BF16) {
+          for (int e = 0; e < 4; e++) acc[n][h][e] = 0.0f;
+      if constexpr (KV == FLOCK_KV_FP8) {
 #pragma unroll
-          for (int h = 0; h < 4; h++) {
-            const uint4 w = lds128(kt + 64 * h);
-            mma16<F16>(acc[0], qa[2 * h], w.x, w.y);
-            mma16<F16>(acc[1], qa[2 * h + 1], w.z, w.w);
-          }
-        } else {
+        for (int h = 0; h < 2; h++) {
+          const uint4 w0 = ld_u4(ka + 64 * h), w1 = ld_u4(ka + 64 * h + 8 * L::K_STRIDE);
 #pragma unroll
-          for (int ks = 0; ks < 8; ks++) {
-            const uint4 w = lds128(kt + 64 * ks);
-            uint32_t b0[3], b1[3];
-            split_bf16(__uint_as_float(w.x), __uint_as_float(w.y), b0);
-            split_bf16(__uint_as_float(w.z), __uint_as_float(w.w), b1);
+          for (int i = 0; i < 4; i++) {
+            const uint32_t x = word_of(w0, i), y = word_of(w1, i);
+            const uint32_t av[4] = {fp8_f16(x), fp8_f16(y), fp8_f16(x >> 16), fp8_f16(y >> 16)};
 #pragma unroll
-            for (int part = 0; part < 3; part++) mma16<F16>(acc[part & 1], qa[ks], b0[part], b1[part]);
+            for (int n = 0; n < NT; n++)
+              mma16<F16>(acc[n][i & 1], av, qb[n][4 * h + i].x, qb[n][4 * h + i].y);
           }
         }
+      } else if constexpr (KV == FLOCK_KV_BF16) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-          s[2 * t + i] = fadd(fadd(acc[0][i], acc[1][i]), fadd(acc[0][2 + i], acc[1][2 + i]));
-          if (!F16) s[2 * t + i] = fadd(s[2 * t + i], __shfl_xor_sync(0xffffffffu, s[2 * t + i], 16));
+        for (int h = 0; h < 4; h++) {
+          const uint4 w0 = ld_u4(ka + 64 * h), w1 = ld_u4(ka + 64 * h + 8 * L::K_STRIDE);
+          const uint32_t a0[4] = {w0.x, w1.x, w0.y, w1.y}, a1[4] = {w0.z, w1.z, w0.w, w1.w};
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+            mma16<F16>(acc[n][0], a0, qb[n][2 * h].x, qb[n][2 * h].y);
+            mma16<F16>(acc[n][1], a1, qb[n][2 * h + 1].x, qb[n][2 * h + 1].y);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < 8; ks++) {
+          const uint4 w0 = ld_u4(ka + 64 * ks), w1 = ld_u4(ka + 64 * ks + 8 * L::K_STRIDE);
+          uint32_t x0[3], x1[3], y0[3], y1[3];
+          split_bf16(__uint_as_float(w0.x), __uint_as_float(w0.y), x0);
+          split_bf16(__uint_as_float(w0.z), __uint_as_float(w0.w), x1);
+          split_bf16(__uint_as_float(w1.x), __uint_as_float(w1.y), y0);
+          split_bf16(__uint_as_float(w1.z), __uint_as_float(w1.w), y1);
+#pragma unroll
+          for (int part = 0; part < 3; part++) {
+            const uint32_t av[4] = {x0[part], y0[part], x1[part], y1[part]};
+#pragma unroll
+            for (int n = 0; n < (part == 2 ? 1 : NT); n++)  // lo lo is below f32's last bit
+              mma16<F16>(acc[n][part & 1], av, qb[n][ks].x, qb[n][ks].y);
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < RL; n++) {
+        s[n][0] = fadd(fadd(acc[n][0][0], acc[n][1][0]), fadd(acc[n][0][1], acc[n][1][1]));
+        s[n][1] = fadd(fadd(acc[n][0][2], acc[n][1][2]), fadd(acc[n][0][3], acc[n][1][3]));
+        if (!F16) {
+          s[n][0] = fadd(s[n][0], fadd(acc[1][0][0], acc[1][1][0]));
+          s[n][1] = fadd(s[n][1], fadd(acc[1][0][2], acc[1][1][2]));
         }
       }
     }
     const int key0 = key_of(grp);
     {  // masks, only where the group is not wholly visible to every row
       const bool sink = grp < sink_groups;
-      const int from = sink ? 0 : row_lo, to = sink ? sk : row_hi;
-      if (__any_sync(0xffffffffu, key0 < from || key0 + KR_GROUP > to)) {
+      if (sink ? key0 + KR_GROUP > sk : key0 < max_lo || key0 + KR_GROUP > min_hi) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int key = key0 + 4 * c + i;
-          // every row sees the tile's sinks; a row's own may reach into the main range
-          const bool seen = sink ? key < sk
-                                 : key >= lo && key < row_hi && (key >= row_lo || key < row_sk);
-          if (!seen) s[i] = -INFINITY;
-        }
+        for (int n = 0; n < RL; n++)
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            const int key = key0 + g + 8 * i;
+            // every row sees the tile's sinks; a row's own may reach into the main range
+            const bool seen = sink ? key < sk
+                                   : key >= lo && key < row_hi[n] && (key >= row_lo[n] || key < row_sk[n]);
+            if (!seen) s[n][i] = -INFINITY;
+          }
       }
     }
     // ------------------------------------------------------------ softmax
-    // the value scales of the lane's four keys, two blocks a word; the largest
-    // magnitude of all sixteen as a bound for the f16 weights
-    uint32_t vs[4][2];
-    float dmax = 0.0f;
+    // 4-bit: the value scales of the lane's two keys, a block's pair a word
+    uint32_t vd[4];
+    uint32_t dmax = 0;
+    bool grow = false;
     if constexpr (Q4) {
-      const uint4 e0 = lds128(stage + L::S_OFF + 128 + 32 * c);
-      const uint4 e1 = lds128(stage + L::S_OFF + 128 + 32 * c + 16);
-      vs[0][0] = e0.x, vs[0][1] = e0.y, vs[1][0] = e0.z, vs[1][1] = e0.w;
-      vs[2][0] = e1.x, vs[2][1] = e1.y, vs[3][0] = e1.z, vs[3][1] = e1.w;
-      auto habs = [](uint32_t x) {
-        const uint32_t u = x & 0x7FFF7FFFu;
-        return *reinterpret_cast<const __half2*>(&u);
-      };
-      __half2 h = habs(vs[0][0]);
-#pragma unroll
-      for (int i = 1; i < 8; i++) h = __hmax2(h, habs(vs[i >> 1][i & 1]));
-      const float2 f = __half22float2(h);
-      dmax = fmaxf(f.x, f.y);
+      const uint2 e0 = ld_u2(stage + L::S_OFF + 128 + 8 * g), e1 = ld_u2(stage + L::S_OFF + 192 + 8 * g);
+      vd[0] = __byte_perm(e0.x, e1.x, 0x5410);
+      vd[1] = __byte_perm(e0.x, e1.x, 0x7632);
+      vd[2] = __byte_perm(e0.y, e1.y, 0x5410);
+      vd[3] = __byte_perm(e0.y, e1.y, 0x7632);
+      const __half2 h = __hmax2(__hmax2(__habs2(as_h2(e0.x)), __habs2(as_h2(e0.y))),
+                                __hmax2(__habs2(as_h2(e1.x)), __habs2(as_h2(e1.y))));
+      grow = __hgt2_mask(h, as_h2(dlim)) != 0;
+      dmax = __half_as_ushort(__hmax(__low2half(h), __high2half(h)));
     }
-    float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmul(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)), unscale);
-    if (__any_sync(0xffffffffu, top > fadd(m, 8.0f) || (Q4 && dmax > dlim))) {
+    float top[RL];
+#pragma unroll
+    for (int n = 0; n < RL; n++) {
+      top[n] = fmaxf(s[n][0], s[n][1]);
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], d));
+      top[n] = fmul(top[n], unscale[n]);
+      grow = grow || top[n] > fadd(m[n], 8.0f);
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+      float fd = 1.0f;
       if (Q4) {
-#pragma unroll
-        for (int x = 1; x < 32; x <<= 1) dmax = fmaxf(dmax, __shfl_xor_sync(0xffffffffu, dmax, x));
-        dexp = max(dexp, min((int)(__float_as_uint(dmax) >> 23) - 126, 16));
-        dlim = __uint_as_float((uint32_t)(127 + dexp) << 23);
+        dmax = __reduce_max_sync(0xffffffffu, dmax);  // magnitudes order as their bits do
+        const int ne = max(dexp, min((int)(dmax >> 10) - 14, 16));  // below 2^(exponent - 14)
+        fd = __uint_as_float((uint32_t)(127 + dexp - ne) << 23);
+        dexp = ne;
+        dlim = ne > 15 ? 0x7BFF7BFFu : (uint32_t)(ne + 15) * 0x04000400u;
+        dnorm = ne < 15 ? (uint32_t)(15 - ne) * 0x04000400u : ne == 15 ? 0x02000200u : 0x01000100u;
       }
-      const float mn = fmaxf(m, top);
-      const float nb = mn == -INFINITY ? 0.0f : fadd(mn, (float)dexp - HEADROOM);
-      const float f = m == -INFINITY ? 0.0f : exp2_approx(fsub(base, nb));
-      l = fmul(l, f);
 #pragma unroll
-      for (int t = 0; t < 16; t++)
+      for (int n = 0; n < RL; n++) {
+        const float mn = fmaxf(m[n], top[n]);
+        const float nb = mn == -INFINITY ? 0.0f : fsub(mn, HEADROOM);
+        const float f = m[n] == -INFINITY ? 0.0f : exp2_approx(fsub(base[n], nb));
+        l[n] = fmul(l[n], f);
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[t][e] = fmul(o[t][e], f);  // rows g and g + 8: one query row
-      m = mn;
-      base = nb;
+        for (int u = 0; u < 8; u++)
+#pragma unroll
+          for (int k = F16 ? n : 0; k < (F16 ? n + 1 : NT); k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[u][k][e] = fmul(o[u][k][e], fmul(f, fd));
+        m[n] = mn;
+        base[n] = nb;
+      }
     }
-    float w[4];
+    float w[RL][2];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      w[i] = exp2_approx(ffma(s[i], unscale, -base));
-      l = fadd(l, w[i]);
-    }
+    for (int n = 0; n < RL; n++)
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        w[n][i] = exp2_approx(ffma(s[n][i], unscale[n], -base[n]));
+        l[n] = fadd(l[n], w[n][i]);
+      }
     // ------------------------------------------------------------- values
-    const uint32_t vaddr = stage + L::V_OFF + c * L::V_GROUP;
+    // lane column c: keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
+    const uint8_t* va = stage + L::V_OFF + c * L::V_PAIR;
     if constexpr (Q4) {
-      uint2 v[4];
+      uint32_t wh[NT], wl[NT];
 #pragma unroll
-      for (int i = 0; i < 4; i++) v[i] = lds64(vaddr + i * 64 + 8 * g);
+      for (int n = 0; n < NT; n++) split_f16(w[n][0], w[n][1], wh[n], wl[n]);
+      const uint2 v0 = ld_u2(va + 8 * g), v1 = ld_u2(va + L::ROW + 8 * g);
+      const uint2 v2 = ld_u2(va + 4 * L::V_PAIR + 8 * g), v3 = ld_u2(va + 4 * L::V_PAIR + L::ROW + 8 * g);
 #pragma unroll
-      for (int hb = 0; hb < 2; hb++) {
-        float2 d[4];
+      for (int b = 0; b < 4; b++) {
+        // block b's two bytes of four keys, keys paired
+        const uint32_t sel = b & 1 ? 0x7632u : 0x5410u;
+        uint32_t x[4], y[4];
+        nib_f16(__byte_perm(b < 2 ? v0.x : v0.y, b < 2 ? v1.x : v1.y, sel), x);
+        nib_f16(__byte_perm(b < 2 ? v2.x : v2.y, b < 2 ? v3.x : v3.y, sel), y);
+        const uint32_t d = hmul2_u(vd[b], dnorm);
+        const uint32_t a0[4] = {x[0], x[1], y[0], y[1]}, a1[4] = {x[2], x[3], y[2], y[3]};
 #pragma unroll
-        for (int i = 0; i < 4; i++) d[i] = h2f2(vs[i][hb]);
-#pragma unroll
-        for (int bb = 0; bb < 2; bb++) {
-          const int b = 2 * hb + bb;
-          uint32_t pa[4];
-          split_f16(fmul(w[0], bb ? d[0].y : d[0].x), fmul(w[1], bb ? d[1].y : d[1].x), pa[0], pa[1]);
-          split_f16(fmul(w[2], bb ? d[2].y : d[2].x), fmul(w[3], bb ? d[3].y : d[3].x), pa[2], pa[3]);
-          // block b's two bytes of four keys, keys paired
-          const uint32_t sel = bb ? 0x7632u : 0x5410u;
-          const uint32_t k01 = __byte_perm(hb ? v[0].y : v[0].x, hb ? v[1].y : v[1].x, sel);
-          const uint32_t k23 = __byte_perm(hb ? v[2].y : v[2].x, hb ? v[3].y : v[3].x, sel);
-          uint32_t x[4], y[4];
-          nib_f16(k01, x);
-          nib_f16(k23, y);
-#pragma unroll
-          for (int e = 0; e < 4; e++)  // tile 4 b + e: nibble e of the halfword
-            mma16<F16>(o[4 * b + e], pa, x[e], y[e]);
+        for (int n = 0; n < NT; n++) {
+          // (hi + lo) d: the product's f16, then what its rounding left plus lo d
+          const uint32_t ph = hmul2_u(wh[n], d);
+          const uint32_t pl = hfma2_u(wl[n], d, hfma2_u(wh[n], d, hneg2_u(ph)));
+          const uint32_t b0 = movm(__byte_perm(ph, pl, 0x5410)), b1 = movm(__byte_perm(ph, pl, 0x7632));
+          mma16<F16>(o[2 * b][n], a0, b0, b1);
+          mma16<F16>(o[2 * b + 1][n], a1, b0, b1);
         }
       }
     } else {
-      uint32_t pa[4];
+      uint32_t pb[NT][2];
       if constexpr (F16) {
-        split_f16(w[0], w[1], pa[0], pa[1]);
-        split_f16(w[2], w[3], pa[2], pa[3]);
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          uint32_t ph, pl;
+          split_f16(w[n][0], w[n][1], ph, pl);
+          pb[n][0] = movm(__byte_perm(ph, pl, 0x5410));
+          pb[n][1] = movm(__byte_perm(ph, pl, 0x7632));
+        }
       } else {
-        uint32_t w0[3], w1[3];
-        split_bf16(w[0], w[1], w0);
-        split_bf16(w[2], w[3], w1);
-        pa[0] = g < 4 ? w0[0] : w0[1];
-        pa[2] = g < 4 ? w1[0] : w1[1];
-        pa[1] = g < 4 ? w0[2] : 0;
-        pa[3] = g < 4 ? w1[2] : 0;
+        uint32_t part[3];
+        split_bf16(w[0][0], w[0][1], part);
+        pb[0][0] = movm(__byte_perm(part[0], part[1], 0x5410));
+        pb[0][1] = movm(__byte_perm(part[0], part[1], 0x7632));
+        pb[1][0] = movm(part[2] & 0x0000FFFFu);
+        pb[1][1] = movm(part[2] >> 16);
       }
-      auto word = [](const uint4& v, int q) { return q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w; };
+      constexpr int K8 = 4 * L::V_PAIR;  // eight keys on
       if constexpr (KV == FLOCK_KV_FP8) {
-        uint4 v[4];
+        const uint4 v0 = ld_u4(va + 16 * g), v1 = ld_u4(va + L::ROW + 16 * g);
+        const uint4 v2 = ld_u4(va + K8 + 16 * g), v3 = ld_u4(va + K8 + L::ROW + 16 * g);
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = lds128(vaddr + i * 128 + 16 * g);
+        for (int u = 0; u < 8; u++) {
+          const int sh = 16 * (u & 1);
+          const uint32_t y0 = fp8_f16(word_of(v0, u >> 1) >> sh), y1 = fp8_f16(word_of(v1, u >> 1) >> sh),
+                         y2 = fp8_f16(word_of(v2, u >> 1) >> sh), y3 = fp8_f16(word_of(v3, u >> 1) >> sh);
+          const uint32_t av[4] = {__byte_perm(y0, y1, 0x5410), __byte_perm(y0, y1, 0x7632),
+                                  __byte_perm(y2, y3, 0x5410), __byte_perm(y2, y3, 0x7632)};
 #pragma unroll
-        for (int q = 0; q < 4; q++)
-#pragma unroll
-          for (int h = 0; h < 2; h++) {
-            uint32_t y[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) y[i] = fp8_f16(word(v[i], q) >> (16 * h));
-            mma16<F16>(o[4 * q + 2 * h], pa, __byte_perm(y[0], y[1], 0x5410),
-                       __byte_perm(y[2], y[3], 0x5410));
-            mma16<F16>(o[4 * q + 2 * h + 1], pa, __byte_perm(y[0], y[1], 0x7632),
-                       __byte_perm(y[2], y[3], 0x7632));
-          }
+          for (int n = 0; n < NT; n++) mma16<F16>(o[u][n], av, pb[n][0], pb[n][1]);
+        }
       } else if constexpr (KV == FLOCK_KV_BF16) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          uint4 v[4];
-#pragma unroll
-          for (int i = 0; i < 4; i++) v[i] = lds128(vaddr + i * 256 + 128 * h + 16 * g);
+          const uint8_t* vh = va + 128 * h + 16 * g;
+          const uint4 v0 = ld_u4(vh), v1 = ld_u4(vh + L::ROW), v2 = ld_u4(vh + K8),
+                      v3 = ld_u4(vh + K8 + L::ROW);
 #pragma unroll
           for (int q = 0; q < 4; q++) {
-            const uint32_t x0 = word(v[0], q), x1 = word(v[1], q), x2 = word(v[2], q),
-                           x3 = word(v[3], q);
-            mma16<F16>(o[8 * h + 2 * q], pa, __byte_perm(x0, x1, 0x5410), __byte_perm(x2, x3, 0x5410));
-            mma16<F16>(o[8 * h + 2 * q + 1], pa, __byte_perm(x0, x1, 0x7632),
-                       __byte_perm(x2, x3, 0x7632));
+            const uint32_t y0 = word_of(v0, q), y1 = word_of(v1, q), y2 = word_of(v2, q), y3 = word_of(v3, q);
+            const uint32_t av[4] = {__byte_perm(y0, y1, 0x5410), __byte_perm(y0, y1, 0x7632),
+                                    __byte_perm(y2, y3, 0x5410), __byte_perm(y2, y3, 0x7632)};
+#pragma unroll
+            for (int n = 0; n < NT; n++) mma16<F16>(o[4 * h + q][n], av, pb[n][0], pb[n][1]);
           }
         }
       } else {
 #pragma unroll
         for (int h = 0; h < 4; h++) {
-          uint4 v[4];
+          const uint8_t* vh = va + 128 * h + 16 * g;
+          const uint4 v0 = ld_u4(vh), v1 = ld_u4(vh + L::ROW), v2 = ld_u4(vh + K8),
+                      v3 = ld_u4(vh + K8 + L::ROW);
 #pragma unroll
-          for (int i = 0; i < 4; i++) v[i] = lds128(vaddr + i * 512 + 128 * h + 16 * g);
+          for (int q = 0; q < 2; q++) {
+            auto f = [&](const uint4& v, int i) { return __uint_as_float(word_of(v, 2 * q + i)); };
+            uint32_t x0[3], x1[3], y0[3], y1[3];
+            split_bf16(f(v0, 0), f(v1, 0), x0);
+            split_bf16(f(v0, 1), f(v1, 1), x1);
+            split_bf16(f(v2, 0), f(v3, 0), y0);
+            split_bf16(f(v2, 1), f(v3, 1), y1);
 #pragma unroll
-          for (int q = 0; q < 4; q++) {
-            uint32_t b0[3], b1[3];
-            split_bf16(__uint_as_float(word(v[0], q)), __uint_as_float(word(v[1], q)), b0);
-            split_bf16(__uint_as_float(word(v[2], q)), __uint_as_float(word(v[3], q)), b1);
+            for (int part = 0; part < 3; part++) {
+              const uint32_t av[4] = {x0[part], x1[part], y0[part], y1[part]};
 #pragma unroll
-            for (int part = 0; part < 3; part++) mma16<F16>(o[4 * h + q], pa, b0[part], b1[part]);
+              for (int n = 0; n < (part == 2 ? 1 : NT); n++)
+                mma16<F16>(o[2 * h + q][n], av, pb[n][0], pb[n][1]);
+            }
           }
         }
       }
@@ -588,24 +701,30 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
   cp_async_wait<0>();
 
   // ---------------------------------------------------------- join the warps
-  l = fadd(l, __shfl_xor_sync(0xffffffffu, l, 1));
-  l = fadd(l, __shfl_xor_sync(0xffffffffu, l, 2));
-  __syncthreads();  // the rings are done with: their memory holds the warps' outputs
-  float* s_o = reinterpret_cast<float*>(kr_smem);  // [warp][RT][128]
+  constexpr int OS = KV_HD + 4;  // row stride of the warps' outputs
   const int live = min(RT, p.rows - tile * RT);
+  __syncthreads();  // the rings are done with: their memory holds the warps' outputs
+  float* s_o = reinterpret_cast<float*>(kr_smem);  // [warp][RT][OS]
 #pragma unroll
-  for (int t = 0; t < 16; t++)
+  for (int n = 0; n < RL; n++) {
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
-      const int at = kr_vdim<KV>(t, 2 * c + e);
-      float* dst = s_o + (warp * RT + j) * KV_HD + at;
-      float x = fadd(o[t][e], o[t][2 + e]);
-      if (!F16) x = fadd(x, __shfl_xor_sync(0xffffffffu, x, 16));
-      if (g < live) *dst = x;
+    for (int d = 4; d < 32; d <<= 1) l[n] = fadd(l[n], __shfl_xor_sync(0xffffffffu, l[n], d));
+    if (4 * n + c < live) {
+      const float back = Q4 ? __uint_as_float((uint32_t)(127 + dexp) << 23) : 1.0f;
+      float* dst = s_o + (warp * RT + 4 * n + c) * OS;
+#pragma unroll
+      for (int u = 0; u < 8; u++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          float x = fadd(o[u][n][2 * h], o[u][n][2 * h + 1]);
+          if (!F16) x = fadd(x, o[u][NT - 1][2 * h]);
+          dst[kr_vdim<KV>(u, h, g)] = fmul(x, back);
+        }
+      if (g == 0) {
+        s_ml[warp][4 * n + c][0] = l[n] > 0.0f ? base[n] : -INFINITY;  // weights are relative to 2^base
+        s_ml[warp][4 * n + c][1] = l[n];
+      }
     }
-  if (g < RT && c == 0) {
-    s_ml[warp][j][0] = l > 0.0f ? base : -INFINITY;  // weights are relative to 2^base
-    s_ml[warp][j][1] = l;
   }
   __syncthreads();
   const int item = head * gridDim.y + tile;
@@ -621,7 +740,7 @@ static __global__ void __launch_bounds__(KrLayout<KV>::THREADS, 1) k_kv_rows(con
 #pragma unroll
     for (int w = 0; w < L::WARPS; w++) {
       const float f = exp2_approx(fsub(s_ml[w][r][0], b));
-      oo = ffma(f, s_o[(w * RT + r) * KV_HD + d], oo);
+      oo = ffma(f, s_o[(w * RT + r) * OS + d], oo);
       ll = ffma(f, s_ml[w][r][1], ll);
     }
     if (p.splits == 1) {
