@@ -266,6 +266,11 @@ FLOCK_DEV uint32_t word_of(const uint4& v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
+#ifdef KR_TRACE
+#define KT(i) if (threadIdx.x == 0) { reinterpret_cast<unsigned long long*>(p.part)[700000 + ((blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * 8 + (i)] = globaltimer_ns(); }
+#else
+#define KT(i)
+#endif
 // Lane (g, c) = (lane / 4, lane % 4).  Scores: keys g and g + 8 of the stage,
 // query row c of each column tile (f16: tile n holds rows 4 n .. 4 n + 3 as hi,
 // lo columns; bf16: tile 0 hi, mid and tile 1 lo of rows 0-3).
@@ -285,6 +290,7 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
   __shared__ int s_last;
   pdl_launch_dependents();
   pdl_wait();
+  KT(0);
   const KvAttnArgs& a = p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
@@ -335,19 +341,24 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
     }
     cp_async_commit();
   };
+  // The query rows' loads go out before the cached bytes': behind the rings'
+  // prefetch (hundreds of KB an SM) they would wait for all of it.
+  static_assert(RT <= L::WARPS, "a warp splits a query row");
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (warp < RT && tile * RT + warp < p.rows) {
+    const int rr = tile * RT + warp;
+    x = __ldg(reinterpret_cast<const float4*>(
+        a.q + (rr / p.group) * a.q_stride + ((int64_t)head * p.group + rr % p.group) * KV_HD +
+        4 * lane));
+  }
 #pragma unroll
   for (int s = 0; s < L::STAGES - 1; s++) fetch(g0 + warp + s * L::WARPS, s);
 
   // The query operand: the parts of q log2(e) / sqrt(128), for f16 scaled by
   // a power of two that brings the row's largest into [2^13, 2^14).  A warp
   // splits a row, four neighbouring dimensions a lane: one entry of each part.
-  for (int r = warp; r < RT; r += L::WARPS) {
-    const int rr = tile * RT + r;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (rr < p.rows)
-      x = __ldg(reinterpret_cast<const float4*>(
-          a.q + (rr / p.group) * a.q_stride + ((int64_t)head * p.group + rr % p.group) * KV_HD +
-          4 * lane));
+  if (warp < RT) {
+    const int r = warp;
     const float k = __double2float_rn(1.4426950408889634 / sqrt(128.0));
     x = make_float4(fmul(x.x, k), fmul(x.y, k), fmul(x.z, k), fmul(x.w, k));
     // where these four dimensions meet a lane's cached bytes: step ks, lane column qc
@@ -398,6 +409,7 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
     }
   }
   __syncthreads();
+  KT(1);
   uint2 qb[NT][8];
   float unscale[RL], corr[RL][4];
 #pragma unroll
@@ -434,6 +446,7 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
   int st = 0;
   for (int grp = g0 + warp; grp < g1; grp += L::WARPS) {
     cp_async_wait<L::STAGES - 2>();
+    KT(2);
     __syncwarp();  // the stage has landed for every lane, and every lane is done with the last one
     fetch(grp + (L::STAGES - 1) * L::WARPS, st == 0 ? L::STAGES - 1 : st - 1);
     const uint8_t* stage = kr_smem + (warp * L::STAGES + st) * L::STAGE;
@@ -699,6 +712,7 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
     st = st + 1 == L::STAGES ? 0 : st + 1;
   }
   cp_async_wait<0>();
+  KT(3);
 
   // ---------------------------------------------------------- join the warps
   constexpr int OS = KV_HD + 4;  // row stride of the warps' outputs
@@ -727,6 +741,7 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
     }
   }
   __syncthreads();
+  KT(4);
   const int item = head * gridDim.y + tile;
   const int n_items = gridDim.y * gridDim.z;
   float* part_ml = p.part + (size_t)n_items * p.splits * RT * KV_HD;
@@ -758,58 +773,88 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
   }
   if (p.splits == 1) return;
   // --------------------------------------------------------- join the splits
-  __threadfence();
+  // one release-acquire arrival per CTA, behind the barrier that orders its
+  // threads' stores before it
   __syncthreads();
-  if (threadIdx.x == 0) s_last = atomicAdd(p.count + item, 1u) == (uint32_t)p.splits - 1;
+  KT(5);
+  if (threadIdx.x == 0) {
+    uint32_t before;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;"
+                 : "=r"(before) : "l"(p.count + item) : "memory");
+    s_last = before == (uint32_t)p.splits - 1;
+    if (s_last) p.count[item] = 0;  // ready for the next call
+  }
   __syncthreads();
+  KT(6);
   if (!s_last) return;
-  __threadfence();
-  if (threadIdx.x == 0) p.count[item] = 0;  // ready for the next call
-  // each split's factor 2^(m_s - m) and sum, [split][RT], then their weighted outputs
-  float* s_f = reinterpret_cast<float*>(kr_smem);
+  // Thread (k, four outputs): the splits k, k + PAR, .. of them, all loads in
+  // flight before the first use; the splits' factors 2^(m_s - m) meanwhile.
+  const int quads = live * (KV_HD / 4);
+  const int par = L::THREADS / quads;
+  const int k = threadIdx.x / quads, r = (threadIdx.x % quads) / (KV_HD / 4),
+            d = 4 * (threadIdx.x % (KV_HD / 4));
+  const bool mine = threadIdx.x < par * quads;
+  float* s_f = reinterpret_cast<float*>(kr_smem);  // [split][RT]
   float* s_l = s_f + p.splits * RT;
+  float4* s_x = reinterpret_cast<float4*>(s_l + p.splits * RT);  // [k][quads]
   const size_t first = (size_t)item * p.splits * RT;
+  constexpr int U = 4;  // loads in flight
+  float4 x4[U];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (mine && s0 + u * par < p.splits)
+        x4[u] = __ldcg(reinterpret_cast<const float4*>(
+            p.part + (first + (size_t)(s0 + u * par) * RT + r) * KV_HD + d));
+  };
+  load(k);
   for (int i = threadIdx.x; i < p.splits * RT; i += L::THREADS) {
     const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml) + first + i);
     s_f[i] = ml.x;
     s_l[i] = ml.y;
   }
   __syncthreads();
-  for (int r = warp; r < live; r += L::WARPS) {
+  if (warp < live) {
     float mm = -INFINITY;
-    for (int s = lane; s < p.splits; s += 32) mm = fmaxf(mm, s_f[s * RT + r]);
+    for (int s = lane; s < p.splits; s += 32) mm = fmaxf(mm, s_f[s * RT + warp]);
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-    for (int s = lane; s < p.splits; s += 32)
-      s_f[s * RT + r] = exp2_approx(fsub(s_f[s * RT + r], mm));
+    for (int x = 1; x < 32; x <<= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
+    float ll = 0.0f;
+    for (int s = lane; s < p.splits; s += 32) {
+      const float f = exp2_approx(fsub(s_f[s * RT + warp], mm));
+      s_f[s * RT + warp] = f;
+      ll = ffma(f, s_l[s * RT + warp], ll);
+    }
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) ll = fadd(ll, __shfl_xor_sync(0xffffffffu, ll, x));
+    if (lane == 0) s_ml[0][warp][1] = ll;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < live * (KV_HD / 4); i += L::THREADS) {
-    const int r = i / (KV_HD / 4), d = 4 * (i % (KV_HD / 4)), rr = tile * RT + r;
-    float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
-    float ll = 0.0f;
-    constexpr int U = 6;  // loads in flight
-    for (int s0 = 0; s0 < p.splits; s0 += U) {
-      float4 x[U];
+  float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = k; mine && s0 < p.splits; s0 += U * par) {
+    if (s0 != k) load(s0);
 #pragma unroll
-      for (int u = 0; u < U; u++)
-        if (s0 + u < p.splits)
-          x[u] = __ldcg(reinterpret_cast<const float4*>(
-              p.part + (first + (size_t)(s0 + u) * RT + r) * KV_HD + d));
-#pragma unroll
-      for (int u = 0; u < U; u++)
-        if (s0 + u < p.splits) {
-          const float f = s_f[(s0 + u) * RT + r];
-          oo = make_float4(ffma(f, x[u].x, oo.x), ffma(f, x[u].y, oo.y), ffma(f, x[u].z, oo.z),
-                           ffma(f, x[u].w, oo.w));
-          ll = ffma(f, s_l[(s0 + u) * RT + r], ll);
-        }
+    for (int u = 0; u < U; u++)
+      if (s0 + u * par < p.splits) {
+        const float f = s_f[(s0 + u * par) * RT + r];
+        oo = make_float4(ffma(f, x4[u].x, oo.x), ffma(f, x4[u].y, oo.y), ffma(f, x4[u].z, oo.z),
+                         ffma(f, x4[u].w, oo.w));
+      }
+  }
+  if (mine) s_x[threadIdx.x] = oo;
+  __syncthreads();
+  if (threadIdx.x < quads) {
+    for (int i = 1; i < par; i++) {
+      const float4 x = s_x[i * quads + threadIdx.x];
+      oo = make_float4(fadd(oo.x, x.x), fadd(oo.y, x.y), fadd(oo.z, x.z), fadd(oo.w, x.w));
     }
-    const float inv = fdiv(1.0f, ll);
+    const float inv = fdiv(1.0f, s_ml[0][r][1]);
+    const int rr = tile * RT + r;
     *reinterpret_cast<float4*>(a.out + (rr / p.group) * a.out_stride +
                                ((int64_t)head * p.group + rr % p.group) * KV_HD + d) =
         make_float4(fmul(oo.x, inv), fmul(oo.y, inv), fmul(oo.z, inv), fmul(oo.w, inv));
   }
+  KT(7);
 }
 
 }  // namespace flock
