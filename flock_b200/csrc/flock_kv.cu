@@ -6,6 +6,7 @@
 
 #include "flock_internal.h"
 #include "kv.cuh"
+#include "kv_prompt.cuh"
 #include "kv_rows.cuh"
 
 using namespace flock;
@@ -112,6 +113,36 @@ int launch_rows(const flock_kv* c, const KvAttnArgs& a, cudaStream_t st) {
   FLOCK_CK(launch_ex(st, k_kv_rows<KV, NT>,
                      dim3((unsigned)p.splits, (unsigned)tiles, (unsigned)a.c.n_kv_heads),
                      dim3(L::THREADS), L::SMEM, true, p));
+  return FLOCK_OK;
+}
+
+// Many query rows: k_kv_prompt on the tensor cores, 128 rows a CTA.
+template <int KV>
+int launch_prompt(const flock_kv* c, const KvAttnArgs& a, cudaStream_t st) {
+  KvPromptArgs p = {};
+  p.a = a;
+  p.group = a.n_heads / a.c.n_kv_heads;
+  p.rows = a.n_queries * p.group;
+  const int tiles = (p.rows + KP_ROWS - 1) / KP_ROWS;
+  const int64_t items = (int64_t)tiles * a.c.n_kv_heads;
+  // key splits of a tile until the GPU is about full, at least two key tiles
+  // each; the workspace holds 125 tiles' partial outputs
+  const int64_t lo = a.window && a.pos + 1 > a.window ? a.pos + 1 - a.window : 0;
+  const int64_t keys = a.pos + a.n_queries - lo + (a.sinks < lo ? a.sinks : lo);
+  const int64_t want = (keys + 2 * KP_KEYS - 1) / (2 * KP_KEYS);
+  constexpr int64_t most = (FLOCK_WORKSPACE_BYTES - KR_PART_OFFSET) / (KP_ROWS * (KV_HD + 2) * 4);
+  const int64_t room = most / items;
+  p.splits = (int)(want < room ? want : room);
+  if (p.splits < 1) p.splits = 1;
+  p.part = reinterpret_cast<float*>(c->workspace + KR_PART_OFFSET);
+  FLOCK_TRY(kernel_setup((const void*)k_kv_prompt<KV>, (int)KP_SMEM<KV>));
+  FLOCK_CK(launch_ex(st, k_kv_prompt<KV>,
+                     dim3((unsigned)tiles, (unsigned)p.splits, (unsigned)a.c.n_kv_heads),
+                     dim3(KP_THREADS), KP_SMEM<KV>, true, p));
+  if (p.splits > 1)
+    FLOCK_CK(launch_ex(st, k_kv_prompt_join,
+                       dim3((unsigned)((p.rows + 7) / 8), (unsigned)a.c.n_kv_heads), dim3(256), 0,
+                       true, p, tiles));
   return FLOCK_OK;
 }
 
@@ -313,18 +344,15 @@ int flock_kv_attention(flock_kv* c, const float* q, int64_t q_stride, int n_head
   a.sinks = sinks;
   const unsigned grid = (unsigned)(((int64_t)n_queries * n_heads + 3) / 4);
   const int64_t rows = (int64_t)n_queries * (n_heads / c->view.n_kv_heads);
-  if (rows <= 16)
-    return by_dtype(c->kv_dtype, [&](auto kv) -> int {
-      constexpr int KV = decltype(kv)::value;
-      // bf16 parts fill two column tiles with four rows; f16 parts one
-      if constexpr (KV == FLOCK_KV_Q4 || KV == FLOCK_KV_FP8)
-        if (rows <= 4) return launch_rows<KV, 1>(c, a, static_cast<cudaStream_t>(stream));
-      return launch_rows<KV, 2>(c, a, static_cast<cudaStream_t>(stream));
-    });
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
   return by_dtype(c->kv_dtype, [&](auto kv) -> int {
-    k_kv_attn<decltype(kv)::value><<<grid, 128, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    FLOCK_CK(cudaGetLastError());
-    return FLOCK_OK;
+    constexpr int KV = decltype(kv)::value;
+    if constexpr (KV == FLOCK_KV_Q4 || KV == FLOCK_KV_FP8) {
+      if (rows > 16) return launch_prompt<KV>(c, a, st);
+      // f16 parts of four rows fill one column tile
+      if (rows <= 4) return launch_rows<KV, 1>(c, a, st);
+    }
+    return launch_rows<KV, 2>(c, a, st);
   });
 }
 

@@ -200,40 +200,4 @@ struct KvAttnArgs {
   int n_queries, n_heads, window, sinks;
 };
 
-// One warp per (query, head): the running maximum and sum of a softmax over
-// the visible keys in order, one key at a time.
-template <int KV>
-static __global__ void __launch_bounds__(128) k_kv_attn(const KvAttnArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (item >= (int64_t)a.n_queries * a.n_heads) return;
-  const int query = (int)(item / a.n_heads), h = (int)(item % a.n_heads);
-  const int head = h / (a.n_heads / a.c.n_kv_heads);
-  const int64_t p = a.pos + query;
-  const int64_t lo = a.window && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
-  const int64_t sinks = a.sinks < lo ? a.sinks : lo;
-  const float scale = __double2float_rn(1.0 / sqrt(128.0));
-  const float4 q = *reinterpret_cast<const float4*>(a.q + query * a.q_stride + h * KV_HD + 4 * lane);
-  float m = -INFINITY, l = 0.0f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int64_t i = 0; i < sinks + p - lo + 1; i++) {
-    const int64_t key = i < sinks ? i : lo + (i - sinks);
-    const float4 kx = kv_load4<KV, true>(a.c, key, head, lane);
-    float s = ffma(q.w, kx.w, ffma(q.z, kx.z, ffma(q.y, kx.y, fmul(q.x, kx.x))));
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) s = fadd(s, __shfl_xor_sync(0xffffffffu, s, d));
-    s = fmul(s, scale);
-    const float mn = fmaxf(m, s);
-    const float e = expf(fsub(s, mn)), f = expf(fsub(m, mn));
-    const float4 vx = kv_load4<KV, false>(a.c, key, head, lane);
-    o = make_float4(ffma(e, vx.x, fmul(f, o.x)), ffma(e, vx.y, fmul(f, o.y)),
-                    ffma(e, vx.z, fmul(f, o.z)), ffma(e, vx.w, fmul(f, o.w)));
-    l = ffma(f, l, e);
-    m = mn;
-  }
-  const float inv = fdiv(1.0f, l);
-  *reinterpret_cast<float4*>(a.out + query * a.out_stride + h * KV_HD + 4 * lane) =
-      make_float4(fmul(o.x, inv), fmul(o.y, inv), fmul(o.z, inv), fmul(o.w, inv));
-}
-
 }  // namespace flock

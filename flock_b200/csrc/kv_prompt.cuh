@@ -1,0 +1,669 @@
+// Attention of many query rows (a prompt chunk, a long draft) over a 4-bit or
+// e4m3 cache on the tcgen05 tensor cores, to f32 accuracy: k_kv_prompt.
+//
+// CTA (row tile of 128 (query, head) rows of a kv head, key split), looping
+// over 128-key tiles; per tile S = Q K^T and O += P V, f32 accumulators in
+// tensor memory.  Bound: the tensor cores' f16 rate times the products below,
+// with the softmax's instructions near it.
+//
+// f32 results from f16 operands.  q (scaled by a power of two per row) and the
+// softmax weights are hi + lo, two f16.  An e4m3 value is an f16 value: two
+// products (hi, lo times it).  A 4-bit value (code - 8) * scale has 15
+// significant bits: hi + lo again, three products (lo lo is below 2^-22).
+//
+// Roles, three warpgroups:
+//   warps 0-3  softmax; thread = row = tensor-memory lane, so a row's maximum
+//              and sum need no exchange.  Reads its 128 scores, writes the
+//              weights' hi and lo parts over them in tensor memory (the A
+//              operand of the second product is read from there).
+//   warps 4-7  widen the next K and V tiles from global memory into the
+//              128-byte-swizzled shared-memory operands (raw bytes are loaded
+//              into registers a tile ahead).  The order of dimensions (K: those
+//              q is given in; V: the output's columns) is whatever unpacks
+//              without shuffling, and is undone at the ends.
+//   warp 8     (9-11 idle) one thread issues the products: S(t+1) before O(t), so the
+//              softmax of a tile has two products' time, and K and V, one
+//              buffer each, are rewritten while the other is being read.
+//
+// The running maximum may lag by 2^8 before the outputs are rescaled (as in
+// k_kv_rows).  Every wait is bounded; a wait that runs out ends the CTA, which
+// then writes NaN.
+#pragma once
+#include "gemm_tc.cuh"
+#include "kv_rows.cuh"
+
+namespace flock {
+
+constexpr int KP_ROWS = 128;     // query rows per CTA
+constexpr int KP_KEYS = 128;     // keys per tile
+constexpr int KP_THREADS = 384;  // three warpgroups
+// Registers a thread: the softmax holds a row's 128 scores.  At launch 168 each
+// (384 threads fill the register file); 128 (240 + 128 + 40) of them are in use.
+constexpr int KP_REGS_SOFTMAX = 240, KP_REGS_WIDEN = 128, KP_REGS_ISSUE = 40;
+static_assert(KP_REGS_SOFTMAX + KP_REGS_WIDEN + KP_REGS_ISSUE <= 3 * 168, "within the launch's registers");
+constexpr int KP_OPND = 128 * 128 * 2;  // bytes of one 128 x 128 f16 operand
+
+struct KvPromptArgs {
+  KvAttnArgs a;
+  int rows, group;  // row r is query r / group, head r % group
+  int splits;
+  float* part;      // [item][split][128 rows][128], then [..][128 rows][2] (base, l)
+};
+
+// 16-byte chunk c (8 columns) of row r of a 128 x 128 operand: two 64-column
+// halves of swizzled 128-byte rows.
+FLOCK_DEV uint32_t kp_off(int r, int c) {
+  return (uint32_t)(c >> 3) * (128u * 128u) + sw128_off(r, c & 7);
+}
+// D (+)= A B^T over 128 K elements; A in tensor memory (a column holds two).
+FLOCK_DEV void kp_mma(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
+  const uint32_t idesc = umma_idesc_f16(128, 128);
+#pragma unroll
+  for (int k = 0; k < 8; k++) {
+    const uint32_t off = (uint32_t)(k >> 2) * (128u * 128u) + (uint32_t)(k & 3) * 32u;
+    const uint64_t desc = umma_desc_sw128(b + off);
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a + 8u * k), "l"(desc), "r"(idesc), "r"(accumulate || k > 0 ? 1u : 0u)
+        : "memory");
+  }
+}
+// 32 columns of this thread's lane; waits for them, so that no use can come before.
+FLOCK_DEV void kp_ld32(uint32_t t, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(t)
+      : "memory");
+}
+FLOCK_DEV void kp_st16(uint32_t t, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16};" ::"r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+      "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+FLOCK_DEV void kp_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+FLOCK_DEV void kp_bar(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// The head dimension of q's column pair word w (0-63), half h, in the K
+// operand's order; and of output column j (0-127), in V's.
+template <int KV>
+FLOCK_DEV constexpr int kp_kdim(int w, int h) {
+  if (KV != FLOCK_KV_Q4) return 2 * w + h;
+  // chunk w / 4 is word c of block b: nibbles at bits 0, 8, 4, 12 of both halfwords
+  const int b = w >> 4, c = (w >> 2) & 3, i = w & 3;
+  return 32 * b + 16 * (i >> 1) + 4 * c + (i & 1) + 2 * h;
+}
+template <int KV>
+FLOCK_DEV constexpr int kp_vcol(int d) {
+  if (KV != FLOCK_KV_Q4) return 8 * (d & 15) + (d >> 4);
+  const int b = d >> 5, hi = (d >> 4) & 1, n = (d & 15) >> 1, byte = d & 1;
+  return 32 * b + 8 * (2 * byte + hi) + n;
+}
+
+// Shared memory: the operands (K hi, V hi, then for 4-bit K lo, V lo), barriers.
+template <int KV>
+constexpr size_t KP_SMEM = (KV == FLOCK_KV_Q4 ? 4 : 2) * (size_t)KP_OPND + 1024;
+
+template <int KV>
+static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvPromptArgs p) {
+  constexpr bool Q4 = KV == FLOCK_KV_Q4;
+  extern __shared__ __align__(16) uint8_t kp_raw[];
+  __shared__ uint64_t s_bar[9];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_err;
+  __shared__ uint32_t s_dmax[2][4];   // converters: a warp's largest scale of K, V
+  __shared__ float s_kscale[4];       // K tile's factor back, by tile % 4
+  __shared__ int s_vexp[4];           // V tile's exponent
+  uint8_t* base = kp_raw + ((1024u - (smem_u32(kp_raw) & 1023u)) & 1023u);
+  uint8_t* sKh = base;
+  uint8_t* sVh = base + KP_OPND;
+  uint8_t* sKl = base + 2 * KP_OPND;
+  uint8_t* sVl = base + 3 * KP_OPND;
+  uint64_t *k_full = s_bar, *k_empty = s_bar + 1, *v_full = s_bar + 2, *v_empty = s_bar + 3,
+           *s_full = s_bar + 4 /* 2 */, *p_full = s_bar + 6, *q_full = s_bar + 7,
+           *drained = s_bar + 8;
+  const KvAttnArgs& a = p.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tile = blockIdx.x, z = blockIdx.y, head = blockIdx.z;
+  if (tid == 0) {
+    mbar_init(k_full, 128);
+    mbar_init(k_empty, 1);
+    mbar_init(v_full, 128);
+    mbar_init(v_empty, 1);
+    mbar_init(s_full, 1);
+    mbar_init(s_full + 1, 1);
+    mbar_init(p_full, 128);
+    mbar_init(q_full, 128);
+    mbar_init(drained, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_err = 0;
+  }
+  if (warp == 8) {
+    tmem_alloc(&s_tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();  // after the allocation: a later grid's cannot hold what this one needs
+  pdl_wait();
+  const uint32_t tmem = s_tmem, tS = tmem, tO = tmem + 256, tQ = tmem + 384;
+
+  // keys that some row of the tile sees: sinks [0, sk), then [lo, hi)
+  const int pos = (int)a.pos;
+  const int first_q = tile * KP_ROWS / p.group;
+  const int last_q = (min(p.rows, (tile + 1) * KP_ROWS) - 1) / p.group;
+  const int hi = pos + last_q + 1;
+  const int lo = a.window && pos + first_q + 1 > a.window ? pos + first_q + 1 - a.window : 0;
+  const int sk = min(a.sinks, lo);
+  const int sink_tiles = (sk + KP_KEYS - 1) / KP_KEYS;
+  const int lo16 = lo & ~15;
+  const int all = sink_tiles + (hi - lo16 + KP_KEYS - 1) / KP_KEYS;
+  const int t0 = (int)((int64_t)z * all / p.splits), t1 = (int)((int64_t)(z + 1) * all / p.splits);
+  const int n = t1 - t0;
+  auto key_of = [&](int t) {
+    return t0 + t < sink_tiles ? (t0 + t) * KP_KEYS : lo16 + (t0 + t - sink_tiles) * KP_KEYS;
+  };
+  auto fail = [&]() { *(volatile int*)&s_err = 1; };
+
+  if (warp < 4) {
+    // ============================================================== softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KP_REGS_SOFTMAX));
+    const uint32_t lanes = (uint32_t)(32 * warp) << 16;
+    const int row = tile * KP_ROWS + tid;
+    const bool live = row < p.rows;
+    const int query = min(row, p.rows - 1) / p.group;
+    const int row_hi = pos + query + 1;
+    const int row_lo = a.window && row_hi > a.window ? row_hi - a.window : 0;
+    const int row_sk = min(a.sinks, row_lo);
+    const int max_lo = a.window && pos + last_q + 1 > a.window ? pos + last_q + 1 - a.window : 0;
+    const int min_hi = pos + first_q + 1;
+    float unscale;
+    {  // q log2(e) / sqrt(128), the row's largest in [2^13, 2^14), hi and lo parts
+      const float* q = a.q + query * a.q_stride +
+                       ((int64_t)head * p.group + min(row, p.rows - 1) % p.group) * KV_HD;
+      const float k = __double2float_rn(1.4426950408889634 / sqrt(128.0));
+      float top = 0.0f;
+#pragma unroll 8
+      for (int i = 0; i < 32; i++) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(q) + i);
+        top = fmaxf(fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+      }
+      top = fmul(top, k);
+      const int biased = (int)(__float_as_uint(top) >> 23);
+      const int e = biased == 0 ? 0 : max(-100, min(100, biased - 127 - 13));
+      const float scale = live ? __uint_as_float((uint32_t)(127 - e) << 23) : 0.0f;
+      unscale = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+      for (int w0 = 0; w0 < 64; w0 += 16) {  // 32 dimensions: one block
+        float x[32];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float4 v = __ldg(reinterpret_cast<const float4*>(q) + w0 / 2 + i);
+          x[4 * i] = fmul(fmul(v.x, k), scale);
+          x[4 * i + 1] = fmul(fmul(v.y, k), scale);
+          x[4 * i + 2] = fmul(fmul(v.z, k), scale);
+          x[4 * i + 3] = fmul(fmul(v.w, k), scale);
+        }
+        uint32_t h[16], l[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+          split_f16(x[kp_kdim<KV>(w0 + i, 0) - 2 * w0], x[kp_kdim<KV>(w0 + i, 1) - 2 * w0], h[i], l[i]);
+        kp_st16(tQ + lanes + w0, h);
+        kp_st16(tQ + lanes + 64 + w0, l);
+      }
+      kp_st_wait();
+      tc_fence_before();
+      mbar_arrive(q_full);
+    }
+    float m = -INFINITY, base_ = 0.0f, l = 0.0f;
+    int vexp = -100;
+    bool ok = true;
+    for (int t = 0; t < n && ok; t++) {
+      const uint32_t S = tS + 128u * (t & 1) + lanes;
+      if (!mbar_wait(s_full + (t & 1), (t >> 1) & 1, &s_err)) {
+        fail();
+        ok = false;
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      float s[128];
+#pragma unroll
+      for (int i = 0; i < 4; i++) kp_ld32(S + 32 * i, s + 32 * i);
+      const float f = Q4 ? fmul(unscale, s_kscale[t & 3]) : unscale;
+      const int ve = Q4 ? s_vexp[t & 3] : 0;
+      const int key0 = key_of(t);
+      const bool sink = t0 + t < sink_tiles;
+      if (sink ? key0 + KP_KEYS > sk : key0 < max_lo || key0 + KP_KEYS > min_hi) {
+        // every row sees the tile's sinks; a row's own may reach into the main range
+        const int from = sink ? 0 : max(lo, row_lo), to = sink ? sk : row_hi;
+        const int also = sink ? 0 : row_sk;
+#pragma unroll
+        for (int i = 0; i < 128; i++) {
+          const int key = key0 + i;
+          if (!((key >= from && key < to) || (key >= lo && key < also))) s[i] = -INFINITY;
+        }
+      }
+      float t4[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int i = 4; i < 128; i++) t4[i & 3] = fmaxf(t4[i & 3], s[i]);
+      const float top = fmul(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])), f);
+      if (__any_sync(0xffffffffu, top > fadd(m, 8.0f) || ve > vexp)) {
+        const float mn = fmaxf(m, top);
+        const float nb = mn == -INFINITY ? 0.0f : fsub(mn, 6.0f);
+        const float g = m == -INFINITY ? 0.0f : exp2_approx(fsub(base_, nb));
+        const int ne = max(vexp, ve);
+        l = fmul(l, g);
+        if (t > 0) {
+          const float go = vexp < -90 ? 0.0f : fmul(g, pow2f(max(vexp - ne, -120)));
+          // the outputs so far: O(t-2) is complete with these scores, O(t-1) is waited
+          // for, and O(t) waits for this thread
+          if (!mbar_wait(v_empty, (t - 1) & 1, &s_err)) {
+            fail();
+            ok = false;
+          }
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          if (__any_sync(0xffffffffu, go != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              float o[32];
+              kp_ld32(tO + lanes + 32 * i, o);
+#pragma unroll
+              for (int j = 0; j < 32; j++) o[j] = fmul(o[j], go);
+              kp_st16(tO + lanes + 32 * i, reinterpret_cast<uint32_t*>(o));
+              kp_st16(tO + lanes + 32 * i + 16, reinterpret_cast<uint32_t*>(o) + 16);
+            }
+          }
+        }
+        m = mn;
+        base_ = nb;
+        vexp = ne;
+      }
+      // weights times the V tile's own power of two over the outputs'
+      const float shift = fsub((float)(ve - vexp), base_);
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; c++) {  // 32 keys
+        uint32_t h[16], w[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float p0 = exp2_approx(ffma(s[32 * c + 2 * i], f, shift));
+          const float p1 = exp2_approx(ffma(s[32 * c + 2 * i + 1], f, shift));
+          sum[i & 1] = fadd(sum[i & 1], p0);
+          sum[2 + (i & 1)] = fadd(sum[2 + (i & 1)], p1);
+          split_f16(p0, p1, h[i], w[i]);
+        }
+        kp_st16(S + 16 * c, h);
+        kp_st16(S + 64 + 16 * c, w);
+      }
+      l = ffma(fadd(fadd(sum[0], sum[1]), fadd(sum[2], sum[3])), pow2f(min(vexp - ve, 120)), l);
+      kp_st_wait();
+      tc_fence_before();
+      mbar_arrive(p_full);
+    }
+    // ------------------------------------------------------------ epilogue
+    // the last scores being there says that O(n-3) is complete: the two phases
+    // after it are waited for in turn (a parity alone tells neighbours apart)
+    for (int t = max(n - 2, 0); t < n; t++)
+      if (ok && !mbar_wait(v_empty, t & 1, &s_err)) {
+        fail();
+        ok = false;
+      }
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    float o[128];
+#pragma unroll
+    for (int i = 0; i < 128; i++) o[i] = 0.0f;
+    if (ok && n > 0) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) kp_ld32(tO + lanes + 32 * i, o + 32 * i);
+    }
+    if (live) {
+      const float back = ok ? (n > 0 ? pow2f(max(vexp, -120)) : 0.0f) : NAN;
+      float* dst;
+      float mul;
+      if (p.splits == 1) {
+        dst = a.out + query * a.out_stride + ((int64_t)head * p.group + row % p.group) * KV_HD;
+        mul = fmul(back, fdiv(1.0f, l));
+      } else {
+        const size_t at = (((size_t)head * gridDim.x + tile) * p.splits + z) * KP_ROWS + tid;
+        dst = p.part + at * KV_HD;
+        float* ml = p.part + (size_t)gridDim.z * gridDim.x * p.splits * KP_ROWS * KV_HD + at * 2;
+        ml[0] = l > 0.0f ? base_ : -INFINITY;
+        ml[1] = l;
+        mul = back;
+      }
+#pragma unroll
+      for (int d = 0; d < 128; d += 4)
+        *reinterpret_cast<float4*>(dst + d) =
+            make_float4(fmul(o[kp_vcol<KV>(d)], mul), fmul(o[kp_vcol<KV>(d + 1)], mul),
+                        fmul(o[kp_vcol<KV>(d + 2)], mul), fmul(o[kp_vcol<KV>(d + 3)], mul));
+    }
+  } else if (warp < 8) {
+    // =========================================================== converters
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_REGS_WIDEN));
+    const int w = tid - 128, cw = warp - 4;
+    const int kg = w >> 3, vn = w & 7;   // V: keys 8 kg .. 8 kg + 7, byte column vn
+    constexpr int KR = Q4 ? 4 : 8;       // 16-byte loads of a K row
+    uint4 kraw[KR];
+    uint2 kd = make_uint2(0, 0);
+    constexpr int VR = Q4 ? 4 : 8;       // 16 bytes each: two keys' 8 (4-bit), one key's 16
+    uint4 vraw[VR];
+    uint2 vd[8], vd_next[8];             // 4-bit: V scales of the thread's eight keys, this tile and the next
+    const size_t hb = Q4 ? q4_row(a.c, 0, head) * 64 : (size_t)head * 128;
+    const int64_t step = Q4 ? 64 : (int64_t)a.c.n_kv_heads * 128;
+    const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + hb;
+    const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + hb;
+    const uint16_t* ks = Q4 ? a.c.ks + q4_row(a.c, 0, head) * 4 : nullptr;
+    const uint16_t* vs = Q4 ? a.c.vs + q4_row(a.c, 0, head) * 4 : nullptr;
+    // keys outside [from, to) are zeros: what lies there cannot reach a product
+    auto range = [&](int t, int& from, int& to) {
+      const bool sink = t0 + t < sink_tiles;
+      from = sink ? 0 : lo;
+      to = sink ? sk : hi;
+    };
+    auto load_k = [&](int t) {
+      int from, to;
+      range(t, from, to);
+      const int key = key_of(t) + w;
+      const bool in = key >= from && key < to;
+#pragma unroll
+      for (int i = 0; i < KR; i++)
+        kraw[i] = in ? __ldg(reinterpret_cast<const uint4*>(kb + (int64_t)key * step) + i)
+                     : make_uint4(0, 0, 0, 0);
+      if (Q4) kd = in ? __ldg(reinterpret_cast<const uint2*>(ks) + key) : make_uint2(0, 0);
+    };
+    auto load_vd = [&](int t) {
+      if (!Q4) return;
+      int from, to;
+      range(t, from, to);
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int key = key_of(t) + 8 * kg + i;
+        vd_next[i] = key >= from && key < to ? __ldg(reinterpret_cast<const uint2*>(vs) + key)
+                                             : make_uint2(0, 0);
+      }
+    };
+    auto load_v = [&](int t) {
+      int from, to;
+      range(t, from, to);
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int key = key_of(t) + 8 * kg + i;
+        const bool in = key >= from && key < to;
+        if (Q4) {
+          const uint2 x = in ? __ldg(reinterpret_cast<const uint2*>(vb + (int64_t)key * 64) + vn)
+                             : make_uint2(0, 0);
+          if (i & 1) {
+            vraw[i >> 1].z = x.x;
+            vraw[i >> 1].w = x.y;
+          } else {
+            vraw[i >> 1].x = x.x;
+            vraw[i >> 1].y = x.y;
+          }
+        } else {
+          vraw[i & (VR - 1)] = in ? __ldg(reinterpret_cast<const uint4*>(vb + (int64_t)key * step) + vn)
+                                  : make_uint4(0, 0, 0, 0);
+        }
+      }
+    };
+    // A tile's scales times 2^e lie below 2^10, so a value (below 2^13) keeps
+    // its lo part; e as far as f16 can hold 2^e.
+    uint32_t knorm = 0, vnorm = 0;  // f16 pairs 2^e of the K and the V tile last looked at
+    auto norms = [&](int t) {
+      if (!Q4) return;
+      auto top = [](__half2 h, uint2 d) {
+        return __hmax2(h, __hmax2(__habs2(as_h2(d.x)), __habs2(as_h2(d.y))));
+      };
+      auto bits = [](__half2 h) { return (uint32_t)__half_as_ushort(__hmax(__low2half(h), __high2half(h))); };
+      const __half2 zero = __float2half2_rn(0.0f);
+      __half2 hv = zero;
+#pragma unroll
+      for (int i = 0; i < 8; i++) hv = top(hv, vd_next[i]);
+      const uint32_t bk = __reduce_max_sync(0xffffffffu, bits(top(zero, kd)));
+      const uint32_t bv = __reduce_max_sync(0xffffffffu, bits(hv));
+      if (lane == 0) {
+        s_dmax[0][cw] = bk;
+        s_dmax[1][cw] = bv;
+      }
+      kp_bar(1, 128);
+      uint32_t mk = 0, mv = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        mk = max(mk, s_dmax[0][i]);
+        mv = max(mv, s_dmax[1][i]);
+      }
+      kp_bar(1, 128);  // read before the next tile's are written
+      // magnitude below 2^(exponent field - 14)
+      const int ek = min(15, 10 - min((int)(mk >> 10) - 14, 16)), ev = min(15, 10 - min((int)(mv >> 10) - 14, 16));
+      // f16 pair 2^e: e in -6 .. 15
+      knorm = (uint32_t)(ek + 15) * 0x04000400u;
+      vnorm = (uint32_t)(ev + 15) * 0x04000400u;
+      if (w == 0) {
+        s_kscale[t & 3] = pow2f(-ek);
+        s_vexp[t & 3] = -ev;
+      }
+    };
+    auto put_k = [&]() {
+      if (Q4) {
+        const uint32_t d01 = hmul2_u(kd.x, knorm), d23 = hmul2_u(kd.y, knorm);
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+          const uint32_t d = __byte_perm(b < 2 ? d01 : d23, 0, b & 1 ? 0x3232 : 0x1010);
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            uint32_t v[4], h[4], l[4];
+            nib_f16(word_of(kraw[c], b), v);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              h[i] = hmul2_u(v[i], d);
+              l[i] = hfma2_u(v[i], d, hneg2_u(h[i]));
+            }
+            const uint32_t off = kp_off(w, 4 * b + c);
+            *reinterpret_cast<uint4*>(sKh + off) = make_uint4(h[0], h[2], h[1], h[3]);
+            *reinterpret_cast<uint4*>(sKl + off) = make_uint4(l[0], l[2], l[1], l[3]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < KR; i++) {
+          uint32_t v[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) v[j] = fp8_f16(word_of(kraw[i], j >> 1) >> (16 * (j & 1)));
+          *reinterpret_cast<uint4*>(sKh + kp_off(w, 2 * i)) = make_uint4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<uint4*>(sKh + kp_off(w, 2 * i + 1)) = make_uint4(v[4], v[5], v[6], v[7]);
+        }
+      }
+    };
+    auto put_v = [&](uint32_t norm) {
+      if (Q4) {
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+          const uint32_t sel = b & 1 ? 0x7632u : 0x5410u;
+          uint32_t h[4][4], l[4][4];  // [nibble][key pair]
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t x = b < 2 ? vraw[i].x : vraw[i].y, y = b < 2 ? vraw[i].z : vraw[i].w;
+            uint32_t v[4];
+            nib_f16(__byte_perm(x, y, sel), v);
+            const uint32_t d = hmul2_u(
+                __byte_perm(b < 2 ? vd[2 * i].x : vd[2 * i].y, b < 2 ? vd[2 * i + 1].x : vd[2 * i + 1].y, sel),
+                norm);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              h[e][i] = hmul2_u(v[e], d);
+              l[e][i] = hfma2_u(v[e], d, hneg2_u(h[e][i]));
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const uint32_t off = kp_off(32 * b + 8 * e + vn, kg);
+            *reinterpret_cast<uint4*>(sVh + off) = make_uint4(h[e][0], h[e][1], h[e][2], h[e][3]);
+            *reinterpret_cast<uint4*>(sVl + off) = make_uint4(l[e][0], l[e][1], l[e][2], l[e][3]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {  // dimensions 16 vn + 2 j, + 1
+          uint32_t x[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++) x[i] = fp8_f16(word_of(vraw[i & (VR - 1)], j >> 1) >> (16 * (j & 1)));
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const uint32_t sel = h ? 0x7632u : 0x5410u;
+            *reinterpret_cast<uint4*>(sVh + kp_off(8 * (2 * j + h) + vn, kg)) =
+                make_uint4(__byte_perm(x[0], x[1], sel), __byte_perm(x[2], x[3], sel),
+                           __byte_perm(x[4], x[5], sel), __byte_perm(x[6], x[7], sel));
+          }
+        }
+      }
+    };
+    bool ok = true;
+    auto wait = [&](uint64_t* b, uint32_t parity) {
+      if (ok && !mbar_wait(b, parity, &s_err)) {
+        fail();
+        ok = false;
+      }
+    };
+    // K(t + 1), then V(t); raw bytes are loaded as soon as the last tile's are
+    // used up.  A failed wait skips the writes but keeps the barriers' counts.
+    uint32_t vnorm_t = 0;  // of the V tile in hand
+    auto next_scales = [&]() {
+      vnorm_t = vnorm;
+      if (Q4) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) vd[i] = vd_next[i];
+      }
+    };
+    auto k_tile = [&](int t) {
+      norms(t);
+      if (t > 0) wait(k_empty, (t - 1) & 1);
+      if (ok) put_k();
+      fence_proxy_async_smem();
+      mbar_arrive(k_full);
+      if (t + 1 < n) load_k(t + 1);
+    };
+    if (n > 0) {
+      load_k(0);
+      load_vd(0);
+      load_v(0);
+      k_tile(0);
+      next_scales();
+      if (n > 1) load_vd(1);
+    }
+    for (int t = 0; t < n; t++) {
+      if (t + 1 < n) k_tile(t + 1);
+      if (t > 0) wait(v_empty, (t - 1) & 1);
+      if (ok) put_v(vnorm_t);
+      fence_proxy_async_smem();
+      mbar_arrive(v_full);
+      if (t + 1 < n) {
+        next_scales();
+        load_v(t + 1);
+        if (t + 2 < n) load_vd(t + 2);
+      }
+    }
+  } else {
+    // ============================================================= products
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_REGS_ISSUE));
+    if (warp == 8 && lane == 0) {
+      bool ok = true;
+      auto wait = [&](uint64_t* b, uint32_t parity) {
+        if (ok && !mbar_wait(b, parity, &s_err)) {
+          fail();
+          ok = false;
+        }
+      };
+      auto scores = [&](int t) {
+        wait(k_full, t & 1);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t d = tS + 128u * (t & 1);
+        kp_mma(d, tQ, smem_u32(sKh), false);
+        kp_mma(d, tQ + 64, smem_u32(sKh), true);
+        if (Q4) kp_mma(d, tQ, smem_u32(sKl), true);
+        umma_commit(k_empty);
+        umma_commit(s_full + (t & 1));
+      };
+      if (n > 0) {
+        wait(q_full, 0);
+        tc_fence_after();
+        scores(0);
+      }
+      for (int t = 0; t < n && ok; t++) {
+        if (t + 1 < n) scores(t + 1);
+        wait(p_full, t & 1);
+        wait(v_full, t & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t P = tS + 128u * (t & 1);
+        kp_mma(tO, P, smem_u32(sVh), t > 0);
+        kp_mma(tO, P + 64, smem_u32(sVh), true);
+        if (Q4) kp_mma(tO, P, smem_u32(sVl), true);
+        umma_commit(v_empty);
+      }
+      if (!ok) {  // let what was issued finish before the memory is given back
+        umma_commit(drained);
+        mbar_wait(drained, 0, &s_err, false);
+      }
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// The rows of one tile from its splits, in order: a warp per row, four
+// outputs a lane.
+static __global__ void __launch_bounds__(256) k_kv_prompt_join(const KvPromptArgs p, int tiles) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), head = blockIdx.y;
+  if (row >= p.rows) return;
+  const int tile = row / KP_ROWS, r = row % KP_ROWS;
+  const size_t first = ((size_t)head * tiles + tile) * p.splits * KP_ROWS + r;
+  const float* ml = p.part + (size_t)gridDim.y * tiles * p.splits * KP_ROWS * KV_HD;
+  float m = -INFINITY;
+  for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, __ldcg(ml + (first + (size_t)s * KP_ROWS) * 2));
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.0f;
+#pragma unroll 4
+  for (int s = 0; s < p.splits; s++) {
+    const size_t at = first + (size_t)s * KP_ROWS;
+    const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part + at * KV_HD) + lane);
+    const float2 b = __ldcg(reinterpret_cast<const float2*>(ml) + at);
+    const float f = exp2_approx(fsub(b.x, m));
+    o = make_float4(ffma(f, x.x, o.x), ffma(f, x.y, o.y), ffma(f, x.z, o.z), ffma(f, x.w, o.w));
+    l = ffma(f, b.y, l);
+  }
+  const float inv = fdiv(1.0f, l);
+  const KvAttnArgs& a = p.a;
+  *reinterpret_cast<float4*>(a.out + (row / p.group) * a.out_stride +
+                             ((int64_t)head * p.group + row % p.group) * KV_HD + 4 * lane) =
+      make_float4(fmul(o.x, inv), fmul(o.y, inv), fmul(o.z, inv), fmul(o.w, inv));
+}
+
+}  // namespace flock
