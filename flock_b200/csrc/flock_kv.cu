@@ -342,7 +342,6 @@ int flock_kv_attention(flock_kv* c, const float* q, int64_t q_stride, int n_head
   a.n_heads = n_heads;
   a.window = window;
   a.sinks = sinks;
-  const unsigned grid = (unsigned)(((int64_t)n_queries * n_heads + 3) / 4);
   const int64_t rows = (int64_t)n_queries * (n_heads / c->view.n_kv_heads);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return by_dtype(c->kv_dtype, [&](auto kv) -> int {

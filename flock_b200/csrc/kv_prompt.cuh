@@ -11,19 +11,21 @@
 // products (hi, lo times it).  A 4-bit value (code - 8) * scale has 15
 // significant bits: hi + lo again, three products (lo lo is below 2^-22).
 //
-// Roles, three warpgroups:
-//   warps 0-3  softmax; thread = row = tensor-memory lane, so a row's maximum
-//              and sum need no exchange.  Reads its 128 scores, writes the
-//              weights' hi and lo parts over them in tensor memory (the A
-//              operand of the second product is read from there).
-//   warps 4-7  widen the next K and V tiles from global memory into the
-//              128-byte-swizzled shared-memory operands (raw bytes are loaded
-//              into registers a tile ahead).  The order of dimensions (K: those
-//              q is given in; V: the output's columns) is whatever unpacks
-//              without shuffling, and is undone at the ends.
-//   warp 8     (9-11 idle) one thread issues the products: S(t+1) before O(t), so the
-//              softmax of a tile has two products' time, and K and V, one
-//              buffer each, are rewritten while the other is being read.
+// Roles, sixteen warps of 128 registers:
+//   warps 0-7   softmax; thread = row = tensor-memory lane, warps 0-3 the
+//               first 64 of its 128 scores, 4-7 the others (one thread a row
+//               took 6500 cycles a tile, its 128 scores' chains alone on a
+//               scheduler).  They agree on the row's maximum in shared memory,
+//               and write the weights' hi and lo parts over the scores in
+//               tensor memory (the second product's A operand is read there).
+//   warps 8-11  widen the next K and V tiles from global memory into the
+//               128-byte-swizzled shared-memory operands (raw bytes are loaded
+//               into registers a tile ahead).  The order of dimensions (K: those
+//               q is given in; V: the output's columns) is whatever unpacks
+//               without shuffling, and is undone at the ends.
+//   warp 12     one thread issues the products: S(t+1) before O(t), so the
+//               softmax of a tile has two products' time, and K and V, one
+//               buffer each, are rewritten while the other is being read.
 //
 // The running maximum may lag by 2^8 before the outputs are rescaled (as in
 // k_kv_rows).  Every wait is bounded; a wait that runs out ends the CTA, which
@@ -36,11 +38,7 @@ namespace flock {
 
 constexpr int KP_ROWS = 128;     // query rows per CTA
 constexpr int KP_KEYS = 128;     // keys per tile
-constexpr int KP_THREADS = 384;  // three warpgroups
-// Registers a thread: the softmax holds a row's 128 scores.  At launch 168 each
-// (384 threads fill the register file); 128 (240 + 128 + 40) of them are in use.
-constexpr int KP_REGS_SOFTMAX = 240, KP_REGS_WIDEN = 128, KP_REGS_ISSUE = 40;
-static_assert(KP_REGS_SOFTMAX + KP_REGS_WIDEN + KP_REGS_ISSUE <= 3 * 168, "within the launch's registers");
+constexpr int KP_THREADS = 512;
 constexpr int KP_OPND = 128 * 128 * 2;  // bytes of one 128 x 128 f16 operand
 
 struct KvPromptArgs {
@@ -124,7 +122,8 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
   extern __shared__ __align__(16) uint8_t kp_raw[];
   __shared__ uint64_t s_bar[9];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_err;
+  __shared__ int s_err, s_ok[2];
+  __shared__ float s_top[2][2][128];  // a row's maximum over either half, by tile parity
   __shared__ uint32_t s_dmax[2][4];   // converters: a warp's largest scale of K, V
   __shared__ float s_kscale[4];       // K tile's factor back, by tile % 4
   __shared__ int s_vexp[4];           // V tile's exponent
@@ -146,13 +145,13 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
     mbar_init(v_empty, 1);
     mbar_init(s_full, 1);
     mbar_init(s_full + 1, 1);
-    mbar_init(p_full, 128);
-    mbar_init(q_full, 128);
+    mbar_init(p_full, 256);
+    mbar_init(q_full, 256);
     mbar_init(drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_err = 0;
   }
-  if (warp == 8) {
+  if (warp == 12) {
     tmem_alloc(&s_tmem, 512);
     tmem_relinquish();
   }
@@ -180,11 +179,11 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
   };
   auto fail = [&]() { *(volatile int*)&s_err = 1; };
 
-  if (warp < 4) {
+  if (warp < 8) {
     // ============================================================== softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KP_REGS_SOFTMAX));
-    const uint32_t lanes = (uint32_t)(32 * warp) << 16;
-    const int row = tile * KP_ROWS + tid;
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+    const int half = warp >> 2, r = tid & 127;  // scores (then output columns) 64 half ..
+    const int row = tile * KP_ROWS + r;
     const bool live = row < p.rows;
     const int query = min(row, p.rows - 1) / p.group;
     const int row_hi = pos + query + 1;
@@ -209,7 +208,8 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       const float scale = live ? __uint_as_float((uint32_t)(127 - e) << 23) : 0.0f;
       unscale = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
-      for (int w0 = 0; w0 < 64; w0 += 16) {  // 32 dimensions: one block
+      for (int b = 0; b < 2; b++) {  // 32 dimensions: one block
+        const int w0 = 32 * half + 16 * b;
         float x[32];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -221,8 +221,8 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         }
         uint32_t h[16], l[16];
 #pragma unroll
-        for (int i = 0; i < 16; i++)
-          split_f16(x[kp_kdim<KV>(w0 + i, 0) - 2 * w0], x[kp_kdim<KV>(w0 + i, 1) - 2 * w0], h[i], l[i]);
+        for (int i = 0; i < 16; i++)  // every block's order is the first one's
+          split_f16(x[kp_kdim<KV>(i, 0)], x[kp_kdim<KV>(i, 1)], h[i], l[i]);
         kp_st16(tQ + lanes + w0, h);
         kp_st16(tQ + lanes + 64 + w0, l);
       }
@@ -235,16 +235,11 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
     bool ok = true;
     for (int t = 0; t < n && ok; t++) {
       const uint32_t S = tS + 128u * (t & 1) + lanes;
-      if (!mbar_wait(s_full + (t & 1), (t >> 1) & 1, &s_err)) {
-        fail();
-        ok = false;
-      }
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+      if (!mbar_wait(s_full + (t & 1), (t >> 1) & 1, &s_err)) fail();
       tc_fence_after();
-      float s[128];
+      float s[64];
 #pragma unroll
-      for (int i = 0; i < 4; i++) kp_ld32(S + 32 * i, s + 32 * i);
+      for (int i = 0; i < 2; i++) kp_ld32(S + 64 * half + 32 * i, s + 32 * i);
       const float f = Q4 ? fmul(unscale, s_kscale[t & 3]) : unscale;
       const int ve = Q4 ? s_vexp[t & 3] : 0;
       const int key0 = key_of(t);
@@ -254,15 +249,22 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         const int from = sink ? 0 : max(lo, row_lo), to = sink ? sk : row_hi;
         const int also = sink ? 0 : row_sk;
 #pragma unroll
-        for (int i = 0; i < 128; i++) {
-          const int key = key0 + i;
+        for (int i = 0; i < 64; i++) {
+          const int key = key0 + 64 * half + i;
           if (!((key >= from && key < to) || (key >= lo && key < also))) s[i] = -INFINITY;
         }
       }
       float t4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int i = 4; i < 128; i++) t4[i & 3] = fmaxf(t4[i & 3], s[i]);
-      const float top = fmul(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])), f);
+      for (int i = 4; i < 64; i++) t4[i & 3] = fmaxf(t4[i & 3], s[i]);
+      float top = fmul(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])), f);
+      // the other half's; behind this barrier both halves have left the scores'
+      // columns, which the weights overwrite
+      s_top[t & 1][half][r] = top;
+      if (tid == 0) s_ok[t & 1] = *(volatile int*)&s_err == 0;
+      kp_bar(2, 256);
+      ok = s_ok[t & 1];  // one thread's look, so that all leave the loop together
+      top = fmaxf(top, s_top[t & 1][half ^ 1][r]);
       if (__any_sync(0xffffffffu, top > fadd(m, 8.0f) || ve > vexp)) {
         const float mn = fmaxf(m, top);
         const float nb = mn == -INFINITY ? 0.0f : fsub(mn, 6.0f);
@@ -270,25 +272,21 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         const int ne = max(vexp, ve);
         l = fmul(l, g);
         if (t > 0) {
-          const float go = vexp < -90 ? 0.0f : fmul(g, pow2f(max(vexp - ne, -120)));
+          const float go = fmul(g, pow2f(max(vexp - ne, -120)));
           // the outputs so far: O(t-2) is complete with these scores, O(t-1) is waited
           // for, and O(t) waits for this thread
-          if (!mbar_wait(v_empty, (t - 1) & 1, &s_err)) {
-            fail();
-            ok = false;
-          }
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
+          if (ok && !mbar_wait(v_empty, (t - 1) & 1, &s_err)) fail();
           tc_fence_after();
           if (__any_sync(0xffffffffu, go != 1.0f)) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < 2; i++) {
+              const uint32_t at = tO + lanes + 64 * half + 32 * i;
               float o[32];
-              kp_ld32(tO + lanes + 32 * i, o);
+              kp_ld32(at, o);
 #pragma unroll
               for (int j = 0; j < 32; j++) o[j] = fmul(o[j], go);
-              kp_st16(tO + lanes + 32 * i, reinterpret_cast<uint32_t*>(o));
-              kp_st16(tO + lanes + 32 * i + 16, reinterpret_cast<uint32_t*>(o) + 16);
+              kp_st16(at, reinterpret_cast<uint32_t*>(o));
+              kp_st16(at + 16, reinterpret_cast<uint32_t*>(o) + 16);
             }
           }
         }
@@ -300,7 +298,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       const float shift = fsub((float)(ve - vexp), base_);
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < 4; c++) {  // 32 keys
+      for (int c = 0; c < 2; c++) {  // 32 keys
         uint32_t h[16], w[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) {
@@ -310,8 +308,8 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
           sum[2 + (i & 1)] = fadd(sum[2 + (i & 1)], p1);
           split_f16(p0, p1, h[i], w[i]);
         }
-        kp_st16(S + 16 * c, h);
-        kp_st16(S + 64 + 16 * c, w);
+        kp_st16(S + 32 * half + 16 * c, h);
+        kp_st16(S + 64 + 32 * half + 16 * c, w);
       }
       l = ffma(fadd(fadd(sum[0], sum[1]), fadd(sum[2], sum[3])), pow2f(min(vexp - ve, 120)), l);
       kp_st_wait();
@@ -322,18 +320,19 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
     // the last scores being there says that O(n-3) is complete: the two phases
     // after it are waited for in turn (a parity alone tells neighbours apart)
     for (int t = max(n - 2, 0); t < n; t++)
-      if (ok && !mbar_wait(v_empty, t & 1, &s_err)) {
-        fail();
-        ok = false;
-      }
-    ok = __all_sync(0xffffffffu, ok);
+      if (ok && !mbar_wait(v_empty, t & 1, &s_err)) fail();
+    kp_bar(2, 256);  // s_top is read, every wait decided
+    s_top[0][half][r] = l;
+    kp_bar(2, 256);
+    ok = *(volatile int*)&s_err == 0;
+    l = fadd(s_top[0][0][r], s_top[0][1][r]);
     tc_fence_after();
-    float o[128];
+    float o[64];
 #pragma unroll
-    for (int i = 0; i < 128; i++) o[i] = 0.0f;
+    for (int i = 0; i < 64; i++) o[i] = 0.0f;
     if (ok && n > 0) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) kp_ld32(tO + lanes + 32 * i, o + 32 * i);
+      for (int i = 0; i < 2; i++) kp_ld32(tO + lanes + 64 * half + 32 * i, o + 32 * i);
     }
     if (live) {
       const float back = ok ? (n > 0 ? pow2f(max(vexp, -120)) : 0.0f) : NAN;
@@ -343,23 +342,27 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         dst = a.out + query * a.out_stride + ((int64_t)head * p.group + row % p.group) * KV_HD;
         mul = fmul(back, fdiv(1.0f, l));
       } else {
-        const size_t at = (((size_t)head * gridDim.x + tile) * p.splits + z) * KP_ROWS + tid;
+        const size_t at = (((size_t)head * gridDim.x + tile) * p.splits + z) * KP_ROWS + r;
         dst = p.part + at * KV_HD;
-        float* ml = p.part + (size_t)gridDim.z * gridDim.x * p.splits * KP_ROWS * KV_HD + at * 2;
-        ml[0] = l > 0.0f ? base_ : -INFINITY;
-        ml[1] = l;
+        if (half == 0) {
+          float* ml = p.part + (size_t)gridDim.z * gridDim.x * p.splits * KP_ROWS * KV_HD + at * 2;
+          ml[0] = l > 0.0f ? base_ : -INFINITY;
+          ml[1] = l;
+        }
         mul = back;
       }
+      // columns 64 half .. hold the dimensions 64 half .. (4-bit), 16 i + 8 half .. (e4m3)
 #pragma unroll
-      for (int d = 0; d < 128; d += 4)
-        *reinterpret_cast<float4*>(dst + d) =
+      for (int i = 0; i < 16; i++) {
+        const int d = Q4 ? 4 * i : 16 * (i >> 1) + 4 * (i & 1);
+        *reinterpret_cast<float4*>(dst + (Q4 ? 64 : 8) * half + d) =
             make_float4(fmul(o[kp_vcol<KV>(d)], mul), fmul(o[kp_vcol<KV>(d + 1)], mul),
                         fmul(o[kp_vcol<KV>(d + 2)], mul), fmul(o[kp_vcol<KV>(d + 3)], mul));
+      }
     }
-  } else if (warp < 8) {
+  } else if (warp < 12) {
     // =========================================================== converters
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_REGS_WIDEN));
-    const int w = tid - 128, cw = warp - 4;
+    const int w = tid - 256, cw = warp - 8;
     const int kg = w >> 3, vn = w & 7;   // V: keys 8 kg .. 8 kg + 7, byte column vn
     constexpr int KR = Q4 ? 4 : 8;       // 16-byte loads of a K row
     uint4 kraw[KR];
@@ -582,8 +585,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
     }
   } else {
     // ============================================================= products
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_REGS_ISSUE));
-    if (warp == 8 && lane == 0) {
+    if (warp == 12 && lane == 0) {
       bool ok = true;
       auto wait = [&](uint64_t* b, uint32_t parity) {
         if (ok && !mbar_wait(b, parity, &s_err)) {
@@ -628,7 +630,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 12) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
