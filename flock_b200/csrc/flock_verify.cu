@@ -13,9 +13,6 @@ namespace {
 constexpr int64_t VERIFY_MAX_VOCAB = 4194304;
 constexpr int64_t VERIFY_MAX_PARTIALS = FLOCK_WORKSPACE_BYTES / 8;
 
-// Vocabulary per CTA whose two rows of f64 exponentials fit its shared memory.
-constexpr int VP_CACHE_MAX = 200 * 1024 / 16;
-
 struct OnDevice {
   int before = -1, want;
   explicit OnDevice(int ordinal) : want(ordinal) {}
@@ -29,16 +26,21 @@ struct OnDevice {
   }
 };
 
-template <bool CACHED>
-int launch_pick(cudaStream_t st, const VerifyArgs& a, int cluster, int L, size_t smem) {
-  auto k = k_verify_pick<CACHED>;
-  FLOCK_TRY(kernel_setup((const void*)k, CACHED ? VP_CACHE_MAX * 16 : 0));
-  if (cluster > 8)
-    FLOCK_CK(cudaFuncSetAttribute((const void*)k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+template <bool KEEP>
+int launch_pick(cudaStream_t st, const VerifyArgs& a, int cluster, int span) {
+  auto k = k_verify_pick<KEEP>;
+  if (cluster > 8) {  // past the portable size: asked for once per device
+    static std::atomic<uint64_t> allowed{0};
+    int dev = 0;
+    FLOCK_CK(cudaGetDevice(&dev));
+    if (!(allowed.load() >> (dev & 63) & 1)) {
+      FLOCK_CK(cudaFuncSetAttribute((const void*)k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+      allowed.fetch_or((uint64_t)1 << (dev & 63));
+    }
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.n_seqs * cluster);
   cfg.blockDim = dim3(VP_THREADS);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -49,7 +51,7 @@ int launch_pick(cudaStream_t st, const VerifyArgs& a, int cluster, int L, size_t
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  FLOCK_CK(cudaLaunchKernelEx(&cfg, k, a, L));
+  FLOCK_CK(cudaLaunchKernelEx(&cfg, k, a, span));
   return FLOCK_OK;
 }
 
@@ -72,7 +74,7 @@ int flock_verify_draft(flock_dev* dev, const float* target, int64_t target_strid
     return FLOCK_E_LIMIT;
   }
   if (!(temperature >= 0.0) || !std::isfinite(temperature) ||
-      (temperature > 0.0 && !std::isfinite(1.0 / temperature))) {
+      (temperature > 0.0 && !std::isfinite(32.0 / temperature))) {
     set_error("verify_draft: temperature %g must be finite and not negative (0: greedy)",
               temperature);
     return FLOCK_E_ARG;
@@ -140,9 +142,11 @@ int flock_verify_draft(flock_dev* dev, const float* target, int64_t target_strid
   // CTAs per sequence: about a thousand tokens each, as many as a cluster may have
   int cluster = 1;
   while (cluster < VP_MAX_CLUSTER && (int64_t)cluster * 1024 < vocab) cluster *= 2;
-  const int L = (int)((vocab + cluster - 1) / cluster);
-  if (L <= VP_CACHE_MAX) return launch_pick<true>(st, a, cluster, L, (size_t)L * 16);
-  return launch_pick<false>(st, a, cluster, L, 0);
+  // each warp's span of the vocabulary, in whole groups of four
+  const int64_t warps = (int64_t)cluster * (VP_THREADS / 32);
+  const int span = (int)(((vocab + warps - 1) / warps + 3) / 4 * 4);
+  return span <= 128 * VP_KEPT ? launch_pick<true>(st, a, cluster, span)
+                               : launch_pick<false>(st, a, cluster, span);
 }
 
 }  // extern "C"

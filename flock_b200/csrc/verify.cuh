@@ -90,23 +90,29 @@ static __global__ void __launch_bounds__(VS_THREADS) k_verify_stats(const Verify
   const float k = (float)(a.inv_t * 1.4426950408889634);
   float m = -INFINITY, s = 0.0f;
   unsigned long long key = 0;
-  constexpr int B = 4;  // 16-byte loads in flight per thread
-  for (int i0 = c0 + 4 * threadIdx.x; i0 < c1; i0 += 4 * B * VS_THREADS) {
-    float v[4 * B];
+  constexpr int B = 4;  // 16-byte loads of a pass; the next pass's are in flight meanwhile
+  float v[4 * B], next[4 * B];
+  auto load = [&](int i0) {
 #pragma unroll
     for (int b = 0; b < B; b++) {
       const int i = i0 + 4 * b * VS_THREADS;
       if (a.vec && i + 4 <= c1) {
         const uint4 w = ldg_stream(x + i);
-        v[4 * b] = __uint_as_float(w.x);
-        v[4 * b + 1] = __uint_as_float(w.y);
-        v[4 * b + 2] = __uint_as_float(w.z);
-        v[4 * b + 3] = __uint_as_float(w.w);
+        next[4 * b] = __uint_as_float(w.x);
+        next[4 * b + 1] = __uint_as_float(w.y);
+        next[4 * b + 2] = __uint_as_float(w.z);
+        next[4 * b + 3] = __uint_as_float(w.w);
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++) v[4 * b + j] = i + j < c1 ? __ldg(x + i + j) : -INFINITY;
+        for (int j = 0; j < 4; j++) next[4 * b + j] = i + j < c1 ? __ldg(x + i + j) : -INFINITY;
       }
     }
+  };
+  load(c0 + 4 * threadIdx.x);
+  for (int i0 = c0 + 4 * threadIdx.x; i0 < c1; i0 += 4 * B * VS_THREADS) {
+#pragma unroll
+    for (int j = 0; j < 4 * B; j++) v[j] = next[j];
+    if (i0 + 4 * B * VS_THREADS < c1) load(i0 + 4 * B * VS_THREADS);
     if (GREEDY) {
 #pragma unroll
       for (int j = 0; j < 4 * B; j++) {
@@ -122,8 +128,11 @@ static __global__ void __launch_bounds__(VS_THREADS) k_verify_stats(const Verify
       for (int j = 0; j < 4 * B; j++) mn = fmaxf(mn, v[j]);
       const float base = mn == -INFINITY ? 0.0f : mn;
       s = fmul(s, ex2(fmul(fsub(m, base), k)));
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 4 * B; j++) s = fadd(s, ex2(fmul(fsub(v[j], base), k)));
+      for (int j = 0; j < 4 * B; j++)
+        part[j & 3] = fadd(part[j & 3], ex2(fmul(fsub(v[j], base), k)));
+      s = fadd(s, fadd(fadd(part[0], part[1]), fadd(part[2], part[3])));
       m = mn;
     }
   }
@@ -171,58 +180,95 @@ FLOCK_DEV void verify_join(const VerifyArgs& a, size_t row, float& m, double& s)
   const int lane = threadIdx.x & 31;
   const float* pm = a.part_m + row * a.chunks;
   const float* ps = a.part_s + row * a.chunks;
-  m = -INFINITY;
-  for (int c = lane; c < a.chunks; c += 32) m = fmaxf(m, pm[c]);
+  // at most 64 chunks: two a lane, all loads in flight together
+  float cm[2], cs[2];
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const int c = lane + 32 * h;
+    cm[h] = c < a.chunks ? pm[c] : -INFINITY;
+    cs[h] = c < a.chunks ? ps[c] : 0.0f;
+  }
+  m = fmaxf(cm[0], cm[1]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
   s = 0.0;
-  for (int c = lane; c < a.chunks; c += 32)  // a chunk of -inf has the sum 0
-    s += pm[c] == -INFINITY ? (double)ps[c]
-                            : exp(((double)pm[c] - (double)m) * a.inv_t) * (double)ps[c];
+#pragma unroll
+  for (int h = 0; h < 2; h++)  // a chunk of -inf has the sum 0
+    s += cm[h] == -INFINITY ? (double)cs[h]
+                            : exp(((double)cm[h] - (double)m) * a.inv_t) * (double)cs[h];
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
 }
 
-// Inclusive sums of one value per thread over the block (VP_THREADS), f64;
-// returns the thread's exclusive sum and the block's total.
-FLOCK_DEV double verify_scan(double v, double* red, double& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  double s = v;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const double o = __shfl_up_sync(0xffffffffu, s, d);
-    if (lane >= d) s += o;
-  }
-  __syncthreads();
-  if (lane == 31) red[warp] = s;
-  __syncthreads();
-  double before = 0.0;
-  total = 0.0;
-  for (int w = 0; w < VP_THREADS / 32; w++) {
-    if (w == warp) before = total;
-    total += red[w];
-  }
-  // the exclusive sum of a thread is the inclusive sum of the one before it
-  const double prev = __shfl_up_sync(0xffffffffu, s, 1);
-  return lane == 0 ? before : before + prev;
+// e^((x - m) / T) for x <= m in f64, c = 16 / (T ln 2): e^z = 2^(n / 16) 2^(r /
+// 16), n the integer nearest 16 z / ln 2 and |r| <= 1/2, 2^(r / 16) by the
+// Taylor polynomial of e^(r ln 2 / 16) of degree 6 (remainder below 5e-16 of
+// it), 2^(j / 16) from a table.  Relative error below 1e-15 for z > -40,
+// growing as |z| 2e-17.  Logits not above `lowest` (m - 700 T, -inf) give 0.
+__constant__ static const double k_pow16[16] = {
+    0x1.0000000000000p+0, 0x1.0b5586cf9890fp+0, 0x1.172b83c7d517bp+0, 0x1.2387a6e756238p+0,
+    0x1.306fe0a31b715p+0, 0x1.3dea64c123422p+0, 0x1.4bfdad5362a27p+0, 0x1.5ab07dd485429p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.7a11473eb0187p+0, 0x1.8ace5422aa0dbp+0, 0x1.9c49182a3f090p+0,
+    0x1.ae89f995ad3adp+0, 0x1.c199bdd85529cp+0, 0x1.d5818dcfba487p+0, 0x1.ea4afa2a490dap+0};
+struct VerifyRow {
+  double m, c;
+  float lowest;
+};
+FLOCK_DEV VerifyRow verify_row_of(float m, double inv_t) {
+  return {(double)m, inv_t * 0x1.71547652b82fep+4, (float)((double)m - 700.0 / inv_t)};
+}
+FLOCK_DEV double verify_exp(float x, const VerifyRow& row, const double* pow16) {
+  const double magic = 6755399441055744.0;  // 1.5 2^52: adding it rounds to an integer
+  const double d = (double)x - row.m;
+  const double t = fma(d, row.c, magic);
+  const double r = fma(d, row.c, magic - t);
+  double p = 0x1.430912f86c787p-37;  // (ln 2 / 16)^k / k!
+  p = fma(p, r, 0x1.5d87fe78a6731p-30);
+  p = fma(p, r, 0x1.3b2ab6fba4e77p-23);
+  p = fma(p, r, 0x1.c6b08d704a0c0p-17);
+  p = fma(p, r, 0x1.ebfbdff82c58fp-11);
+  p = fma(p, r, 0x1.62e42fefa39efp-5);
+  p = fma(p, r, 1.0);
+  const int k = __double2loint(t);  // n, two's complement
+  const double e = p * pow16[k & 15];
+  return x > row.lowest
+             ? __hiloint2double(__double2hiint(e) + ((k >> 4) << 20), __double2loint(e)) : 0.0;
 }
 
-// One cluster per sequence; CTA `rank` holds vocabulary [rank L, (rank + 1) L),
-// thread t of it the contiguous elements [t E, (t + 1) E) of that.  CACHED: the
-// f64 exponentials of both rows stay in shared memory between the passes (V /
-// cluster * 16 bytes); a vocabulary too long for that computes them again.
-template <bool CACHED>
-static __global__ void __launch_bounds__(VP_THREADS) k_verify_pick(const VerifyArgs a, int L) {
+// The sum of one value per thread over the block, f64, the same in every
+// thread; red: VP_THREADS / 32 values.
+FLOCK_DEV double verify_sum(double v, double* red) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.0;
+#pragma unroll
+  for (int w = 0; w < VP_THREADS / 32; w++) v += red[w];
+  return v;
+}
+
+// One cluster per sequence.  Every warp of it takes a contiguous `span` of the
+// vocabulary, so that a sum per warp, added up in order, is the running sum at
+// the warps' borders; the warp whose span holds u W then looks inside it.
+// KEEP: a lane's exponentials of both rows stay in registers between the
+// passes (spans up to 128 KEPT: V = 151936 in a cluster of 16); longer
+// vocabularies compute them again.
+constexpr int VP_KEPT = 5;
+template <bool KEEP>
+static __global__ void __launch_bounds__(VP_THREADS) k_verify_pick(const VerifyArgs a, int span) {
   namespace cg = cooperative_groups;
-  extern __shared__ double vp_smem[];
+  constexpr int WARPS = VP_THREADS / 32;
   __shared__ int s_first;
   __shared__ float s_rm[2 * VERIFY_MAX_DRAFTS + 1];   // each row's maximum and sum
   __shared__ double s_rs[2 * VERIFY_MAX_DRAFTS + 1];
-  __shared__ double s_red[VP_THREADS / 32];
-  __shared__ double s_sum[2], s_total;  // read by the cluster's other CTAs
+  __shared__ double s_red[WARPS], s_pow16[16];
+  __shared__ double s_sum[2], s_total[2];  // read by the cluster's other CTAs
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), nr = (int)cluster.num_blocks();
-  const int seq = blockIdx.x / nr, t = threadIdx.x;
+  const int seq = blockIdx.x / nr, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  if (t < 16) s_pow16[t] = k_pow16[t];
   pdl_wait();  // the partials
   const int len = verify_len(a, seq);
   const bool sampled = a.draft != nullptr;
@@ -233,12 +279,12 @@ static __global__ void __launch_bounds__(VP_THREADS) k_verify_pick(const VerifyA
 
   // every CTA decides the first refused draft for itself
   if (t == 0) s_first = len;
-  for (int row = t >> 5; row < rows; row += VP_THREADS / 32) {
+  for (int row = warp; row < rows; row += WARPS) {
     if (row <= a.n ? row > len : row - a.n - 1 >= len) continue;  // not read: no partials
     float m;
     double s;
     verify_join(a, row0 + row, m, s);
-    if ((t & 31) == 0) {
+    if (lane == 0) {
       s_rm[row] = m;
       s_rs[row] = s;
     }
@@ -262,7 +308,8 @@ static __global__ void __launch_bounds__(VP_THREADS) k_verify_pick(const VerifyA
   const bool residual = refused && sampled;
   // one-hot draft: its token cannot be drawn again
   const int skip = refused && !sampled ? ids[r] : -1;
-  const double mp = s_rm[r], mq = residual ? s_rm[a.n + 1 + r] : 0.0f;
+  const VerifyRow mp = verify_row_of(s_rm[r], a.inv_t);
+  const VerifyRow mq = verify_row_of(residual ? s_rm[a.n + 1 + r] : 0.0f, a.inv_t);
   auto summable = [&](int row) { return s_rs[row] > 0.0 && s_rs[row] < (double)INFINITY; };
   const bool has = summable(r) && (!residual || summable(a.n + 1 + r));
   if (rank == 0) {
@@ -275,101 +322,177 @@ static __global__ void __launch_bounds__(VP_THREADS) k_verify_pick(const VerifyA
 
   const float* xp = verify_row(a, seq, r);
   const float* xq = residual ? verify_row(a, seq, a.n + 1 + r) : nullptr;
-  const int v0 = rank * L, v1 = min(a.vocab, v0 + L);
-  double* ep = vp_smem;
-  double* eq = vp_smem + L;
-  auto expo = [&](const float* x, int i, double m) {
-    return exp(((double)__ldg(x + i) - m) * a.inv_t);
-  };
-  // the rows' f64 sums over the cluster (only a residual needs them)
-  double sp = 1.0, sq = 1.0;
-  if (CACHED || residual) {
-    double a0 = 0.0, a1 = 0.0;
-    for (int i = v0 + t; i < v1; i += VP_THREADS) {
-      const double e = expo(xp, i, mp);
-      a0 += e;
-      if (CACHED) ep[i - v0] = e;
-      if (residual) {
-        const double f = expo(xq, i, mq);
-        a1 += f;
-        if (CACHED) eq[i - v0] = f;
-      }
-    }
-    if (residual) {
-      double t0, t1;
-      verify_scan(a0, s_red, t0);
-      verify_scan(a1, s_red, t1);
-      if (t == 0) {
-        s_sum[0] = t0;
-        s_sum[1] = t1;
-      }
-      cluster.sync();
-      sp = sq = 0.0;
-      for (int c = 0; c < nr; c++) {
-        const double* o = cluster.map_shared_rank(s_sum, c);
-        sp += o[0];
-        sq += o[1];
-      }
+  const int64_t from = ((int64_t)rank * WARPS + warp) * span;
+  const int v0 = (int)(from < a.vocab ? from : a.vocab), v1 = (int)(from + span < a.vocab ? from + span : a.vocab);
+  // four neighbouring logits from i on, -inf past the span
+  auto four = [&](const float* x, int i, float (&v)[4]) {
+    if (a.vec && i + 4 <= v1) {
+      const float4 w = __ldg(reinterpret_cast<const float4*>(x + i));
+      v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
     } else {
-      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] = i + j < v1 ? __ldg(x + i + j) : -INFINITY;
     }
-  }
-  const double ip = 1.0 / sp, iq = 1.0 / sq;
-  const int E = (L + VP_THREADS - 1) / VP_THREADS;
-  const int j0 = min(v1, v0 + t * E), j1 = min(v1, j0 + E);
-  // all: the weights are the target's own (nothing was left of the residual)
-  auto weight = [&](int i, bool all) {
-    const double e = CACHED ? ep[i - v0] : expo(xp, i, mp);
-    if (all) return e;
-    if (residual) return fmax(e * ip - (CACHED ? eq[i - v0] : expo(xq, i, mq)) * iq, 0.0);
-    return i == skip ? 0.0 : e;
   };
-  bool all = !refused;
-  double mine, before, total, w = 0.0;
-  while (true) {
-    mine = 0.0;
-    for (int i = j0; i < j1; i++) mine += weight(i, all);
-    before = verify_scan(mine, s_red, total);
-    if (t == 0) s_total = total;
-    cluster.sync();
-    double base = 0.0;
-    w = 0.0;
-    for (int c = 0; c < nr; c++) {
-      if (c == rank) base = w;
-      w += *cluster.map_shared_rank(&s_total, c);
+  // f(index, exponential, draft's exponential) over the span, a lane four at a
+  // time; the first of two passes computes them (KEEP) or both do
+  double ke[KEEP ? VP_KEPT : 1][4], kf[KEEP ? VP_KEPT : 1][4];
+  auto compute = [&](const float (&x)[4], const float (&y)[4], double (&e)[4], double (&f)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      e[j] = verify_exp(x[j], mp, s_pow16);
+      f[j] = residual ? verify_exp(y[j], mq, s_pow16) : 0.0;
     }
-    before += base;
-    cluster.sync();  // s_total is read before it is written again, and before any CTA leaves
-    if (w > 0.0 || all) break;
+  };
+  auto each = [&](bool first, auto f) {
+    if constexpr (KEEP) {
+      if (first) {
+        float x[VP_KEPT][4], y[VP_KEPT][4];
+#pragma unroll
+        for (int b = 0; b < VP_KEPT; b++) {
+          four(xp, v0 + 4 * lane + 128 * b, x[b]);
+          if (residual) four(xq, v0 + 4 * lane + 128 * b, y[b]);
+        }
+#pragma unroll
+        for (int b = 0; b < VP_KEPT; b++) compute(x[b], y[b], ke[b], kf[b]);
+      }
+#pragma unroll
+      for (int b = 0; b < VP_KEPT; b++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) f(v0 + 4 * lane + 128 * b + j, ke[b][j], kf[b][j]);
+    } else {
+      for (int i = v0 + 4 * lane; i < v1; i += 128) {
+        float x[4], y[4];
+        four(xp, i, x);
+        if (residual) four(xq, i, y);
+        compute(x, y, ke[0], kf[0]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) f(i + j, ke[0][j], kf[0][j]);
+      }
+    }
+  };
+  double ip = 1.0, iq = 1.0;
+  if (residual) {  // the rows' f64 sums
+    double a0 = 0.0, a1 = 0.0;
+    each(true, [&](int, double e, double f) {
+      a0 += e;
+      a1 += f;
+    });
+    a0 = verify_sum(a0, s_red);
+    a1 = verify_sum(a1, s_red);
+    if (t == 0) {
+      s_sum[0] = a0;
+      s_sum[1] = a1;
+    }
+    cluster.sync();
+    // a lane per CTA: the remote loads (0.2 us each) in flight together
+    double sp = 0.0, sq = 0.0;
+    if (lane < nr) {
+      const double* o = cluster.map_shared_rank(s_sum, lane);
+      sp = o[0];
+      sq = o[1];
+    }
+#pragma unroll
+    for (int d = VP_MAX_CLUSTER / 2; d > 0; d >>= 1) {
+      sp += __shfl_xor_sync(0xffffffffu, sp, d);
+      sq += __shfl_xor_sync(0xffffffffu, sq, d);
+    }
+    sp = __shfl_sync(0xffffffffu, sp, 0);
+    sq = __shfl_sync(0xffffffffu, sq, 0);
+    ip = 1.0 / sp;
+    iq = 1.0 / sq;
+  }
+  // all: the weights are the target's own (nothing was left of the residual)
+  auto weight = [&](int i, double e, double f, bool all) {
+    return all ? e : residual ? fmax(e * ip - f * iq, 0.0) : i == skip ? 0.0 : e;
+  };
+  double before = 0.0, end = 0.0, w = 0.0;
+  bool all = !refused;
+  for (int turn = 0; turn < 2; turn++) {
+    double mine = 0.0;
+    each(turn == 0 && !residual, [&](int i, double e, double f) { mine += weight(i, e, f, all); });
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+    __syncthreads();
+    if (lane == 0) s_red[warp] = mine;
+    __syncthreads();
+    if (t == 0) {
+      double sum = 0.0;
+      for (int i = 0; i < WARPS; i++) sum += s_red[i];
+      s_total[turn] = sum;
+    }
+    cluster.sync();
+    // running sums over the CTAs, a lane each, the same in every CTA
+    double run = lane < nr ? *cluster.map_shared_rank(s_total + turn, lane) : 0.0;
+#pragma unroll
+    for (int d = 1; d < VP_MAX_CLUSTER; d <<= 1) {
+      const double o = __shfl_up_sync(0xffffffffu, run, d);
+      if (lane >= d) run += o;
+    }
+    before = rank == 0 ? 0.0 : __shfl_sync(0xffffffffu, run, rank - 1);
+    end = __shfl_sync(0xffffffffu, run, rank);
+    w = __shfl_sync(0xffffffffu, run, nr - 1);
+    if (w > 0.0 || all) break;  // the whole cluster agrees
     all = true;
   }
-  // The first index whose running sum passes u W.  The threads' half-open
-  // ranges [before, end) cut [0, W) without gaps, `end` being the next
-  // thread's `before`, so one thread draws.
+  // no CTA leaves while another may read its shared memory
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  // this warp's [before, end) of the running sum: its CTA's, cut at the warps
+  // before it; the last warp's end is the next CTA's beginning
+  const double cta_end = end;
+  for (int i = 0; i < warp; i++) before += s_red[i];
+  end = warp + 1 < WARPS ? before + s_red[warp] : cta_end;
   double goal = (double)u[a.n] * w;
   if (!(goal < w)) goal = w * 0.9999999999999999;
-  double end = __shfl_down_sync(0xffffffffu, before, 1);
-  const int lane = t & 31, warp = t >> 5;
-  __syncthreads();
-  if (lane == 0) s_red[warp] = before;
-  if (t == 0) s_sum[0] = before;  // this CTA's first running sum
-  cluster.sync();
-  if (lane == 31)
-    end = warp + 1 < VP_THREADS / 32 ? s_red[warp + 1]
-          : rank + 1 < nr            ? cluster.map_shared_rank(s_sum, rank + 1)[0]
-                                     : w;
   if (before <= goal && goal < end) {
+    int pick = -1, last = v0;
     double c = before;
-    int pick = min(j0, a.vocab - 1);
-    for (int i = j0; i < j1; i++) {
-      const double x = weight(i, all);
-      c += x;
-      if (x > 0.0) pick = i;
-      if (c > goal) break;
+    auto look = [&](int i, const double (&e)[4], const double (&f)[4]) {
+      double v[4], sum = 0.0;
+      int top = -1;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        v[j] = weight(i + j, e[j], f[j], all);
+        sum += v[j];
+        if (v[j] > 0.0) top = i + j;
+      }
+      double run = sum;  // inclusive over the lanes
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const double o = __shfl_up_sync(0xffffffffu, run, d);
+        if (lane >= d) run += o;
+      }
+      const uint32_t over = __ballot_sync(0xffffffffu, c + run > goal);
+      if (over && pick < 0) {
+        int found = top;  // rounding may leave it to the lane's last weight
+        double upto = c + (run - sum) + sum;
+#pragma unroll
+        for (int j = 3; j >= 0; j--) {
+          if (v[j] > 0.0 && upto > goal) found = i + j;
+          upto -= v[j];
+        }
+        pick = __shfl_sync(0xffffffffu, found, __ffs(over) - 1);
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      last = top >= 0 ? top : last;
+      c += __shfl_sync(0xffffffffu, run, 31);
+    };
+    if constexpr (KEEP) {
+#pragma unroll
+      for (int b = 0; b < VP_KEPT; b++)
+        if (pick < 0) look(v0 + 4 * lane + 128 * b, ke[b], kf[b]);
+    } else {
+      for (int i0 = v0; i0 < v1 && pick < 0; i0 += 128) {
+        float x[4], y[4];
+        four(xp, i0 + 4 * lane, x);
+        if (residual) four(xq, i0 + 4 * lane, y);
+        compute(x, y, ke[0], kf[0]);
+        look(i0 + 4 * lane, ke[0], kf[0]);
+      }
     }
-    a.tokens[(size_t)seq * (a.n + 1) + r] = pick;
+    if (lane == 0) a.tokens[(size_t)seq * (a.n + 1) + r] = pick >= 0 ? pick : last;
   }
-  cluster.sync();  // s_sum is read before its CTA leaves
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // Greedy: drafts are kept while they equal the target's argmax (the lowest
