@@ -119,8 +119,8 @@ int flock_verify_draft(flock_dev* dev, const float* target, int64_t target_strid
   // none under one pass of a CTA's loads
   const int64_t pass = 16 * VS_THREADS;
   int64_t chunks = (4 * (int64_t)dev->sm_count + rows - 1) / rows;
-  const int64_t most = (vocab + pass - 1) / pass;
-  chunks = chunks < 1 ? 1 : chunks > most ? most : chunks;
+  const int64_t passes = (vocab + pass - 1) / pass;
+  chunks = chunks < 1 ? 1 : chunks > passes ? passes : chunks;
   if (chunks > 64) chunks = 64;
   if (chunks * rows > VERIFY_MAX_PARTIALS) chunks = VERIFY_MAX_PARTIALS / rows;
   a.chunk_len = (int)(((vocab + chunks - 1) / chunks + 3) / 4 * 4);
@@ -139,13 +139,18 @@ int flock_verify_draft(flock_dev* dev, const float* target, int64_t target_strid
   }
   k_verify_stats<false><<<grid, VS_THREADS, 0, st>>>(a);
   FLOCK_CK(cudaGetLastError());
-  // CTAs per sequence: about a thousand tokens each, as many as a cluster may have
+  // CTAs per sequence: about a thousand tokens each, as many as a cluster may
+  // have.  More sequences than such clusters find room (seven of 16 CTAs that
+  // fill an SM each) do better in clusters of eight whose CTAs share SMs and
+  // compute the exponentials twice (32 sequences: 90 us against 101).
+  const bool many = (int64_t)n_seqs * VP_MAX_CLUSTER > dev->sm_count;
+  const int most = many ? VP_MAX_CLUSTER / 2 : VP_MAX_CLUSTER;
   int cluster = 1;
-  while (cluster < VP_MAX_CLUSTER && (int64_t)cluster * 1024 < vocab) cluster *= 2;
+  while (cluster < most && (int64_t)cluster * 1024 < vocab) cluster *= 2;
   // each warp's span of the vocabulary, in whole groups of four
   const int64_t warps = (int64_t)cluster * (VP_THREADS / 32);
   const int span = (int)(((vocab + warps - 1) / warps + 3) / 4 * 4);
-  return span <= 128 * VP_KEPT ? launch_pick<true>(st, a, cluster, span)
+  return span <= 128 * VP_KEPT && !many ? launch_pick<true>(st, a, cluster, span)
                                : launch_pick<false>(st, a, cluster, span);
 }
 

@@ -26,19 +26,32 @@ HEAD_DIM = 128
 WORKSPACE_BYTES = _abi.FLOCK_WORKSPACE_BYTES
 
 # __cuda_array_interface__ type strings and torch dtype names of an element
-_TYPES = {"f32": ("<f4", "torch.float32"), "bf16": ("<u2", "torch.bfloat16"),
-          "fp8": ("|u1", "torch.float8_e4m3fn"), "u8": ("|u1", "torch.uint8"),
-          "f16": ("<f2", "torch.float16"), "i32": ("<i4", "torch.int32")}
+_TYPES = {"f32": ("<f4", "float32"), "bf16": ("<u2", "bfloat16"), "fp8": ("|u1", "float8_e4m3fn"),
+          "u8": ("|u1", "uint8"), "f16": ("<f2", "float16"), "i32": ("<i4", "int32")}
+_torch_types: dict = {}  # torch dtype -> element name, filled when a tensor comes by
+
+
+def _torch_type(t) -> str | None:
+    if not _torch_types:
+        import torch  # a torch tensor is here, so torch is loaded
+        _torch_types.update({getattr(torch, n): e for e, (_, n) in _TYPES.items()})
+    return _torch_types.get(t)
 
 
 def _array(a, dtype: str, ordinal: int, what: str):
     """(device address, shape, strides in elements or None when dense)."""
-    if hasattr(a, "data_ptr"):  # a torch tensor
-        if str(a.dtype) != _TYPES[dtype][1]:
-            raise ValueError(f"{what} is {a.dtype}, want {_TYPES[dtype][1]}")
-        if not a.is_cuda or a.get_device() != ordinal:
-            raise ValueError(f"{what} is on {a.device}, the cache's device is cuda:{ordinal}")
-        return a.data_ptr(), a.shape, None if a.is_contiguous() else a.stride()
+    try:
+        t, p = a.dtype, a.data_ptr()
+    except AttributeError:
+        return _interface(a, dtype, what)
+    if (_torch_types.get(t) or _torch_type(t)) != dtype:
+        raise ValueError(f"{what} is {t}, want torch.{_TYPES[dtype][1]}")
+    if a.get_device() != ordinal:  # -1 on the host
+        raise ValueError(f"{what} is on {a.device}, the cache's device is cuda:{ordinal}")
+    return p, a.shape, None if a.is_contiguous() else a.stride()
+
+
+def _interface(a, dtype: str, what: str):
     i = getattr(a, "__cuda_array_interface__", None)
     if i is None:
         raise ValueError(f"{what} is a {type(a).__name__}, not a device array")
@@ -50,9 +63,9 @@ def _array(a, dtype: str, ordinal: int, what: str):
 
 def _dense(a, dtype: str, ordinal: int, what: str, shape: tuple) -> int:
     p, got, strides = _array(a, dtype, ordinal, what)
-    if tuple(got) != tuple(shape) or strides is not None:
+    if strides is not None or tuple(got) != shape:
         raise ValueError(f"{what} is {tuple(got)}{'' if strides is None else ' with strides'}, "
-                         f"want a dense {tuple(shape)}")
+                         f"want a dense {shape}")
     return p
 
 
