@@ -69,6 +69,10 @@ int check_range(const flock_kv* c, const char* who, int64_t pos, int n) {
   return FLOCK_OK;
 }
 
+dim3 row_grid(const flock_kv* c, int n) {  // 8 tokens a CTA, a warp each
+  return dim3((unsigned)((n + 7) / 8), (unsigned)c->view.n_kv_heads);
+}
+
 size_t plane_bytes(int kv_dtype, int n_kv_heads, int64_t capacity) {
   const size_t values = (size_t)capacity * n_kv_heads * KV_HD;
   return kv_dtype == FLOCK_KV_Q4     ? values / 2
@@ -273,11 +277,10 @@ int flock_kv_append(flock_kv* c, const float* k, const float* v, int64_t row_str
   if (n == 0) return FLOCK_OK;
   OnDevice on(c->dev->ordinal);
   FLOCK_TRY(on.enter());
-  const unsigned grid = (unsigned)(((int64_t)n * c->view.n_kv_heads + 7) / 8);
+  const dim3 grid = row_grid(c, n);
   return by_dtype(c->kv_dtype, [&](auto kv) -> int {
-    k_kv_append<decltype(kv)::value><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
-        c->view, k, v, row_stride, pos, n);
-    FLOCK_CK(cudaGetLastError());
+    FLOCK_CK(launch_ex(static_cast<cudaStream_t>(stream), k_kv_append<decltype(kv)::value>,
+                       grid, dim3(256), 0, true, c->view, k, v, row_stride, pos, n));
     return FLOCK_OK;
   });
 }
@@ -291,11 +294,10 @@ int flock_kv_read(flock_kv* c, int64_t pos, int n, float* k, float* v, void* str
   if (n == 0) return FLOCK_OK;
   OnDevice on(c->dev->ordinal);
   FLOCK_TRY(on.enter());
-  const unsigned grid = (unsigned)(((int64_t)n * c->view.n_kv_heads + 7) / 8);
+  const dim3 grid = row_grid(c, n);
   return by_dtype(c->kv_dtype, [&](auto kv) -> int {
-    k_kv_read<decltype(kv)::value><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
-        c->view, pos, n, k, v);
-    FLOCK_CK(cudaGetLastError());
+    FLOCK_CK(launch_ex(static_cast<cudaStream_t>(stream), k_kv_read<decltype(kv)::value>,
+                       grid, dim3(256), 0, true, c->view, pos, n, k, v));
     return FLOCK_OK;
   });
 }

@@ -84,42 +84,64 @@ FLOCK_DEV float4 kv_load4(const KvView& c, int64_t key, int head, int lane) {
 
 // One row (lane: elements 4 lane .. 4 lane + 3) into the 4-bit cache.
 //
-// The code of x is decided in f64, x * (1 / d) + 8.5 with one rounding each,
-// as flock_quant_q4 decides it: the codes of a row are the host's bytes.  A
-// block with a NaN gets a NaN scale (every value of it reads back NaN).
+// The code of x is floor(x * (1 / d) + 8.5) in f64 with one rounding each, as
+// flock_quant_q4 decides it: the codes of a row are the host's bytes.  f32
+// gives the same wherever it lands further from an integer than its own error
+// (2.5e-6: a reciprocal and a product of relative error 2^-22, the sum's 2^-20);
+// a warp with a value within 1e-5 of one works its codes out in f64.  A block
+// with a NaN gets a NaN scale (every value of it reads back NaN).
 template <bool IS_K>
 FLOCK_DEV void q4_store_row(const KvView& c, int64_t key, int head, float4 x4, int lane) {
   float x[4] = {x4.x, x4.y, x4.z, x4.w};
-  bool nan = false;
-  float top = 0.0f;  // this lane's first value of largest magnitude
-  int at = 4 * (lane & 7);
+  auto mag = [](float v) { return __float_as_uint(v) & 0x7FFFFFFFu; };
+  uint32_t top_bits = max(max(mag(x[0]), mag(x[1])), max(mag(x[2]), mag(x[3])));
+  const bool nan = top_bits > 0x7F800000u;
+  if (__any_sync(0xffffffffu, top_bits > __float_as_uint(Q4_VALUE_MAX))) {
+    top_bits = 0;
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    nan |= x[i] != x[i];
-    x[i] = fminf(fmaxf(x[i], -Q4_VALUE_MAX), Q4_VALUE_MAX);
-    if (fabsf(x[i]) > fabsf(top)) {
-      top = x[i];
-      at = 4 * (lane & 7) + i;
+    for (int i = 0; i < 4; i++) {  // a NaN becomes a bound, its block is marked below
+      x[i] = fminf(fmaxf(x[i], -Q4_VALUE_MAX), Q4_VALUE_MAX);
+      top_bits = max(top_bits, mag(x[i]));
     }
   }
+  const uint32_t own = top_bits;
 #pragma unroll
-  for (int s = 1; s < 8; s <<= 1) {  // over the block's 8 lanes; the lower index wins a tie
-    const float o = __shfl_xor_sync(0xffffffffu, top, s);
-    const int oa = __shfl_xor_sync(0xffffffffu, at, s);
-    if (fabsf(o) > fabsf(top) || (fabsf(o) == fabsf(top) && oa < at)) {
-      top = o;
-      at = oa;
-    }
-    nan |= __shfl_xor_sync(0xffffffffu, (int)nan, s) != 0;
-  }
-  const double d = (double)top / -8.0;
-  const double inv = d == 0.0 ? 0.0 : 1.0 / d;
+  for (int s = 1; s < 8; s <<= 1)  // over the block's 8 lanes
+    top_bits = max(top_bits, __shfl_xor_sync(0xffffffffu, top_bits, s));
+  // the first value of that magnitude: the first such lane's first
+  const uint32_t octet = 0xFFu << (lane & 24);
+  const int at = __ffs(__ballot_sync(0xffffffffu, own == top_bits) & octet) - 1;
+  const float first = mag(x[0]) == own   ? x[0]
+                      : mag(x[1]) == own ? x[1]
+                      : mag(x[2]) == own ? x[2]
+                                         : x[3];
+  const float top = __shfl_sync(0xffffffffu, first, at);
+  const bool nan_block = (__ballot_sync(0xffffffffu, nan) & octet) != 0;
+
   uint32_t code = 0;
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(top));
+  inv = top == 0.0f ? 0.0f : fmul(inv, -8.0f);
+  // too small for f32's reciprocal: also f64
+  bool close = top != 0.0f && fabsf(top) < 1e-30f;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    const double t = floor(__dadd_rn(__dmul_rn((double)x[i], inv), 8.5));
-    const int q = t < 0.0 ? 0 : t > 15.0 ? 15 : (int)t;
-    code |= (uint32_t)q << (8 * i);
+    const float t = ffma(x[i], inv, 8.5f);
+    // 2^23 added rounding down leaves floor(t) in the low bits
+    const float f = __fadd_rd(t, 8388608.0f);
+    const float frac = fsub(t, fsub(f, 8388608.0f));
+    close |= frac < 1e-5f || frac > 0.99999f;
+    code |= min(__float_as_uint(f) & 31u, 15u) << (8 * i);
+  }
+  if (__any_sync(0xffffffffu, close)) {
+    const double d = (double)top / -8.0;
+    const double inv64 = d == 0.0 ? 0.0 : 1.0 / d;
+    code = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const double t = __dadd_rn(__dmul_rn((double)x[i], inv64), 8.5);
+      code |= (uint32_t)min(__double2loint(__dadd_rd(t, 4503599627370496.0)), 15) << (8 * i);
+    }
   }
   // lanes 0-3 of a block hold values 0..15 (low nibbles), lanes 4-7 16..31
   const uint32_t high = __shfl_xor_sync(0xffffffffu, code, 4);
@@ -135,9 +157,9 @@ FLOCK_DEV void q4_store_row(const KvView& c, int64_t key, int head, float4 x4, i
       *reinterpret_cast<uint16_t*>(r + 16 * p + 8 + 2 * b) = (uint16_t)(w >> 16);
     }
   }
-  if (p == 0)
+  if (p == 0)  // top / -8 is exact in f32 down to its subnormals, which round to a zero scale
     (IS_K ? c.ks : c.vs)[row * 4 + b] =
-        nan ? (uint16_t)0x7E00u : __half_as_ushort(__float2half_rn((float)d));
+        nan_block ? (uint16_t)0x7E00u : __half_as_ushort(__float2half_rn(fmul(top, -0.125f)));
 }
 
 template <int KV, bool IS_K>
@@ -158,16 +180,20 @@ FLOCK_DEV void kv_store4(const KvView& c, int64_t key, int head, float4 x, int l
   }
 }
 
-// One warp per cached row: k and v of (token, head) rounded into the cache.
+// One warp per (token, head), a row of k and one of v; grid (8 tokens, head), so
+// no index is divided (64-bit divisions were half the instructions).  Bound: the
+// f32 rows' bytes.  Two or four tokens a warp, to have more loads in flight,
+// measured slower.
 template <int KV>
 static __global__ void __launch_bounds__(256) k_kv_append(KvView c, const float* k, const float* v,
                                                           int64_t row_stride, int64_t pos, int n) {
+  pdl_launch_dependents();
+  pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (item >= (int64_t)n * c.n_kv_heads) return;
-  const int64_t tok = item / c.n_kv_heads;
-  const int head = (int)(item % c.n_kv_heads);
-  const size_t src = (size_t)tok * row_stride + (size_t)head * KV_HD + 4 * lane;
+  const int64_t tok = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int head = blockIdx.y;
+  if (tok >= n) return;
+  const int64_t src = tok * row_stride + (int64_t)head * KV_HD + 4 * lane;
   const float4 kx = __ldg(reinterpret_cast<const float4*>(k + src));
   const float4 vx = __ldg(reinterpret_cast<const float4*>(v + src));
   kv_store4<KV, true>(c, pos + tok, head, kx, lane);
@@ -178,14 +204,17 @@ static __global__ void __launch_bounds__(256) k_kv_append(KvView c, const float*
 template <int KV>
 static __global__ void __launch_bounds__(256) k_kv_read(KvView c, int64_t pos, int n, float* k,
                                                         float* v) {
+  pdl_launch_dependents();
+  pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (item >= (int64_t)n * c.n_kv_heads) return;
-  const int64_t tok = item / c.n_kv_heads;
-  const int head = (int)(item % c.n_kv_heads);
-  const size_t dst = (size_t)item * KV_HD + 4 * lane;
-  *reinterpret_cast<float4*>(k + dst) = kv_load4<KV, true>(c, pos + tok, head, lane);
-  *reinterpret_cast<float4*>(v + dst) = kv_load4<KV, false>(c, pos + tok, head, lane);
+  const int64_t tok = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int head = blockIdx.y;
+  if (tok >= n) return;
+  const size_t dst = ((size_t)tok * c.n_kv_heads + head) * KV_HD + 4 * lane;
+  const float4 kx = kv_load4<KV, true>(c, pos + tok, head, lane);
+  const float4 vx = kv_load4<KV, false>(c, pos + tok, head, lane);
+  *reinterpret_cast<float4*>(k + dst) = kx;
+  *reinterpret_cast<float4*>(v + dst) = vx;
 }
 
 // Queries at positions pos .. pos + n_queries - 1, row i of q [n_heads][128]

@@ -120,7 +120,10 @@ class KVCache:
         _abi.call("flock_kv_create", dev.handle, KV_DTYPES[dtype], n_kv_heads, head_dim, capacity,
                   *planes, ws, ctypes.byref(h))
         self.handle = h
-        self._attention = _abi.lib().flock_kv_attention
+        # the entry points, looked up once
+        lib = _abi.lib()
+        self._append, self._read = lib.flock_kv_append, lib.flock_kv_read
+        self._attention = lib.flock_kv_attention
 
     def free(self) -> None:
         if self.handle:
@@ -140,14 +143,17 @@ class KVCache:
         vp, nv, _, vs = _rows(v, self.dev.ordinal, "v", self.n_kv_heads)
         if n != nv or ks != vs:
             raise ValueError(f"k has {n} rows at stride {ks}, v {nv} at {vs}")
-        _abi.call("flock_kv_append", self.handle, kp, vp, ks, pos, n, stream or None)
+        rc = self._append(self.handle, kp, vp, ks, pos, n, stream or None)
+        if rc:
+            _abi.check(rc)
 
     def read(self, pos: int, n: int, k, v, stream: int = 0) -> None:
         """The cached rows pos .. pos + n - 1 into f32 k and v [n][n_kv_heads][128]."""
         shape = (n, self.n_kv_heads, HEAD_DIM)
-        _abi.call("flock_kv_read", self.handle, pos, n,
-                  _dense(k, "f32", self.dev.ordinal, "k", shape),
-                  _dense(v, "f32", self.dev.ordinal, "v", shape), stream or None)
+        rc = self._read(self.handle, pos, n, _dense(k, "f32", self.dev.ordinal, "k", shape),
+                        _dense(v, "f32", self.dev.ordinal, "v", shape), stream or None)
+        if rc:
+            _abi.check(rc)
 
     def attention(self, q, pos: int, out, window: int = 0, sinks: int = 0,
                   stream: int = 0) -> None:
