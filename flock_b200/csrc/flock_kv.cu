@@ -348,11 +348,9 @@ int flock_kv_attention(flock_kv* c, const float* q, int64_t q_stride, int n_head
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return by_dtype(c->kv_dtype, [&](auto kv) -> int {
     constexpr int KV = decltype(kv)::value;
-    if constexpr (KV == FLOCK_KV_Q4 || KV == FLOCK_KV_FP8) {
-      if (rows > 16) return launch_prompt<KV>(c, a, st);
-      // f16 parts of four rows fill one column tile
-      if (rows <= 4) return launch_rows<KV, 1>(c, a, st);
-    }
+    if (rows > 16) return launch_prompt<KV>(c, a, st);
+    if constexpr (KV == FLOCK_KV_Q4 || KV == FLOCK_KV_FP8)
+      if (rows <= 4) return launch_rows<KV, 1>(c, a, st);  // f16 parts of four rows: one column tile
     return launch_rows<KV, 2>(c, a, st);
   });
 }

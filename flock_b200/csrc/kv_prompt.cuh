@@ -1,5 +1,5 @@
-// Attention of many query rows (a prompt chunk, a long draft) over a 4-bit or
-// e4m3 cache on the tcgen05 tensor cores, to f32 accuracy: k_kv_prompt.
+// Attention of many query rows (a prompt chunk, a long draft) over a cache on
+// the tcgen05 tensor cores, to f32 accuracy: k_kv_prompt.
 //
 // CTA (row tile of 128 (query, head) rows of a kv head, key split), looping
 // over 128-key tiles; per tile S = Q K^T and O += P V, f32 accumulators in
@@ -8,8 +8,10 @@
 //
 // f32 results from f16 operands.  q (scaled by a power of two per row) and the
 // softmax weights are hi + lo, two f16.  An e4m3 value is an f16 value: two
-// products (hi, lo times it).  A 4-bit value (code - 8) * scale has 15
-// significant bits: hi + lo again, three products (lo lo is below 2^-22).
+// products (hi, lo times it), and so is a bf16 value once its tile is scaled by a
+// power of two into f16's range.  A 4-bit value (code - 8) * scale has 15
+// significant bits, an f32 24: hi + lo again, three products (lo lo is below
+// 2^-22).
 //
 // Roles, sixteen warps of 128 registers:
 //   warps 0-7   softmax; thread = row = tensor-memory lane, warps 0-3 the
@@ -27,6 +29,12 @@
 //               softmax of a tile has two products' time, and K and V, one
 //               buffer each, are rewritten while the other is being read.
 //
+// The tensor cores' accumulators do not round to nearest: each step loses half a
+// last bit on average, towards zero, so a sum of n steps shrinks by about n
+// 2^-25 (1128 steps over 6000 keys: 2.3e-5).  The small products of a score go
+// first, and the outputs move to an f32 sum in shared memory every KP_FLUSH
+// tiles, added there in f32 (96 steps: 1e-6).
+//
 // The running maximum may lag by 2^8 before the outputs are rescaled (as in
 // k_kv_rows).  Every wait is bounded; a wait that runs out ends the CTA, which
 // then writes NaN.
@@ -39,6 +47,8 @@ namespace flock {
 constexpr int KP_ROWS = 128;     // query rows per CTA
 constexpr int KP_KEYS = 128;     // keys per tile
 constexpr int KP_THREADS = 512;
+constexpr int KP_FLUSH = 4;      // key tiles an output accumulator takes
+constexpr int KP_SUM_STRIDE = 132;  // floats of a row of the outputs' sum: rows 4 banks apart
 constexpr int KP_OPND = 128 * 128 * 2;  // bytes of one 128 x 128 f16 operand
 
 struct KvPromptArgs {
@@ -112,13 +122,18 @@ FLOCK_DEV constexpr int kp_vcol(int d) {
   return 32 * b + 8 * (2 * byte + hi) + n;
 }
 
-// Shared memory: the operands (K hi, V hi, then for 4-bit K lo, V lo), barriers.
+// Shared memory: the operands K hi, V hi, then K lo, V lo, and the outputs' sum.
 template <int KV>
-constexpr size_t KP_SMEM = (KV == FLOCK_KV_Q4 ? 4 : 2) * (size_t)KP_OPND + 1024;
+constexpr bool KP_LO = KV == FLOCK_KV_Q4 || KV == FLOCK_KV_F32;  // K and V in two parts
+template <int KV>
+constexpr size_t KP_SMEM =
+    (KP_LO<KV> ? 4 : 2) * (size_t)KP_OPND + 128 * KP_SUM_STRIDE * 4 + 1024;
 
 template <int KV>
 static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvPromptArgs p) {
-  constexpr bool Q4 = KV == FLOCK_KV_Q4;
+  constexpr bool Q4 = KV == FLOCK_KV_Q4, LO = KP_LO<KV>;
+  constexpr bool WIDE = KV == FLOCK_KV_F32 || KV == FLOCK_KV_BF16;  // elements scaled by tile
+  constexpr bool SCALED = KV != FLOCK_KV_FP8;
   extern __shared__ __align__(16) uint8_t kp_raw[];
   __shared__ uint64_t s_bar[9];
   __shared__ uint32_t s_tmem;
@@ -132,6 +147,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
   uint8_t* sVh = base + KP_OPND;
   uint8_t* sKl = base + 2 * KP_OPND;
   uint8_t* sVl = base + 3 * KP_OPND;
+  float* s_sum = reinterpret_cast<float*>(base + (LO ? 4 : 2) * KP_OPND);
   uint64_t *k_full = s_bar, *k_empty = s_bar + 1, *v_full = s_bar + 2, *v_empty = s_bar + 3,
            *s_full = s_bar + 4 /* 2 */, *p_full = s_bar + 6, *q_full = s_bar + 7,
            *drained = s_bar + 8;
@@ -231,7 +247,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       mbar_arrive(q_full);
     }
     float m = -INFINITY, base_ = 0.0f, l = 0.0f;
-    int vexp = -100;
+    int vexp = -1000;
     bool ok = true;
     for (int t = 0; t < n && ok; t++) {
       const uint32_t S = tS + 128u * (t & 1) + lanes;
@@ -240,8 +256,8 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       float s[64];
 #pragma unroll
       for (int i = 0; i < 2; i++) kp_ld32(S + 64 * half + 32 * i, s + 32 * i);
-      const float f = Q4 ? fmul(unscale, s_kscale[t & 3]) : unscale;
-      const int ve = Q4 ? s_vexp[t & 3] : 0;
+      const float f = SCALED ? fmul(unscale, s_kscale[t & 3]) : unscale;
+      const int ve = SCALED ? s_vexp[t & 3] : 0;
       const int key0 = key_of(t);
       const bool sink = t0 + t < sink_tiles;
       if (sink ? key0 + KP_KEYS > sk : key0 < max_lo || key0 + KP_KEYS > min_hi) {
@@ -265,34 +281,47 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       kp_bar(2, 256);
       ok = s_ok[t & 1];  // one thread's look, so that all leave the loop together
       top = fmaxf(top, s_top[t & 1][half ^ 1][r]);
-      if (__any_sync(0xffffffffu, top > fadd(m, 8.0f) || ve > vexp)) {
+      const bool grow = __any_sync(0xffffffffu, top > fadd(m, 8.0f) || ve > vexp);
+      const bool flush = t > 0 && t % KP_FLUSH == 0;
+      float go = 1.0f;  // the outputs so far, in the new units
+      if (grow) {
         const float mn = fmaxf(m, top);
         const float nb = mn == -INFINITY ? 0.0f : fsub(mn, 6.0f);
         const float g = m == -INFINITY ? 0.0f : exp2_approx(fsub(base_, nb));
         const int ne = max(vexp, ve);
         l = fmul(l, g);
-        if (t > 0) {
-          const float go = fmul(g, pow2f(max(vexp - ne, -120)));
-          // the outputs so far: O(t-2) is complete with these scores, O(t-1) is waited
-          // for, and O(t) waits for this thread
-          if (ok && !mbar_wait(v_empty, (t - 1) & 1, &s_err)) fail();
-          tc_fence_after();
-          if (__any_sync(0xffffffffu, go != 1.0f)) {
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-              const uint32_t at = tO + lanes + 64 * half + 32 * i;
-              float o[32];
-              kp_ld32(at, o);
-#pragma unroll
-              for (int j = 0; j < 32; j++) o[j] = fmul(o[j], go);
-              kp_st16(at, reinterpret_cast<uint32_t*>(o));
-              kp_st16(at + 16, reinterpret_cast<uint32_t*>(o) + 16);
-            }
-          }
-        }
+        go = fmul(g, pow2f(max(vexp - ne, -120)));
         m = mn;
         base_ = nb;
         vexp = ne;
+      }
+      if (t > 0 && (flush || __any_sync(0xffffffffu, go != 1.0f))) {
+        // O(t-2) is complete with these scores, O(t-1) is waited for, and O(t)
+        // waits for this thread
+        if (ok && !mbar_wait(v_empty, (t - 1) & 1, &s_err)) fail();
+        tc_fence_after();
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          const uint32_t at = tO + lanes + 64 * half + 32 * i;
+          float4* sum = reinterpret_cast<float4*>(s_sum + r * KP_SUM_STRIDE + 64 * half + 32 * i);
+          float o[32];
+          kp_ld32(at, o);
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            float4 x = t > KP_FLUSH ? sum[j] : make_float4(0.f, 0.f, 0.f, 0.f);
+            if (flush)
+              x = make_float4(fadd(x.x, o[4 * j]), fadd(x.y, o[4 * j + 1]), fadd(x.z, o[4 * j + 2]),
+                              fadd(x.w, o[4 * j + 3]));
+            if (flush || t > KP_FLUSH)
+              sum[j] = make_float4(fmul(x.x, go), fmul(x.y, go), fmul(x.z, go), fmul(x.w, go));
+          }
+          if (!flush) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) o[j] = fmul(o[j], go);
+            kp_st16(at, reinterpret_cast<uint32_t*>(o));
+            kp_st16(at + 16, reinterpret_cast<uint32_t*>(o) + 16);
+          }
+        }
       }
       // weights times the V tile's own power of two over the outputs'
       const float shift = fsub((float)(ve - vexp), base_);
@@ -333,6 +362,17 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
     if (ok && n > 0) {
 #pragma unroll
       for (int i = 0; i < 2; i++) kp_ld32(tO + lanes + 64 * half + 32 * i, o + 32 * i);
+      if (n > KP_FLUSH) {
+        const float4* sum = reinterpret_cast<const float4*>(s_sum + r * KP_SUM_STRIDE + 64 * half);
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+          const float4 x = sum[j];
+          o[4 * j] = fadd(o[4 * j], x.x);
+          o[4 * j + 1] = fadd(o[4 * j + 1], x.y);
+          o[4 * j + 2] = fadd(o[4 * j + 2], x.z);
+          o[4 * j + 3] = fadd(o[4 * j + 3], x.w);
+        }
+      }
     }
     if (live) {
       const float back = ok ? (n > 0 ? pow2f(max(vexp, -120)) : 0.0f) : NAN;
@@ -364,14 +404,15 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
     // =========================================================== converters
     const int w = tid - 256, cw = warp - 8;
     const int kg = w >> 3, vn = w & 7;   // V: keys 8 kg .. 8 kg + 7, byte column vn
-    constexpr int KR = Q4 ? 4 : 8;       // 16-byte loads of a K row
+    constexpr int KR = Q4 ? 4 : WIDE ? 1 : 8;  // 16-byte loads of a K row held a tile ahead
     uint4 kraw[KR];
     uint2 kd = make_uint2(0, 0);
     constexpr int VR = Q4 ? 4 : 8;       // 16 bytes each: two keys' 8 (4-bit), one key's 16
     uint4 vraw[VR];
     uint2 vd[8], vd_next[8];             // 4-bit: V scales of the thread's eight keys, this tile and the next
-    const size_t hb = Q4 ? q4_row(a.c, 0, head) * 64 : (size_t)head * 128;
-    const int64_t step = Q4 ? 64 : (int64_t)a.c.n_kv_heads * 128;
+    constexpr int ROW = Q4 ? 64 : KV == FLOCK_KV_FP8 ? 128 : KV == FLOCK_KV_BF16 ? 256 : 512;
+    const size_t hb = Q4 ? q4_row(a.c, 0, head) * 64 : (size_t)head * ROW;
+    const int64_t step = Q4 ? 64 : (int64_t)a.c.n_kv_heads * ROW;
     const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + hb;
     const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + hb;
     const uint16_t* ks = Q4 ? a.c.ks + q4_row(a.c, 0, head) * 4 : nullptr;
@@ -383,6 +424,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       to = sink ? sk : hi;
     };
     auto load_k = [&](int t) {
+      if (WIDE) return;
       int from, to;
       range(t, from, to);
       const int key = key_of(t) + w;
@@ -405,6 +447,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       }
     };
     auto load_v = [&](int t) {
+      if (WIDE) return;
       int from, to;
       range(t, from, to);
 #pragma unroll
@@ -427,11 +470,69 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         }
       }
     };
+    // f32 and bf16 rows are too long to hold: read for the tile's largest
+    // magnitude, and again (from L2) when their buffer is free.
+    auto wide4 = [&](const uint8_t* base, int key, int from, int to, int d) {
+      if (key < from || key >= to) return make_float4(0.f, 0.f, 0.f, 0.f);
+      const uint8_t* row = base + (int64_t)key * step;
+      if constexpr (KV == FLOCK_KV_BF16) {
+        const uint2 x = __ldg(reinterpret_cast<const uint2*>(row + 2 * d));
+        const float2 lo2 = bf16x2_widen(x.x), hi2 = bf16x2_widen(x.y);
+        return make_float4(lo2.x, lo2.y, hi2.x, hi2.y);
+      } else {
+        return __ldg(reinterpret_cast<const float4*>(row + 4 * d));
+      }
+    };
+    int vrun = -1000;  // the largest exponent of a V tile so far
     // A tile's scales times 2^e lie below 2^10, so a value (below 2^13) keeps
     // its lo part; e as far as f16 can hold 2^e.
     uint32_t knorm = 0, vnorm = 0;  // f16 pairs 2^e of the K and the V tile last looked at
     auto norms = [&](int t) {
-      if (!Q4) return;
+      if (!SCALED) return;
+      if (WIDE) {
+        int from, to;
+        range(t, from, to);
+        auto mag = [](uint32_t m, float4 x) {
+          const uint32_t y = 0x7FFFFFFFu;
+          return max(max(m, max(__float_as_uint(x.x) & y, __float_as_uint(x.y) & y)),
+                     max(__float_as_uint(x.z) & y, __float_as_uint(x.w) & y));
+        };
+        uint32_t bk = 0, bv = 0;
+#pragma unroll 8
+        for (int d = 0; d < 128; d += 4) bk = mag(bk, wide4(kb, key_of(t) + w, from, to, d));
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+          for (int d = 0; d < 16; d += 4)
+            bv = mag(bv, wide4(vb, key_of(t) + 8 * kg + i, from, to, 16 * vn + d));
+        bk = __reduce_max_sync(0xffffffffu, bk);
+        bv = __reduce_max_sync(0xffffffffu, bv);
+        if (lane == 0) {
+          s_dmax[0][cw] = bk;
+          s_dmax[1][cw] = bv;
+        }
+        kp_bar(1, 128);
+        uint32_t mk = 0, mv = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          mk = max(mk, s_dmax[0][i]);
+          mv = max(mv, s_dmax[1][i]);
+        }
+        kp_bar(1, 128);  // read before the next tile's are written
+        // magnitudes lie below 2^(exponent field - 126): times 2^e below 2^13
+        auto exponent = [](uint32_t m) { return max(-120, min(120, 139 - (int)(m >> 23))); };
+        const int ek = exponent(mk);
+        // a tile of far smaller values than an earlier one need not fill f16
+        vrun = max(vrun, -exponent(mv));
+        const int ev = -max(-exponent(mv), vrun - 30);
+        knorm = __float_as_uint(pow2f(ek));
+        vnorm = __float_as_uint(pow2f(ev));
+        if (w == 0) {
+          s_kscale[t & 3] = pow2f(-ek);
+          s_vexp[t & 3] = -ev;
+        }
+        return;
+      }
       auto top = [](__half2 h, uint2 d) {
         return __hmax2(h, __hmax2(__habs2(as_h2(d.x)), __habs2(as_h2(d.y))));
       };
@@ -464,8 +565,24 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         s_vexp[t & 3] = -ev;
       }
     };
-    auto put_k = [&]() {
-      if (Q4) {
+    auto put_k = [&](int t) {
+      if constexpr (WIDE) {
+        int from, to;
+        range(t, from, to);
+        const float f = __uint_as_float(knorm);
+#pragma unroll 4
+        for (int c = 0; c < 16; c++) {
+          const float4 x = wide4(kb, key_of(t) + w, from, to, 8 * c);
+          const float4 y = wide4(kb, key_of(t) + w, from, to, 8 * c + 4);
+          uint32_t h[4], l[4];
+          split_f16(fmul(x.x, f), fmul(x.y, f), h[0], l[0]);
+          split_f16(fmul(x.z, f), fmul(x.w, f), h[1], l[1]);
+          split_f16(fmul(y.x, f), fmul(y.y, f), h[2], l[2]);
+          split_f16(fmul(y.z, f), fmul(y.w, f), h[3], l[3]);
+          *reinterpret_cast<uint4*>(sKh + kp_off(w, c)) = make_uint4(h[0], h[1], h[2], h[3]);
+          if (LO) *reinterpret_cast<uint4*>(sKl + kp_off(w, c)) = make_uint4(l[0], l[1], l[2], l[3]);
+        }
+      } else if constexpr (Q4) {
         const uint32_t d01 = hmul2_u(kd.x, knorm), d23 = hmul2_u(kd.y, knorm);
 #pragma unroll
         for (int b = 0; b < 4; b++) {
@@ -495,8 +612,31 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         }
       }
     };
-    auto put_v = [&](uint32_t norm) {
-      if (Q4) {
+    auto put_v = [&](int t, uint32_t norm) {
+      if constexpr (WIDE) {
+        int from, to;
+        range(t, from, to);
+        const float f = __uint_as_float(norm);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {  // dimensions 16 vn + 4 i ..
+          float4 x[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            x[j] = wide4(vb, key_of(t) + 8 * kg + j, from, to, 16 * vn + 4 * i);
+          auto at = [&](int j, int e) {
+            return fmul(e == 0 ? x[j].x : e == 1 ? x[j].y : e == 2 ? x[j].z : x[j].w, f);
+          };
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) split_f16(at(2 * j, e), at(2 * j + 1, e), h[j], l[j]);
+            const uint32_t off = kp_off(8 * (4 * i + e) + vn, kg);
+            *reinterpret_cast<uint4*>(sVh + off) = make_uint4(h[0], h[1], h[2], h[3]);
+            if (LO) *reinterpret_cast<uint4*>(sVl + off) = make_uint4(l[0], l[1], l[2], l[3]);
+          }
+        }
+      } else if constexpr (Q4) {
 #pragma unroll
         for (int b = 0; b < 4; b++) {
           const uint32_t sel = b & 1 ? 0x7632u : 0x5410u;
@@ -558,7 +698,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
     auto k_tile = [&](int t) {
       norms(t);
       if (t > 0) wait(k_empty, (t - 1) & 1);
-      if (ok) put_k();
+      if (ok) put_k(t);
       fence_proxy_async_smem();
       mbar_arrive(k_full);
       if (t + 1 < n) load_k(t + 1);
@@ -574,7 +714,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
     for (int t = 0; t < n; t++) {
       if (t + 1 < n) k_tile(t + 1);
       if (t > 0) wait(v_empty, (t - 1) & 1);
-      if (ok) put_v(vnorm_t);
+      if (ok) put_v(t, vnorm_t);
       fence_proxy_async_smem();
       mbar_arrive(v_full);
       if (t + 1 < n) {
@@ -598,9 +738,9 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         if (!ok) return;
         tc_fence_after();
         const uint32_t d = tS + 128u * (t & 1);
-        kp_mma(d, tQ, smem_u32(sKh), false);
-        kp_mma(d, tQ + 64, smem_u32(sKh), true);
-        if (Q4) kp_mma(d, tQ, smem_u32(sKl), true);
+        kp_mma(d, tQ + 64, smem_u32(sKh), false);  // the small products first
+        if (LO) kp_mma(d, tQ, smem_u32(sKl), true);
+        kp_mma(d, tQ, smem_u32(sKh), true);
         umma_commit(k_empty);
         umma_commit(s_full + (t & 1));
       };
@@ -616,9 +756,9 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         if (!ok) break;
         tc_fence_after();
         const uint32_t P = tS + 128u * (t & 1);
-        kp_mma(tO, P, smem_u32(sVh), t > 0);
-        kp_mma(tO, P + 64, smem_u32(sVh), true);
-        if (Q4) kp_mma(tO, P, smem_u32(sVl), true);
+        kp_mma(tO, P + 64, smem_u32(sVh), t % KP_FLUSH != 0);
+        if (LO) kp_mma(tO, P, smem_u32(sVl), true);
+        kp_mma(tO, P, smem_u32(sVh), true);
         umma_commit(v_empty);
       }
       if (!ok) {  // let what was issued finish before the memory is given back
