@@ -20,12 +20,12 @@
 // of 8 bits.  The parts sit in neighbouring COLUMNS, which a lane's accumulator
 // holds side by side: one instruction multiplies both, an addition joins them.
 //
-// 4-bit blocks.  Scores: a code c in an f16's low bits is the subnormal c
-// 2^-24, an operand for one AND; sum (c - 8) q = sum c q - 8 sum q, the second
-// term being a constant of the query that the accumulator starts from.  A
-// block's sum is multiplied by the key's scale in f32.  Values: codes minus 8
-// (over many keys the uncentred sum would cancel), the scale joins the weight,
-// so the weight operand differs per block.
+// 4-bit blocks.  Codes minus 8 are the operands.  (A code left in an f16's low
+// bits is the subnormal c 2^-24 and needs no more than an AND, but the tensor
+// cores align a subnormal's product as if it were normal and drop the bits below:
+// errors of 3e-6 instead of 3e-7.)  A block's products are multiplied by the
+// key's scale in f32, one accumulator per block.  Values: the scale joins the
+// weight, so the weight operand differs per block.
 //
 // Work split: CTA (split z, row tile, kv head), its warps taking 16-key groups
 // in turn, each with its own cp.async ring, running maximum, sum and output;
@@ -49,12 +49,6 @@ struct KvRowsArgs {
   float* part;      // [item][split][RT][128], then [item][split][RT][2] (m, l)
 };
 
-#ifndef KR_W1
-#define KR_W1 16
-#define KR_S1 5
-#define KR_W2 12
-#define KR_S2 5
-#endif
 // Shared-memory layout of one warp's 16-key stage, per cached type, for NT
 // column tiles.  Key rows are read 16 bytes a lane, eight lanes covering 64
 // bytes of two keys; value rows 8 or 16 bytes a lane, eight lanes covering
@@ -63,8 +57,7 @@ template <int KV, int NT>
 struct KrTile;
 template <int NT>
 struct KrTile<FLOCK_KV_Q4, NT> {
-  static constexpr int ROW = 64, K_STRIDE = 64, WARPS = NT == 1 ? KR_W1 : KR_W2,
-                       STAGES = NT == 1 ? KR_S1 : KR_S2;
+  static constexpr int ROW = 64, K_STRIDE = 64, WARPS = NT == 1 ? 16 : 12, STAGES = 5;
   static constexpr int SCALES = 2 * KR_GROUP * 8;
 };
 template <int NT>
@@ -191,15 +184,6 @@ FLOCK_DEV uint32_t movm(uint32_t a) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
   return r;
 }
-// The eight codes of a word as f16 pairs of the subnormals c 2^-24 (v[0],
-// v[2]) and 16 c 2^-24 (v[1], v[3]).  v[e]: bits 4 e .. 4 e + 3 of both halfwords.
-FLOCK_DEV void nib_sub(uint32_t w, uint32_t (&v)[4]) {
-  const uint32_t hi = w >> 8;
-  v[0] = w & 0x000F000Fu;
-  v[1] = w & 0x00F000F0u;
-  v[2] = hi & 0x000F000Fu;
-  v[3] = hi & 0x00F000F0u;
-}
 // The eight codes of a word -> (code - 8) as four f16 pairs: 0x6400 | code is
 // the f16 1024 + code, 0x6400 | 16 code is 1024 + 16 code, and the rest is
 // taken off exactly.  v[e]: bits 4 e .. 4 e + 3 of both halfwords.
@@ -266,11 +250,6 @@ FLOCK_DEV uint32_t word_of(const uint4& v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
-#ifdef KR_TRACE
-#define KT(i) if (threadIdx.x == 0) { reinterpret_cast<unsigned long long*>(p.part)[700000 + ((blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * 8 + (i)] = globaltimer_ns(); }
-#else
-#define KT(i)
-#endif
 // Lane (g, c) = (lane / 4, lane % 4).  Scores: keys g and g + 8 of the stage,
 // query row c of each column tile (f16: tile n holds rows 4 n .. 4 n + 3 as hi,
 // lo columns; bf16: tile 0 hi, mid and tile 1 lo of rows 0-3).
@@ -285,12 +264,10 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
   extern __shared__ __align__(16) uint8_t kr_smem[];
   __shared__ float s_ml[L::WARPS][RT][2];
   __shared__ uint2 s_q[NT][8][32];    // the query operand: [tile][QK step][lane]
-  __shared__ float s_corr[RT][4];     // 4-bit: -8 2^-24 sum of a block's query parts
   __shared__ float s_unscale[RT];
   __shared__ int s_last;
   pdl_launch_dependents();
   pdl_wait();
-  KT(0);
   const KvAttnArgs& a = p.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
@@ -371,9 +348,8 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
       const int biased = (int)(__float_as_uint(top) >> 23);
-      const int e = biased == 0 ? 0 : max(-90, min(90, biased - 127 - 13));
-      // high nibbles (4-bit, odd steps) are read as 16 c
-      const float scale = __uint_as_float((uint32_t)(127 - e - (Q4 && (ks & 1) ? 4 : 0)) << 23);
+      const int e = biased == 0 ? 0 : max(-100, min(100, biased - 127 - 13));
+      const float scale = __uint_as_float((uint32_t)(127 - e) << 23);
       if (Q4) {  // pairs two apart: bytes 0 and 2, 1 and 3 of a code word
         const float y = x.y;
         x.y = x.z;
@@ -384,20 +360,7 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
       split_f16(fmul(x.z, scale), fmul(x.w, scale), h.y, l.y);
       s_q[r / 4][ks][4 * (2 * (r % 4)) + qc] = h;
       s_q[r / 4][ks][4 * (2 * (r % 4) + 1) + qc] = l;
-      if (Q4) {
-        float sum = 0.0f;
-        const uint32_t parts[4] = {l.x, l.y, h.x, h.y};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float2 f = h2f2(parts[i]);
-          sum = fadd(sum, fadd(f.x, f.y));
-        }
-        sum = ks & 1 ? fmul(sum, 16.0f) : sum;
-#pragma unroll
-        for (int d = 1; d < 8; d <<= 1) sum = fadd(sum, __shfl_xor_sync(0xffffffffu, sum, d));
-        if ((lane & 7) == 0) s_corr[r][lane >> 3] = fmul(sum, -4.76837158203125e-7f);  // -8 2^-24
-      }
-      if (lane == 0) s_unscale[r] = __uint_as_float((uint32_t)(127 + e + (Q4 ? 24 : 0)) << 23);
+      if (lane == 0) s_unscale[r] = __uint_as_float((uint32_t)(127 + e) << 23);
     } else {
       uint32_t w0[3], w1[3];
       split_bf16(x.x, x.y, w0);
@@ -409,19 +372,14 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
     }
   }
   __syncthreads();
-  KT(1);
   uint2 qb[NT][8];
-  float unscale[RL], corr[RL][4];
+  float unscale[RL];
 #pragma unroll
   for (int n = 0; n < NT; n++)
 #pragma unroll
     for (int ks = 0; ks < 8; ks++) qb[n][ks] = s_q[n][ks][lane];
 #pragma unroll
-  for (int n = 0; n < RL; n++) {
-    unscale[n] = F16 ? s_unscale[4 * n + c] : 1.0f;
-#pragma unroll
-    for (int b = 0; b < 4; b++) corr[n][b] = Q4 ? s_corr[4 * n + c][b] : 0.0f;
-  }
+  for (int n = 0; n < RL; n++) unscale[n] = F16 ? s_unscale[4 * n + c] : 1.0f;
   float o[8][NT][4];
 #pragma unroll
   for (int u = 0; u < 8; u++)
@@ -446,7 +404,6 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
   int st = 0;
   for (int grp = g0 + warp; grp < g1; grp += L::WARPS) {
     cp_async_wait<L::STAGES - 2>();
-    KT(2);
     __syncwarp();  // the stage has landed for every lane, and every lane is done with the last one
     fetch(grp + (L::STAGES - 1) * L::WARPS, st == 0 ? L::STAGES - 1 : st - 1);
     const uint8_t* stage = kr_smem + (warp * L::STAGES + st) * L::STAGE;
@@ -461,14 +418,14 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
 #pragma unroll
       for (int b = 0; b < 4; b++) {
         uint32_t x[4], y[4];
-        nib_sub(word_of(w0, b), x);
-        nib_sub(word_of(w1, b), y);
+        nib_f16(word_of(w0, b), x);
+        nib_f16(word_of(w1, b), y);
         const float2 d0 = h2f2(b < 2 ? e0.x : e0.y), d1 = h2f2(b < 2 ? e1.x : e1.y);
 #pragma unroll
         for (int n = 0; n < NT; n++) {
           float acc[4];
           const uint32_t a0[4] = {x[0], y[0], x[2], y[2]}, a1[4] = {x[1], y[1], x[3], y[3]};
-          mma16<F16>(acc, a0, qb[n][2 * b].x, qb[n][2 * b].y, corr[n][b], 0.f, corr[n][b], 0.f);
+          mma16<F16>(acc, a0, qb[n][2 * b].x, qb[n][2 * b].y, 0.f, 0.f, 0.f, 0.f);
           mma16<F16>(acc, a1, qb[n][2 * b + 1].x, qb[n][2 * b + 1].y);
           s[n][0] = ffma(b & 1 ? d0.y : d0.x, fadd(acc[0], acc[1]), s[n][0]);
           s[n][1] = ffma(b & 1 ? d1.y : d1.x, fadd(acc[2], acc[3]), s[n][1]);
@@ -712,7 +669,6 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
     st = st + 1 == L::STAGES ? 0 : st + 1;
   }
   cp_async_wait<0>();
-  KT(3);
 
   // ---------------------------------------------------------- join the warps
   constexpr int OS = KV_HD + 4;  // row stride of the warps' outputs
@@ -741,7 +697,6 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
     }
   }
   __syncthreads();
-  KT(4);
   const int item = head * gridDim.y + tile;
   const int n_items = gridDim.y * gridDim.z;
   float* part_ml = p.part + (size_t)n_items * p.splits * RT * KV_HD;
@@ -776,7 +731,6 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
   // one release-acquire arrival per CTA, behind the barrier that orders its
   // threads' stores before it
   __syncthreads();
-  KT(5);
   if (threadIdx.x == 0) {
     uint32_t before;
     asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;"
@@ -785,7 +739,6 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
     if (s_last) p.count[item] = 0;  // ready for the next call
   }
   __syncthreads();
-  KT(6);
   if (!s_last) return;
   // Thread (k, four outputs): the splits k, k + PAR, .. of them, all loads in
   // flight before the first use; the splits' factors 2^(m_s - m) meanwhile.
@@ -854,7 +807,6 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
                                ((int64_t)head * p.group + rr % p.group) * KV_HD + d) =
         make_float4(fmul(oo.x, inv), fmul(oo.y, inv), fmul(oo.z, inv), fmul(oo.w, inv));
   }
-  KT(7);
 }
 
 }  // namespace flock
