@@ -118,6 +118,7 @@ SIGNATURES = {
     "flock_layer_reset": [_vp],
     "flock_layer_n_keys": [_vp, _ip],
     "flock_layer_rewind": [_vp, _i],
+    "flock_layer_set_window": [_vp, _i, _i],
     "flock_layer_read_cache": [_vp, _fp, _fp],
     "flock_layer_write_cache": [_vp, _fp, _fp, _i],
     "flock_range_forward": [_pp, _i, _fp, _i, _i, _i, _fp],
@@ -154,6 +155,7 @@ SIGNATURES = {
     "flock_model_rewind": [_vp, _i],
     "flock_model_pos": [_vp, _ip],
     "flock_model_held": [_vp, _ip],
+    "flock_model_set_window": [_vp, _i, _i],
     "flock_model_set_token": [_vp, ctypes.c_int32],
     "flock_model_set_decode_mode": [_vp, _i],
     "flock_model_get_decode_mode": [_vp, _ip],

@@ -21,6 +21,7 @@
 #include "flock_internal.h"
 #include "gemv.cuh"
 #include "gemv_fast.cuh"
+#include "kv_layer.h"
 #include "ops.cuh"
 
 namespace flock {
@@ -372,8 +373,10 @@ static int check_cfg(const flock_layer_config& c) {
               c.ffn);
     return FLOCK_E_UNSUPPORTED;
   }
-  if (c.kv_dtype != FLOCK_KV_F32 && c.kv_dtype != FLOCK_KV_BF16 && c.kv_dtype != FLOCK_KV_FP8) {
-    set_error("kv_dtype %d is not FLOCK_KV_F32, FLOCK_KV_BF16 or FLOCK_KV_FP8", c.kv_dtype);
+  if (c.kv_dtype != FLOCK_KV_F32 && c.kv_dtype != FLOCK_KV_BF16 && c.kv_dtype != FLOCK_KV_FP8 &&
+      c.kv_dtype != FLOCK_KV_Q4) {
+    set_error("kv_dtype %d is not FLOCK_KV_F32, FLOCK_KV_BF16, FLOCK_KV_FP8 or FLOCK_KV_Q4",
+              c.kv_dtype);
     return FLOCK_E_ARG;
   }
   if (c.matvec != FLOCK_MATVEC_EXACT && c.matvec != FLOCK_MATVEC_FAST) {
@@ -383,7 +386,7 @@ static int check_cfg(const flock_layer_config& c) {
   if (c.kv_dtype != FLOCK_KV_F32 &&
       (c.attention != FLOCK_ATTN_FAST || c.prefill != FLOCK_PREFILL_TENSOR)) {
     set_error("a %s KV cache needs FLOCK_ATTN_FAST and FLOCK_PREFILL_TENSOR (the exact "
-              "kernels read f32)", c.kv_dtype == FLOCK_KV_BF16 ? "bf16" : "fp8");
+              "kernels read f32)", kv_dtype_name(c.kv_dtype));
     return FLOCK_E_UNSUPPORTED;
   }
   if (c.attention == FLOCK_ATTN_EXACT && c.max_keys > 48 * 1024) {
@@ -394,14 +397,28 @@ static int check_cfg(const flock_layer_config& c) {
   return FLOCK_OK;
 }
 
+static int kv_workspace(Workspace* ws) {
+  if (ws->kv_ws.p) return FLOCK_OK;
+  FLOCK_TRY(ws->kv_ws.alloc(FLOCK_WORKSPACE_BYTES));
+  FLOCK_CK(cudaMemset(ws->kv_ws.p, 0, FLOCK_WORKSPACE_BYTES));
+  FLOCK_CK(cudaStreamSynchronize(nullptr));
+  return FLOCK_OK;
+}
+
 int layer_init(flock_layer* L, flock_dev* dev, const flock_layer_config& cfg, Workspace* ws,
                int* shared_ctl) {
   FLOCK_TRY(check_cfg(cfg));
   L->dev = dev_retain(dev);
   L->cfg = cfg;
-  const size_t kv = (size_t)cfg.max_keys * cfg.n_kv_heads * cfg.head_dim * kv_elem_bytes(cfg);
+  const size_t values = (size_t)kv_capacity(cfg) * cfg.n_kv_heads * cfg.head_dim;
+  const bool q4 = cfg.kv_dtype == FLOCK_KV_Q4;
+  const size_t kv = q4 ? values / 2 : values * kv_elem_bytes(cfg);
   FLOCK_TRY(L->kcache.alloc(kv));
   FLOCK_TRY(L->vcache.alloc(kv));
+  if (q4) {
+    FLOCK_TRY(L->kscales.alloc(values / 32 * sizeof(uint16_t)));
+    FLOCK_TRY(L->vscales.alloc(values / 32 * sizeof(uint16_t)));
+  }
   std::vector<float> inv(cfg.head_dim / 2);
   // layer.ts:180 invFreqOf: fr(1 / base^(2j/headDim)), on the host.
   for (int j = 0; j < cfg.head_dim / 2; j++)
@@ -423,7 +440,36 @@ int layer_init(flock_layer* L, flock_dev* dev, const flock_layer_config& cfg, Wo
     L->ws = &L->ws_own;
     L->owns_ws = true;
   }
+  if (q4) FLOCK_TRY(kv_workspace(L->ws));
   return FLOCK_OK;
+}
+
+int layer_set_window(flock_layer* L, int window, int sinks) {
+  if (window < 0 || sinks < 0 || (window == 0 && sinks > 0)) {
+    set_error("window %d and sinks %d must not be negative, sinks 0 without a window", window,
+              sinks);
+    return FLOCK_E_ARG;
+  }
+  if (window > 0 && L->cfg.attention != FLOCK_ATTN_FAST) {
+    set_error("a window needs FLOCK_ATTN_FAST (the exact kernels read every key)");
+    return FLOCK_E_UNSUPPORTED;
+  }
+  if (window > 0) FLOCK_TRY(kv_workspace(L->ws));
+  L->window = window;
+  L->sinks = sinks;
+  return FLOCK_OK;
+}
+
+// The layer's cache as flock_kv.cu's kernels see it.
+static KvView layer_kv_view(const flock_layer* L) {
+  KvView c = {};
+  c.k = L->kcache.p;
+  c.v = L->vcache.p;
+  c.ks = L->kscales.as<uint16_t>();
+  c.vs = L->vscales.as<uint16_t>();
+  c.capacity = kv_capacity(L->cfg);
+  c.n_kv_heads = L->cfg.n_kv_heads;
+  return c;
 }
 
 // q/k norm + RoPE + KV append, then attention over n >= 1 queries: in
@@ -451,7 +497,8 @@ static int enqueue_qk_attn(flock_layer* L, int n, bool pdl, bool tensor_cores) {
   qa.neox = c.rope_pairing == FLOCK_ROPE_NEOX;
   pf_add(qa.pf, L->w[W_GATE]);
   const int img_tiles = (c.max_keys + ATC_K - 1) / ATC_K;
-  if (n > 1 && tensor_cores) {
+  const bool kv_ops = layer_uses_kv_ops(L);
+  if (n > 1 && tensor_cores && !kv_ops) {
     qa.kv_img = ws->kv_img.as<uint8_t>();
     qa.img_tiles = img_tiles;
     qa.q_img = ws->q_img.as<uint8_t>();
@@ -460,16 +507,33 @@ static int enqueue_qk_attn(flock_layer* L, int n, bool pdl, bool tensor_cores) {
   qa.rope_cs = ws->rope.as<float2>();
   qa.rope_rows = ws->rope_rows;
   const int kv = c.kv_dtype;
-  if (kv != FLOCK_KV_F32 && !(n > 1 && tensor_cores)) {
+  if (kv != FLOCK_KV_F32 && !(n > 1 && tensor_cores) && !kv_ops) {
     set_error("a %s KV cache runs decode on FLOCK_ATTN_FAST and prefill on the tensor cores",
-              kv == FLOCK_KV_BF16 ? "bf16" : "fp8");
+              kv_dtype_name(kv));
     return FLOCK_E_UNSUPPORTED;
   }
+  if (kv == FLOCK_KV_Q4) qa.q4 = layer_kv_view(L);
   FLOCK_CK(launch_ex(d->stream,
-                     kv == FLOCK_KV_FP8 ? k_qk_norm_rope_append<FLOCK_KV_FP8>
+                     kv == FLOCK_KV_Q4 ? k_qk_norm_rope_append<FLOCK_KV_Q4>
+                     : kv == FLOCK_KV_FP8 ? k_qk_norm_rope_append<FLOCK_KV_FP8>
                      : kv == FLOCK_KV_BF16 ? k_qk_norm_rope_append<FLOCK_KV_BF16>
                                            : k_qk_norm_rope_append<FLOCK_KV_F32>,
                      dim3((n * (c.n_heads + c.n_kv_heads) + 7) / 8), dim3(256), 0, pdl, qa));
+  if (kv_ops) {
+    KvAttnArgs ka = {};
+    ka.c = layer_kv_view(L);
+    ka.q = ws->qn.as<float>();
+    ka.out = ws->attn.as<float>();
+    ka.q_stride = ka.out_stride = (int64_t)c.n_heads * c.head_dim;
+    ka.ctl = L->ctl;  // the position; below, the bound that sizes the launch
+    ka.pos = n == 1 ? c.max_keys - 1 : L->n_keys;
+    ka.n_queries = n;
+    ka.n_heads = c.n_heads;
+    ka.window = L->window;
+    ka.sinks = L->sinks;
+    ws->atc_nz = 1;
+    return kv_attention_enqueue(d->sm_count, kv, ka, ws->kv_ws.as<uint8_t>(), d->stream);
+  }
   AttnArgs aa = {};
   aa.q = ws->qn.as<float>();
   aa.kcache = L->kcache.as<float>();
@@ -718,7 +782,7 @@ int layer_enqueue(flock_layer* L, int n, bool advance, const PrefetchList& pf_ne
     FLOCK_TRY(launch_gemv(d, QT_Q8, EPI_STORE, a, pdl));
   }
   // 2-3. q/k norm + RoPE + KV append, attention
-  if (n == 1 && c.attention == FLOCK_ATTN_FAST) {
+  if (n == 1 && c.attention == FLOCK_ATTN_FAST && !layer_uses_kv_ops(L)) {
     AttnFastArgs a = {};
     a.q = ws->q.as<float>();
     a.k = ws->k.as<float>();
@@ -1555,6 +1619,16 @@ int flock_layer_rewind(flock_layer* L, int n_keys) {
   return FLOCK_OK;
 }
 
+int flock_layer_set_window(flock_layer* L, int window, int sinks) {
+  if (!L) return FLOCK_E_ARG;
+  if (!L->owns_ws) {
+    set_error("this layer belongs to a model: use flock_model_set_window");
+    return FLOCK_E_STATE;
+  }
+  FLOCK_CK(cudaSetDevice(L->dev->ordinal));
+  return layer_set_window(L, window, sinks);
+}
+
 int flock_layer_reset(flock_layer* L) { return flock_layer_rewind(L, 0); }
 
 int flock_layer_n_keys(const flock_layer* L, int* out) {
@@ -1595,7 +1669,18 @@ static uint8_t host_fp8_bits(float x) {
 int flock_layer_read_cache(flock_layer* L, float* k, float* v) {
   if (!L || !k || !v) return FLOCK_E_ARG;
   const size_t count = (size_t)L->n_keys * L->cfg.n_kv_heads * L->cfg.head_dim;
-  if (count && L->cfg.kv_dtype == FLOCK_KV_FP8) {
+  if (count && L->cfg.kv_dtype == FLOCK_KV_Q4) {
+    FLOCK_CK(cudaSetDevice(L->dev->ordinal));
+    DBuf kd, vd;
+    FLOCK_TRY(kd.alloc(count * 4));
+    FLOCK_TRY(vd.alloc(count * 4));
+    k_kv_read<FLOCK_KV_Q4><<<dim3((L->n_keys + 7) / 8, L->cfg.n_kv_heads), 256, 0, L->dev->stream>>>(
+        layer_kv_view(L), 0, L->n_keys, kd.as<float>(), vd.as<float>());
+    FLOCK_CK(cudaGetLastError());
+    FLOCK_CK(cudaMemcpyAsync(k, kd.p, count * 4, cudaMemcpyDeviceToHost, L->dev->stream));
+    FLOCK_CK(cudaMemcpyAsync(v, vd.p, count * 4, cudaMemcpyDeviceToHost, L->dev->stream));
+    FLOCK_CK(cudaStreamSynchronize(L->dev->stream));  // before the copies' sources go
+  } else if (count && L->cfg.kv_dtype == FLOCK_KV_FP8) {
     // e4m3 -> f32 exactly
     std::vector<uint8_t> kb(count), vb(count);
     FLOCK_CK(cudaMemcpyAsync(kb.data(), L->kcache.p, count, cudaMemcpyDeviceToHost,
@@ -1640,7 +1725,19 @@ int flock_layer_write_cache(flock_layer* L, const float* k, const float* v, int 
   if (!L || !k || !v || n_keys < 0 || L->n_keys + n_keys > L->cfg.max_keys) return FLOCK_E_ARG;
   const size_t elems = (size_t)L->cfg.n_kv_heads * L->cfg.head_dim;
   const size_t row = elems * kv_elem_bytes(L->cfg);
-  if (L->cfg.kv_dtype == FLOCK_KV_FP8) {
+  if (n_keys > 0 && L->cfg.kv_dtype == FLOCK_KV_Q4) {
+    FLOCK_CK(cudaSetDevice(L->dev->ordinal));
+    DBuf kd, vd;
+    FLOCK_TRY(kd.alloc(elems * n_keys * 4));
+    FLOCK_TRY(vd.alloc(elems * n_keys * 4));
+    FLOCK_CK(cudaMemcpyAsync(kd.p, k, elems * n_keys * 4, cudaMemcpyHostToDevice, L->dev->stream));
+    FLOCK_CK(cudaMemcpyAsync(vd.p, v, elems * n_keys * 4, cudaMemcpyHostToDevice, L->dev->stream));
+    k_kv_append<FLOCK_KV_Q4><<<dim3((n_keys + 7) / 8, L->cfg.n_kv_heads), 256, 0, L->dev->stream>>>(
+        layer_kv_view(L), kd.as<float>(), vd.as<float>(), (int64_t)elems, L->n_keys, n_keys);
+    FLOCK_CK(cudaGetLastError());
+    FLOCK_CK(cudaStreamSynchronize(L->dev->stream));  // before its inputs go
+  } else if (L->cfg.kv_dtype == FLOCK_KV_Q4) {
+  } else if (L->cfg.kv_dtype == FLOCK_KV_FP8) {
     const size_t count = elems * (size_t)n_keys;
     std::vector<uint8_t> kb(count), vb(count);
     for (size_t i = 0; i < count; i++) {

@@ -108,6 +108,7 @@ struct Workspace {
   int down_pending = 0;
   DBuf tp_part, tp_all;         // tensor parallel: this rank's partial [P][H], all ranks
   DBuf wire;                    // FLK1 frames: the f16 payload on the device
+  DBuf kv_ws;                   // attention over a 4-bit cache or in a window (kv_attention_enqueue)
   // tp_ranks >= 1 (a tensor-parallel model, one rank included): also the
   // partial / all-gather buffers; 0 = no tensor parallelism
   int alloc(const flock_layer_config& c, int sm_count, int tp_ranks = 0);
@@ -173,6 +174,8 @@ struct flock_layer {
   flock_layer_config cfg{};
   const flock_tensor* w[flock::W_COUNT] = {};
   flock::DBuf kcache, vcache, ctl_own, inv_freq;
+  flock::DBuf kscales, vscales;  // FLOCK_KV_Q4 (capacity kv_capacity())
+  int window = 0, sinks = 0;   // flock_layer_set_window; 0: every key
   int* ctl = nullptr;          // {pos, n_last} on the device (own or the model's)
   int n_keys = 0;              // host mirror
   // tensor parallel: this layer is one rank's slice; o_proj and down give
@@ -186,7 +189,8 @@ struct flock_layer {
 };
 
 namespace flock {
-// Bytes per cached key/value element: 4 (FLOCK_KV_F32) or 2 (FLOCK_KV_BF16).
+// Bytes per cached key/value element: 4 (FLOCK_KV_F32) or 2 (FLOCK_KV_BF16);
+// not for FLOCK_KV_Q4, whose planes are bytes and scales.
 inline size_t kv_elem_bytes(const flock_layer_config& c) {
   return c.kv_dtype == FLOCK_KV_BF16 ? 2 : c.kv_dtype == FLOCK_KV_FP8 ? 1 : 4;
 }
@@ -194,6 +198,19 @@ inline size_t kv_elem_bytes(const flock_layer_config& c) {
 // `advance` = this launch advances the layer's ctl; pf_next = L2 prefetch
 // hint for whatever follows the layer (may be empty).
 int layer_enqueue(flock_layer* L, int n, bool advance, const PrefetchList& pf_next, bool pdl);
+// Keys a layer's planes hold: max_keys, in whole 16-key groups for FLOCK_KV_Q4.
+inline int64_t kv_capacity(const flock_layer_config& c) {
+  return c.kv_dtype == FLOCK_KV_Q4 ? ((int64_t)c.max_keys + 15) / 16 * 16 : c.max_keys;
+}
+inline const char* kv_dtype_name(int kv) {
+  return kv == FLOCK_KV_BF16 ? "bf16" : kv == FLOCK_KV_FP8 ? "fp8" : kv == FLOCK_KV_Q4 ? "4-bit" : "f32";
+}
+// Attention through kv_attention_enqueue (flock_kv.cu) instead of the layers'
+// own fused kernels: over a 4-bit cache, or in a window.
+inline bool layer_uses_kv_ops(const flock_layer* L) {
+  return L->cfg.kv_dtype == FLOCK_KV_Q4 || L->window > 0;
+}
+int layer_set_window(flock_layer* L, int window, int sinks);
 int layer_init(flock_layer* L, flock_dev* dev, const flock_layer_config& cfg, Workspace* ws,
                int* shared_ctl);
 int comm_send(flock_comm* c, const void* p, size_t n_f32, int peer);

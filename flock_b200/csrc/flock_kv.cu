@@ -6,6 +6,7 @@
 
 #include "flock_internal.h"
 #include "kv.cuh"
+#include "kv_layer.h"
 #include "kv_prompt.cuh"
 #include "kv_rows.cuh"
 
@@ -93,7 +94,7 @@ int by_dtype(int kv_dtype, F f) {
 
 // A few query rows per kv head: k_kv_rows.
 template <int KV, int NT>
-int launch_rows(const flock_kv* c, const KvAttnArgs& a, cudaStream_t st) {
+int launch_rows(int sm_count, uint8_t* workspace, const KvAttnArgs& a, cudaStream_t st) {
   using L = KrLayout<KV, NT>;
   constexpr int RT = L::RT;
   KvRowsArgs p = {};
@@ -102,27 +103,26 @@ int launch_rows(const flock_kv* c, const KvAttnArgs& a, cudaStream_t st) {
   p.rows = a.n_queries * p.group;
   const int tiles = (p.rows + RT - 1) / RT;
   const int64_t items = (int64_t)tiles * a.c.n_kv_heads;
-  // Key splits: one CTA per SM, each warp at least a group of keys.  Joining
-  // splits costs about 2.5 us, a group about 0.5: up to four groups a warp one
-  // CTA reads them all (320 keys: 4.4 us against 6.1 in two splits).
-  const int64_t lo = a.window && a.pos + 1 > a.window ? a.pos + 1 - a.window : 0;
-  const int64_t keys = a.pos + a.n_queries - lo + (a.sinks < lo ? a.sinks : lo);
-  const int64_t want = (keys + KR_GROUP * L::WARPS - 1) / (KR_GROUP * L::WARPS);
-  const int64_t room = c->dev->sm_count / items;
-  p.splits = want <= 4 ? 1 : (int)(want < room ? want : room);
-  if (p.splits < 1) p.splits = 1;
-  p.count = reinterpret_cast<uint32_t*>(c->workspace);
-  p.part = reinterpret_cast<float*>(c->workspace + KR_PART_OFFSET);
+  // one CTA per SM; with the position on the device the kernel decides, at most
+  // the splits of the bound (sink and window groups, two of them cut)
+  const int64_t lo = a.window && !a.ctl && a.pos + 1 > a.window ? a.pos + 1 - a.window : 0;
+  int64_t keys = a.pos + a.n_queries - lo + (a.sinks < lo ? a.sinks : lo);
+  if (a.ctl && a.window && keys > (int64_t)a.window + a.n_queries + a.sinks)
+    keys = (int64_t)a.window + a.n_queries + a.sinks;
+  const int64_t room = items < KR_MAX_ITEMS ? sm_count / items : 1;
+  const int splits = kr_splits(keys / KR_GROUP + 3, L::WARPS, room);
+  p.count = reinterpret_cast<uint32_t*>(workspace);
+  p.part = reinterpret_cast<float*>(workspace + KR_PART_OFFSET);
   FLOCK_TRY(kernel_setup((const void*)k_kv_rows<KV, NT>, (int)L::SMEM));
   FLOCK_CK(launch_ex(st, k_kv_rows<KV, NT>,
-                     dim3((unsigned)p.splits, (unsigned)tiles, (unsigned)a.c.n_kv_heads),
+                     dim3((unsigned)splits, (unsigned)tiles, (unsigned)a.c.n_kv_heads),
                      dim3(L::THREADS), L::SMEM, true, p));
   return FLOCK_OK;
 }
 
 // Many query rows: k_kv_prompt on the tensor cores, 128 rows a CTA.
 template <int KV>
-int launch_prompt(const flock_kv* c, const KvAttnArgs& a, cudaStream_t st) {
+int launch_prompt(uint8_t* workspace, const KvAttnArgs& a, cudaStream_t st) {
   KvPromptArgs p = {};
   p.a = a;
   p.group = a.n_heads / a.c.n_kv_heads;
@@ -138,7 +138,7 @@ int launch_prompt(const flock_kv* c, const KvAttnArgs& a, cudaStream_t st) {
   const int64_t room = most / items;
   p.splits = (int)(want < room ? want : room);
   if (p.splits < 1) p.splits = 1;
-  p.part = reinterpret_cast<float*>(c->workspace + KR_PART_OFFSET);
+  p.part = reinterpret_cast<float*>(workspace + KR_PART_OFFSET);
   FLOCK_TRY(kernel_setup((const void*)k_kv_prompt<KV>, (int)KP_SMEM<KV>));
   FLOCK_CK(launch_ex(st, k_kv_prompt<KV>,
                      dim3((unsigned)tiles, (unsigned)p.splits, (unsigned)a.c.n_kv_heads),
@@ -151,6 +151,21 @@ int launch_prompt(const flock_kv* c, const KvAttnArgs& a, cudaStream_t st) {
 }
 
 }  // namespace
+
+int flock::kv_attention_enqueue(int sm_count, int kv_dtype, const KvAttnArgs& a,
+                                uint8_t* workspace, cudaStream_t st) {
+  const int64_t rows = (int64_t)a.n_queries * (a.n_heads / a.c.n_kv_heads);
+  return by_dtype(kv_dtype, [&](auto kv) -> int {
+    constexpr int KV = decltype(kv)::value;
+    // 16 rows: three tiles of k_kv_rows' smallest, where it and one mostly empty
+    // tile of the tensor cores meet (6 queries of 16 / 8 heads at 8191 keys 15 us
+    // against 22; 16 at 3000 keys 19 us on either)
+    if (rows > 16) return launch_prompt<KV>(workspace, a, st);
+    if constexpr (KV == FLOCK_KV_Q4 || KV == FLOCK_KV_FP8)
+      if (rows <= 4) return launch_rows<KV, 1>(sm_count, workspace, a, st);  // one column tile
+    return launch_rows<KV, 2>(sm_count, workspace, a, st);
+  });
+}
 
 extern "C" {
 
@@ -344,15 +359,8 @@ int flock_kv_attention(flock_kv* c, const float* q, int64_t q_stride, int n_head
   a.n_heads = n_heads;
   a.window = window;
   a.sinks = sinks;
-  const int64_t rows = (int64_t)n_queries * (n_heads / c->view.n_kv_heads);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return by_dtype(c->kv_dtype, [&](auto kv) -> int {
-    constexpr int KV = decltype(kv)::value;
-    if (rows > 16) return launch_prompt<KV>(c, a, st);
-    if constexpr (KV == FLOCK_KV_Q4 || KV == FLOCK_KV_FP8)
-      if (rows <= 4) return launch_rows<KV, 1>(c, a, st);  // f16 parts of four rows: one column tile
-    return launch_rows<KV, 2>(c, a, st);
-  });
+  return kv_attention_enqueue(c->dev->sm_count, c->kv_dtype, a, c->workspace,
+                              static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -31,6 +31,7 @@ struct flock_model {
   Workspace ws;
   DBuf ctl, ids, hist, logits, normed, am_val, am_idx, am_count, am_best_val;
   int pos = 0;  // host mirror of ctl[0] after the last step
+  int window = 0;  // flock_model_set_window
   // the kernel graph of one decode step, and of DECODE_GRAPH_TOKENS steps
   // in a row (device-fed decode runs: no graph boundary, so each step's
   // first launch overlaps the previous step's last one)
@@ -58,6 +59,14 @@ struct flock_model {
 };
 
 namespace {
+
+// The one-launch engines read every key: a model in a window runs the kernel graph.
+bool use_stream(const flock_model* m) {
+  return m->decode_mode == FLOCK_DECODE_STREAM && m->st.ok && m->window == 0;
+}
+bool use_mk(const flock_model* m) {
+  return m->decode_mode == FLOCK_DECODE_PERSISTENT && m->mk_ok && m->window == 0;
+}
 
 int enqueue_embed(flock_model* m, int n) {
   EmbedArgs a = {};
@@ -253,7 +262,8 @@ int mk_prepare(flock_model* m) {
   const flock_layer_config& c = m->cfg;
   m->mk_ok = false;
   if (c.attention != FLOCK_ATTN_FAST || !m->embd || !m->head || m->held < 1 || c.head_dim != 128 ||
-      c.n_heads / c.n_kv_heads > 4 || c.hidden > 4096 || m->tp || c.matvec != FLOCK_MATVEC_EXACT)
+      c.n_heads / c.n_kv_heads > 4 || c.hidden > 4096 || m->tp || c.matvec != FLOCK_MATVEC_EXACT ||
+      c.kv_dtype == FLOCK_KV_Q4)
     return FLOCK_OK;
   int dev = m->dev->ordinal, coop = 0, smem_optin = 0;
   FLOCK_CK(cudaDeviceGetAttribute(&coop, cudaDevAttrCooperativeLaunch, dev));
@@ -465,7 +475,7 @@ int st_prepare(flock_model* m) {
     m->st.why = "its matvecs are the exact-order ones (FLOCK_MATVEC_EXACT)";
     return FLOCK_OK;
   }
-  if (c.kv_dtype == FLOCK_KV_FP8) {
+  if (c.kv_dtype == FLOCK_KV_FP8 || c.kv_dtype == FLOCK_KV_Q4) {
     m->st.why = "its attention reads f32 or bf16 caches";
     return FLOCK_OK;
   }
@@ -589,7 +599,7 @@ void drop_decode_graphs(flock_model* m) {
 // barrier reset plus one cooperative launch; no graph, so profilers see the
 // kernel) or the captured kernel graph.
 int launch_decode(flock_model* m) {
-  if (m->decode_mode == FLOCK_DECODE_STREAM && m->st.ok) {
+  if (use_stream(m)) {
     // the layers in one streaming launch, then the graph's head GEMV (its
     // 296-CTA register-pipelined stream beats the persistent grid's 148 CTAs
     // on the 165 MB head) with the fused argmax, and the history record
@@ -597,7 +607,7 @@ int launch_decode(flock_model* m) {
     FLOCK_TRY(enqueue_head(m, 0));
     return enqueue_record(m);
   }
-  if (m->decode_mode == FLOCK_DECODE_PERSISTENT && m->mk_ok) return enqueue_mk(m);
+  if (use_mk(m)) return enqueue_mk(m);
   if (m->decode_mode == FLOCK_DECODE_EAGER) {
     FLOCK_TRY(enqueue_embed(m, 1));
     FLOCK_TRY(enqueue_layers(m, 1));
@@ -614,8 +624,8 @@ int launch_decode(flock_model* m) {
 // as n single-step launches); the other engines, and tensor-parallel ranks
 // (whose graphs hold collectives), one step at a time.
 int launch_decode_run(flock_model* m, int n) {
-  const bool graph = !m->tp && !(m->decode_mode == FLOCK_DECODE_STREAM && m->st.ok) &&
-                     !(m->decode_mode == FLOCK_DECODE_PERSISTENT && m->mk_ok) &&
+  const bool graph = !m->tp && !(use_stream(m)) &&
+                     !(use_mk(m)) &&
                      m->decode_mode != FLOCK_DECODE_EAGER;
   int i = 0;
   if (graph && n >= DECODE_GRAPH_TOKENS) {
@@ -778,7 +788,7 @@ int flock_model_set_decode_mode(flock_model* m, int mode) {
 
 int flock_model_trace(flock_model* m, int enable) {
   if (!m) return FLOCK_E_ARG;
-  if (m->decode_mode == FLOCK_DECODE_STREAM && m->st.ok) return stream_trace(&m->st, enable != 0);
+  if (use_stream(m)) return stream_trace(&m->st, enable != 0);
   if (!m->mk_ok) {
     set_error("phase tracing needs the persistent decode kernel, which this model cannot run");
     return FLOCK_E_UNSUPPORTED;
@@ -794,7 +804,7 @@ int flock_model_trace(flock_model* m, int enable) {
 
 int flock_model_trace_read(flock_model* m, uint64_t* out, int64_t cap, int* n_ctas, int* stride) {
   if (!m || !n_ctas || !stride) return FLOCK_E_ARG;
-  if (m->decode_mode == FLOCK_DECODE_STREAM && m->st.ok) {
+  if (use_stream(m)) {
     *n_ctas = m->st.grid;
     *stride = stream_trace_stride(&m->st);
     const int64_t n = (int64_t)*n_ctas * *stride;
@@ -811,6 +821,15 @@ int flock_model_trace_read(flock_model* m, uint64_t* out, int64_t cap, int* n_ct
   if (!out || cap < n) return FLOCK_E_LIMIT;
   FLOCK_TRY(sync_model(m));
   FLOCK_CK(cudaMemcpy(out, m->mk_trace.p, (size_t)n * 8, cudaMemcpyDeviceToHost));
+  return FLOCK_OK;
+}
+
+int flock_model_set_window(flock_model* m, int window, int sinks) {
+  if (!m) return FLOCK_E_ARG;
+  FLOCK_CK(cudaSetDevice(m->dev->ordinal));
+  for (auto* L : m->layers) FLOCK_TRY(layer_set_window(L, window, sinks));
+  m->window = window;
+  drop_decode_graphs(m);  // their launches hold the window
   return FLOCK_OK;
 }
 
@@ -838,8 +857,8 @@ int flock_model_get_tp_exchange(const flock_model* m, int* mode) {
 
 int flock_model_get_decode_mode(const flock_model* m, int* mode) {
   if (!m || !mode) return FLOCK_E_ARG;
-  *mode = ((m->decode_mode == FLOCK_DECODE_PERSISTENT && !m->mk_ok) ||
-           (m->decode_mode == FLOCK_DECODE_STREAM && !m->st.ok))
+  *mode = ((m->decode_mode == FLOCK_DECODE_PERSISTENT && !use_mk(m)) ||
+           (m->decode_mode == FLOCK_DECODE_STREAM && !use_stream(m)))
               ? FLOCK_DECODE_KERNELS
               : m->decode_mode;
   return FLOCK_OK;

@@ -14,6 +14,7 @@
 // Head-major planes keep a head's keys contiguous: its scales (8 bytes a key)
 // fill whole sectors, where [key][head] rows would use 8 bytes of each 32.
 #pragma once
+#include "../../include/flock_cuda.h"
 #include "common.cuh"
 #include "mbar.cuh"
 
@@ -226,7 +227,10 @@ struct KvAttnArgs {
   float* out;
   int64_t q_stride, out_stride;
   int64_t pos;
+  const int* ctl;  // a layer's step control: the position is ctl[0], pos its bound; or null
   int n_queries, n_heads, window, sinks;
 };
+// After griddepcontrol.wait: an earlier kernel of the step writes ctl.
+FLOCK_DEV int kv_attn_pos(const KvAttnArgs& a) { return a.ctl ? a.ctl[0] : (int)a.pos; }
 
 }  // namespace flock

@@ -179,7 +179,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
   const uint32_t tmem = s_tmem, tS = tmem, tO = tmem + 256, tQ = tmem + 384;
 
   // keys that some row of the tile sees: sinks [0, sk), then [lo, hi)
-  const int pos = (int)a.pos;
+  const int pos = kv_attn_pos(a);
   const int first_q = tile * KP_ROWS / p.group;
   const int last_q = (min(p.rows, (tile + 1) * KP_ROWS) - 1) / p.group;
   const int hi = pos + last_q + 1;

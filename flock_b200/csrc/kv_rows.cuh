@@ -44,9 +44,8 @@ struct KvRowsArgs {
   KvAttnArgs a;
   int rows;         // n_queries * group: row r is query r / group, head r % group
   int group;        // query heads per kv head
-  int splits;
   uint32_t* count;  // [items], zero between calls
-  float* part;      // [item][split][RT][128], then [item][split][RT][2] (m, l)
+  float* part;      // [item][gridDim.x][RT][128], then [item][gridDim.x][RT][2] (m, l)
 };
 
 // Shared-memory layout of one warp's 16-key stage, per cached type, for NT
@@ -244,6 +243,14 @@ FLOCK_DEV void kr_load(uint32_t stage, const uint8_t* kb, const uint8_t* vb, con
   }
 }
 
+// Key splits of a row tile: every warp at least a group of keys, as far as the
+// grid allows.  Joining splits costs about 2.5 us, a group about 0.5: up to four
+// groups a warp one CTA reads them all (320 keys: 4.9 us against 7 in two).
+__host__ __device__ inline int kr_splits(int64_t groups, int warps, int64_t most) {
+  const int64_t want = (groups + warps - 1) / warps;
+  return want <= 4 || most < 2 ? 1 : (int)(want < most ? want : most);
+}
+
 FLOCK_DEV uint4 ld_u4(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 FLOCK_DEV uint2 ld_u2(const uint8_t* p) { return *reinterpret_cast<const uint2*>(p); }
 FLOCK_DEV uint32_t word_of(const uint4& v, int i) {
@@ -275,14 +282,17 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
   const int first_q = tile * RT / p.group;
   const int last_q = (min(p.rows, (tile + 1) * RT) - 1) / p.group;
   // keys that some row of the tile sees: sinks [0, sk), then [lo, hi)
-  const int pos = (int)a.pos;
+  const int pos = kv_attn_pos(a);
   const int hi = pos + last_q + 1;
   const int lo = a.window && pos + first_q + 1 > a.window ? pos + first_q + 1 - a.window : 0;
   const int sk = min(a.sinks, lo);
   const int sink_groups = (sk + KR_GROUP - 1) / KR_GROUP;
   const int lo16 = lo & ~(KR_GROUP - 1);
   const int groups = sink_groups + (hi - lo16 + KR_GROUP - 1) / KR_GROUP;
-  const int g0 = (int)((int64_t)z * groups / p.splits), g1 = (int)((int64_t)(z + 1) * groups / p.splits);
+  // the splits these groups are worth, of those the grid has (see kr_splits)
+  const int splits = kr_splits(groups, L::WARPS, gridDim.x);
+  if (z >= splits) return;
+  const int g0 = (int)((int64_t)z * groups / splits), g1 = (int)((int64_t)(z + 1) * groups / splits);
   // a row's own keys: sinks [0, row_sk), then [row_lo, row_hi)
   int row_lo[RL], row_hi[RL], row_sk[RL];
   int max_lo = 0, min_hi = hi;  // a group inside [max_lo, min_hi) is visible to every row
@@ -699,7 +709,7 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
   __syncthreads();
   const int item = head * gridDim.y + tile;
   const int n_items = gridDim.y * gridDim.z;
-  float* part_ml = p.part + (size_t)n_items * p.splits * RT * KV_HD;
+  float* part_ml = p.part + (size_t)n_items * gridDim.x * RT * KV_HD;
   for (int i = threadIdx.x; i < live * KV_HD; i += L::THREADS) {
     const int r = i / KV_HD, d = i % KV_HD;
     float mm = -INFINITY;
@@ -713,12 +723,12 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
       oo = ffma(f, s_o[(w * RT + r) * OS + d], oo);
       ll = ffma(f, s_ml[w][r][1], ll);
     }
-    if (p.splits == 1) {
+    if (splits == 1) {
       const int rr = tile * RT + r;
       a.out[(rr / p.group) * a.out_stride + ((int64_t)head * p.group + rr % p.group) * KV_HD + d] =
           fdiv(oo, ll);
     } else {
-      const size_t at = ((size_t)item * p.splits + z) * RT + r;
+      const size_t at = ((size_t)item * gridDim.x + z) * RT + r;
       p.part[at * KV_HD + d] = oo;
       if (d == 0) {
         part_ml[at * 2] = mm;
@@ -726,7 +736,7 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
       }
     }
   }
-  if (p.splits == 1) return;
+  if (splits == 1) return;
   // --------------------------------------------------------- join the splits
   // one release-acquire arrival per CTA, behind the barrier that orders its
   // threads' stores before it
@@ -735,7 +745,7 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
     uint32_t before;
     asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;"
                  : "=r"(before) : "l"(p.count + item) : "memory");
-    s_last = before == (uint32_t)p.splits - 1;
+    s_last = before == (uint32_t)splits - 1;
     if (s_last) p.count[item] = 0;  // ready for the next call
   }
   __syncthreads();
@@ -748,20 +758,20 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
             d = 4 * (threadIdx.x % (KV_HD / 4));
   const bool mine = threadIdx.x < par * quads;
   float* s_f = reinterpret_cast<float*>(kr_smem);  // [split][RT]
-  float* s_l = s_f + p.splits * RT;
-  float4* s_x = reinterpret_cast<float4*>(s_l + p.splits * RT);  // [k][quads]
-  const size_t first = (size_t)item * p.splits * RT;
+  float* s_l = s_f + splits * RT;
+  float4* s_x = reinterpret_cast<float4*>(s_l + splits * RT);  // [k][quads]
+  const size_t first = (size_t)item * gridDim.x * RT;
   constexpr int U = 4;  // loads in flight
   float4 x4[U];
   auto load = [&](int s0) {
 #pragma unroll
     for (int u = 0; u < U; u++)
-      if (mine && s0 + u * par < p.splits)
+      if (mine && s0 + u * par < splits)
         x4[u] = __ldcg(reinterpret_cast<const float4*>(
             p.part + (first + (size_t)(s0 + u * par) * RT + r) * KV_HD + d));
   };
   load(k);
-  for (int i = threadIdx.x; i < p.splits * RT; i += L::THREADS) {
+  for (int i = threadIdx.x; i < splits * RT; i += L::THREADS) {
     const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml) + first + i);
     s_f[i] = ml.x;
     s_l[i] = ml.y;
@@ -769,11 +779,11 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
   __syncthreads();
   if (warp < live) {
     float mm = -INFINITY;
-    for (int s = lane; s < p.splits; s += 32) mm = fmaxf(mm, s_f[s * RT + warp]);
+    for (int s = lane; s < splits; s += 32) mm = fmaxf(mm, s_f[s * RT + warp]);
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
     float ll = 0.0f;
-    for (int s = lane; s < p.splits; s += 32) {
+    for (int s = lane; s < splits; s += 32) {
       const float f = exp2_approx(fsub(s_f[s * RT + warp], mm));
       s_f[s * RT + warp] = f;
       ll = ffma(f, s_l[s * RT + warp], ll);
@@ -784,11 +794,11 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
   }
   __syncthreads();
   float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = k; mine && s0 < p.splits; s0 += U * par) {
+  for (int s0 = k; mine && s0 < splits; s0 += U * par) {
     if (s0 != k) load(s0);
 #pragma unroll
     for (int u = 0; u < U; u++)
-      if (s0 + u * par < p.splits) {
+      if (s0 + u * par < splits) {
         const float f = s_f[(s0 + u * par) * RT + r];
         oo = make_float4(ffma(f, x4[u].x, oo.x), ffma(f, x4[u].y, oo.y), ffma(f, x4[u].z, oo.z),
                          ffma(f, x4[u].w, oo.w));

@@ -15,6 +15,7 @@
 #pragma once
 #include <cuda_fp16.h>
 #include "common.cuh"
+#include "kv.cuh"
 
 namespace flock {
 
@@ -84,6 +85,7 @@ struct QkArgs {
   // RoPE (cos, sin) table [rope_rows][hd / 2] (k_rope_table), or null
   const float2* rope_cs;
   int rope_rows;
+  KvView q4;  // k_qk_norm_rope_append<FLOCK_KV_Q4>: the cache
 };
 
 // Byte offset of element (row, 8-element chunk c16) of a 128 x 128 f16
@@ -205,7 +207,7 @@ static __global__ void k_rope_table(const float* inv_freq, int n_pos, float2* ou
 // One warp per 128-vector (8 per CTA): q heads -> qn, k heads -> the cache at
 // position pos0 + token with v copied beside it.  norm_rope_warp's arithmetic
 // is the WG = 128 RMSNorm and RoPE above, bit for bit.  KV: the cache's
-// element (FLOCK_KV_F32 / _BF16 / _FP8); for bf16 and e4m3 the rotated key is
+// element (FLOCK_KV_F32 / _BF16 / _FP8 / _Q4); for bf16 and e4m3 the rotated key is
 // staged in shared memory and stored rounded to nearest even, as is v.
 template <int KV>
 static __global__ void __launch_bounds__(256) k_qk_norm_rope_append(const QkArgs a) {
@@ -247,7 +249,18 @@ static __global__ void __launch_bounds__(256) k_qk_norm_rope_append(const QkArgs
     const float* k = a.k + ((size_t)tok * a.n_kv_heads + kvh) * hd;
     const float* v = a.v + ((size_t)tok * a.n_kv_heads + kvh) * hd;
     float kf[4], vf[4];  // the values the cache now holds (for the f16 image)
-    if constexpr (KV == 2) {
+    if constexpr (KV == FLOCK_KV_Q4) {
+      // no f16 image: attention over the 4-bit cache reads its codes
+      float* ks = kstage + warp * 128;
+      if (table)
+        norm_rope_warp_cs(k, a.k_norm, a.eps, cs, a.neox, ks, lane);
+      else
+        norm_rope_warp(k, a.k_norm, a.eps, pos, a.inv_freq, a.neox, ks, lane);
+      __syncwarp();
+      q4_store_row<true>(a.q4, pos, kvh, reinterpret_cast<const float4*>(ks)[lane], lane);
+      q4_store_row<false>(a.q4, pos, kvh, reinterpret_cast<const float4*>(v)[lane], lane);
+      return;
+    } else if constexpr (KV == 2) {
       float* ks = kstage + warp * 128;
       if (table)
         norm_rope_warp_cs(k, a.k_norm, a.eps, cs, a.neox, ks, lane);

@@ -45,9 +45,9 @@ class LayerConfig:
     # "tensor" (tcgen05 tensor cores, f16 operands, 1e-2 relative tolerance)
     prefill: str = "exact"
     # KV cache element type: "f32" (the reference's), "bf16" (half the bytes
-    # per key) or "fp8" (e4m3, a quarter; magnitudes past 448 saturate);
-    # appends round to nearest even; both need attention="fast" and
-    # prefill="tensor"
+    # per key) or "fp8" (e4m3, a quarter; magnitudes past 448 saturate), whose
+    # appends round to nearest even, or "q4" (blocks of 32 in Q4_0's rule, 0.14);
+    # all three need attention="fast" and prefill="tensor"
     kv: str = "f32"
     # one-token matvecs: "exact" (cpuMatmulQ8F32(coop(64))'s order, bit-identical)
     # or "fast" (the decode LM head on the int8 tensor cores, reassociated,
@@ -55,8 +55,8 @@ class LayerConfig:
     matvec: str = "exact"
 
     def to_c(self) -> _abi.LayerConfigC:
-        if self.kv not in ("f32", "bf16", "fp8"):
-            raise ValueError(f"kv must be 'f32', 'bf16' or 'fp8', not {self.kv!r}")
+        if self.kv not in ("f32", "bf16", "fp8", "q4"):
+            raise ValueError(f"kv must be 'f32', 'bf16', 'fp8' or 'q4', not {self.kv!r}")
         if self.matvec not in ("exact", "fast"):
             raise ValueError(f"matvec must be 'exact' or 'fast', not {self.matvec!r}")
         return _abi.LayerConfigC(
@@ -65,7 +65,8 @@ class LayerConfig:
             _abi.FLOCK_ROPE_NEOX if self.rope_pairing == "neox" else _abi.FLOCK_ROPE_NORM,
             _abi.FLOCK_ATTN_EXACT if self.attention == "exact" else _abi.FLOCK_ATTN_FAST,
             _abi.FLOCK_PREFILL_TENSOR if self.prefill == "tensor" else _abi.FLOCK_PREFILL_EXACT,
-            {"bf16": _abi.FLOCK_KV_BF16, "fp8": _abi.FLOCK_KV_FP8}.get(self.kv, _abi.FLOCK_KV_F32),
+            {"bf16": _abi.FLOCK_KV_BF16, "fp8": _abi.FLOCK_KV_FP8,
+             "q4": _abi.FLOCK_KV_Q4}.get(self.kv, _abi.FLOCK_KV_F32),
             _abi.FLOCK_MATVEC_FAST if self.matvec == "fast" else _abi.FLOCK_MATVEC_EXACT)
 
     def with_(self, **kw) -> "LayerConfig":
@@ -152,6 +153,11 @@ class Layer:
 
     def rewind(self, n_keys: int) -> None:
         _abi.call("flock_layer_rewind", self.handle, n_keys)
+
+    def set_window(self, window: int, sinks: int = 0) -> None:
+        """From the next step on queries see the ``window`` newest keys and the
+        first ``sinks`` only; 0: every key (needs attention="fast")."""
+        _abi.call("flock_layer_set_window", self.handle, window, sinks)
 
     @property
     def n_keys(self) -> int:

@@ -204,6 +204,11 @@ class Model:
     def rewind(self, n_keys: int) -> None:
         _abi.call("flock_model_rewind", self.handle, n_keys)
 
+    def set_window(self, window: int, sinks: int = 0) -> None:
+        """From the next step on queries see the ``window`` newest keys and the
+        first ``sinks`` only; 0: every key (needs attention="fast")."""
+        _abi.call("flock_model_set_window", self.handle, window, sinks)
+
     @property
     def pos(self) -> int:
         n = ctypes.c_int()

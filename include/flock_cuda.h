@@ -71,7 +71,10 @@ extern "C" {
                            scale) once and every read widens it exactly.  Needs
                            FLOCK_ATTN_FAST and FLOCK_PREFILL_TENSOR. */
 #define FLOCK_KV_Q4 3   /* 4-bit KV cache: blocks of 32 values along the head in the Q4_0 rule
-                           (lib.ts:64), 4.5 bits a value, 0.14 of f32's bytes per key */
+                           (lib.ts:64), 4.5 bits a value, 0.14 of f32's bytes per key; every
+                           read takes the stored values exactly.  Needs FLOCK_ATTN_FAST and
+                           FLOCK_PREFILL_TENSOR; attention is flock_kv_attention's, the
+                           one-launch decode engines fall back to the kernel graph. */
 
 #define FLOCK_MATVEC_EXACT 0 /* one-token matvecs in cpuMatmulQ8F32(coop(64))'s f32 order
                                 (lib.ts:213), bit-identical */
@@ -103,7 +106,7 @@ typedef struct flock_layer_config {
   int32_t rope_pairing; /* FLOCK_ROPE_NEOX | FLOCK_ROPE_NORM */
   int32_t attention;    /* FLOCK_ATTN_EXACT | FLOCK_ATTN_FAST */
   int32_t prefill;      /* FLOCK_PREFILL_EXACT | FLOCK_PREFILL_TENSOR (multi-token steps) */
-  int32_t kv_dtype;     /* FLOCK_KV_F32 (0, the default) | FLOCK_KV_BF16 | FLOCK_KV_FP8 */
+  int32_t kv_dtype;     /* FLOCK_KV_F32 (0, the default) | FLOCK_KV_BF16 | _FP8 | _Q4 */
   int32_t matvec;       /* FLOCK_MATVEC_EXACT (0, the default) | FLOCK_MATVEC_FAST */
 } flock_layer_config;
 
@@ -371,6 +374,13 @@ FLOCK_API int flock_layer_reset(flock_layer* layer);
 FLOCK_API int flock_layer_n_keys(const flock_layer* layer, int* out);
 /* Drop the cache back to n_keys (model.ts:529 rewind, per layer). */
 FLOCK_API int flock_layer_rewind(flock_layer* layer, int n_keys);
+/* From the next step on every query sees the `window` newest keys (itself
+ * among them) and the first `sinks` keys only; window 0: every key again.  No
+ * counterpart in the reference.  The cache keeps all keys (max_keys bounds the
+ * conversation), attention reads the visible ones (flock_kv_attention).  Needs
+ * FLOCK_ATTN_FAST; a model's layers take it from flock_model_set_window, which
+ * also makes the one-launch decode engines fall back to the kernel graph. */
+FLOCK_API int flock_layer_set_window(flock_layer* layer, int window, int sinks);
 /* kernels/layer.ts:792 cacheBuffers(): copy keys/values [n_keys][nKV][hd] as f32
  * (a bf16 cache is widened exactly). */
 FLOCK_API int flock_layer_read_cache(flock_layer* layer, float* k_out, float* v_out);
@@ -479,6 +489,8 @@ FLOCK_API int flock_model_get_decode_mode(const flock_model* m, int* mode);
 FLOCK_API int flock_model_trace(flock_model* m, int enable);
 FLOCK_API int flock_model_trace_read(flock_model* m, uint64_t* out, int64_t cap, int* n_ctas,
                                      int* stride);
+/* flock_layer_set_window for every layer of the model. */
+FLOCK_API int flock_model_set_window(flock_model* m, int window, int sinks);
 /* Set the token the next device-fed decode step consumes (ids[0]). */
 FLOCK_API int flock_model_set_token(flock_model* m, int32_t id);
 /* kernels/model.ts:541 currentToken(). */

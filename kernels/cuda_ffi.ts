@@ -137,6 +137,8 @@ export const symbols = {
   flock_layer_n_keys: { parameters: ["pointer", "buffer"], result: "i32" },
   // (layer, n_keys)
   flock_layer_rewind: { parameters: ["pointer", "i32"], result: "i32" },
+  // (layer, window, sinks)
+  flock_layer_set_window: { parameters: ["pointer", "i32", "i32"], result: "i32" },
   // (layer, k_out, v_out)
   flock_layer_read_cache: { parameters: ["pointer", "buffer", "buffer"], result: "i32" },
   // (layer, k, v, n_keys)
@@ -187,6 +189,8 @@ export const symbols = {
   flock_model_trace: { parameters: ["pointer", "i32"], result: "i32" },
   // (m, out, cap, n_ctas, stride)
   flock_model_trace_read: { parameters: ["pointer", "buffer", "i64", "buffer", "buffer"], result: "i32" },
+  // (m, window, sinks)
+  flock_model_set_window: { parameters: ["pointer", "i32", "i32"], result: "i32" },
   // (m, id)
   flock_model_set_token: { parameters: ["pointer", "i32"], result: "i32" },
   // (m, out)

@@ -154,6 +154,11 @@ export class Model {
     check(flock().flock_model_rewind(this.handle, nKeys));
   }
 
+  /** From the next step on queries see the newest `window` keys and the first `sinks` (0: all). */
+  setWindow(window: number, sinks = 0): void {
+    check(flock().flock_model_set_window(this.handle, window, sinks));
+  }
+
   /** model.ts:541 currentToken: the id the device argmax holds. */
   currentToken(): Promise<number> {
     const out = new Int32Array(1);

@@ -53,7 +53,9 @@ def build() -> str:
 def lib():
     global _lib
     if _lib is None:
-        if not os.path.exists(_LIB_PATH):
+        sources = [os.path.join(_HERE, f) for f in ("flock_oracle.c", "flock_oracle.h")]
+        if (not os.path.exists(_LIB_PATH)
+                or os.path.getmtime(_LIB_PATH) < max(map(os.path.getmtime, sources))):
             build()
         L = ctypes.CDLL(_LIB_PATH)
         sig = {
@@ -93,6 +95,8 @@ def lib():
             "fo_cache_set_bf16": (None, [ctypes.c_void_p, _int]),
             "fo_bf16_round": (ctypes.c_float, [ctypes.c_float]),
             "fo_cache_set_fp8": (None, [ctypes.c_void_p, _int]),
+            "fo_cache_set_q4": (None, [ctypes.c_void_p, _int]),
+            "fo_cache_set_window": (None, [ctypes.c_void_p, _int, _int]),
             "fo_fp8_round": (ctypes.c_float, [ctypes.c_float]),
             "fo_layer_forward": (_int, [_f32p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                         _f32p]),
@@ -322,12 +326,13 @@ class RefLayer:
     (shard_ref.ts:353), the arithmetic of a tensor-parallel layer.
     kv="bf16": every appended key/value is rounded to bf16 (nearest even), the
     cache a FLOCK_KV_BF16 layer keeps; kv="fp8": to e4m3 (fo_fp8_round, the
-    FLOCK_KV_FP8 cache); attention then reads the rounded values."""
+    FLOCK_KV_FP8 cache); kv="q4": in blocks of 32 as fo_quant_row_q4 stores
+    them (FLOCK_KV_Q4); attention then reads the rounded values."""
 
     def __init__(self, weights: dict, cfg: dict, max_keys: int = 4096, tp: int = 1,
                  kv: str = "f32"):
-        if kv not in ("f32", "bf16", "fp8"):
-            raise ValueError(f"kv must be 'f32', 'bf16' or 'fp8', not {kv!r}")
+        if kv not in ("f32", "bf16", "fp8", "q4"):
+            raise ValueError(f"kv must be 'f32', 'bf16', 'fp8' or 'q4', not {kv!r}")
         self.tp = int(tp)
         self._keep = {}
         w = _W()
@@ -349,6 +354,8 @@ class RefLayer:
         lib().fo_cache_set_bf16(self._cache, 1 if kv == "bf16" else 0)
         if kv == "fp8":
             lib().fo_cache_set_fp8(self._cache, 1)
+        if kv == "q4":
+            lib().fo_cache_set_q4(self._cache, 1)
 
     def __del__(self):
         try:
@@ -362,6 +369,9 @@ class RefLayer:
 
     def reset(self) -> None:
         lib().fo_cache_reset(self._cache)
+
+    def set_window(self, window: int, sinks: int = 0) -> None:
+        lib().fo_cache_set_window(self._cache, window, sinks)
 
     def fill_cache(self, k: np.ndarray, v: np.ndarray) -> None:
         k, v = _f32(k), _f32(v)

@@ -516,6 +516,23 @@ float fo_bf16_round(float x) {
   return x;
 }
 void fo_cache_set_fp8(fo_cache* c, int on) { c->bf16 = on ? 2 : 0; }
+void fo_cache_set_q4(fo_cache* c, int on) { c->bf16 = on ? 3 : 0; }
+void fo_cache_set_window(fo_cache* c, int window, int sinks) {
+  c->window = window;
+  c->sinks = sinks;
+}
+/* n values (a multiple of 32) through Q4_0 blocks: (code - 8) * d, d in f16 */
+static void q4_round(float* x, int64_t n) {
+  uint8_t blk[18];
+  for (int64_t b = 0; b < n / 32; b++) {
+    fo_quant_row_q4(x + b * 32, 32, blk);
+    const double d = fo_f16to32(rd16(blk));
+    for (int i = 0; i < 32; i++) {
+      const int code = i < 16 ? blk[2 + i] & 15 : blk[2 + i - 16] >> 4;
+      x[b * 32 + i] = (float)((code - 8) * d);
+    }
+  }
+}
 float fo_fp8_round(float x) {
   if (isnan(x)) return x;
   const float a = fabsf(x);
@@ -545,8 +562,41 @@ int fo_cache_fill(fo_cache* c, const float* k, const float* v, int n) {
       kd[i] = fo_fp8_round(kd[i]);
       vd[i] = fo_fp8_round(vd[i]);
     }
+  else if (c->bf16 == 3) {
+    q4_round(kd, (int64_t)count);
+    q4_round(vd, (int64_t)count);
+  }
   c->n += n;
   return 0;
+}
+
+/* Attention of n queries from pos0 on over the keys each sees, in f64. */
+static void attn_window(const float* q, const fo_cache* c, int n_heads, int n_kv_heads,
+                        int head_dim, int n, int pos0, float* out) {
+  const int group = n_heads / n_kv_heads;
+  const double scale = 1.0 / sqrt((double)head_dim);
+  double* p = (double*)malloc(sizeof(double) * (size_t)(pos0 + n));
+  for (int qi = 0; qi < n; qi++)
+    for (int h = 0; h < n_heads; h++) {
+      const float* qr = q + ((int64_t)qi * n_heads + h) * head_dim;
+      const int pos = pos0 + qi;
+      double max = -INFINITY, sum = 0;
+      for (int t = 0; t <= pos; t++) {
+        const float* kr = c->k + ((int64_t)t * n_kv_heads + h / group) * head_dim;
+        double s = 0;
+        for (int i = 0; i < head_dim; i++) s += (double)qr[i] * kr[i];
+        p[t] = t < c->sinks || t > pos - c->window ? s * scale : -INFINITY;
+        if (p[t] > max) max = p[t];
+      }
+      for (int t = 0; t <= pos; t++) sum += p[t] = exp(p[t] - max);
+      for (int i = 0; i < head_dim; i++) {
+        double o = 0;
+        for (int t = 0; t <= pos; t++)
+          if (p[t] > 0) o += p[t] * c->v[((int64_t)t * n_kv_heads + h / group) * head_dim + i];
+        out[((int64_t)qi * n_heads + h) * head_dim + i] = (float)(o / sum);
+      }
+    }
+  free(p);
 }
 
 #define COOP_LANES 64 /* layer_ref.ts:12, must match q8_coop.wgsl */
@@ -618,7 +668,9 @@ int fo_layer_prefill_tp(const float* hidden, int n, const fo_layer_w* w, const f
   fo_rope(qn, n, nH, hd, pos0, inv_freq, cfg->neox, q);
   fo_rope(kn, n, nKV, hd, pos0, inv_freq, cfg->neox, k);
   fo_cache_fill(cache, k, v, n);
-  if (n == 1)
+  if (cache->window > 0)
+    attn_window(q, cache, nH, nKV, hd, n, pos0, attn);
+  else if (n == 1)
     fo_attn(q, cache->k, cache->v, nH, nKV, hd, cache->n, attn);
   else
     fo_attn_prefill(q, cache->k, cache->v, nH, nKV, hd, n, pos0, 64, 128, attn);

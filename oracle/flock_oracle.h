@@ -116,7 +116,8 @@ typedef struct fo_cache {
   int cap; /* capacity in keys */
   int kvw; /* nKV*hd */
   int bf16; /* 1: every key/value is rounded to bf16 (nearest even) as it is stored;
-               2: to e4m3 (FLOCK_KV_FP8) */
+               2: to e4m3 (FLOCK_KV_FP8); 3: blocks of 32 to Q4_0 (FLOCK_KV_Q4) */
+  int window, sinks; /* flock_layer_set_window; window 0: every key is seen */
 } fo_cache;
 
 fo_cache* fo_cache_new(int cap, int kvw);
@@ -137,6 +138,12 @@ void fo_cache_set_fp8(fo_cache* c, int on);
  * become 448 with the sign, NaN stays NaN), as an f32: the rounding of the
  * device's cvt.rn.satfinite.e4m3x2.f32. */
 float fo_fp8_round(float x);
+/* A 4-bit KV cache (FLOCK_KV_Q4): from now on fo_cache_fill stores each block
+ * of 32 values as fo_quant_row_q4's codes and scale give it back. */
+void fo_cache_set_q4(fo_cache* c, int on);
+/* From now on a query at position p sees keys p - window + 1 .. p and the first
+ * `sinks` keys only (plain attention in f64, rounded once to f32). */
+void fo_cache_set_window(fo_cache* c, int window, int sinks);
 /* Preload n keys (e.g. a synthetic cache); returns 0 or -1 if over capacity. */
 int fo_cache_fill(fo_cache* c, const float* k, const float* v, int n);
 
