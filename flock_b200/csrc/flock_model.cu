@@ -32,6 +32,8 @@ struct flock_model {
   DBuf ctl, ids, hist, logits, normed, am_val, am_idx, am_count, am_best_val;
   int pos = 0;  // host mirror of ctl[0] after the last step
   int window = 0;  // flock_model_set_window
+  // flock_model_step_draft: every row's logits; tokens [n], accepted, u [n]; scratch
+  DBuf draft_logits, draft_io, draft_ws;
   // the kernel graph of one decode step, and of DECODE_GRAPH_TOKENS steps
   // in a row (device-fed decode runs: no graph boundary, so each step's
   // first launch overlaps the previous step's last one)
@@ -187,6 +189,28 @@ int enqueue_head(flock_model* m, int row) {
                                             m->ids.as<int32_t>());
   FLOCK_CK(cudaGetLastError());
   return FLOCK_OK;
+}
+
+// output_norm + lm-head over the first n rows of ws.h, logits [n][vocab].
+int enqueue_head_rows(flock_model* m, int n, float* logits) {
+  GemvArgs a = {};
+  GemvSeg s;
+  s.qs = m->head->qs.as<uint8_t>();
+  s.sc = m->head->sc.as<uint16_t>();
+  s.out = logits;
+  s.rows = (int)m->head->rows;
+  s.sc_stride = m->head->sc_stride;
+  s.out_stride = m->vocab;
+  a.seg[0] = s;
+  a.nseg = 1;
+  a.K = m->cfg.hidden;
+  a.n_tokens = n;
+  a.x = m->ws.h.as<float>();
+  a.x_stride = m->cfg.hidden;
+  a.norm_gain = m->out_norm->data.as<float>();
+  a.eps = m->cfg.eps;
+  return m->cfg.matvec == FLOCK_MATVEC_FAST ? launch_gemv_fast(m->dev, QT_Q8, EPI_STORE, a, true)
+                                            : launch_gemv(m->dev, QT_Q8, EPI_STORE, a, true);
 }
 
 // Wait for the model's stream: bounded by the communicator's deadline (which
@@ -931,6 +955,61 @@ int flock_model_step(flock_model* m, const int32_t* ids, int n, int32_t* next_id
   FLOCK_CK(cudaMemcpyAsync(next_id, m->ids.p, 4, cudaMemcpyDeviceToHost, m->dev->stream));
   FLOCK_TRY(sync_model(m));
   return check_device_errors(m);
+}
+
+int flock_model_step_draft(flock_model* m, const int32_t* ids, int n, const float* draft,
+                           const float* u, double temperature, int32_t* tokens, int* n_tokens) {
+  if (!m || !ids || !tokens || !n_tokens || (!u && temperature != 0.0)) {
+    set_error("step_draft: the model, ids, tokens and n_tokens must not be NULL, u only at "
+              "temperature 0");
+    return FLOCK_E_ARG;
+  }
+  FLOCK_TRY(need_head(m));
+  if (m->tp) {
+    set_error("step_draft: not for tensor-parallel models (a rank holds a slice of the logits)");
+    return FLOCK_E_UNSUPPORTED;
+  }
+  if (n < 1 || n > m->cfg.max_prefill || n > 513) {
+    set_error("step_draft: %d tokens, want 1 .. min(maxPrefill %d, 513)", n, m->cfg.max_prefill);
+    return FLOCK_E_LIMIT;
+  }
+  FLOCK_CK(cudaSetDevice(m->dev->ordinal));
+  const size_t row = (size_t)m->vocab * 4;
+  if (m->draft_logits.bytes < n * row) FLOCK_TRY(m->draft_logits.alloc(n * row));
+  if (!m->draft_io.p) FLOCK_TRY(m->draft_io.alloc((size_t)(2 * 513 + 1) * 4));
+  if (!m->draft_ws.p) FLOCK_TRY(m->draft_ws.alloc(FLOCK_WORKSPACE_BYTES));
+  int32_t* d_tokens = m->draft_io.as<int32_t>();
+  float* d_u = m->draft_io.as<float>() + 514;
+  cudaStream_t st = m->dev->stream;
+  const int start = m->pos;
+  int32_t got[514];  // tokens [n], accepted at n
+  auto run = [&]() -> int {
+    int last = 0;
+    FLOCK_TRY(encode_tokens(m, ids, n, &last));  // ids now also at m->ids
+    FLOCK_TRY(enqueue_head_rows(m, n, m->draft_logits.as<float>()));
+    if (u) FLOCK_CK(cudaMemcpyAsync(d_u, u, (size_t)n * 4, cudaMemcpyHostToDevice, st));
+    FLOCK_TRY(flock_verify_draft(m->dev, m->draft_logits.as<float>(), 0, draft, 0,
+                                 m->ids.as<int32_t>() + 1, d_u, nullptr, 1, n - 1, m->vocab,
+                                 temperature, d_tokens, d_tokens + n, m->draft_ws.p, st));
+    FLOCK_CK(cudaMemcpyAsync(got, d_tokens, (size_t)(n + 1) * 4, cudaMemcpyDeviceToHost, st));
+    FLOCK_TRY(sync_model(m));
+    FLOCK_TRY(check_device_errors(m));
+    if (got[got[n]] < 0) {
+      set_error("step_draft: the logits after %d drafts have no distribution", got[n]);
+      return FLOCK_E_STATE;
+    }
+    return FLOCK_OK;
+  };
+  const int rc = run();
+  if (rc) {
+    if (m->pos != start) flock_model_rewind(m, start);
+    return rc;
+  }
+  *n_tokens = got[n] + 1;
+  for (int i = 0; i < n; i++) tokens[i] = got[i];
+  // the certain positions: the consumed token's and the kept drafts'
+  FLOCK_CK(cudaMemcpyAsync(m->ids.p, d_tokens + got[n], 4, cudaMemcpyDeviceToDevice, st));
+  return flock_model_rewind(m, start + *n_tokens);
 }
 
 int flock_model_decode_device(flock_model* m, int n_steps, int32_t* out_ids) {

@@ -123,6 +123,26 @@ class Model:
                   ctypes.byref(out))
         return out.value
 
+    def step_draft(self, ids, draft=None, u=None, temperature: float = 0.0) -> list:
+        """Feed ids[0] and check the drafts ids[1:] of what follows it
+        (flock_model_step_draft): the kept drafts and the token after them.
+        ``draft``: device f32 [len(ids) - 1][vocab], the logits the drafts were
+        drawn from, or None; ``u``: len(ids) uniform numbers in [0, 1)."""
+        ids = self._ids(ids)
+        if u is not None:
+            u = np.ascontiguousarray(u, np.float32)
+            if u.size != ids.size:
+                raise ValueError(f"u is {u.size} numbers, want {ids.size}")
+        if draft is not None:
+            from .kv import _dense
+            draft = _dense(draft, "f32", self.dev.ordinal, "draft", (ids.size - 1, self.vocab))
+        out = np.empty(max(1, ids.size), np.int32)
+        n = ctypes.c_int()
+        _abi.call("flock_model_step_draft", self.handle, _abi.ptr(ids, _abi._i32p), ids.size,
+                  draft, None if u is None else _abi.ptr(u, _abi._fp), temperature,
+                  _abi.ptr(out, _abi._i32p), ctypes.byref(n))
+        return out[: n.value].tolist()
+
     def logits(self, ids) -> np.ndarray:
         """kernels/model.ts:400"""
         ids = self._ids(ids)

@@ -491,6 +491,21 @@ FLOCK_API int flock_model_trace_read(flock_model* m, uint64_t* out, int64_t cap,
                                      int* stride);
 /* flock_layer_set_window for every layer of the model. */
 FLOCK_API int flock_model_set_window(flock_model* m, int window, int sinks);
+/* One step of several greedy or sampled tokens (no counterpart in the
+ * reference): ids[0] is the token to consume, ids[1 .. n-1] drafts of what
+ * follows it (a small model's, or a lookup's).  All n run in one multi-token
+ * step, flock_verify_draft decides on the logits after each, and the caches go
+ * back to what is certain: pos has grown by *n_tokens = kept drafts + 1, tokens
+ * [n] holds the kept drafts and the token after them (then -1), which is also
+ * the one the next device-fed decode step consumes.  draft: device logits
+ * [n - 1][vocab] the drafts were drawn from, or NULL; u: n uniform numbers
+ * (host), or NULL at temperature 0.  n at most maxPrefill and 513; all n
+ * positions need room below maxKeys.  After an error the caches are as before
+ * the call; FLOCK_E_STATE also where the logits after the kept drafts have no
+ * distribution (a NaN).  Not for tensor-parallel models. */
+FLOCK_API int flock_model_step_draft(flock_model* m, const int32_t* ids, int n, const float* draft,
+                                     const float* u, double temperature, int32_t* tokens,
+                                     int* n_tokens);
 /* Set the token the next device-fed decode step consumes (ids[0]). */
 FLOCK_API int flock_model_set_token(flock_model* m, int32_t id);
 /* kernels/model.ts:541 currentToken(). */

@@ -149,6 +149,19 @@ export class Model {
     return Promise.resolve(Array.from(out.subarray(0, n)));
   }
 
+  /**
+   * Feed ids[0] and check the drafts ids[1..] of what follows it: the kept
+   * drafts and the token after them (flock_model_step_draft without draft
+   * logits).  `u`: one uniform number an id, at a temperature above 0.
+   */
+  stepDraft(ids: number[], u: Float32Array | null = null, temperature = 0): Promise<number[]> {
+    const out = new Int32Array(Math.max(1, ids.length));
+    const n = new Int32Array(1);
+    const fed = Int32Array.from(ids);
+    check(flock().flock_model_step_draft(this.handle, fed, fed.length, null, u, temperature, out, n));
+    return Promise.resolve(Array.from(out.subarray(0, n[0])));
+  }
+
   /** model.ts:529 rewind: drop the caches back to nKeys. */
   rewind(nKeys: number): void {
     check(flock().flock_model_rewind(this.handle, nKeys));
