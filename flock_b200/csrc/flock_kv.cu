@@ -120,14 +120,15 @@ int launch_rows(int sm_count, uint8_t* workspace, const KvAttnArgs& a, cudaStrea
   return FLOCK_OK;
 }
 
-// Many query rows: k_kv_prompt on the tensor cores, 128 rows a CTA.
-template <int KV>
+// Many query rows: k_kv_prompt on the tensor cores, 128 rows a CTA, alone or in pairs.
+template <int KV, bool PAIR>
 int launch_prompt(uint8_t* workspace, const KvAttnArgs& a, cudaStream_t st) {
   KvPromptArgs p = {};
   p.a = a;
   p.group = a.n_heads / a.c.n_kv_heads;
   p.rows = a.n_queries * p.group;
-  const int tiles = (p.rows + KP_ROWS - 1) / KP_ROWS;
+  int tiles = (p.rows + KP_ROWS - 1) / KP_ROWS;
+  if (PAIR) tiles = (tiles + 1) & ~1;
   const int64_t items = (int64_t)tiles * a.c.n_kv_heads;
   // key splits of a tile until the GPU is about full, at least two key tiles
   // each; the workspace holds 125 tiles' partial outputs
@@ -139,10 +140,20 @@ int launch_prompt(uint8_t* workspace, const KvAttnArgs& a, cudaStream_t st) {
   p.splits = (int)(want < room ? want : room);
   if (p.splits < 1) p.splits = 1;
   p.part = reinterpret_cast<float*>(workspace + KR_PART_OFFSET);
-  FLOCK_TRY(kernel_setup((const void*)k_kv_prompt<KV>, (int)KP_SMEM<KV>));
-  FLOCK_CK(launch_ex(st, k_kv_prompt<KV>,
-                     dim3((unsigned)tiles, (unsigned)p.splits, (unsigned)a.c.n_kv_heads),
-                     dim3(KP_THREADS), KP_SMEM<KV>, true, p));
+  FLOCK_TRY(kernel_setup((const void*)k_kv_prompt<KV, PAIR>, (int)KP_SMEM<KV>));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)tiles, (unsigned)p.splits, (unsigned)a.c.n_kv_heads);
+  cfg.blockDim = dim3(KP_THREADS);
+  cfg.dynamicSmemBytes = KP_SMEM<KV>;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {PAIR ? 2u : 1u, 1u, 1u};
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 2 : 1;
+  FLOCK_CK(cudaLaunchKernelEx(&cfg, k_kv_prompt<KV, PAIR>, p));
   if (p.splits > 1)
     FLOCK_CK(launch_ex(st, k_kv_prompt_join,
                        dim3((unsigned)((p.rows + 7) / 8), (unsigned)a.c.n_kv_heads), dim3(256), 0,
@@ -160,7 +171,17 @@ int flock::kv_attention_enqueue(int sm_count, int kv_dtype, const KvAttnArgs& a,
     // 16 rows: three tiles of k_kv_rows' smallest, where it and one mostly empty
     // tile of the tensor cores meet (6 queries of 16 / 8 heads at 8191 keys 15 us
     // against 22; 16 at 3000 keys 19 us on either)
-    if (rows > 16) return launch_prompt<KV>(workspace, a, st);
+    if (rows > 16) {
+      // Two tiles as a pair of CTAs where the operands are widened at a cost: 1024
+      // queries at 3000 keys of 16 / 8 heads 105 us against 119 (4-bit), 226
+      // against 283 (bf16); e4m3 gains 2% and loses 10% in a window.  A tile
+      // without a partner costs one: three tiles at 4000 keys 51 us against 43,
+      // thirteen 36 against 38.
+      const int64_t tiles = (rows + KP_ROWS - 1) / KP_ROWS;
+      if constexpr (KV != FLOCK_KV_FP8)
+        if (tiles % 2 == 0 || tiles > 8) return launch_prompt<KV, true>(workspace, a, st);
+      return launch_prompt<KV, false>(workspace, a, st);
+    }
     if constexpr (KV == FLOCK_KV_Q4 || KV == FLOCK_KV_FP8)
       if (rows <= 4) return launch_rows<KV, 1>(sm_count, workspace, a, st);  // one column tile
     return launch_rows<KV, 2>(sm_count, workspace, a, st);

@@ -13,31 +13,41 @@
 // significant bits, an f32 24: hi + lo again, three products (lo lo is below
 // 2^-22).
 //
+// Alone (PAIR false) a CTA widens every key for its 128 rows.  A pair, two CTAs
+// of a cluster with neighbouring row tiles and the same keys, shares that work:
+// the products are cta_group::2, 256 rows over both CTAs' tensor memory, and
+// either CTA widens and keeps half of a B operand's rows (keys of K, output
+// columns of V), in two stages.  1024 queries over 8192 4-bit keys, 16 / 8 heads:
+// 193 us against 222; three products an operand pair at the sustained rate are
+// 136, and the clock falls to 1.55 GHz under them.
+//
 // Roles, sixteen warps of 128 registers:
 //   warps 0-7   softmax; thread = row = tensor-memory lane, warps 0-3 the
 //               first 64 of its 128 scores, 4-7 the others (one thread a row
 //               took 6500 cycles a tile, its 128 scores' chains alone on a
-//               scheduler).  They agree on the row's maximum in shared memory,
-//               and write the weights' hi and lo parts over the scores in
+//               scheduler; so 3100).  They agree on the row's maximum in shared
+//               memory, and write the weights' hi and lo parts over the scores in
 //               tensor memory (the second product's A operand is read there).
 //   warps 8-11  widen the next K and V tiles from global memory into the
 //               128-byte-swizzled shared-memory operands (raw bytes are loaded
 //               into registers a tile ahead).  The order of dimensions (K: those
 //               q is given in; V: the output's columns) is whatever unpacks
 //               without shuffling, and is undone at the ends.
-//   warp 12     one thread issues the products: S(t+1) before O(t), so the
-//               softmax of a tile has two products' time, and K and V, one
-//               buffer each, are rewritten while the other is being read.
+//   warp 12     one thread (of the pair's first CTA) issues the products: O(t),
+//               then S(t+2) over its weights, while the softmax of t+1 goes on.
+//
+// A barrier that a thread may find two phases on is two barriers, by the tile's
+// parity: the weights' and the outputs'.
 //
 // The tensor cores' accumulators do not round to nearest: each step loses half a
 // last bit on average, towards zero, so a sum of n steps shrinks by about n
 // 2^-25 (1128 steps over 6000 keys: 2.3e-5).  The small products of a score go
 // first, and the outputs move to an f32 sum in shared memory every KP_FLUSH
-// tiles, added there in f32 (96 steps: 1e-6).
+// tiles, added there in f32 (96 steps: 1e-6; 16 us of the 193).
 //
 // The running maximum may lag by 2^8 before the outputs are rescaled (as in
 // k_kv_rows).  Every wait is bounded; a wait that runs out ends the CTA, which
-// then writes NaN.
+// then writes NaN (and so does its partner).
 #pragma once
 #include "gemm_tc.cuh"
 #include "kv_rows.cuh"
@@ -58,23 +68,86 @@ struct KvPromptArgs {
   float* part;      // [item][split][128 rows][128], then [..][128 rows][2] (base, l)
 };
 
-// 16-byte chunk c (8 columns) of row r of a 128 x 128 operand: two 64-column
-// halves of swizzled 128-byte rows.
+// 16-byte chunk c (8 columns) of row r of an operand of ROWS rows and 128
+// columns: two 64-column halves of swizzled 128-byte rows.
+template <int ROWS>
 FLOCK_DEV uint32_t kp_off(int r, int c) {
-  return (uint32_t)(c >> 3) * (128u * 128u) + sw128_off(r, c & 7);
+  return (uint32_t)(c >> 3) * (ROWS * 128u) + sw128_off(r, c & 7);
 }
 // D (+)= A B^T over 128 K elements; A in tensor memory (a column holds two).
+// PAIR: both CTAs' 128 rows of A and D, half of B's 128 rows in either.
+template <bool PAIR>
 FLOCK_DEV void kp_mma(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
-  const uint32_t idesc = umma_idesc_f16(128, 128);
+  const uint32_t idesc = umma_idesc_f16(PAIR ? 256 : 128, 128);
 #pragma unroll
   for (int k = 0; k < 8; k++) {
-    const uint32_t off = (uint32_t)(k >> 2) * (128u * 128u) + (uint32_t)(k & 3) * 32u;
+    const uint32_t off = (uint32_t)(k >> 2) * (PAIR ? 8192u : 16384u) + (uint32_t)(k & 3) * 32u;
     const uint64_t desc = umma_desc_sw128(b + off);
+    const uint32_t acc = accumulate || k > 0 ? 1u : 0u;
+    if constexpr (PAIR)
+      asm volatile(
+          "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+          " tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+          "r"(a + 8u * k), "l"(desc), "r"(idesc), "r"(acc)
+          : "memory");
+    else
+      asm volatile(
+          "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+          " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+          "r"(a + 8u * k), "l"(desc), "r"(idesc), "r"(acc)
+          : "memory");
+  }
+}
+// The barrier (of both CTAs) arrives once the products issued so far are done.
+template <bool PAIR>
+FLOCK_DEV void kp_commit(uint64_t* b) {
+  if constexpr (PAIR)
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a + 8u * k), "l"(desc), "r"(idesc), "r"(accumulate || k > 0 ? 1u : 0u)
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(smem_u32(b)), "h"((uint16_t)3)
         : "memory");
+  else
+    umma_commit(b);
+}
+template <bool PAIR>
+FLOCK_DEV void kp_alloc(uint32_t* slot) {  // all 512 columns
+  if constexpr (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                     smem_u32(slot))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tmem_alloc(slot, 512);
+    tmem_relinquish();
+  }
+}
+template <bool PAIR>
+FLOCK_DEV void kp_free(uint32_t t) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(t) : "memory");
+  else
+    tmem_dealloc(t, 512);
+}
+FLOCK_DEV void kp_cluster_sync() {  // every thread of both CTAs
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// What a thread arrives for (PAIR: its warp, at the first CTA's barrier, whose
+// thread issues the products of both).  What the barrier hands on, shared-memory
+// operands and tensor memory, each thread has ordered itself before it arrives
+// (proxy fence; store wait and tcgen05 fence), so the arrival need not be a
+// release over the cluster, which waits 1000 cycles for every access of the warp.
+template <bool PAIR>
+FLOCK_DEV void kp_arrive(uint64_t* b) {
+  if constexpr (PAIR) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0)
+      asm volatile(
+          "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, 0;\n"
+          " mbarrier.arrive.shared::cluster.b64 _, [a];\n}\n" ::"r"(smem_u32(b))
+          : "memory");
+  } else {
+    mbar_arrive(b);
   }
 }
 // 32 columns of this thread's lane; waits for them, so that no use can come before.
@@ -129,13 +202,15 @@ template <int KV>
 constexpr size_t KP_SMEM =
     (KP_LO<KV> ? 4 : 2) * (size_t)KP_OPND + 128 * KP_SUM_STRIDE * 4 + 1024;
 
-template <int KV>
+template <int KV, bool PAIR>
 static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvPromptArgs p) {
+  // operand rows here (keys of K, output columns of V), stages of them, their bytes
+  constexpr int OR = PAIR ? 64 : 128, NB = PAIR ? 2 : 1, OP = KP_OPND / NB;
   constexpr bool Q4 = KV == FLOCK_KV_Q4, LO = KP_LO<KV>;
   constexpr bool WIDE = KV == FLOCK_KV_F32 || KV == FLOCK_KV_BF16;  // elements scaled by tile
   constexpr bool SCALED = KV != FLOCK_KV_FP8;
   extern __shared__ __align__(16) uint8_t kp_raw[];
-  __shared__ uint64_t s_bar[9];
+  __shared__ uint64_t s_bar[14];
   __shared__ uint32_t s_tmem;
   __shared__ int s_err, s_ok[2];
   __shared__ float s_top[2][2][128];  // a row's maximum over either half, by tile parity
@@ -148,40 +223,42 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
   uint8_t* sKl = base + 2 * KP_OPND;
   uint8_t* sVl = base + 3 * KP_OPND;
   float* s_sum = reinterpret_cast<float*>(base + (LO ? 4 : 2) * KP_OPND);
-  uint64_t *k_full = s_bar, *k_empty = s_bar + 1, *v_full = s_bar + 2, *v_empty = s_bar + 3,
-           *s_full = s_bar + 4 /* 2 */, *p_full = s_bar + 6, *q_full = s_bar + 7,
-           *drained = s_bar + 8;
+  uint64_t *k_full = s_bar, *k_empty = s_bar + 2, *v_full = s_bar + 4, *v_empty = s_bar + 6,
+           *s_full = s_bar + 8, *p_full = s_bar + 10, *q_full = s_bar + 12, *drained = s_bar + 13;
+  auto stage = [](int t) { return NB == 2 ? t & 1 : 0; };
+  auto phase = [](int t) { return (uint32_t)(NB == 2 ? t >> 1 : t) & 1; };
   const KvAttnArgs& a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int tile = blockIdx.x, z = blockIdx.y, head = blockIdx.z;
+  const int rank = PAIR ? tile & 1 : 0;
   if (tid == 0) {
-    mbar_init(k_full, 128);
-    mbar_init(k_empty, 1);
-    mbar_init(v_full, 128);
-    mbar_init(v_empty, 1);
-    mbar_init(s_full, 1);
-    mbar_init(s_full + 1, 1);
-    mbar_init(p_full, 256);
-    mbar_init(q_full, 256);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(k_full + i, PAIR ? 8 : 128);
+      mbar_init(k_empty + i, 1);
+      mbar_init(v_full + i, PAIR ? 8 : 128);
+      mbar_init(v_empty + i, 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, PAIR ? 16 : 256);
+    }
+    mbar_init(q_full, PAIR ? 16 : 256);
     mbar_init(drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_err = 0;
   }
-  if (warp == 12) {
-    tmem_alloc(&s_tmem, 512);
-    tmem_relinquish();
-  }
+  if (warp == 12) kp_alloc<PAIR>(&s_tmem);
   tc_fence_before();
   __syncthreads();
+  if (PAIR) kp_cluster_sync();  // the other CTA's barriers are there to arrive at
   tc_fence_after();
   pdl_launch_dependents();  // after the allocation: a later grid's cannot hold what this one needs
   pdl_wait();
   const uint32_t tmem = s_tmem, tS = tmem, tO = tmem + 256, tQ = tmem + 384;
 
-  // keys that some row of the tile sees: sinks [0, sk), then [lo, hi)
+  // keys that some row of the tile (of both tiles of a pair) sees: sinks [0, sk),
+  // then [lo, hi)
   const int pos = kv_attn_pos(a);
-  const int first_q = tile * KP_ROWS / p.group;
-  const int last_q = (min(p.rows, (tile + 1) * KP_ROWS) - 1) / p.group;
+  const int first_q = (tile - rank) * KP_ROWS / p.group;
+  const int last_q = (min(p.rows, (tile - rank + NB) * KP_ROWS) - 1) / p.group;
   const int hi = pos + last_q + 1;
   const int lo = a.window && pos + first_q + 1 > a.window ? pos + first_q + 1 - a.window : 0;
   const int sk = min(a.sinks, lo);
@@ -205,8 +282,10 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
     const int row_hi = pos + query + 1;
     const int row_lo = a.window && row_hi > a.window ? row_hi - a.window : 0;
     const int row_sk = min(a.sinks, row_lo);
-    const int max_lo = a.window && pos + last_q + 1 > a.window ? pos + last_q + 1 - a.window : 0;
-    const int min_hi = pos + first_q + 1;
+    // keys in [max_lo, min_hi) are seen by every row of this CTA
+    const int own_last = (min(p.rows, (tile + 1) * KP_ROWS) - 1) / p.group;
+    const int max_lo = a.window && pos + own_last + 1 > a.window ? pos + own_last + 1 - a.window : 0;
+    const int min_hi = pos + min(tile * KP_ROWS, p.rows - 1) / p.group + 1;
     float unscale;
     {  // q log2(e) / sqrt(128), the row's largest in [2^13, 2^14), hi and lo parts
       const float* q = a.q + query * a.q_stride +
@@ -244,7 +323,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       }
       kp_st_wait();
       tc_fence_before();
-      mbar_arrive(q_full);
+      kp_arrive<PAIR>(q_full);
     }
     float m = -INFINITY, base_ = 0.0f, l = 0.0f;
     int vexp = -1000;
@@ -298,7 +377,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       if (t > 0 && (flush || __any_sync(0xffffffffu, go != 1.0f))) {
         // O(t-2) is complete with these scores, O(t-1) is waited for, and O(t)
         // waits for this thread
-        if (ok && !mbar_wait(v_empty, (t - 1) & 1, &s_err)) fail();
+        if (ok && !mbar_wait(v_empty + ((t - 1) & 1), ((t - 1) >> 1) & 1, &s_err)) fail();
         tc_fence_after();
 #pragma unroll
         for (int i = 0; i < 2; i++) {
@@ -325,35 +404,48 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       }
       // weights times the V tile's own power of two over the outputs'
       const float shift = fsub((float)(ve - vexp), base_);
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t f2 = pack2(f, f), shift2 = pack2(shift, shift), one2 = pack2(1.0f, 1.0f);
+      uint64_t sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
 #pragma unroll
       for (int c = 0; c < 2; c++) {  // 32 keys
         uint32_t h[16], w[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-          const float p0 = exp2_approx(ffma(s[32 * c + 2 * i], f, shift));
-          const float p1 = exp2_approx(ffma(s[32 * c + 2 * i + 1], f, shift));
-          sum[i & 1] = fadd(sum[i & 1], p0);
-          sum[2 + (i & 1)] = fadd(sum[2 + (i & 1)], p1);
-          split_f16(p0, p1, h[i], w[i]);
+          const float2 x =
+              unpack2(ffma2(pack2(s[32 * c + 2 * i], s[32 * c + 2 * i + 1]), f2, shift2));
+          const float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+          const uint64_t e2 = pack2(e.x, e.y);
+          sum[i & 1] = ffma2(e2, one2, sum[i & 1]);
+          h[i] = hf2(e.x, e.y);
+          const float2 hi = h2f2(h[i]);
+          const float2 rest = unpack2(fsub2(e2, pack2(hi.x, hi.y)));
+          w[i] = hf2(rest.x, rest.y);
         }
         kp_st16(S + 32 * half + 16 * c, h);
         kp_st16(S + 64 + 32 * half + 16 * c, w);
       }
-      l = ffma(fadd(fadd(sum[0], sum[1]), fadd(sum[2], sum[3])), pow2f(min(vexp - ve, 120)), l);
+      const float2 sum0 = unpack2(sum[0]), sum1 = unpack2(sum[1]);
+      l = ffma(fadd(fadd(sum0.x, sum0.y), fadd(sum1.x, sum1.y)), pow2f(min(vexp - ve, 120)), l);
       kp_st_wait();
       tc_fence_before();
-      mbar_arrive(p_full);
+      kp_arrive<PAIR>(p_full + (t & 1));
     }
     // ------------------------------------------------------------ epilogue
-    // the last scores being there says that O(n-3) is complete: the two phases
-    // after it are waited for in turn (a parity alone tells neighbours apart)
+    // the last scores being there says that O(n-3) is complete: either of the two
+    // after it has a barrier of its own, so that its parity says which
     for (int t = max(n - 2, 0); t < n; t++)
-      if (ok && !mbar_wait(v_empty, t & 1, &s_err)) fail();
+      if (ok && !mbar_wait(v_empty + (t & 1), (t >> 1) & 1, &s_err)) fail();
     kp_bar(2, 256);  // s_top is read, every wait decided
     s_top[0][half][r] = l;
     kp_bar(2, 256);
     ok = *(volatile int*)&s_err == 0;
+    if (PAIR) {  // the other CTA's keys and columns are in these rows too
+      int other;
+      asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n"
+                   " ld.volatile.shared::cluster.s32 %0, [a];\n}\n"
+                   : "=r"(other) : "r"(smem_u32(&s_err)), "r"(rank ^ 1) : "memory");
+      ok = ok && other == 0;
+    }
     l = fadd(s_top[0][0][r], s_top[0][1][r]);
     tc_fence_after();
     float o[64];
@@ -403,13 +495,19 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
   } else if (warp < 12) {
     // =========================================================== converters
     const int w = tid - 256, cw = warp - 8;
+    // K: the thread's key of the tile and which part of its row; of a pair either
+    // CTA widens half of the keys
+    const int kk = PAIR ? 64 * rank + (w & 63) : w, kr = PAIR ? w & 63 : w, kh = PAIR ? w >> 6 : 0;
     const int kg = w >> 3, vn = w & 7;   // V: keys 8 kg .. 8 kg + 7, byte column vn
-    constexpr int KR = Q4 ? 4 : WIDE ? 1 : 8;  // 16-byte loads of a K row held a tile ahead
+    constexpr int KR = (Q4 ? 4 : WIDE ? 2 : 8) / NB;  // 16-byte loads of a K row held a tile ahead
     uint4 kraw[KR];
-    uint2 kd = make_uint2(0, 0);
-    constexpr int VR = Q4 ? 4 : 8;       // 16 bytes each: two keys' 8 (4-bit), one key's 16
-    uint4 vraw[VR];
-    uint2 vd[8], vd_next[8];             // 4-bit: V scales of the thread's eight keys, this tile and the next
+    constexpr int VW = (Q4 ? 2 : 4) / NB;  // words of a key held for V
+    uint32_t vraw[8][VW];
+    // 4-bit: the scales of the thread's K row and V rows, and, for the tile's
+    // largest, those of key w
+    uint2 kd = make_uint2(0, 0), k_any = make_uint2(0, 0), v_any = make_uint2(0, 0);
+    constexpr int DW = 2 / NB;
+    uint32_t vd[8][DW];
     constexpr int ROW = Q4 ? 64 : KV == FLOCK_KV_FP8 ? 128 : KV == FLOCK_KV_BF16 ? 256 : 512;
     const size_t hb = Q4 ? q4_row(a.c, 0, head) * 64 : (size_t)head * ROW;
     const int64_t step = Q4 ? 64 : (int64_t)a.c.n_kv_heads * ROW;
@@ -423,27 +521,34 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       from = sink ? 0 : lo;
       to = sink ? sk : hi;
     };
+    auto load_words = [](const uint8_t* at, bool in, auto& out) {
+      constexpr int N = sizeof(out) / 4;
+      if constexpr (N == 1) {
+        out[0] = in ? __ldg(reinterpret_cast<const uint32_t*>(at)) : 0;
+      } else if constexpr (N == 2) {
+        const uint2 x = in ? __ldg(reinterpret_cast<const uint2*>(at)) : make_uint2(0, 0);
+        out[0] = x.x, out[1] = x.y;
+      } else {
+        const uint4 x = in ? __ldg(reinterpret_cast<const uint4*>(at)) : make_uint4(0, 0, 0, 0);
+        out[0] = x.x, out[1] = x.y, out[2] = x.z, out[3] = x.w;
+      }
+    };
     auto load_k = [&](int t) {
       if (WIDE) return;
       int from, to;
       range(t, from, to);
-      const int key = key_of(t) + w;
+      const int key = key_of(t) + kk;
       const bool in = key >= from && key < to;
 #pragma unroll
       for (int i = 0; i < KR; i++)
-        kraw[i] = in ? __ldg(reinterpret_cast<const uint4*>(kb + (int64_t)key * step) + i)
+        kraw[i] = in ? __ldg(reinterpret_cast<const uint4*>(kb + (int64_t)key * step) + KR * kh + i)
                      : make_uint4(0, 0, 0, 0);
-      if (Q4) kd = in ? __ldg(reinterpret_cast<const uint2*>(ks) + key) : make_uint2(0, 0);
-    };
-    auto load_vd = [&](int t) {
-      if (!Q4) return;
-      int from, to;
-      range(t, from, to);
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const int key = key_of(t) + 8 * kg + i;
-        vd_next[i] = key >= from && key < to ? __ldg(reinterpret_cast<const uint2*>(vs) + key)
-                                             : make_uint2(0, 0);
+      if (Q4) {
+        const int any = key_of(t) + w;
+        const bool has = any >= from && any < to;
+        kd = in ? __ldg(reinterpret_cast<const uint2*>(ks) + key) : make_uint2(0, 0);
+        k_any = has ? __ldg(reinterpret_cast<const uint2*>(ks) + any) : make_uint2(0, 0);
+        v_any = has ? __ldg(reinterpret_cast<const uint2*>(vs) + any) : make_uint2(0, 0);
       }
     };
     auto load_v = [&](int t) {
@@ -454,20 +559,8 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       for (int i = 0; i < 8; i++) {
         const int key = key_of(t) + 8 * kg + i;
         const bool in = key >= from && key < to;
-        if (Q4) {
-          const uint2 x = in ? __ldg(reinterpret_cast<const uint2*>(vb + (int64_t)key * 64) + vn)
-                             : make_uint2(0, 0);
-          if (i & 1) {
-            vraw[i >> 1].z = x.x;
-            vraw[i >> 1].w = x.y;
-          } else {
-            vraw[i >> 1].x = x.x;
-            vraw[i >> 1].y = x.y;
-          }
-        } else {
-          vraw[i & (VR - 1)] = in ? __ldg(reinterpret_cast<const uint4*>(vb + (int64_t)key * step) + vn)
-                                  : make_uint4(0, 0, 0, 0);
-        }
+        load_words(vb + (int64_t)key * step + 4 * VW * (NB * vn + rank), in, vraw[i]);
+        if (Q4) load_words(reinterpret_cast<const uint8_t*>(vs) + (int64_t)key * 8 + 4 * rank, in, vd[i]);
       }
     };
     // f32 and bf16 rows are too long to hold: read for the tile's largest
@@ -538,11 +631,8 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       };
       auto bits = [](__half2 h) { return (uint32_t)__half_as_ushort(__hmax(__low2half(h), __high2half(h))); };
       const __half2 zero = __float2half2_rn(0.0f);
-      __half2 hv = zero;
-#pragma unroll
-      for (int i = 0; i < 8; i++) hv = top(hv, vd_next[i]);
-      const uint32_t bk = __reduce_max_sync(0xffffffffu, bits(top(zero, kd)));
-      const uint32_t bv = __reduce_max_sync(0xffffffffu, bits(hv));
+      const uint32_t bk = __reduce_max_sync(0xffffffffu, bits(top(zero, k_any)));
+      const uint32_t bv = __reduce_max_sync(0xffffffffu, bits(top(zero, v_any)));
       if (lane == 0) {
         s_dmax[0][cw] = bk;
         s_dmax[1][cw] = bv;
@@ -566,21 +656,23 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       }
     };
     auto put_k = [&](int t) {
+      uint8_t *oh = sKh + stage(t) * OP, *ol = sKl + stage(t) * OP;
       if constexpr (WIDE) {
         int from, to;
         range(t, from, to);
         const float f = __uint_as_float(knorm);
 #pragma unroll 4
-        for (int c = 0; c < 16; c++) {
-          const float4 x = wide4(kb, key_of(t) + w, from, to, 8 * c);
-          const float4 y = wide4(kb, key_of(t) + w, from, to, 8 * c + 4);
+        for (int i = 0; i < 16 / NB; i++) {
+          const int c = 8 * kh + i;
+          const float4 x = wide4(kb, key_of(t) + kk, from, to, 8 * c);
+          const float4 y = wide4(kb, key_of(t) + kk, from, to, 8 * c + 4);
           uint32_t h[4], l[4];
           split_f16(fmul(x.x, f), fmul(x.y, f), h[0], l[0]);
           split_f16(fmul(x.z, f), fmul(x.w, f), h[1], l[1]);
           split_f16(fmul(y.x, f), fmul(y.y, f), h[2], l[2]);
           split_f16(fmul(y.z, f), fmul(y.w, f), h[3], l[3]);
-          *reinterpret_cast<uint4*>(sKh + kp_off(w, c)) = make_uint4(h[0], h[1], h[2], h[3]);
-          if (LO) *reinterpret_cast<uint4*>(sKl + kp_off(w, c)) = make_uint4(l[0], l[1], l[2], l[3]);
+          *reinterpret_cast<uint4*>(oh + kp_off<OR>(kr, c)) = make_uint4(h[0], h[1], h[2], h[3]);
+          if (LO) *reinterpret_cast<uint4*>(ol + kp_off<OR>(kr, c)) = make_uint4(l[0], l[1], l[2], l[3]);
         }
       } else if constexpr (Q4) {
         const uint32_t d01 = hmul2_u(kd.x, knorm), d23 = hmul2_u(kd.y, knorm);
@@ -588,7 +680,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         for (int b = 0; b < 4; b++) {
           const uint32_t d = __byte_perm(b < 2 ? d01 : d23, 0, b & 1 ? 0x3232 : 0x1010);
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
+          for (int c = 0; c < KR; c++) {
             uint32_t v[4], h[4], l[4];
             nib_f16(word_of(kraw[c], b), v);
 #pragma unroll
@@ -596,9 +688,9 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
               h[i] = hmul2_u(v[i], d);
               l[i] = hfma2_u(v[i], d, hneg2_u(h[i]));
             }
-            const uint32_t off = kp_off(w, 4 * b + c);
-            *reinterpret_cast<uint4*>(sKh + off) = make_uint4(h[0], h[2], h[1], h[3]);
-            *reinterpret_cast<uint4*>(sKl + off) = make_uint4(l[0], l[2], l[1], l[3]);
+            const uint32_t off = kp_off<OR>(kr, 4 * b + KR * kh + c);
+            *reinterpret_cast<uint4*>(oh + off) = make_uint4(h[0], h[2], h[1], h[3]);
+            *reinterpret_cast<uint4*>(ol + off) = make_uint4(l[0], l[2], l[1], l[3]);
           }
         }
       } else {
@@ -607,22 +699,24 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
           uint32_t v[8];
 #pragma unroll
           for (int j = 0; j < 8; j++) v[j] = fp8_f16(word_of(kraw[i], j >> 1) >> (16 * (j & 1)));
-          *reinterpret_cast<uint4*>(sKh + kp_off(w, 2 * i)) = make_uint4(v[0], v[1], v[2], v[3]);
-          *reinterpret_cast<uint4*>(sKh + kp_off(w, 2 * i + 1)) = make_uint4(v[4], v[5], v[6], v[7]);
+          const int c = 2 * (KR * kh + i);
+          *reinterpret_cast<uint4*>(oh + kp_off<OR>(kr, c)) = make_uint4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<uint4*>(oh + kp_off<OR>(kr, c + 1)) = make_uint4(v[4], v[5], v[6], v[7]);
         }
       }
     };
     auto put_v = [&](int t, uint32_t norm) {
+      uint8_t *oh = sVh + stage(t) * OP, *ol = sVl + stage(t) * OP;
       if constexpr (WIDE) {
         int from, to;
         range(t, from, to);
         const float f = __uint_as_float(norm);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {  // dimensions 16 vn + 4 i ..
+        for (int i = 0; i < 4 / NB; i++) {  // dimensions 16 vn + 8 rank + 4 i ..
           float4 x[8];
 #pragma unroll
           for (int j = 0; j < 8; j++)
-            x[j] = wide4(vb, key_of(t) + 8 * kg + j, from, to, 16 * vn + 4 * i);
+            x[j] = wide4(vb, key_of(t) + 8 * kg + j, from, to, 16 * vn + 8 * rank + 4 * i);
           auto at = [&](int j, int e) {
             return fmul(e == 0 ? x[j].x : e == 1 ? x[j].y : e == 2 ? x[j].z : x[j].w, f);
           };
@@ -631,24 +725,22 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
             uint32_t h[4], l[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) split_f16(at(2 * j, e), at(2 * j + 1, e), h[j], l[j]);
-            const uint32_t off = kp_off(8 * (4 * i + e) + vn, kg);
-            *reinterpret_cast<uint4*>(sVh + off) = make_uint4(h[0], h[1], h[2], h[3]);
-            if (LO) *reinterpret_cast<uint4*>(sVl + off) = make_uint4(l[0], l[1], l[2], l[3]);
+            const uint32_t off = kp_off<OR>(8 * (4 * i + e) + vn, kg);
+            *reinterpret_cast<uint4*>(oh + off) = make_uint4(h[0], h[1], h[2], h[3]);
+            if (LO) *reinterpret_cast<uint4*>(ol + off) = make_uint4(l[0], l[1], l[2], l[3]);
           }
         }
       } else if constexpr (Q4) {
 #pragma unroll
-        for (int b = 0; b < 4; b++) {
+        for (int b = 0; b < 4 / NB; b++) {  // blocks (2 rank +) b
           const uint32_t sel = b & 1 ? 0x7632u : 0x5410u;
           uint32_t h[4][4], l[4][4];  // [nibble][key pair]
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            const uint32_t x = b < 2 ? vraw[i].x : vraw[i].y, y = b < 2 ? vraw[i].z : vraw[i].w;
             uint32_t v[4];
-            nib_f16(__byte_perm(x, y, sel), v);
-            const uint32_t d = hmul2_u(
-                __byte_perm(b < 2 ? vd[2 * i].x : vd[2 * i].y, b < 2 ? vd[2 * i + 1].x : vd[2 * i + 1].y, sel),
-                norm);
+            nib_f16(__byte_perm(vraw[2 * i][b >> 1], vraw[2 * i + 1][b >> 1], sel), v);
+            const uint32_t d =
+                hmul2_u(__byte_perm(vd[2 * i][b >> 1], vd[2 * i + 1][b >> 1], sel), norm);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
               h[e][i] = hmul2_u(v[e], d);
@@ -657,21 +749,21 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
           }
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const uint32_t off = kp_off(32 * b + 8 * e + vn, kg);
-            *reinterpret_cast<uint4*>(sVh + off) = make_uint4(h[e][0], h[e][1], h[e][2], h[e][3]);
-            *reinterpret_cast<uint4*>(sVl + off) = make_uint4(l[e][0], l[e][1], l[e][2], l[e][3]);
+            const uint32_t off = kp_off<OR>(32 * b + 8 * e + vn, kg);
+            *reinterpret_cast<uint4*>(oh + off) = make_uint4(h[e][0], h[e][1], h[e][2], h[e][3]);
+            *reinterpret_cast<uint4*>(ol + off) = make_uint4(l[e][0], l[e][1], l[e][2], l[e][3]);
           }
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {  // dimensions 16 vn + 2 j, + 1
+        for (int j = 0; j < 2 * VW; j++) {  // dimensions 16 vn (+ 8 rank) + 2 j, + 1
           uint32_t x[8];
 #pragma unroll
-          for (int i = 0; i < 8; i++) x[i] = fp8_f16(word_of(vraw[i & (VR - 1)], j >> 1) >> (16 * (j & 1)));
+          for (int i = 0; i < 8; i++) x[i] = fp8_f16(vraw[i][(j >> 1) & (VW - 1)] >> (16 * (j & 1)));
 #pragma unroll
           for (int h = 0; h < 2; h++) {
             const uint32_t sel = h ? 0x7632u : 0x5410u;
-            *reinterpret_cast<uint4*>(sVh + kp_off(8 * (2 * j + h) + vn, kg)) =
+            *reinterpret_cast<uint4*>(oh + kp_off<OR>(8 * (2 * j + h) + vn, kg)) =
                 make_uint4(__byte_perm(x[0], x[1], sel), __byte_perm(x[2], x[3], sel),
                            __byte_perm(x[4], x[5], sel), __byte_perm(x[6], x[7], sel));
           }
@@ -688,44 +780,34 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
     // K(t + 1), then V(t); raw bytes are loaded as soon as the last tile's are
     // used up.  A failed wait skips the writes but keeps the barriers' counts.
     uint32_t vnorm_t = 0;  // of the V tile in hand
-    auto next_scales = [&]() {
-      vnorm_t = vnorm;
-      if (Q4) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) vd[i] = vd_next[i];
-      }
-    };
     auto k_tile = [&](int t) {
       norms(t);
-      if (t > 0) wait(k_empty, (t - 1) & 1);
+      if (t >= NB) wait(k_empty + stage(t - NB), phase(t - NB));
       if (ok) put_k(t);
       fence_proxy_async_smem();
-      mbar_arrive(k_full);
+      kp_arrive<PAIR>(k_full + stage(t));
       if (t + 1 < n) load_k(t + 1);
     };
     if (n > 0) {
       load_k(0);
-      load_vd(0);
       load_v(0);
       k_tile(0);
-      next_scales();
-      if (n > 1) load_vd(1);
+      vnorm_t = vnorm;
     }
     for (int t = 0; t < n; t++) {
       if (t + 1 < n) k_tile(t + 1);
-      if (t > 0) wait(v_empty, (t - 1) & 1);
+      if (t >= NB) wait(v_empty + ((t - NB) & 1), ((t - NB) >> 1) & 1);
       if (ok) put_v(t, vnorm_t);
       fence_proxy_async_smem();
-      mbar_arrive(v_full);
+      kp_arrive<PAIR>(v_full + stage(t));
       if (t + 1 < n) {
-        next_scales();
+        vnorm_t = vnorm;
         load_v(t + 1);
-        if (t + 2 < n) load_vd(t + 2);
       }
     }
   } else {
     // ============================================================= products
-    if (warp == 12 && lane == 0) {
+    if (warp == 12 && lane == 0 && rank == 0) {
       bool ok = true;
       auto wait = [&](uint64_t* b, uint32_t parity) {
         if (ok && !mbar_wait(b, parity, &s_err)) {
@@ -734,35 +816,40 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         }
       };
       auto scores = [&](int t) {
-        wait(k_full, t & 1);
         if (!ok) return;
         tc_fence_after();
-        const uint32_t d = tS + 128u * (t & 1);
-        kp_mma(d, tQ + 64, smem_u32(sKh), false);  // the small products first
-        if (LO) kp_mma(d, tQ, smem_u32(sKl), true);
-        kp_mma(d, tQ, smem_u32(sKh), true);
-        umma_commit(k_empty);
-        umma_commit(s_full + (t & 1));
+        const uint32_t d = tS + 128u * (t & 1), kh = smem_u32(sKh) + stage(t) * OP;
+        kp_mma<PAIR>(d, tQ + 64, kh, false);  // the small products first
+        if (LO) kp_mma<PAIR>(d, tQ, smem_u32(sKl) + stage(t) * OP, true);
+        kp_mma<PAIR>(d, tQ, kh, true);
+        kp_commit<PAIR>(k_empty + stage(t));
+        kp_commit<PAIR>(s_full + (t & 1));
       };
-      if (n > 0) {
-        wait(q_full, 0);
-        tc_fence_after();
-        scores(0);
+      wait(q_full, 0);
+      for (int t = 0; t < min(n, 2); t++) {
+        wait(k_full + stage(t), phase(t));
+        scores(t);
       }
+      // O(t), then S(t + 2) over O(t)'s weights: the softmax of two tiles is under
+      // way.  The operands are there long before the weights.
       for (int t = 0; t < n && ok; t++) {
-        if (t + 1 < n) scores(t + 1);
-        wait(p_full, t & 1);
-        wait(v_full, t & 1);
+        wait(v_full + stage(t), phase(t));
+        if (NB == 2 && t + 2 < n) wait(k_full + stage(t), phase(t + 2));
+        wait(p_full + (t & 1), (t >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t P = tS + 128u * (t & 1);
-        kp_mma(tO, P + 64, smem_u32(sVh), t % KP_FLUSH != 0);
-        if (LO) kp_mma(tO, P, smem_u32(sVl), true);
-        kp_mma(tO, P, smem_u32(sVh), true);
-        umma_commit(v_empty);
+        const uint32_t P = tS + 128u * (t & 1), vh = smem_u32(sVh) + stage(t) * OP;
+        kp_mma<PAIR>(tO, P + 64, vh, t % KP_FLUSH != 0);
+        if (LO) kp_mma<PAIR>(tO, P, smem_u32(sVl) + stage(t) * OP, true);
+        kp_mma<PAIR>(tO, P, vh, true);
+        kp_commit<PAIR>(v_empty + (t & 1));
+        if (t + 2 < n) {
+          if (NB == 1) wait(k_full, phase(t + 2));
+          scores(t + 2);
+        }
       }
       if (!ok) {  // let what was issued finish before the memory is given back
-        umma_commit(drained);
+        kp_commit<PAIR>(drained);
         mbar_wait(drained, 0, &s_err, false);
       }
     }
@@ -770,9 +857,10 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) kp_cluster_sync();  // nothing of the pair's is in flight, or will be read
   if (warp == 12) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    kp_free<PAIR>(tmem);
   }
 }
 

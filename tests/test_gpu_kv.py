@@ -395,3 +395,21 @@ def test_refusals(torch, dev):
     unaligned = torch.zeros(2 * 4 * HD + 1, device="cuda")[1:].view(2, 4, HD)
     refused(FLOCK_E_ARG, "aligned", lambda: cache.attention(unaligned, 3, o))
     refused(FLOCK_E_ARG, "aligned", lambda: cache.append(unaligned[:, :2], unaligned[:, 2:], 3))
+
+
+# Row tiles (128 rows of a kv head) that run in pairs, with and without a partner
+# or live rows in it: two full tiles, a last tile of few rows, nine tiles (the
+# tenth empty), splits of a pair's keys, several heads a kv head.
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,kv_heads,n,pos,window,sinks", [
+    (2, 1, 128, 0, 0, 0), (4, 2, 70, 900, 0, 0), (2, 1, 577, 3, 0, 0), (8, 2, 259, 150, 0, 0),
+    (4, 2, 200, 300, 77, 5), (1, 1, 1100, 0, 33, 0), (3, 1, 43, 2000, 1500, 200)])
+def test_attention_in_pairs(torch, dev, dtype, heads, kv_heads, n, pos, window, sinks):
+    keys = pos + n
+    k, v, q = rows(91, keys, kv_heads), rows(92, keys, kv_heads), rows(93, n, heads)
+    cache = filled(torch, dev, dtype, k, v, -(-(keys + 5) // 16) * 16, garbage=True)
+    check(torch, cache, dtype, q, k, v, pos, window, sinks)
+    out = [torch.empty(q.shape, device="cuda") for _ in range(2)]
+    for o in out:   # the same bits from call to call
+        cache.attention(torch.from_numpy(q).cuda(), pos, o, window=window, sinks=sinks)
+    assert torch.equal(*out)
