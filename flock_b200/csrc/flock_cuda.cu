@@ -460,6 +460,12 @@ int layer_set_window(flock_layer* L, int window, int sinks) {
   return FLOCK_OK;
 }
 
+int layer_few_rows(flock_layer* L, bool on) {
+  if (on) FLOCK_TRY(kv_workspace(L->ws));
+  L->few_rows = on;
+  return FLOCK_OK;
+}
+
 // The layer's cache as flock_kv.cu's kernels see it.
 static KvView layer_kv_view(const flock_layer* L) {
   KvView c = {};

@@ -176,6 +176,7 @@ struct flock_layer {
   flock::DBuf kcache, vcache, ctl_own, inv_freq;
   flock::DBuf kscales, vscales;  // FLOCK_KV_Q4 (capacity kv_capacity())
   int window = 0, sinks = 0;   // flock_layer_set_window; 0: every key
+  bool few_rows = false;       // a step of a few tokens that reads the cache directly
   int* ctl = nullptr;          // {pos, n_last} on the device (own or the model's)
   int n_keys = 0;              // host mirror
   // tensor parallel: this layer is one rank's slice; o_proj and down give
@@ -206,10 +207,13 @@ inline const char* kv_dtype_name(int kv) {
   return kv == FLOCK_KV_BF16 ? "bf16" : kv == FLOCK_KV_FP8 ? "fp8" : kv == FLOCK_KV_Q4 ? "4-bit" : "f32";
 }
 // Attention through kv_attention_enqueue (flock_kv.cu) instead of the layers'
-// own fused kernels: over a 4-bit cache, or in a window.
+// own fused kernels: over a 4-bit cache, in a window, or for the drafts of a
+// long conversation, where the tensor-core prefill would first lay out an f16
+// image of every cached key (layer_few_rows).
 inline bool layer_uses_kv_ops(const flock_layer* L) {
-  return L->cfg.kv_dtype == FLOCK_KV_Q4 || L->window > 0;
+  return L->cfg.kv_dtype == FLOCK_KV_Q4 || L->window > 0 || L->few_rows;
 }
+int layer_few_rows(flock_layer* L, bool on);
 int layer_set_window(flock_layer* L, int window, int sinks);
 int layer_init(flock_layer* L, flock_dev* dev, const flock_layer_config& cfg, Workspace* ws,
                int* shared_ctl);

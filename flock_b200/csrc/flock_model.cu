@@ -983,9 +983,18 @@ int flock_model_step_draft(flock_model* m, const int32_t* ids, int n, const floa
   cudaStream_t st = m->dev->stream;
   const int start = m->pos;
   int32_t got[514];  // tokens [n], accepted at n
+  // up to 16 rows a kv head (k_kv_rows): 6 tokens at 32000 keys of the 28-layer
+  // 0.6B shape 6.0 ms against 15 over the f32 cache, 3.3 against 14 over bf16
+  const bool few = m->cfg.attention == FLOCK_ATTN_FAST && n > 1 &&
+                   n * (m->cfg.n_heads / m->cfg.n_kv_heads) <= 16;
   auto run = [&]() -> int {
     int last = 0;
-    FLOCK_TRY(encode_tokens(m, ids, n, &last));  // ids now also at m->ids
+    int rc = FLOCK_OK;
+    for (auto* L : m->layers)
+      if (few && !rc) rc = layer_few_rows(L, true);
+    if (!rc) rc = encode_tokens(m, ids, n, &last);  // ids now also at m->ids
+    for (auto* L : m->layers) layer_few_rows(L, false);
+    FLOCK_TRY(rc);
     FLOCK_TRY(enqueue_head_rows(m, n, m->draft_logits.as<float>()));
     if (u) FLOCK_CK(cudaMemcpyAsync(d_u, u, (size_t)n * 4, cudaMemcpyHostToDevice, st));
     FLOCK_TRY(flock_verify_draft(m->dev, m->draft_logits.as<float>(), 0, draft, 0,

@@ -110,6 +110,7 @@ def test_sampled_drafts(dev, oracle, model_data, kv, with_logits):
     import torch
     oracle.set_fma_mode(False)
     m, _ = _prompted(dev, model_data, FAST.with_(kv=kv))
+    m.set_window(FAST.max_keys)   # sees every key; steps of any kind use the same attention
     H = FAST.hidden
 
     def rows(ids):
