@@ -366,6 +366,11 @@ int flock_kv_attention(flock_kv* c, const float* q, int64_t q_stride, int n_head
               (long long)row);
     return FLOCK_E_ARG;
   }
+  if ((int64_t)n_queries * (n_heads / c->view.n_kv_heads) > (int64_t)1 << 30) {
+    set_error("kv_attention: %d queries of %d heads over %d kv heads are more than 2^30 rows",
+              n_queries, n_heads, c->view.n_kv_heads);
+    return FLOCK_E_LIMIT;
+  }
   if (n_queries == 0) return FLOCK_OK;
   OnDevice on(c->dev->ordinal);
   FLOCK_TRY(on.enter());

@@ -23,6 +23,7 @@ from .lib import Device
 KV_DTYPES = {"f32": _abi.FLOCK_KV_F32, "bf16": _abi.FLOCK_KV_BF16, "fp8": _abi.FLOCK_KV_FP8,
              "q4": _abi.FLOCK_KV_Q4}
 HEAD_DIM = 128
+_INT_MAX = 2 ** 31 - 1  # no cache is longer: a window past it sees every key
 WORKSPACE_BYTES = _abi.FLOCK_WORKSPACE_BYTES
 
 # __cuda_array_interface__ type strings and torch dtype names of an element
@@ -165,8 +166,8 @@ class KVCache:
         op, no, _, os_ = _rows(out, self.dev.ordinal, "out", heads)
         if no != n:
             raise ValueError(f"out has {no} rows, q {n}")
-        rc = self._attention(self.handle, qp, qs, heads, n, pos, window, sinks, op, os_,
-                             stream or None)
+        rc = self._attention(self.handle, qp, qs, heads, n, pos, min(window, _INT_MAX),
+                             min(sinks, _INT_MAX), op, os_, stream or None)
         if rc:
             _abi.check(rc)
 

@@ -157,7 +157,8 @@ class Layer:
     def set_window(self, window: int, sinks: int = 0) -> None:
         """From the next step on queries see the ``window`` newest keys and the
         first ``sinks`` only; 0: every key (needs attention="fast")."""
-        _abi.call("flock_layer_set_window", self.handle, window, sinks)
+        _abi.call("flock_layer_set_window", self.handle, min(window, 2 ** 31 - 1),
+                  min(sinks, 2 ** 31 - 1))
 
     @property
     def n_keys(self) -> int:

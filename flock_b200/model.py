@@ -227,7 +227,8 @@ class Model:
     def set_window(self, window: int, sinks: int = 0) -> None:
         """From the next step on queries see the ``window`` newest keys and the
         first ``sinks`` only; 0: every key (needs attention="fast")."""
-        _abi.call("flock_model_set_window", self.handle, window, sinks)
+        _abi.call("flock_model_set_window", self.handle, min(window, 2 ** 31 - 1),
+                  min(sinks, 2 ** 31 - 1))
 
     @property
     def pos(self) -> int:

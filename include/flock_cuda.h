@@ -313,7 +313,7 @@ FLOCK_API int flock_kv_read(flock_kv* c, int64_t pos, int n, float* k, float* v,
  * kv heads in order (n_heads a multiple of n_kv_heads).  Keys no query sees
  * are not read into the result, whatever they hold; a NaN or infinity in a
  * key or value that only some queries of the call see makes the others'
- * outputs undefined. */
+ * outputs undefined.  At most 2^30 rows (queries times heads a kv head). */
 FLOCK_API int flock_kv_attention(flock_kv* c, const float* q, int64_t q_stride, int n_heads,
                                  int n_queries, int64_t pos, int window, int sinks, float* out,
                                  int64_t out_stride, void* stream);

@@ -413,3 +413,53 @@ def test_attention_in_pairs(torch, dev, dtype, heads, kv_heads, n, pos, window, 
     for o in out:   # the same bits from call to call
         cache.attention(torch.from_numpy(q).cuda(), pos, o, window=window, sinks=sinks)
     assert torch.equal(*out)
+
+
+def test_more_rows_than_an_int_are_refused(torch, dev):
+    from flock_b200._abi import FLOCK_E_LIMIT
+    from flock_b200.kv import KVCache
+    cache = KVCache(dev, "f32", 2, 32)
+    q = torch.zeros(4, device="cuda")   # refused before anything is read
+    rc = cache._attention(cache.handle, q.data_ptr(), 0, 2 << 26, 32, 0, 0, 0, q.data_ptr(), 0, None)
+    assert rc == FLOCK_E_LIMIT
+
+
+def test_a_window_past_32_bits_sees_every_key(torch, dev):
+    k, v, q = rows(94, 60, 2), rows(95, 60, 2), rows(96, 3, 4)
+    cache = filled(torch, dev, "q4", k, v, 64)
+    out = [torch.empty(q.shape, device="cuda") for _ in range(2)]
+    for o, w in zip(out, (0, 2 ** 32 + 5)):
+        cache.attention(torch.from_numpy(q).cuda(), 57, o, window=w)
+    assert torch.equal(*out)
+
+
+@pytest.mark.parametrize("dtype", ["q4", "bf16"])
+def test_pairs_in_two_graphs_at_once(torch, dev, dtype):
+    """Two captured prompt steps, a cache (and workspace) each, replayed together
+    on two streams, three times; a decode step on a third meanwhile."""
+    n, nkv, heads, nq = 700, 2, 4, 300
+    k, v, q = rows(97, n, nkv), rows(98, n, nkv), torch.from_numpy(rows(99, nq, heads)).cuda()
+    caches = [filled(torch, dev, dtype, k, v, 704) for _ in range(3)]
+    want = torch.empty(q.shape, device="cuda")
+    caches[0].attention(q, n - nq, want)
+    outs = [torch.zeros(q.shape, device="cuda") for _ in range(2)]
+    one, first = torch.zeros(1, heads, HD, device="cuda"), torch.zeros(1, heads, HD, device="cuda")
+    caches[2].attention(q[-1:], n - 1, first)
+    torch.cuda.synchronize()
+    streams, graphs = [torch.cuda.Stream() for _ in range(3)], []
+    for c, o, st in zip(caches, outs, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            c.attention(q, n - nq, o, stream=st.cuda_stream)
+        graphs.append(g)
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        caches[2].attention(q[-1:], n - 1, one, stream=streams[2].cuda_stream)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+        assert torch.equal(one, first)
