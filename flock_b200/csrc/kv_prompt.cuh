@@ -288,16 +288,29 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
     const int min_hi = pos + min(tile * KP_ROWS, p.rows - 1) / p.group + 1;
     float unscale;
     {  // q log2(e) / sqrt(128), the row's largest in [2^13, 2^14), hi and lo parts
-      const float* q = a.q + query * a.q_stride +
-                       ((int64_t)head * p.group + min(row, p.rows - 1) % p.group) * KV_HD;
+      // A warp reads whole rows (sixteen, 512 bytes each at once); a thread takes
+      // its own from the outputs' sum, which is not in use yet.  (A thread's
+      // own row straight from memory: 8 us.)
       const float k = __double2float_rn(1.4426950408889634 / sqrt(128.0));
-      float top = 0.0f;
-#pragma unroll 8
-      for (int i = 0; i < 32; i++) {
-        const float4 x = __ldg(reinterpret_cast<const float4*>(q) + i);
-        top = fmaxf(fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+      float4* sq = reinterpret_cast<float4*>(s_sum);
+      float4 x16[16];
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int rr = min(tile * KP_ROWS + 16 * warp + i, p.rows - 1);
+        x16[i] = __ldg(reinterpret_cast<const float4*>(
+                           a.q + (rr / p.group) * a.q_stride +
+                           ((int64_t)head * p.group + rr % p.group) * KV_HD) + lane);
       }
-      top = fmul(top, k);
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        auto mag = [](float y) { return __float_as_uint(y) & 0x7FFFFFFFu; };
+        const uint32_t most = __reduce_max_sync(
+            0xffffffffu, max(max(mag(x16[i].x), mag(x16[i].y)), max(mag(x16[i].z), mag(x16[i].w))));
+        if (lane == 0) s_top[0][0][16 * warp + i] = __uint_as_float(most);
+        sq[(16 * warp + i) * (KP_SUM_STRIDE / 4) + lane] = x16[i];
+      }
+      kp_bar(2, 256);
+      const float top = fmul(s_top[0][0][r], k);
       const int biased = (int)(__float_as_uint(top) >> 23);
       const int e = biased == 0 ? 0 : max(-100, min(100, biased - 127 - 13));
       const float scale = live ? __uint_as_float((uint32_t)(127 - e) << 23) : 0.0f;
@@ -308,7 +321,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         float x[32];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-          const float4 v = __ldg(reinterpret_cast<const float4*>(q) + w0 / 2 + i);
+          const float4 v = sq[r * (KP_SUM_STRIDE / 4) + w0 / 2 + i];
           x[4 * i] = fmul(fmul(v.x, k), scale);
           x[4 * i + 1] = fmul(fmul(v.y, k), scale);
           x[4 * i + 2] = fmul(fmul(v.z, k), scale);
@@ -466,31 +479,36 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         }
       }
     }
-    if (live) {
-      const float back = ok ? (n > 0 ? pow2f(max(vexp, -120)) : 0.0f) : NAN;
-      float* dst;
-      float mul;
-      if (p.splits == 1) {
-        dst = a.out + query * a.out_stride + ((int64_t)head * p.group + row % p.group) * KV_HD;
-        mul = fmul(back, fdiv(1.0f, l));
-      } else {
-        const size_t at = (((size_t)head * gridDim.x + tile) * p.splits + z) * KP_ROWS + r;
-        dst = p.part + at * KV_HD;
-        if (half == 0) {
-          float* ml = p.part + (size_t)gridDim.z * gridDim.x * p.splits * KP_ROWS * KV_HD + at * 2;
-          ml[0] = l > 0.0f ? base_ : -INFINITY;
-          ml[1] = l;
-        }
-        mul = back;
-      }
-      // columns 64 half .. hold the dimensions 64 half .. (4-bit), 16 i + 8 half .. (e4m3)
+    // through shared memory, so that a warp writes whole rows (a thread its own
+    // straight to memory: 4 us)
+    const float mul = fmul(ok ? (n > 0 ? pow2f(max(vexp, -120)) : 0.0f) : NAN,
+                           p.splits == 1 ? fdiv(1.0f, l) : 1.0f);
+    const size_t part_row = (((size_t)head * gridDim.x + tile) * p.splits + z) * KP_ROWS;
+    if (live && half == 0 && p.splits > 1) {
+      float* ml = p.part + (size_t)gridDim.z * gridDim.x * p.splits * KP_ROWS * KV_HD +
+                  (part_row + r) * 2;
+      ml[0] = l > 0.0f ? base_ : -INFINITY;
+      ml[1] = l;
+    }
+    kp_bar(2, 256);  // the sums are read
+    // columns 64 half .. hold the dimensions 64 half .. (4-bit), 16 i + 8 half .. (e4m3)
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const int d = Q4 ? 4 * i : 16 * (i >> 1) + 4 * (i & 1);
-        *reinterpret_cast<float4*>(dst + (Q4 ? 64 : 8) * half + d) =
-            make_float4(fmul(o[kp_vcol<KV>(d)], mul), fmul(o[kp_vcol<KV>(d + 1)], mul),
-                        fmul(o[kp_vcol<KV>(d + 2)], mul), fmul(o[kp_vcol<KV>(d + 3)], mul));
-      }
+    for (int i = 0; i < 16; i++) {
+      const int d = Q4 ? 4 * i : 16 * (i >> 1) + 4 * (i & 1);
+      *reinterpret_cast<float4*>(s_sum + r * KP_SUM_STRIDE + (Q4 ? 64 : 8) * half + d) =
+          make_float4(fmul(o[kp_vcol<KV>(d)], mul), fmul(o[kp_vcol<KV>(d + 1)], mul),
+                      fmul(o[kp_vcol<KV>(d + 2)], mul), fmul(o[kp_vcol<KV>(d + 3)], mul));
+    }
+    kp_bar(2, 256);
+#pragma unroll 4
+    for (int i = 0; i < 16; i++) {
+      const int rr = tile * KP_ROWS + 16 * warp + i;
+      if (rr >= p.rows) break;
+      float* dst = p.splits == 1 ? a.out + (rr / p.group) * a.out_stride +
+                                       ((int64_t)head * p.group + rr % p.group) * KV_HD
+                                 : p.part + (part_row + 16 * warp + i) * KV_HD;
+      reinterpret_cast<float4*>(dst)[lane] =
+          reinterpret_cast<const float4*>(s_sum)[(16 * warp + i) * (KP_SUM_STRIDE / 4) + lane];
     }
   } else if (warp < 12) {
     // =========================================================== converters
