@@ -92,6 +92,27 @@ int by_dtype(int kv_dtype, F f) {
   }
 }
 
+// Keys that some query of the call sees, sinks included (with the position on
+// the device and a window: of the bound).
+int64_t visible_keys(const KvAttnArgs& a) {
+  const int64_t lo = a.window && a.pos + 1 > a.window ? a.pos + 1 - a.window : 0;
+  return a.pos + a.n_queries - lo + (a.sinks < lo ? a.sinks : lo);
+}
+
+// k_kv_rows or k_kv_prompt.  The first's time grows with rows times keys, the
+// second's starts at 12 to 25 us and grows with the keys of 128 rows.  us, first
+// against second, 8 kv heads, rows @ keys:
+//   4-bit  32 @ 32000 59 / 67   48 @ 32000 75 / 68    48 @ 8169 26 / 32    64 @ 8169 35 / 32
+//   e4m3   24 @ 32000 43 / 51   32 @ 32000 60 / 51    48 @ 8169 26 / 27    64 @ 8169 34 / 27
+//   bf16   32 @ 32000 139 / 193 48 @ 32000 266 / 194  128 @ 1000 26 / 27   48 @ 8169 74 / 56
+//   f32    16 @ 32000 208 / 227 24 @ 32000 272 / 226  32 @ 1000 21 / 31    48 @ 1000 32 / 31
+template <int KV>
+bool few_rows(int64_t rows, int64_t keys, int64_t n_kv_heads) {
+  constexpr int always = KV == FLOCK_KV_F32 ? 16 : KV == FLOCK_KV_FP8 ? 24 : 32;
+  constexpr int64_t work = KV == FLOCK_KV_F32 ? 300000 : KV == FLOCK_KV_BF16 ? 1024000 : 3200000;
+  return rows <= always || (rows <= 128 && rows * keys * n_kv_heads <= work);
+}
+
 // A few query rows per kv head: k_kv_rows.
 template <int KV, int NT>
 int launch_rows(int sm_count, uint8_t* workspace, const KvAttnArgs& a, cudaStream_t st) {
@@ -132,9 +153,7 @@ int launch_prompt(uint8_t* workspace, const KvAttnArgs& a, cudaStream_t st) {
   const int64_t items = (int64_t)tiles * a.c.n_kv_heads;
   // key splits of a tile until the GPU is about full, at least two key tiles
   // each; the workspace holds 125 tiles' partial outputs
-  const int64_t lo = a.window && a.pos + 1 > a.window ? a.pos + 1 - a.window : 0;
-  const int64_t keys = a.pos + a.n_queries - lo + (a.sinks < lo ? a.sinks : lo);
-  const int64_t want = (keys + 2 * KP_KEYS - 1) / (2 * KP_KEYS);
+  const int64_t want = (visible_keys(a) + 2 * KP_KEYS - 1) / (2 * KP_KEYS);
   constexpr int64_t most = (FLOCK_WORKSPACE_BYTES - KR_PART_OFFSET) / (KP_ROWS * (KV_HD + 2) * 4);
   const int64_t room = most / items;
   p.splits = (int)(want < room ? want : room);
@@ -168,15 +187,12 @@ int flock::kv_attention_enqueue(int sm_count, int kv_dtype, const KvAttnArgs& a,
   const int64_t rows = (int64_t)a.n_queries * (a.n_heads / a.c.n_kv_heads);
   return by_dtype(kv_dtype, [&](auto kv) -> int {
     constexpr int KV = decltype(kv)::value;
-    // 16 rows: three tiles of k_kv_rows' smallest, where it and one mostly empty
-    // tile of the tensor cores meet (6 queries of 16 / 8 heads at 8191 keys 15 us
-    // against 22; 16 at 3000 keys 19 us on either)
-    if (rows > 16) {
+    if (!few_rows<KV>(rows, visible_keys(a), a.c.n_kv_heads)) {
       // Two tiles as a pair of CTAs where the operands are widened at a cost: 1024
-      // queries at 3000 keys of 16 / 8 heads 105 us against 119 (4-bit), 226
-      // against 283 (bf16); e4m3 gains 2% and loses 10% in a window.  A tile
-      // without a partner costs one: three tiles at 4000 keys 51 us against 43,
-      // thirteen 36 against 38.
+      // queries at 3000 keys of 16 / 8 heads 99 us against 114 (4-bit), 221
+      // against 276 (bf16); e4m3 gains 3% and loses 15% in a window.  A tile
+      // without a partner costs one: three tiles at 4000 keys 45 us against 36,
+      // thirteen in a window of 1500 keys 51 against 56.
       const int64_t tiles = (rows + KP_ROWS - 1) / KP_ROWS;
       if constexpr (KV != FLOCK_KV_FP8)
         if (tiles % 2 == 0 || tiles > 8) return launch_prompt<KV, true>(workspace, a, st);

@@ -18,7 +18,7 @@
 // the products are cta_group::2, 256 rows over both CTAs' tensor memory, and
 // either CTA widens and keeps half of a B operand's rows (keys of K, output
 // columns of V), in two stages.  1024 queries over 8192 4-bit keys, 16 / 8 heads:
-// 193 us against 222; three products an operand pair at the sustained rate are
+// 187 us against 216; three products an operand pair at the sustained rate are
 // 136, and the clock falls to 1.55 GHz under them.
 //
 // Roles, sixteen warps of 128 registers:
@@ -43,7 +43,7 @@
 // last bit on average, towards zero, so a sum of n steps shrinks by about n
 // 2^-25 (1128 steps over 6000 keys: 2.3e-5).  The small products of a score go
 // first, and the outputs move to an f32 sum in shared memory every KP_FLUSH
-// tiles, added there in f32 (96 steps: 1e-6; 16 us of the 193).
+// tiles, added there in f32 (96 steps: 1e-6; 16 us of the 187).
 //
 // The running maximum may lag by 2^8 before the outputs are rescaled (as in
 // k_kv_rows).  Every wait is bounded; a wait that runs out ends the CTA, which

@@ -403,7 +403,8 @@ def test_refusals(torch, dev):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("heads,kv_heads,n,pos,window,sinks", [
     (2, 1, 128, 0, 0, 0), (4, 2, 70, 900, 0, 0), (2, 1, 577, 3, 0, 0), (8, 2, 259, 150, 0, 0),
-    (4, 2, 200, 300, 77, 5), (1, 1, 1100, 0, 33, 0), (3, 1, 43, 2000, 1500, 200)])
+    (4, 2, 200, 300, 77, 5), (1, 1, 1100, 0, 33, 0), (3, 1, 43, 2000, 1500, 200),
+    (4, 2, 50, 17000, 0, 0), (4, 2, 45, 17000, 16500, 40)])   # one tile, alone, many keys
 def test_attention_in_pairs(torch, dev, dtype, heads, kv_heads, n, pos, window, sinks):
     keys = pos + n
     k, v, q = rows(91, keys, kv_heads), rows(92, keys, kv_heads), rows(93, n, heads)
