@@ -535,6 +535,7 @@ static int enqueue_qk_attn(flock_layer* L, int n, bool pdl, bool tensor_cores) {
     ka.pos = n == 1 ? c.max_keys - 1 : L->n_keys;
     ka.n_queries = n;
     ka.n_heads = c.n_heads;
+    ka.err = ws->tc_err.as<int>();
     ka.window = L->window;
     ka.sinks = L->sinks;
     ws->atc_nz = 1;

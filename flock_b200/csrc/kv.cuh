@@ -228,6 +228,7 @@ struct KvAttnArgs {
   int64_t q_stride, out_stride;
   int64_t pos;
   const int* ctl;  // a layer's step control: the position is ctl[0], pos its bound; or null
+  int* err;        // a layer's error word: nonzero when a bounded wait ran out; or null
   int n_queries, n_heads, window, sinks;
 };
 // After griddepcontrol.wait: an earlier kernel of the step writes ctl.

@@ -47,7 +47,7 @@
 //
 // The running maximum may lag by 2^8 before the outputs are rescaled (as in
 // k_kv_rows).  Every wait is bounded; a wait that runs out ends the CTA, which
-// then writes NaN (and so does its partner).
+// then writes NaN (and so does its partner) and sets a layer's error word.
 #pragma once
 #include "gemm_tc.cuh"
 #include "kv_rows.cuh"
@@ -270,7 +270,10 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
   auto key_of = [&](int t) {
     return t0 + t < sink_tiles ? (t0 + t) * KP_KEYS : lo16 + (t0 + t - sink_tiles) * KP_KEYS;
   };
-  auto fail = [&]() { *(volatile int*)&s_err = 1; };
+  auto fail = [&]() {
+    *(volatile int*)&s_err = 1;
+    if (a.err) atomicCAS(a.err, 0, 1);
+  };
 
   if (warp < 8) {
     // ============================================================== softmax

@@ -313,7 +313,9 @@ FLOCK_API int flock_kv_read(flock_kv* c, int64_t pos, int n, float* k, float* v,
  * kv heads in order (n_heads a multiple of n_kv_heads).  Keys no query sees
  * are not read into the result, whatever they hold; a NaN or infinity in a
  * key or value that only some queries of the call see makes the others'
- * outputs undefined.  At most 2^30 rows (queries times heads a kv head). */
+ * outputs undefined.  At most 2^30 rows (queries times heads a kv head).  The waits
+ * inside the many-row kernel are bounded (2 s); one that ran out, which nothing
+ * but a lost kernel of the device can cause, leaves NaN in its rows. */
 FLOCK_API int flock_kv_attention(flock_kv* c, const float* q, int64_t q_stride, int n_heads,
                                  int n_queries, int64_t pos, int window, int sinks, float* out,
                                  int64_t out_stride, void* stream);
