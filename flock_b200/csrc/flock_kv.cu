@@ -4,6 +4,7 @@
 
 #include <new>
 
+#include "arg_checks.h"
 #include "flock_internal.h"
 #include "kv.cuh"
 #include "kv_layer.h"
@@ -62,9 +63,9 @@ int check_device_pointer(const flock_dev* dev, const void* p, const char* what) 
 }
 
 int check_range(const flock_kv* c, const char* who, int64_t pos, int n) {
-  if (pos < 0 || n < 0 || pos + n > c->view.capacity) {
-    set_error("%s: positions %lld .. %lld are not inside a cache of %lld keys", who,
-              (long long)pos, (long long)pos + n - 1, (long long)c->view.capacity);
+  if (!range_inside(pos, n, c->view.capacity)) {
+    set_error("%s: %d positions from %lld on are not inside a cache of %lld keys", who, n,
+              (long long)pos, (long long)c->view.capacity);
     return FLOCK_E_STATE;
   }
   return FLOCK_OK;
