@@ -23,13 +23,25 @@ from .lib import Device
 KV_DTYPES = {"f32": _abi.FLOCK_KV_F32, "bf16": _abi.FLOCK_KV_BF16, "fp8": _abi.FLOCK_KV_FP8,
              "q4": _abi.FLOCK_KV_Q4}
 HEAD_DIM = 128
-_INT_MAX = 2 ** 31 - 1  # no cache is longer: a window past it sees every key
+# ctypes keeps an integer's low bits, so what the C types cannot hold is brought
+# to the nearest number that they can: no cache is as long as either.
+_INT_MAX = 2 ** 31 - 1   # a window past it sees every key
+_POS_MAX = 2 ** 63 - 1   # outside of every cache, as is -1
 WORKSPACE_BYTES = _abi.FLOCK_WORKSPACE_BYTES
 
 # __cuda_array_interface__ type strings and torch dtype names of an element
 _TYPES = {"f32": ("<f4", "float32"), "bf16": ("<u2", "bfloat16"), "fp8": ("|u1", "float8_e4m3fn"),
           "u8": ("|u1", "uint8"), "f16": ("<f2", "float16"), "i32": ("<i4", "int32")}
 _torch_types: dict = {}  # torch dtype -> element name, filled when a tensor comes by
+
+
+def _position(pos: int) -> int:
+    return -1 if pos < 0 else pos if pos <= _POS_MAX else _POS_MAX
+
+
+def _window(n: int) -> int:
+    """A window or a number of sinks; negative ones stay so, to be refused."""
+    return -1 if n < 0 else n if n <= _INT_MAX else _INT_MAX
 
 
 def _torch_type(t) -> str | None:
@@ -144,14 +156,14 @@ class KVCache:
         vp, nv, _, vs = _rows(v, self.dev.ordinal, "v", self.n_kv_heads)
         if n != nv or ks != vs:
             raise ValueError(f"k has {n} rows at stride {ks}, v {nv} at {vs}")
-        rc = self._append(self.handle, kp, vp, ks, pos, n, stream or None)
+        rc = self._append(self.handle, kp, vp, ks, _position(pos), n, stream or None)
         if rc:
             _abi.check(rc)
 
     def read(self, pos: int, n: int, k, v, stream: int = 0) -> None:
         """The cached rows pos .. pos + n - 1 into f32 k and v [n][n_kv_heads][128]."""
         shape = (n, self.n_kv_heads, HEAD_DIM)
-        rc = self._read(self.handle, pos, n, _dense(k, "f32", self.dev.ordinal, "k", shape),
+        rc = self._read(self.handle, _position(pos), n, _dense(k, "f32", self.dev.ordinal, "k", shape),
                         _dense(v, "f32", self.dev.ordinal, "v", shape), stream or None)
         if rc:
             _abi.check(rc)
@@ -166,8 +178,8 @@ class KVCache:
         op, no, _, os_ = _rows(out, self.dev.ordinal, "out", heads)
         if no != n:
             raise ValueError(f"out has {no} rows, q {n}")
-        rc = self._attention(self.handle, qp, qs, heads, n, pos, min(window, _INT_MAX),
-                             min(sinks, _INT_MAX), op, os_, stream or None)
+        rc = self._attention(self.handle, qp, qs, heads, n, _position(pos), _window(window),
+                             _window(sinks), op, os_, stream or None)
         if rc:
             _abi.check(rc)
 

@@ -16,6 +16,7 @@ from dataclasses import dataclass, replace
 import numpy as np
 
 from . import _abi
+from .kv import _window
 from .lib import Device, GpuTensor
 
 TENSOR_NAMES = ("attn_q.weight", "attn_k.weight", "attn_v.weight", "attn_output.weight",
@@ -157,8 +158,7 @@ class Layer:
     def set_window(self, window: int, sinks: int = 0) -> None:
         """From the next step on queries see the ``window`` newest keys and the
         first ``sinks`` only; 0: every key (needs attention="fast")."""
-        _abi.call("flock_layer_set_window", self.handle, min(window, 2 ** 31 - 1),
-                  min(sinks, 2 ** 31 - 1))
+        _abi.call("flock_layer_set_window", self.handle, _window(window), _window(sinks))
 
     @property
     def n_keys(self) -> int:

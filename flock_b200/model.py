@@ -15,6 +15,7 @@ import ctypes
 import numpy as np
 
 from . import _abi
+from .kv import _dense, _window
 from .layer import QWEN3_06B, TENSOR_NAMES, LayerConfig, upload_layer
 from .lib import Device, GpuTensor
 
@@ -134,7 +135,6 @@ class Model:
             if u.size != ids.size:
                 raise ValueError(f"u is {u.size} numbers, want {ids.size}")
         if draft is not None:
-            from .kv import _dense
             draft = _dense(draft, "f32", self.dev.ordinal, "draft", (ids.size - 1, self.vocab))
         out = np.empty(max(1, ids.size), np.int32)
         n = ctypes.c_int()
@@ -227,8 +227,7 @@ class Model:
     def set_window(self, window: int, sinks: int = 0) -> None:
         """From the next step on queries see the ``window`` newest keys and the
         first ``sinks`` only; 0: every key (needs attention="fast")."""
-        _abi.call("flock_model_set_window", self.handle, min(window, 2 ** 31 - 1),
-                  min(sinks, 2 ** 31 - 1))
+        _abi.call("flock_model_set_window", self.handle, _window(window), _window(sinks))
 
     @property
     def pos(self) -> int:

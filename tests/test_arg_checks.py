@@ -1,12 +1,15 @@
 """The entry points' argument checks without a GPU: csrc/arg_checks.h compiled by
-itself."""
+itself, and the integers that kv.py and the model classes hand on."""
 import ctypes
 import os
 import subprocess
+import types
 
 import pytest
 
 from flock_b200 import _abi, kv
+from flock_b200.layer import Layer
+from flock_b200.model import Model
 
 CSRC = os.path.join(os.path.dirname(_abi.__file__), "csrc")
 I64_MAX, I64_MIN = 2 ** 63 - 1, -2 ** 63
@@ -35,6 +38,60 @@ def test_positions_inside_a_cache(checks, capacity):
         for n in (-1, 0, 1, 2, 32, capacity, 2 ** 31 - 1):
             want = pos >= 0 and n >= 0 and pos + n <= capacity
             assert checks.range_inside(pos, n, capacity) == want, (pos, n, capacity)
+
+
+class OnDevice:
+    """What a CUDA array shows of itself; nothing reads the address here."""
+
+    def __init__(self, *shape):
+        self.__cuda_array_interface__ = dict(shape=shape, typestr="<f4", strides=None,
+                                             data=(4096, False), version=3)
+
+
+def _cache(name):
+    """A KVCache whose `name` entry point records what reaches the C call."""
+    seen = []
+    c = object.__new__(kv.KVCache)
+    c.handle, c.dev, c.n_kv_heads = None, types.SimpleNamespace(ordinal=0), 2
+    proto = ctypes.CFUNCTYPE(ctypes.c_int, *_abi.SIGNATURES[f"flock_kv_{name}"])
+    c._entry = proto(lambda *a: seen.append(a) or 0)
+    setattr(c, f"_{name}", c._entry)
+    return c, seen
+
+
+@pytest.mark.parametrize("pos", [2 ** 63, 2 ** 64, 2 ** 64 + 3, -2 ** 63 - 1, -2 ** 64])
+def test_a_position_past_64_bits_is_not_another_one(checks, pos):
+    """ctypes keeps the low 64 bits of an integer: 2^64 + 3 must not become 3."""
+    x = OnDevice(1, 2, 128)
+    for name, at, call in [("append", 4, lambda c: c.append(x, x, pos)),
+                           ("read", 1, lambda c: c.read(pos, 1, x, x)),
+                           ("attention", 5, lambda c: c.attention(x, pos, x))]:
+        c, seen = _cache(name)
+        call(c)
+        assert not checks.range_inside(seen[0][at], 1, 2 ** 30), name
+
+
+@pytest.mark.parametrize("window,sinks", [(-2 ** 32, 0), (5, -2 ** 32), (-2 ** 31 - 1, 1)])
+def test_a_negative_window_stays_negative(monkeypatch, window, sinks):
+    x = OnDevice(1, 2, 128)
+    c, seen = _cache("attention")
+    c.attention(x, 0, x, window=window, sinks=sinks)
+    assert seen[0][6] < 0 or seen[0][7] < 0
+    for cls, name in ((Layer, "flock_layer_set_window"), (Model, "flock_model_set_window")):
+        args = []
+        monkeypatch.setattr(_abi, "call", lambda fn, handle, *a: args.append((fn, a)))
+        o = object.__new__(cls)
+        o.handle = None
+        o.set_window(window, sinks)
+        fn, (w, s) = args[0]
+        assert fn == name and -2 ** 31 <= min(w, s) < 0 and max(w, s) < 2 ** 31
+
+
+def test_windows_past_32_bits_see_every_key():
+    x = OnDevice(1, 2, 128)
+    c, seen = _cache("attention")
+    c.attention(x, 0, x, window=2 ** 40, sinks=2 ** 33)
+    assert seen[0][6] == seen[0][7] == 2 ** 31 - 1
 
 
 @pytest.mark.gpu
