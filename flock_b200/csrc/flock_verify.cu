@@ -85,6 +85,15 @@ int flock_verify_draft(flock_dev* dev, const float* target, int64_t target_strid
     set_error("verify_draft: target, ids, u, tokens, accepted and workspace must not be NULL");
     return FLOCK_E_ARG;
   }
+  // floats and ints at 4 bytes, the workspace's 8-byte keys and more at 16: a
+  // misaligned address would fault the GPU
+  auto off = [](const void* p, uintptr_t align) { return (reinterpret_cast<uintptr_t>(p) & (align - 1)) != 0; };
+  if (off(workspace, 16) || off(target, 4) || off(draft, 4) || off(ids, 4) || off(u, 4) ||
+      off(lens, 4) || off(tokens, 4) || off(accepted, 4)) {
+    set_error("verify_draft: the workspace must be 16-byte aligned, every other address 4-byte "
+              "aligned");
+    return FLOCK_E_ARG;
+  }
   if (target_stride == 0) target_stride = vocab;
   if (draft_stride == 0) draft_stride = vocab;
   if (target_stride < vocab || draft_stride < vocab) {

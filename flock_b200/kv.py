@@ -187,12 +187,14 @@ class KVCache:
 class DraftVerifier:
     """flock_verify_draft over a vocabulary: drafted tokens checked against the
     target's logits with given uniform numbers.  ``workspace``: WORKSPACE_BYTES
-    of device uint8 that no overlapping call uses."""
+    of device uint8, 16-byte aligned, that no overlapping call uses."""
 
     def __init__(self, dev: Device, vocab: int, workspace):
         self.dev, self.vocab = dev, vocab
         self._keep = workspace
         self._ws = _workspace(workspace, dev.ordinal)
+        if self._ws & 15:
+            raise ValueError("the workspace is not 16-byte aligned")
         self._verify = _abi.lib().flock_verify_draft
 
     def _logits(self, a, what: str, n: int, rows: int) -> tuple:

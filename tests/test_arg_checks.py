@@ -110,3 +110,41 @@ def test_positions_whose_end_passes_64_bits_are_refused(dtype):
             assert e.value.code == _abi.FLOCK_E_STATE
     cache.append(x, x, 30)
     cache.attention(x, 30, out)
+
+
+# ------------------------------------------------- draft verification's addresses
+# target, draft, ids, u, lens, tokens, accepted, workspace: argument numbers
+ADDRESSES = dict(target=1, draft=3, ids=5, u=6, lens=7, tokens=12, accepted=13, workspace=14)
+
+
+def _verify(temperature, **at):
+    """flock_verify_draft with made-up addresses, refused before a device is touched."""
+    dev = ctypes.create_string_buffer(1024)   # no device; its first bytes say ordinal 0
+    args = [ctypes.addressof(dev), 4096, 0, 4096, 0, 4096, 4096, 4096, 1, 2, 100, temperature,
+            4096, 4096, 4096, None]
+    for name, a in at.items():
+        args[ADDRESSES[name]] = a
+    lib = _abi.lib()
+    return lib.flock_verify_draft(*args), lib.flock_last_error().decode()
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+@pytest.mark.parametrize("name,off", [("workspace", 1), ("workspace", 4), ("workspace", 8)] +
+                         [(n, 2) for n in ADDRESSES if n != "workspace"])
+def test_misaligned_addresses_are_refused(name, off, temperature):
+    rc, text = _verify(temperature, **{name: 4096 + off})
+    assert rc == _abi.FLOCK_E_ARG and "aligned" in text
+
+
+class Bytes:
+    def __init__(self, at):
+        self.__cuda_array_interface__ = dict(shape=(kv.WORKSPACE_BYTES,), typestr="|u1",
+                                             strides=None, data=(at, False), version=3)
+
+
+def test_a_misaligned_workspace_is_refused():
+    dev = types.SimpleNamespace(ordinal=0, handle=None)
+    kv.DraftVerifier(dev, 100, Bytes(4096))
+    for at in (4097, 4100, 4104):
+        with pytest.raises(ValueError, match="workspace.*aligned"):
+            kv.DraftVerifier(dev, 100, Bytes(at))
