@@ -158,6 +158,7 @@ SIGNATURES = {
     "flock_model_set_window": [_vp, _i, _i],
     "flock_model_step_draft": [_vp, _i32p, _i, _vp, _fp, ctypes.c_double, _i32p,
                                ctypes.POINTER(_i)],
+    "flock_model_wait_stream": [_vp, _vp],
     "flock_model_set_token": [_vp, ctypes.c_int32],
     "flock_model_set_decode_mode": [_vp, _i],
     "flock_model_get_decode_mode": [_vp, _ip],

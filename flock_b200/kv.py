@@ -74,6 +74,15 @@ def _interface(a, dtype: str, what: str):
     return i["data"][0], tuple(i["shape"]), strides and tuple(s // size for s in strides)
 
 
+def _stream_of(a) -> int:
+    """The stream that a device array is written on, as far as it says: torch's
+    current one, or the interface's (none named: 0, the default stream)."""
+    if hasattr(a, "data_ptr"):
+        import torch
+        return torch.cuda.current_stream(a.device).cuda_stream if a.is_cuda else 0
+    return getattr(a, "__cuda_array_interface__", {}).get("stream") or 0
+
+
 def _dense(a, dtype: str, ordinal: int, what: str, shape: tuple) -> int:
     p, got, strides = _array(a, dtype, ordinal, what)
     if strides is not None or tuple(got) != shape:

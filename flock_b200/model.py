@@ -15,7 +15,7 @@ import ctypes
 import numpy as np
 
 from . import _abi
-from .kv import _dense, _window
+from .kv import _dense, _stream_of, _window
 from .layer import QWEN3_06B, TENSOR_NAMES, LayerConfig, upload_layer
 from .lib import Device, GpuTensor
 
@@ -124,18 +124,25 @@ class Model:
                   ctypes.byref(out))
         return out.value
 
-    def step_draft(self, ids, draft=None, u=None, temperature: float = 0.0) -> list:
+    def step_draft(self, ids, draft=None, u=None, temperature: float = 0.0,
+                   stream: int | None = None) -> list:
         """Feed ids[0] and check the drafts ids[1:] of what follows it
         (flock_model_step_draft): the kept drafts and the token after them.
         ``draft``: device f32 [len(ids) - 1][vocab], the logits the drafts were
-        drawn from, or None; ``u``: len(ids) uniform numbers in [0, 1)."""
+        drawn from, or None; ``u``: len(ids) uniform numbers in [0, 1).
+        ``stream``: the cudaStream_t that ``draft`` is written on, whose work so
+        far is waited for; by default torch's current stream, or the one that
+        ``__cuda_array_interface__`` names, or the default stream."""
         ids = self._ids(ids)
         if u is not None:
             u = np.ascontiguousarray(u, np.float32)
             if u.size != ids.size:
                 raise ValueError(f"u is {u.size} numbers, want {ids.size}")
         if draft is not None:
+            on = _stream_of(draft) if stream is None else stream
             draft = _dense(draft, "f32", self.dev.ordinal, "draft", (ids.size - 1, self.vocab))
+            if on:  # the default stream is waited for in any case
+                _abi.call("flock_model_wait_stream", self.handle, on)
         out = np.empty(max(1, ids.size), np.int32)
         n = ctypes.c_int()
         _abi.call("flock_model_step_draft", self.handle, _abi.ptr(ids, _abi._i32p), ids.size,

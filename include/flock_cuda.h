@@ -504,10 +504,17 @@ FLOCK_API int flock_model_set_window(flock_model* m, int window, int sinks);
  * (host), or NULL at temperature 0.  n at most maxPrefill and 513; all n
  * positions need room below maxKeys.  After an error the caches are as before
  * the call; FLOCK_E_STATE also where the logits after the kept drafts have no
- * distribution (a NaN).  Not for tensor-parallel models. */
+ * distribution (a NaN).  Not for tensor-parallel models.  draft is read on a
+ * stream of the model's own, behind what the default stream holds at the call;
+ * what writes it on another stream has to be done, or waited for with
+ * flock_model_wait_stream. */
 FLOCK_API int flock_model_step_draft(flock_model* m, const int32_t* ids, int n, const float* draft,
                                      const float* u, double temperature, int32_t* tokens,
                                      int* n_tokens);
+/* What the model enqueues from now on runs after the work that `stream` (a
+ * cudaStream_t of the model's device, NULL: the default stream) holds now.
+ * Nothing waits on the host.  FLOCK_E_STATE while `stream` is being captured. */
+FLOCK_API int flock_model_wait_stream(flock_model* m, void* stream);
 /* Set the token the next device-fed decode step consumes (ids[0]). */
 FLOCK_API int flock_model_set_token(flock_model* m, int32_t id);
 /* kernels/model.ts:541 currentToken(). */

@@ -193,6 +193,8 @@ export const symbols = {
   flock_model_set_window: { parameters: ["pointer", "i32", "i32"], result: "i32" },
   // (m, ids, n, draft, u, temperature, tokens, n_tokens)
   flock_model_step_draft: { parameters: ["pointer", "buffer", "i32", "buffer", "buffer", "f64", "buffer", "buffer"], result: "i32" },
+  // (m, stream)
+  flock_model_wait_stream: { parameters: ["pointer", "buffer"], result: "i32" },
   // (m, id)
   flock_model_set_token: { parameters: ["pointer", "i32"], result: "i32" },
   // (m, out)

@@ -148,3 +148,18 @@ def test_a_misaligned_workspace_is_refused():
     for at in (4097, 4100, 4104):
         with pytest.raises(ValueError, match="workspace.*aligned"):
             kv.DraftVerifier(dev, 100, Bytes(at))
+
+
+# ------------------------------------------------------- where an array is written
+def test_the_stream_that_an_array_names():
+    class On:
+        def __init__(self, **kw):
+            self.__cuda_array_interface__ = dict(shape=(1,), typestr="<f4", data=(4096, False),
+                                                 version=3, **kw)
+    assert [kv._stream_of(On()), kv._stream_of(On(stream=None)), kv._stream_of(On(stream=2)),
+            kv._stream_of(On(stream=77)), kv._stream_of([1.0])] == [0, 0, 2, 77, 0]
+
+
+def test_wait_stream_wants_a_model():
+    assert _abi.lib().flock_model_wait_stream(None, None) == _abi.FLOCK_E_ARG
+    assert "wait_stream" in _abi.lib().flock_last_error().decode()
