@@ -1,8 +1,6 @@
 // Draft verification (include/flock_cuda.h flock_verify_draft).
 #include <cuda_runtime.h>
 
-#include <cmath>
-
 #include "flock_internal.h"
 #include "verify.cuh"
 
@@ -73,10 +71,9 @@ int flock_verify_draft(flock_dev* dev, const float* target, int64_t target_strid
               VERIFY_MAX_DRAFTS, (long long)vocab, (long long)VERIFY_MAX_VOCAB);
     return FLOCK_E_LIMIT;
   }
-  if (!(temperature >= 0.0) || !std::isfinite(temperature) ||
-      (temperature > 0.0 && !std::isfinite(32.0 / temperature))) {
-    set_error("verify_draft: temperature %g must be finite and not negative (0: greedy)",
-              temperature);
+  // log2(e) / temperature has to be a normal f32 (k_verify_stats)
+  if (temperature != 0.0 && !(temperature >= 1e-38 && temperature <= 1e38)) {
+    set_error("verify_draft: temperature %g must be 0 (greedy) or in 1e-38 .. 1e38", temperature);
     return FLOCK_E_ARG;
   }
   if (n_seqs == 0) return FLOCK_OK;

@@ -204,7 +204,9 @@ FLOCK_DEV void verify_join(const VerifyArgs& a, size_t row, float& m, double& s)
 // 16), n the integer nearest 16 z / ln 2 and |r| <= 1/2, 2^(r / 16) by the
 // Taylor polynomial of e^(r ln 2 / 16) of degree 6 (remainder below 5e-16 of
 // it), 2^(j / 16) from a table.  Relative error below 1e-15 for z > -40,
-// growing as |z| 2e-17.  Logits not above `lowest` (m - 700 T, -inf) give 0.
+// growing as |z| 2e-17.  z below -700, and a logit of -inf, give 0: decided on n,
+// since a border m - 700 T in f32 is m itself at a small T, and would take the
+// row's maximum with it.
 __constant__ static const double k_pow16[16] = {
     0x1.0000000000000p+0, 0x1.0b5586cf9890fp+0, 0x1.172b83c7d517bp+0, 0x1.2387a6e756238p+0,
     0x1.306fe0a31b715p+0, 0x1.3dea64c123422p+0, 0x1.4bfdad5362a27p+0, 0x1.5ab07dd485429p+0,
@@ -212,10 +214,9 @@ __constant__ static const double k_pow16[16] = {
     0x1.ae89f995ad3adp+0, 0x1.c199bdd85529cp+0, 0x1.d5818dcfba487p+0, 0x1.ea4afa2a490dap+0};
 struct VerifyRow {
   double m, c;
-  float lowest;
 };
 FLOCK_DEV VerifyRow verify_row_of(float m, double inv_t) {
-  return {(double)m, inv_t * 0x1.71547652b82fep+4, (float)((double)m - 700.0 / inv_t)};
+  return {(double)m, inv_t * 0x1.71547652b82fep+4};
 }
 FLOCK_DEV double verify_exp(float x, const VerifyRow& row, const double* pow16) {
   const double magic = 6755399441055744.0;  // 1.5 2^52: adding it rounds to an integer
@@ -231,7 +232,8 @@ FLOCK_DEV double verify_exp(float x, const VerifyRow& row, const double* pow16) 
   p = fma(p, r, 1.0);
   const int k = __double2loint(t);  // n, two's complement
   const double e = p * pow16[k & 15];
-  return x > row.lowest
+  // t is 1.5 2^52 + n, whose bits count in ones; far down, or -inf, they are fewer
+  return __double_as_longlong(t) > 0x4338000000000000ll - 16160
              ? __hiloint2double(__double2hiint(e) + ((k >> 4) << 20), __double2loint(e)) : 0.0;
 }
 
@@ -314,8 +316,8 @@ static __global__ void __launch_bounds__(VP_THREADS) k_verify_pick(const VerifyA
   const bool has = summable(r) && (!residual || summable(a.n + 1 + r));
   if (rank == 0) {
     int32_t* out = a.tokens + (size_t)seq * (a.n + 1);
-    for (int i = t; i <= a.n; i += VP_THREADS)
-      if (i != r || !has) out[i] = i < r ? ids[i] : -1;
+    // token r too: the warp that draws it writes it behind the cluster's barriers
+    for (int i = t; i <= a.n; i += VP_THREADS) out[i] = i < r ? ids[i] : -1;
     if (t == 0) a.accepted[seq] = r;
   }
   if (!has) return;  // the whole cluster agrees

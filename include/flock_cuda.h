@@ -338,7 +338,7 @@ FLOCK_API int flock_kv_attention(flock_kv* c, const float* q, int64_t q_stride, 
  * every one before it was.  At the first refusal r the next token is drawn
  * from max(p_r - q_r, 0), normalised (from p_r where nothing is left), after
  * `lens` kept drafts from p: the lowest index whose running sum passes
- * u_{n_drafts} of the total.  temperature 0: drafts are kept while they equal
+ * u_{n_drafts} of the total.  temperature is 0 or in 1e-38 .. 1e38; at 0 drafts are kept while they equal
  * the argmax (lowest index among the maxima, NaN never one), draft and u are
  * not read.  tokens [n_seqs][n_drafts + 1]: the kept drafts, the next token,
  * then -1; accepted [n_seqs]: how many were kept.
