@@ -204,9 +204,8 @@ FLOCK_DEV void verify_join(const VerifyArgs& a, size_t row, float& m, double& s)
 // 16), n the integer nearest 16 z / ln 2 and |r| <= 1/2, 2^(r / 16) by the
 // Taylor polynomial of e^(r ln 2 / 16) of degree 6 (remainder below 5e-16 of
 // it), 2^(j / 16) from a table.  Relative error below 1e-15 for z > -40,
-// growing as |z| 2e-17.  z below -700, and a logit of -inf, give 0: decided on n,
-// since a border m - 700 T in f32 is m itself at a small T, and would take the
-// row's maximum with it.
+// growing as |z| 2e-17.  Logits below `lowest` (m - 700 T rounded up: at a small T
+// it is m itself, which counts; above -inf at a large one) give 0.
 __constant__ static const double k_pow16[16] = {
     0x1.0000000000000p+0, 0x1.0b5586cf9890fp+0, 0x1.172b83c7d517bp+0, 0x1.2387a6e756238p+0,
     0x1.306fe0a31b715p+0, 0x1.3dea64c123422p+0, 0x1.4bfdad5362a27p+0, 0x1.5ab07dd485429p+0,
@@ -214,9 +213,10 @@ __constant__ static const double k_pow16[16] = {
     0x1.ae89f995ad3adp+0, 0x1.c199bdd85529cp+0, 0x1.d5818dcfba487p+0, 0x1.ea4afa2a490dap+0};
 struct VerifyRow {
   double m, c;
+  float lowest;
 };
 FLOCK_DEV VerifyRow verify_row_of(float m, double inv_t) {
-  return {(double)m, inv_t * 0x1.71547652b82fep+4};
+  return {(double)m, inv_t * 0x1.71547652b82fep+4, __double2float_ru((double)m - 700.0 / inv_t)};
 }
 FLOCK_DEV double verify_exp(float x, const VerifyRow& row, const double* pow16) {
   const double magic = 6755399441055744.0;  // 1.5 2^52: adding it rounds to an integer
@@ -232,8 +232,7 @@ FLOCK_DEV double verify_exp(float x, const VerifyRow& row, const double* pow16) 
   p = fma(p, r, 1.0);
   const int k = __double2loint(t);  // n, two's complement
   const double e = p * pow16[k & 15];
-  // t is 1.5 2^52 + n, whose bits count in ones; far down, or -inf, they are fewer
-  return __double_as_longlong(t) > 0x4338000000000000ll - 16160
+  return x >= row.lowest
              ? __hiloint2double(__double2hiint(e) + ((k >> 4) << 20), __double2loint(e)) : 0.0;
 }
 
@@ -424,13 +423,22 @@ static __global__ void __launch_bounds__(VP_THREADS) k_verify_pick(const VerifyA
       s_total[turn] = sum;
     }
     cluster.sync();
-    // running sums over the CTAs, a lane each, the same in every CTA
-    double run = lane < nr ? *cluster.map_shared_rank(s_total + turn, lane) : 0.0;
+    // running sums over the CTAs, a lane each, the same in every CTA: one after the
+    // other in fours, and so the fours, which never fall and stay as they are over a
+    // CTA without weight (a scan by doubling adds neighbours in different orders)
+    const double total = lane < nr ? *cluster.map_shared_rank(s_total + turn, lane) : 0.0;
+    double run = 0.0, fours = 0.0;
 #pragma unroll
-    for (int d = 1; d < VP_MAX_CLUSTER; d <<= 1) {
-      const double o = __shfl_up_sync(0xffffffffu, run, d);
-      if (lane >= d) run += o;
+    for (int i = 0; i < 4; i++) {
+      const double o = __shfl_sync(0xffffffffu, total, (lane & ~3) + i);
+      run += i <= (lane & 3) ? o : 0.0;
     }
+#pragma unroll
+    for (int i = 0; i + 1 < VP_MAX_CLUSTER / 4; i++) {
+      const double o = __shfl_sync(0xffffffffu, run, 4 * i + 3);
+      fours += i < lane >> 2 ? o : 0.0;
+    }
+    run += fours;
     before = rank == 0 ? 0.0 : __shfl_sync(0xffffffffu, run, rank - 1);
     end = __shfl_sync(0xffffffffu, run, rank);
     w = __shfl_sync(0xffffffffu, run, nr - 1);
@@ -439,14 +447,18 @@ static __global__ void __launch_bounds__(VP_THREADS) k_verify_pick(const VerifyA
   }
   // no CTA leaves while another may read its shared memory
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  // this warp's [before, end) of the running sum: its CTA's, cut at the warps
-  // before it; the last warp's end is the next CTA's beginning
+  // This warp's [before, end) of the running sum: its CTA's, cut at the warps
+  // before it, and none without weight.  The CTA's end and the warps' sums round
+  // apart: cut at that end, and the last warp of weight reaches it, the parts cover
+  // [0, w) once, so one warp draws, and it has a token to draw.
   const double cta_end = end;
+  const uint32_t weighted = __ballot_sync(0xffffffffu, lane < WARPS && s_red[lane % WARPS] > 0.0);
   for (int i = 0; i < warp; i++) before += s_red[i];
-  end = warp + 1 < WARPS ? before + s_red[warp] : cta_end;
+  end = weighted >> warp > 1 ? fmin(before + s_red[warp], cta_end) : cta_end;
+  const bool some = weighted >> warp & 1;
   double goal = (double)u[a.n] * w;
   if (!(goal < w)) goal = w * 0.9999999999999999;
-  if (before <= goal && goal < end) {
+  if (some && before <= goal && goal < end) {
     int pick = -1, last = v0;
     double c = before;
     auto look = [&](int i, const double (&e)[4], const double (&f)[4]) {
@@ -464,7 +476,8 @@ static __global__ void __launch_bounds__(VP_THREADS) k_verify_pick(const VerifyA
         const double o = __shfl_up_sync(0xffffffffu, run, d);
         if (lane >= d) run += o;
       }
-      const uint32_t over = __ballot_sync(0xffffffffu, c + run > goal);
+      // of the lanes with weight: the others' sums may pass it by their rounding
+      const uint32_t over = __ballot_sync(0xffffffffu, top >= 0 && c + run > goal);
       if (over && pick < 0) {
         int found = top;  // rounding may leave it to the lane's last weight
         double upto = c + (run - sum) + sum;

@@ -68,3 +68,42 @@ def test_temperatures_out_of_range_are_refused(torch, dev, scratch):  # noqa: F8
         with pytest.raises(FlockError, match="temperature") as e:
             run(torch, dev, scratch, target, draft, ids, u, None, t)
         assert e.value.code == FLOCK_E_ARG
+
+
+@pytest.mark.parametrize("n,d,v", [(2, 2, 900), (30, 1, 5001)])
+def test_uniform_numbers_outside_their_range(torch, dev, scratch, n, d, v):  # noqa: F811
+    """Some token is drawn wherever there is a distribution."""
+    target, draft, ids, u, _ = inputs(33, n, d, v)
+    ends = [(1.0, 1 - 2.0 ** -24), (7.0, 1 - 2.0 ** -24), (np.inf, 1 - 2.0 ** -24)]
+    for probs in (draft, None):
+        for bad, near in ends:
+            got = []
+            for last in (bad, near):
+                x = u.copy()
+                x[:, d] = last
+                got.append(run(torch, dev, scratch, target, probs, ids, x, None, 1.0))
+            (tok, acc), (want, want_acc) = got
+            at = np.arange(n), acc
+            assert (acc == want_acc).all() and (tok[at] >= 0).all() and (tok[at] < v).all()
+            # the last token, or one before it of less than 2^-24 in all
+            assert (tok[at] >= want[at]).all()
+
+
+@pytest.mark.parametrize("n", [9, 64])
+def test_a_draw_on_the_border_of_two_blocks(torch, dev, scratch, n):  # noqa: F811
+    """Eight times the same 8192 logits, the last 513 of them -inf: at u = k / 8 the
+    goal is a running sum but for its rounding, at the end of a block of a cluster (of
+    8 or 16 blocks) whose last warps hold no weight.  One warp draws: the last token
+    of weight before the border or the first behind it, the same each time."""
+    v, period = 65536, 8192
+    for seed in range(12):
+        r = np.random.default_rng(seed)
+        one = (r.standard_normal((n, 1, period)) * 2).astype(np.float32)
+        one[:, :, -513:] = -np.inf
+        target = np.tile(one, (1, 1, v // period))
+        for k in range(1, 8):
+            u = np.full((n, 1), k / 8, np.float32)
+            got = [run(torch, dev, scratch, target, None, np.zeros((n, 0), np.int32), u, None,
+                       1.0)[0][:, 0] for _ in range(2)]
+            np.testing.assert_array_equal(*got)
+            assert np.isin(got[0], (period * k - 514, period * k)).all(), (seed, k, got[0])
