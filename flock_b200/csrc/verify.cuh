@@ -456,7 +456,7 @@ static __global__ void __launch_bounds__(VP_THREADS) k_verify_pick(const VerifyA
   for (int i = 0; i < warp; i++) before += s_red[i];
   end = weighted >> warp > 1 ? fmin(before + s_red[warp], cta_end) : cta_end;
   const bool some = weighted >> warp & 1;
-  double goal = (double)u[a.n] * w;
+  double goal = fmax((double)u[a.n], 0.0) * w;  // fmax: 0 for a NaN
   if (!(goal < w)) goal = w * 0.9999999999999999;
   if (some && before <= goal && goal < end) {
     int pick = -1, last = v0;

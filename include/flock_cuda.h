@@ -331,7 +331,8 @@ FLOCK_API int flock_kv_attention(flock_kv* c, const float* q, int64_t q_stride, 
  * the tokens before draft i, rows target_stride floats apart (0: dense).
  * draft: the logits [n_seqs][n_drafts][vocab] the drafts were drawn from at
  * the same temperature, or NULL when each draft was certain (a lookup).
- * u [n_seqs][n_drafts + 1]: uniform numbers in [0, 1).
+ * u [n_seqs][n_drafts + 1]: uniform numbers in [0, 1); the draw takes another
+ * as the nearest of them (NaN as 0).
  *
  * With p_i and q_i the softmax of the rows / temperature (q_i = 1 at ids[i]
  * without draft logits), draft i is kept iff u_i q_i(ids[i]) < p_i(ids[i]) and

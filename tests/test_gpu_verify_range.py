@@ -72,9 +72,11 @@ def test_temperatures_out_of_range_are_refused(torch, dev, scratch):  # noqa: F8
 
 @pytest.mark.parametrize("n,d,v", [(2, 2, 900), (30, 1, 5001)])
 def test_uniform_numbers_outside_their_range(torch, dev, scratch, n, d, v):  # noqa: F811
-    """Some token is drawn wherever there is a distribution."""
+    """A draw takes what is not in [0, 1) as the nearest number that is, NaN as 0:
+    some token is drawn wherever there is a distribution."""
     target, draft, ids, u, _ = inputs(33, n, d, v)
-    ends = [(1.0, 1 - 2.0 ** -24), (7.0, 1 - 2.0 ** -24), (np.inf, 1 - 2.0 ** -24)]
+    ends = [(-1e-30, 0.0), (-1.0, 0.0), (-np.inf, 0.0), (np.nan, 0.0), (1.0, 1 - 2.0 ** -24),
+            (7.0, 1 - 2.0 ** -24), (np.inf, 1 - 2.0 ** -24)]
     for probs in (draft, None):
         for bad, near in ends:
             got = []
@@ -85,8 +87,10 @@ def test_uniform_numbers_outside_their_range(torch, dev, scratch, n, d, v):  # n
             (tok, acc), (want, want_acc) = got
             at = np.arange(n), acc
             assert (acc == want_acc).all() and (tok[at] >= 0).all() and (tok[at] < v).all()
-            # the last token, or one before it of less than 2^-24 in all
-            assert (tok[at] >= want[at]).all()
+            if near == 0.0:   # the first token of any weight
+                np.testing.assert_array_equal(tok, want)
+            else:             # the last one, or one before it of less than 2^-24 in all
+                assert (tok[at] >= want[at]).all()
 
 
 @pytest.mark.parametrize("n", [9, 64])
