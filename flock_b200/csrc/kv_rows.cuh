@@ -25,18 +25,23 @@
 // cores align a subnormal's product as if it were normal and drop the bits below:
 // errors of 3e-6 instead of 3e-7.)  A block's products are multiplied by the
 // key's scale in f32, one accumulator per block.  Values: the scale joins the
-// weight, so the weight operand differs per block.
+// weight, so the weight operand differs per block.  Scales further apart than
+// 2^KR_SPREAD (a warp keeps watch) would leave the smaller ones' products too few
+// bits in f16: the warp then begins again with the products as three bf16 parts.
 //
 // Work split: CTA (split z, row tile, kv head), its warps taking 16-key groups
 // in turn, each with its own cp.async ring, running maximum, sum and output;
 // warps join in shared memory, CTAs in the workspace, the last to arrive adding
 // the splits in order (results do not depend on who is last).
 #pragma once
+#include <type_traits>
+
 #include "kv.cuh"
 
 namespace flock {
 
 constexpr int KR_GROUP = 16;  // keys per warp step
+constexpr int KR_SPREAD = 12;  // 4-bit value scales a warp takes in f16: 2^12 apart
 constexpr int KR_MAX_ITEMS = 4096;  // (row tile, kv head) pairs that may be split: arrival counters
 constexpr size_t KR_PART_OFFSET = KR_MAX_ITEMS * 4;
 
@@ -391,292 +396,345 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
 #pragma unroll
   for (int n = 0; n < RL; n++) unscale[n] = F16 ? s_unscale[4 * n + c] : 1.0f;
   float o[8][NT][4];
-#pragma unroll
-  for (int u = 0; u < 8; u++)
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) o[u][n][e] = 0.0f;
-  // Weights are 2^(s - base), base = m - 6, m a running maximum that may lag by
-  // 2^8: at most 2^14, inside f16, and a lo part loses nothing above 2^-31 of
+  // Weights are 2^(s - base), base = m - 10, m a running maximum that may lag by
+  // 2^4: at most 2^14, inside f16, and a lo part loses nothing above 2^-35 of
   // the largest.  Value scales are divided by 2^dexp, a bound on those so far,
-  // which the outputs get back at the end.
-  constexpr float HEADROOM = F16 ? 6.0f : 0.0f;
+  // which the outputs get back at the end; those down to 2^-12 of it leave the
+  // largest weight's products at 2^-2 and up, 2^23 of a lo part's last bit.
+  constexpr float HEADROOM = F16 ? 10.0f : 0.0f, LAG = F16 ? 4.0f : 8.0f;
   float m[RL], l[RL], base[RL];
-#pragma unroll
-  for (int n = 0; n < RL; n++) {
-    m[n] = -INFINITY;
-    l[n] = base[n] = 0.0f;
-  }
   int dexp = -14;
-  uint32_t dlim = 0x04000400u, dnorm = 0x74007400u;  // f16 pairs 2^dexp and 2^-dexp
-
-  int st = 0;
-  for (int grp = g0 + warp; grp < g1; grp += L::WARPS) {
-    cp_async_wait<L::STAGES - 2>();
-    __syncwarp();  // the stage has landed for every lane, and every lane is done with the last one
-    fetch(grp + (L::STAGES - 1) * L::WARPS, st == 0 ? L::STAGES - 1 : st - 1);
-    const uint8_t* stage = kr_smem + (warp * L::STAGES + st) * L::STAGE;
-    // ------------------------------------------------------------- scores
-    float s[RL][2];  // keys g, g + 8
-    const uint8_t* ka = stage + g * L::K_STRIDE + 16 * c;
-    if constexpr (Q4) {
-      const uint4 w0 = ld_u4(ka), w1 = ld_u4(ka + 8 * L::K_STRIDE);
-      const uint2 e0 = ld_u2(stage + L::S_OFF + 8 * g), e1 = ld_u2(stage + L::S_OFF + 8 * g + 64);
+  // The warp's groups; false: the value scales lie too far apart, and nothing of
+  // this pass counts.  WIDE: whatever the scales.
+  auto pass = [&](auto wide) -> bool {
+    constexpr bool WIDE = decltype(wide)::value;
 #pragma unroll
-      for (int n = 0; n < RL; n++) s[n][0] = s[n][1] = 0.0f;
-#pragma unroll
-      for (int b = 0; b < 4; b++) {
-        uint32_t x[4], y[4];
-        nib_f16(word_of(w0, b), x);
-        nib_f16(word_of(w1, b), y);
-        const float2 d0 = h2f2(b < 2 ? e0.x : e0.y), d1 = h2f2(b < 2 ? e1.x : e1.y);
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-          float acc[4];
-          const uint32_t a0[4] = {x[0], y[0], x[2], y[2]}, a1[4] = {x[1], y[1], x[3], y[3]};
-          mma16<F16>(acc, a0, qb[n][2 * b].x, qb[n][2 * b].y, 0.f, 0.f, 0.f, 0.f);
-          mma16<F16>(acc, a1, qb[n][2 * b + 1].x, qb[n][2 * b + 1].y);
-          s[n][0] = ffma(b & 1 ? d0.y : d0.x, fadd(acc[0], acc[1]), s[n][0]);
-          s[n][1] = ffma(b & 1 ? d1.y : d1.x, fadd(acc[2], acc[3]), s[n][1]);
-        }
-      }
-    } else {
-      float acc[NT][2][4];
+    for (int u = 0; u < 8; u++)
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) acc[n][h][e] = 0.0f;
-      if constexpr (KV == FLOCK_KV_FP8) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const uint4 w0 = ld_u4(ka + 64 * h), w1 = ld_u4(ka + 64 * h + 8 * L::K_STRIDE);
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const uint32_t x = word_of(w0, i), y = word_of(w1, i);
-            const uint32_t av[4] = {fp8_f16(x), fp8_f16(y), fp8_f16(x >> 16), fp8_f16(y >> 16)};
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-              mma16<F16>(acc[n][i & 1], av, qb[n][4 * h + i].x, qb[n][4 * h + i].y);
-          }
-        }
-      } else if constexpr (KV == FLOCK_KV_BF16) {
-#pragma unroll
-        for (int h = 0; h < 4; h++) {
-          const uint4 w0 = ld_u4(ka + 64 * h), w1 = ld_u4(ka + 64 * h + 8 * L::K_STRIDE);
-          const uint32_t a0[4] = {w0.x, w1.x, w0.y, w1.y}, a1[4] = {w0.z, w1.z, w0.w, w1.w};
-#pragma unroll
-          for (int n = 0; n < NT; n++) {
-            mma16<F16>(acc[n][0], a0, qb[n][2 * h].x, qb[n][2 * h].y);
-            mma16<F16>(acc[n][1], a1, qb[n][2 * h + 1].x, qb[n][2 * h + 1].y);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < 8; ks++) {
-          const uint4 w0 = ld_u4(ka + 64 * ks), w1 = ld_u4(ka + 64 * ks + 8 * L::K_STRIDE);
-          uint32_t x0[3], x1[3], y0[3], y1[3];
-          split_bf16(__uint_as_float(w0.x), __uint_as_float(w0.y), x0);
-          split_bf16(__uint_as_float(w0.z), __uint_as_float(w0.w), x1);
-          split_bf16(__uint_as_float(w1.x), __uint_as_float(w1.y), y0);
-          split_bf16(__uint_as_float(w1.z), __uint_as_float(w1.w), y1);
-#pragma unroll
-          for (int part = 0; part < 3; part++) {
-            const uint32_t av[4] = {x0[part], y0[part], x1[part], y1[part]};
-#pragma unroll
-            for (int n = 0; n < (part == 2 ? 1 : NT); n++)  // lo lo is below f32's last bit
-              mma16<F16>(acc[n][part & 1], av, qb[n][ks].x, qb[n][ks].y);
-          }
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < RL; n++) {
-        s[n][0] = fadd(fadd(acc[n][0][0], acc[n][1][0]), fadd(acc[n][0][1], acc[n][1][1]));
-        s[n][1] = fadd(fadd(acc[n][0][2], acc[n][1][2]), fadd(acc[n][0][3], acc[n][1][3]));
-        if (!F16) {
-          s[n][0] = fadd(s[n][0], fadd(acc[1][0][0], acc[1][1][0]));
-          s[n][1] = fadd(s[n][1], fadd(acc[1][0][2], acc[1][1][2]));
-        }
-      }
-    }
-    const int key0 = key_of(grp);
-    {  // masks, only where the group is not wholly visible to every row
-      const bool sink = grp < sink_groups;
-      if (sink ? key0 + KR_GROUP > sk : key0 < max_lo || key0 + KR_GROUP > min_hi) {
-#pragma unroll
-        for (int n = 0; n < RL; n++)
-#pragma unroll
-          for (int i = 0; i < 2; i++) {
-            const int key = key0 + g + 8 * i;
-            // every row sees the tile's sinks; a row's own may reach into the main range
-            const bool seen = sink ? key < sk
-                                   : key >= lo && key < row_hi[n] && (key >= row_lo[n] || key < row_sk[n]);
-            if (!seen) s[n][i] = -INFINITY;
-          }
-      }
-    }
-    // ------------------------------------------------------------ softmax
-    // 4-bit: the value scales of the lane's two keys, a block's pair a word
-    uint32_t vd[4];
-    uint32_t dmax = 0;
-    bool grow = false;
-    if constexpr (Q4) {
-      const uint2 e0 = ld_u2(stage + L::S_OFF + 128 + 8 * g), e1 = ld_u2(stage + L::S_OFF + 192 + 8 * g);
-      vd[0] = __byte_perm(e0.x, e1.x, 0x5410);
-      vd[1] = __byte_perm(e0.x, e1.x, 0x7632);
-      vd[2] = __byte_perm(e0.y, e1.y, 0x5410);
-      vd[3] = __byte_perm(e0.y, e1.y, 0x7632);
-      const __half2 h = __hmax2(__hmax2(__habs2(as_h2(e0.x)), __habs2(as_h2(e0.y))),
-                                __hmax2(__habs2(as_h2(e1.x)), __habs2(as_h2(e1.y))));
-      grow = __hgt2_mask(h, as_h2(dlim)) != 0;
-      dmax = __half_as_ushort(__hmax(__low2half(h), __high2half(h)));
-    }
-    float top[RL];
+        for (int e = 0; e < 4; e++) o[u][n][e] = 0.0f;
 #pragma unroll
     for (int n = 0; n < RL; n++) {
-      top[n] = fmaxf(s[n][0], s[n][1]);
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1) top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], d));
-      top[n] = fmul(top[n], unscale[n]);
-      grow = grow || top[n] > fadd(m[n], 8.0f);
+      m[n] = -INFINITY;
+      l[n] = base[n] = 0.0f;
     }
-    if (__any_sync(0xffffffffu, grow)) {
-      float fd = 1.0f;
-      if (Q4) {
-        dmax = __reduce_max_sync(0xffffffffu, dmax);  // magnitudes order as their bits do
-        const int ne = max(dexp, min((int)(dmax >> 10) - 14, 16));  // below 2^(exponent - 14)
-        fd = __uint_as_float((uint32_t)(127 + dexp - ne) << 23);
-        dexp = ne;
-        dlim = ne > 15 ? 0x7BFF7BFFu : (uint32_t)(ne + 15) * 0x04000400u;
-        dnorm = ne < 15 ? (uint32_t)(15 - ne) * 0x04000400u : ne == 15 ? 0x02000200u : 0x01000100u;
-      }
+    dexp = WIDE ? 0 : -14;
+    uint32_t dlim = 0x04000400u, dnorm = 0x74007400u;  // f16 pairs 2^dexp and 2^-dexp
+    uint32_t dlow = 0, dmin = 0xFFFFFFFFu;  // u16 pairs: 2^(dexp - KR_SPREAD); smallest scale but 0, less 1
+
+    int st = 0;
+    for (int grp = g0 + warp; grp < g1; grp += L::WARPS) {
+      cp_async_wait<L::STAGES - 2>();
+      __syncwarp();  // the stage has landed for every lane, and every lane is done with the last one
+      fetch(grp + (L::STAGES - 1) * L::WARPS, st == 0 ? L::STAGES - 1 : st - 1);
+      const uint8_t* stage = kr_smem + (warp * L::STAGES + st) * L::STAGE;
+      // ------------------------------------------------------------- scores
+      float s[RL][2];  // keys g, g + 8
+      const uint8_t* ka = stage + g * L::K_STRIDE + 16 * c;
+      if constexpr (Q4) {
+        const uint4 w0 = ld_u4(ka), w1 = ld_u4(ka + 8 * L::K_STRIDE);
+        const uint2 e0 = ld_u2(stage + L::S_OFF + 8 * g), e1 = ld_u2(stage + L::S_OFF + 8 * g + 64);
 #pragma unroll
-      for (int n = 0; n < RL; n++) {
-        const float mn = fmaxf(m[n], top[n]);
-        const float nb = mn == -INFINITY ? 0.0f : fsub(mn, HEADROOM);
-        const float f = m[n] == -INFINITY ? 0.0f : exp2_approx(fsub(base[n], nb));
-        l[n] = fmul(l[n], f);
+        for (int n = 0; n < RL; n++) s[n][0] = s[n][1] = 0.0f;
 #pragma unroll
-        for (int u = 0; u < 8; u++)
+        for (int b = 0; b < 4; b++) {
+          uint32_t x[4], y[4];
+          nib_f16(word_of(w0, b), x);
+          nib_f16(word_of(w1, b), y);
+          const float2 d0 = h2f2(b < 2 ? e0.x : e0.y), d1 = h2f2(b < 2 ? e1.x : e1.y);
 #pragma unroll
-          for (int k = F16 ? n : 0; k < (F16 ? n + 1 : NT); k++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[u][k][e] = fmul(o[u][k][e], fmul(f, fd));
-        m[n] = mn;
-        base[n] = nb;
-      }
-    }
-    float w[RL][2];
-#pragma unroll
-    for (int n = 0; n < RL; n++)
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        w[n][i] = exp2_approx(ffma(s[n][i], unscale[n], -base[n]));
-        l[n] = fadd(l[n], w[n][i]);
-      }
-    // ------------------------------------------------------------- values
-    // lane column c: keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
-    const uint8_t* va = stage + L::V_OFF + c * L::V_PAIR;
-    if constexpr (Q4) {
-      uint32_t wh[NT], wl[NT];
-#pragma unroll
-      for (int n = 0; n < NT; n++) split_f16(w[n][0], w[n][1], wh[n], wl[n]);
-      const uint2 v0 = ld_u2(va + 8 * g), v1 = ld_u2(va + L::ROW + 8 * g);
-      const uint2 v2 = ld_u2(va + 4 * L::V_PAIR + 8 * g), v3 = ld_u2(va + 4 * L::V_PAIR + L::ROW + 8 * g);
-#pragma unroll
-      for (int b = 0; b < 4; b++) {
-        // block b's two bytes of four keys, keys paired
-        const uint32_t sel = b & 1 ? 0x7632u : 0x5410u;
-        uint32_t x[4], y[4];
-        nib_f16(__byte_perm(b < 2 ? v0.x : v0.y, b < 2 ? v1.x : v1.y, sel), x);
-        nib_f16(__byte_perm(b < 2 ? v2.x : v2.y, b < 2 ? v3.x : v3.y, sel), y);
-        const uint32_t d = hmul2_u(vd[b], dnorm);
-        const uint32_t a0[4] = {x[0], x[1], y[0], y[1]}, a1[4] = {x[2], x[3], y[2], y[3]};
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-          // (hi + lo) d: the product's f16, then what its rounding left plus lo d
-          const uint32_t ph = hmul2_u(wh[n], d);
-          const uint32_t pl = hfma2_u(wl[n], d, hfma2_u(wh[n], d, hneg2_u(ph)));
-          const uint32_t b0 = movm(__byte_perm(ph, pl, 0x5410)), b1 = movm(__byte_perm(ph, pl, 0x7632));
-          mma16<F16>(o[2 * b][n], a0, b0, b1);
-          mma16<F16>(o[2 * b + 1][n], a1, b0, b1);
-        }
-      }
-    } else {
-      uint32_t pb[NT][2];
-      if constexpr (F16) {
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-          uint32_t ph, pl;
-          split_f16(w[n][0], w[n][1], ph, pl);
-          pb[n][0] = movm(__byte_perm(ph, pl, 0x5410));
-          pb[n][1] = movm(__byte_perm(ph, pl, 0x7632));
+          for (int n = 0; n < NT; n++) {
+            float acc[4];
+            const uint32_t a0[4] = {x[0], y[0], x[2], y[2]}, a1[4] = {x[1], y[1], x[3], y[3]};
+            mma16<F16>(acc, a0, qb[n][2 * b].x, qb[n][2 * b].y, 0.f, 0.f, 0.f, 0.f);
+            mma16<F16>(acc, a1, qb[n][2 * b + 1].x, qb[n][2 * b + 1].y);
+            s[n][0] = ffma(b & 1 ? d0.y : d0.x, fadd(acc[0], acc[1]), s[n][0]);
+            s[n][1] = ffma(b & 1 ? d1.y : d1.x, fadd(acc[2], acc[3]), s[n][1]);
+          }
         }
       } else {
-        uint32_t part[3];
-        split_bf16(w[0][0], w[0][1], part);
-        pb[0][0] = movm(__byte_perm(part[0], part[1], 0x5410));
-        pb[0][1] = movm(__byte_perm(part[0], part[1], 0x7632));
-        pb[1][0] = movm(part[2] & 0x0000FFFFu);
-        pb[1][1] = movm(part[2] >> 16);
-      }
-      constexpr int K8 = 4 * L::V_PAIR;  // eight keys on
-      if constexpr (KV == FLOCK_KV_FP8) {
-        const uint4 v0 = ld_u4(va + 16 * g), v1 = ld_u4(va + L::ROW + 16 * g);
-        const uint4 v2 = ld_u4(va + K8 + 16 * g), v3 = ld_u4(va + K8 + L::ROW + 16 * g);
+        float acc[NT][2][4];
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
-          const int sh = 16 * (u & 1);
-          const uint32_t y0 = fp8_f16(word_of(v0, u >> 1) >> sh), y1 = fp8_f16(word_of(v1, u >> 1) >> sh),
-                         y2 = fp8_f16(word_of(v2, u >> 1) >> sh), y3 = fp8_f16(word_of(v3, u >> 1) >> sh);
-          const uint32_t av[4] = {__byte_perm(y0, y1, 0x5410), __byte_perm(y0, y1, 0x7632),
-                                  __byte_perm(y2, y3, 0x5410), __byte_perm(y2, y3, 0x7632)};
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int n = 0; n < NT; n++) mma16<F16>(o[u][n], av, pb[n][0], pb[n][1]);
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[n][h][e] = 0.0f;
+        if constexpr (KV == FLOCK_KV_FP8) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const uint4 w0 = ld_u4(ka + 64 * h), w1 = ld_u4(ka + 64 * h + 8 * L::K_STRIDE);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const uint32_t x = word_of(w0, i), y = word_of(w1, i);
+              const uint32_t av[4] = {fp8_f16(x), fp8_f16(y), fp8_f16(x >> 16), fp8_f16(y >> 16)};
+#pragma unroll
+              for (int n = 0; n < NT; n++)
+                mma16<F16>(acc[n][i & 1], av, qb[n][4 * h + i].x, qb[n][4 * h + i].y);
+            }
+          }
+        } else if constexpr (KV == FLOCK_KV_BF16) {
+#pragma unroll
+          for (int h = 0; h < 4; h++) {
+            const uint4 w0 = ld_u4(ka + 64 * h), w1 = ld_u4(ka + 64 * h + 8 * L::K_STRIDE);
+            const uint32_t a0[4] = {w0.x, w1.x, w0.y, w1.y}, a1[4] = {w0.z, w1.z, w0.w, w1.w};
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+              mma16<F16>(acc[n][0], a0, qb[n][2 * h].x, qb[n][2 * h].y);
+              mma16<F16>(acc[n][1], a1, qb[n][2 * h + 1].x, qb[n][2 * h + 1].y);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < 8; ks++) {
+            const uint4 w0 = ld_u4(ka + 64 * ks), w1 = ld_u4(ka + 64 * ks + 8 * L::K_STRIDE);
+            uint32_t x0[3], x1[3], y0[3], y1[3];
+            split_bf16(__uint_as_float(w0.x), __uint_as_float(w0.y), x0);
+            split_bf16(__uint_as_float(w0.z), __uint_as_float(w0.w), x1);
+            split_bf16(__uint_as_float(w1.x), __uint_as_float(w1.y), y0);
+            split_bf16(__uint_as_float(w1.z), __uint_as_float(w1.w), y1);
+#pragma unroll
+            for (int part = 0; part < 3; part++) {
+              const uint32_t av[4] = {x0[part], y0[part], x1[part], y1[part]};
+#pragma unroll
+              for (int n = 0; n < (part == 2 ? 1 : NT); n++)  // lo lo is below f32's last bit
+                mma16<F16>(acc[n][part & 1], av, qb[n][ks].x, qb[n][ks].y);
+            }
+          }
         }
-      } else if constexpr (KV == FLOCK_KV_BF16) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const uint8_t* vh = va + 128 * h + 16 * g;
-          const uint4 v0 = ld_u4(vh), v1 = ld_u4(vh + L::ROW), v2 = ld_u4(vh + K8),
-                      v3 = ld_u4(vh + K8 + L::ROW);
+        for (int n = 0; n < RL; n++) {
+          s[n][0] = fadd(fadd(acc[n][0][0], acc[n][1][0]), fadd(acc[n][0][1], acc[n][1][1]));
+          s[n][1] = fadd(fadd(acc[n][0][2], acc[n][1][2]), fadd(acc[n][0][3], acc[n][1][3]));
+          if (!F16) {
+            s[n][0] = fadd(s[n][0], fadd(acc[1][0][0], acc[1][1][0]));
+            s[n][1] = fadd(s[n][1], fadd(acc[1][0][2], acc[1][1][2]));
+          }
+        }
+      }
+      const int key0 = key_of(grp);
+      {  // masks, only where the group is not wholly visible to every row
+        const bool sink = grp < sink_groups;
+        if (sink ? key0 + KR_GROUP > sk : key0 < max_lo || key0 + KR_GROUP > min_hi) {
 #pragma unroll
-          for (int q = 0; q < 4; q++) {
-            const uint32_t y0 = word_of(v0, q), y1 = word_of(v1, q), y2 = word_of(v2, q), y3 = word_of(v3, q);
+          for (int n = 0; n < RL; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const int key = key0 + g + 8 * i;
+              // every row sees the tile's sinks; a row's own may reach into the main range
+              const bool seen = sink ? key < sk
+                                     : key >= lo && key < row_hi[n] && (key >= row_lo[n] || key < row_sk[n]);
+              if (!seen) s[n][i] = -INFINITY;
+            }
+        }
+      }
+      // ------------------------------------------------------------ softmax
+      // 4-bit: the value scales of the lane's two keys, a block's pair a word
+      uint32_t vd[4];
+      uint32_t dmax = 0;
+      bool grow = false;
+      if constexpr (Q4) {
+        const uint2 e0 = ld_u2(stage + L::S_OFF + 128 + 8 * g), e1 = ld_u2(stage + L::S_OFF + 192 + 8 * g);
+        vd[0] = __byte_perm(e0.x, e1.x, 0x5410);
+        vd[1] = __byte_perm(e0.x, e1.x, 0x7632);
+        vd[2] = __byte_perm(e0.y, e1.y, 0x5410);
+        vd[3] = __byte_perm(e0.y, e1.y, 0x7632);
+        if (!WIDE) {
+          // magnitudes order as their bits do
+          const uint32_t m0 = e0.x & 0x7FFF7FFFu, m1 = e0.y & 0x7FFF7FFFu, m2 = e1.x & 0x7FFF7FFFu,
+                         m3 = e1.y & 0x7FFF7FFFu;
+          const uint32_t h = __vimax3_u16x2(__vmaxu2(m0, m1), m2, m3);
+          dmin = __viaddmin_u16x2(m3, 0xFFFFFFFFu,
+                 __viaddmin_u16x2(m2, 0xFFFFFFFFu,
+                 __viaddmin_u16x2(m1, 0xFFFFFFFFu, __viaddmin_u16x2(m0, 0xFFFFFFFFu, dmin))));
+          grow = (__hgt2_mask(as_h2(h), as_h2(dlim)) | __hlt2_mask(as_h2(dmin), as_h2(dlow))) != 0;
+          dmax = max(h & 0xFFFFu, h >> 16);
+        }
+      }
+      float top[RL];
+#pragma unroll
+      for (int n = 0; n < RL; n++) {
+        top[n] = fmaxf(s[n][0], s[n][1]);
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) top[n] = fmaxf(top[n], __shfl_xor_sync(0xffffffffu, top[n], d));
+        top[n] = fmul(top[n], unscale[n]);
+        grow = grow || top[n] > fadd(m[n], LAG);
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+        float fd = 1.0f;
+        if (Q4 && !WIDE) {
+          dmax = __reduce_max_sync(0xffffffffu, dmax);
+          const int ne = max(dexp, min((int)(dmax >> 10) - 14, 16));  // below 2^(exponent - 14)
+          fd = __uint_as_float((uint32_t)(127 + dexp - ne) << 23);
+          dexp = ne;
+          dlim = ne > 15 ? 0x7BFF7BFFu : (uint32_t)(ne + 15) * 0x04000400u;
+          dnorm = ne < 15 ? (uint32_t)(15 - ne) * 0x04000400u : ne == 15 ? 0x02000200u : 0x01000100u;
+          // 2^(ne - KR_SPREAD) as f16 bits, below 2^-14 a subnormal, below 2^-24 nothing
+          const int le = ne - KR_SPREAD;
+          const uint32_t low = le >= -14 ? (uint32_t)(le + 15) << 10 : le >= -24 ? 1u << (le + 24) : 0u;
+          dlow = low * 0x00010001u;
+          if (__reduce_min_sync(0xffffffffu, min(dmin & 0xFFFFu, dmin >> 16)) + 1 < low) return false;
+        }
+#pragma unroll
+        for (int n = 0; n < RL; n++) {
+          const float mn = fmaxf(m[n], top[n]);
+          const float nb = mn == -INFINITY ? 0.0f : fsub(mn, HEADROOM);
+          const float f = m[n] == -INFINITY ? 0.0f : exp2_approx(fsub(base[n], nb));
+          l[n] = fmul(l[n], f);
+#pragma unroll
+          for (int u = 0; u < 8; u++)
+#pragma unroll
+            for (int k = F16 ? n : 0; k < (F16 ? n + 1 : NT); k++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) o[u][k][e] = fmul(o[u][k][e], fmul(f, fd));
+          m[n] = mn;
+          base[n] = nb;
+        }
+      }
+      float w[RL][2];
+#pragma unroll
+      for (int n = 0; n < RL; n++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          w[n][i] = exp2_approx(ffma(s[n][i], unscale[n], -base[n]));
+          l[n] = fadd(l[n], w[n][i]);
+        }
+      // ------------------------------------------------------------- values
+      // lane column c: keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
+      const uint8_t* va = stage + L::V_OFF + c * L::V_PAIR;
+      if constexpr (Q4) {
+        uint32_t wh[NT], wl[NT];
+#pragma unroll
+        for (int n = 0; !WIDE && n < NT; n++) split_f16(w[n][0], w[n][1], wh[n], wl[n]);
+        const uint2 v0 = ld_u2(va + 8 * g), v1 = ld_u2(va + L::ROW + 8 * g);
+        const uint2 v2 = ld_u2(va + 4 * L::V_PAIR + 8 * g), v3 = ld_u2(va + 4 * L::V_PAIR + L::ROW + 8 * g);
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+          // block b's two bytes of four keys, keys paired
+          const uint32_t sel = b & 1 ? 0x7632u : 0x5410u;
+          uint32_t x[4], y[4];
+          nib_f16(__byte_perm(b < 2 ? v0.x : v0.y, b < 2 ? v1.x : v1.y, sel), x);
+          nib_f16(__byte_perm(b < 2 ? v2.x : v2.y, b < 2 ? v3.x : v3.y, sel), y);
+          if (WIDE) {  // codes in bf16, weight times scale in f32 and as three bf16 parts
+            uint32_t av[2][4];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              const float2 v = h2f2(i & 2 ? y[(i & 1) + 2 * (i >> 2)] : x[(i & 1) + 2 * (i >> 2)]);
+              av[i >> 2][i & 3] = bf2(v.x, v.y);
+            }
+            const float2 d = h2f2(vd[b]);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+              uint32_t part[3];
+              split_bf16(fmul(w[n][0], d.x), fmul(w[n][1], d.y), part);
+              const uint32_t b0 = movm(__byte_perm(part[0], part[1], 0x5410)),
+                             b1 = movm(__byte_perm(part[0], part[1], 0x7632)),
+                             b2 = movm(part[2] & 0x0000FFFFu), b3 = movm(part[2] >> 16);
+#pragma unroll
+              for (int i = 0; i < 2; i++) {
+                mma16<false>(o[2 * b + i][n], av[i], b2, b3);
+                mma16<false>(o[2 * b + i][n], av[i], b0, b1);
+              }
+            }
+            continue;
+          }
+          const uint32_t d = hmul2_u(vd[b], dnorm);
+          const uint32_t a0[4] = {x[0], x[1], y[0], y[1]}, a1[4] = {x[2], x[3], y[2], y[3]};
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+            // (hi + lo) d: the product's f16, then what its rounding left plus lo d
+            const uint32_t ph = hmul2_u(wh[n], d);
+            const uint32_t pl = hfma2_u(wl[n], d, hfma2_u(wh[n], d, hneg2_u(ph)));
+            const uint32_t b0 = movm(__byte_perm(ph, pl, 0x5410)), b1 = movm(__byte_perm(ph, pl, 0x7632));
+            mma16<F16>(o[2 * b][n], a0, b0, b1);
+            mma16<F16>(o[2 * b + 1][n], a1, b0, b1);
+          }
+        }
+      } else {
+        uint32_t pb[NT][2];
+        if constexpr (F16) {
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+            uint32_t ph, pl;
+            split_f16(w[n][0], w[n][1], ph, pl);
+            pb[n][0] = movm(__byte_perm(ph, pl, 0x5410));
+            pb[n][1] = movm(__byte_perm(ph, pl, 0x7632));
+          }
+        } else {
+          uint32_t part[3];
+          split_bf16(w[0][0], w[0][1], part);
+          pb[0][0] = movm(__byte_perm(part[0], part[1], 0x5410));
+          pb[0][1] = movm(__byte_perm(part[0], part[1], 0x7632));
+          pb[1][0] = movm(part[2] & 0x0000FFFFu);
+          pb[1][1] = movm(part[2] >> 16);
+        }
+        constexpr int K8 = 4 * L::V_PAIR;  // eight keys on
+        if constexpr (KV == FLOCK_KV_FP8) {
+          const uint4 v0 = ld_u4(va + 16 * g), v1 = ld_u4(va + L::ROW + 16 * g);
+          const uint4 v2 = ld_u4(va + K8 + 16 * g), v3 = ld_u4(va + K8 + L::ROW + 16 * g);
+#pragma unroll
+          for (int u = 0; u < 8; u++) {
+            const int sh = 16 * (u & 1);
+            const uint32_t y0 = fp8_f16(word_of(v0, u >> 1) >> sh), y1 = fp8_f16(word_of(v1, u >> 1) >> sh),
+                           y2 = fp8_f16(word_of(v2, u >> 1) >> sh), y3 = fp8_f16(word_of(v3, u >> 1) >> sh);
             const uint32_t av[4] = {__byte_perm(y0, y1, 0x5410), __byte_perm(y0, y1, 0x7632),
                                     __byte_perm(y2, y3, 0x5410), __byte_perm(y2, y3, 0x7632)};
 #pragma unroll
-            for (int n = 0; n < NT; n++) mma16<F16>(o[4 * h + q][n], av, pb[n][0], pb[n][1]);
+            for (int n = 0; n < NT; n++) mma16<F16>(o[u][n], av, pb[n][0], pb[n][1]);
           }
-        }
-      } else {
+        } else if constexpr (KV == FLOCK_KV_BF16) {
 #pragma unroll
-        for (int h = 0; h < 4; h++) {
-          const uint8_t* vh = va + 128 * h + 16 * g;
-          const uint4 v0 = ld_u4(vh), v1 = ld_u4(vh + L::ROW), v2 = ld_u4(vh + K8),
-                      v3 = ld_u4(vh + K8 + L::ROW);
+          for (int h = 0; h < 2; h++) {
+            const uint8_t* vh = va + 128 * h + 16 * g;
+            const uint4 v0 = ld_u4(vh), v1 = ld_u4(vh + L::ROW), v2 = ld_u4(vh + K8),
+                        v3 = ld_u4(vh + K8 + L::ROW);
 #pragma unroll
-          for (int q = 0; q < 2; q++) {
-            auto f = [&](const uint4& v, int i) { return __uint_as_float(word_of(v, 2 * q + i)); };
-            uint32_t x0[3], x1[3], y0[3], y1[3];
-            split_bf16(f(v0, 0), f(v1, 0), x0);
-            split_bf16(f(v0, 1), f(v1, 1), x1);
-            split_bf16(f(v2, 0), f(v3, 0), y0);
-            split_bf16(f(v2, 1), f(v3, 1), y1);
+            for (int q = 0; q < 4; q++) {
+              const uint32_t y0 = word_of(v0, q), y1 = word_of(v1, q), y2 = word_of(v2, q), y3 = word_of(v3, q);
+              const uint32_t av[4] = {__byte_perm(y0, y1, 0x5410), __byte_perm(y0, y1, 0x7632),
+                                      __byte_perm(y2, y3, 0x5410), __byte_perm(y2, y3, 0x7632)};
 #pragma unroll
-            for (int part = 0; part < 3; part++) {
-              const uint32_t av[4] = {x0[part], x1[part], y0[part], y1[part]};
+              for (int n = 0; n < NT; n++) mma16<F16>(o[4 * h + q][n], av, pb[n][0], pb[n][1]);
+            }
+          }
+        } else {
 #pragma unroll
-              for (int n = 0; n < (part == 2 ? 1 : NT); n++)
-                mma16<F16>(o[2 * h + q][n], av, pb[n][0], pb[n][1]);
+          for (int h = 0; h < 4; h++) {
+            const uint8_t* vh = va + 128 * h + 16 * g;
+            const uint4 v0 = ld_u4(vh), v1 = ld_u4(vh + L::ROW), v2 = ld_u4(vh + K8),
+                        v3 = ld_u4(vh + K8 + L::ROW);
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+              auto f = [&](const uint4& v, int i) { return __uint_as_float(word_of(v, 2 * q + i)); };
+              uint32_t x0[3], x1[3], y0[3], y1[3];
+              split_bf16(f(v0, 0), f(v1, 0), x0);
+              split_bf16(f(v0, 1), f(v1, 1), x1);
+              split_bf16(f(v2, 0), f(v3, 0), y0);
+              split_bf16(f(v2, 1), f(v3, 1), y1);
+#pragma unroll
+              for (int part = 0; part < 3; part++) {
+                const uint32_t av[4] = {x0[part], x1[part], y0[part], y1[part]};
+#pragma unroll
+                for (int n = 0; n < (part == 2 ? 1 : NT); n++)
+                  mma16<F16>(o[2 * h + q][n], av, pb[n][0], pb[n][1]);
+              }
             }
           }
         }
       }
+      st = st + 1 == L::STAGES ? 0 : st + 1;
     }
-    st = st + 1 == L::STAGES ? 0 : st + 1;
+    return true;
+  };
+  if (!pass(std::false_type())) {
+    if constexpr (Q4) {
+      cp_async_wait<0>();
+      __syncwarp();  // the ring is this warp's alone
+#pragma unroll
+      for (int s = 0; s < L::STAGES - 1; s++) fetch(g0 + warp + s * L::WARPS, s);
+      pass(std::true_type());
+    }
   }
   cp_async_wait<0>();
 
