@@ -351,7 +351,8 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       float s[64];
 #pragma unroll
       for (int i = 0; i < 2; i++) kp_ld32(S + 64 * half + 32 * i, s + 32 * i);
-      const float f = SCALED ? fmul(unscale, s_kscale[t & 3]) : unscale;
+      // not 0, which times a masked score is NaN; below 2^-126 a score is 0 anyway
+      const float f = SCALED ? fmaxf(fmul(unscale, s_kscale[t & 3]), 0x1p-126f) : unscale;
       const int ve = SCALED ? s_vexp[t & 3] : 0;
       const int key0 = key_of(t);
       const bool sink = t0 + t < sink_tiles;

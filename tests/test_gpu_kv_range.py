@@ -120,3 +120,17 @@ def test_many_scales_in_four_bits(torch, dev, nq, window, sinks):  # noqa: F811
     k, v, q = rows(10, N, NKV, 0.3), rows(11, N, NKV), few(12, nq)
     v *= 2.0 ** np.random.default_rng(13).integers(-18, 18, (N, NKV, 1)).astype(np.float32)
     check(torch, dev, "q4", q, k, v, N - nq, window, sinks)
+
+
+# ------------------------------------------------------- many rows (k_kv_prompt)
+# 40 and 300 queries of two heads a kv head: one tile of 128 rows, and five (in pairs)
+MANY = (40, 300)
+WIDE = ("f32", "bf16")
+
+
+@pytest.mark.parametrize("dtype", WIDE + ("fp8", "q4"))
+@pytest.mark.parametrize("scale", [0.0, 1e-30, 1e-7, 1.0])
+@pytest.mark.parametrize("nq", (1, 8) + MANY)
+def test_keys_of_zero_see_the_mean(torch, dev, nq, scale, dtype):  # noqa: F811
+    k, v, q = np.zeros((N, NKV, HD), np.float32), rows(38, N, NKV), rows(39, nq, HEADS, scale)
+    check(torch, dev, dtype, q, k, v, N - nq, window=90, sinks=3)
