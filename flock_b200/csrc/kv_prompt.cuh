@@ -45,8 +45,22 @@
 // first, and the outputs move to an f32 sum in shared memory every KP_FLUSH
 // tiles, added there in f32 (96 steps: 1e-6; 16 us of the 187).
 //
-// The running maximum may lag by 2^8 before the outputs are rescaled (as in
-// k_kv_rows).  Every wait is bounded; a wait that runs out ends the CTA, which
+// The running maximum may lag by 2^4 before the outputs are rescaled (as in
+// k_kv_rows).
+//
+// f16 parts hold a number to 2^-22 of itself down to 2^-15 of its tile's largest,
+// below that to 2^-38 of the largest.  That is enough while the largest is no
+// outlier.  Where it is, a CTA's rows are worked out again in f32, a warp a row
+// (kp_exact_rows), after a look at bounds that cost next to nothing:
+//   scores  a row's largest |q| times a tile's largest |k| bounds what the lost
+//           bits of q and k can move a score by;
+//   values  the tiles' largest (4-bit: all scales) further apart than 2^KR_SPREAD,
+//           or more than a few of a tile's elements below 2^-15 of its largest (a
+//           key or a column of such is more; of 4096 normal ones about one).
+// Large keys or values may belong to keys that a row does not see, to others'
+// dimensions, or be infinite or NaN: the f32 rows are free of them.
+//
+// Every wait is bounded; a wait that runs out ends the CTA, which
 // then writes NaN (and so does its partner) and sets a layer's error word.
 #pragma once
 #include "gemm_tc.cuh"
@@ -60,6 +74,15 @@ constexpr int KP_THREADS = 512;
 constexpr int KP_FLUSH = 4;      // key tiles an output accumulator takes
 constexpr int KP_SUM_STRIDE = 132;  // floats of a row of the outputs' sum: rows 4 banks apart
 constexpr int KP_OPND = 128 * 128 * 2;  // bytes of one 128 x 128 f16 operand
+
+// Bounds of that look.  Scores: q's and k's f16 parts are off by 2^-25 each at
+// most (q up to 2^14, k to 2^13), 128 terms by 2^-3.4, typically 2^-8, in units f: f up
+// to 2^-12 moves a score by 2^-15.4, typically 2^-20.  e4m3 keys are exact, up to 448:
+// 2^-9.2 of q's unit, typically 2^-13.
+constexpr float KP_MAX_UNIT = 0x1p-12f, KP_MAX_UNIT_FP8 = 0x1p-6f;
+// Values: elements of a warp's 32 keys below 2^-15 of the tile's largest (2^-2 as scaled).
+constexpr float KP_SMALL = 0.25f;
+constexpr int KP_FEW = 24;
 
 struct KvPromptArgs {
   KvAttnArgs a;
@@ -202,6 +225,109 @@ template <int KV>
 constexpr size_t KP_SMEM =
     (KP_LO<KV> ? 4 : 2) * (size_t)KP_OPND + 128 * KP_SUM_STRIDE * 4 + 1024;
 
+// Sixteen rows of a tile from the keys of tiles [t0, t1) in f32, by one warp, four
+// rows and four keys at a time: outputs (normalised where nothing is joined later)
+// into the rows' part of s_sum, (base, l) into part_ml.  A key that a row does not
+// see is not part of its arithmetic, whatever it holds.  The sixteen scores are
+// added up over the lanes together, each step halving the values a lane holds:
+// lane 2 (4 i + j) has row i's with key j.  Rare, and slow: 1024 queries at 3000
+// keys, 16 / 8 heads, 4 to 6 ms where the tensor cores take 0.1 to 0.25.
+template <int KV>
+FLOCK_DEV void kp_exact_rows(const KvPromptArgs& p, int tile, int head, int pos, int lo, int hi,
+                             int sk, int t0, int t1, float* s_sum, float* part_ml) {
+  const KvAttnArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sink_tiles = (sk + KP_KEYS - 1) / KP_KEYS, lo16 = lo & ~15;
+  const float scale = __double2float_rn(1.4426950408889634 / sqrt(128.0));
+#pragma unroll 1
+  for (int i0 = 0; i0 < 16; i0 += 4) {
+    const int row0 = tile * KP_ROWS + 16 * warp + i0;
+    if (row0 >= p.rows) return;
+    float4 q[4], o[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int r = min(row0 + i, p.rows - 1);
+      const float4 x = __ldg(reinterpret_cast<const float4*>(
+                                 a.q + (r / p.group) * a.q_stride +
+                                 ((int64_t)head * p.group + r % p.group) * KV_HD) + lane);
+      q[i] = make_float4(fmul(x.x, scale), fmul(x.y, scale), fmul(x.z, scale), fmul(x.w, scale));
+      o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    // the lane's row (and its key of four): bounds, running maximum and sum
+    const int row_hi = pos + min(row0 + (lane >> 3), p.rows - 1) / p.group + 1;
+    const int row_lo = a.window && row_hi > a.window ? row_hi - a.window : 0;
+    const int row_sk = min(a.sinks, row_lo);
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll 1
+    for (int t = t0; t < t1; t++) {
+      const bool sink = t < sink_tiles;
+      const int key0 = sink ? t * KP_KEYS : lo16 + (t - sink_tiles) * KP_KEYS;
+      const int from = max(key0, sink ? 0 : lo), to = min(key0 + KP_KEYS, sink ? sk : hi);
+#pragma unroll 1
+      for (int key = from; key < to; key += 4) {
+        float4 k[4], v[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          k[j] = v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (key + j < to) {
+            k[j] = kv_load4<KV, true>(a.c, key + j, head, lane);
+            v[j] = kv_load4<KV, false>(a.c, key + j, head, lane);
+          }
+        }
+        float s[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float4 x = q[i >> 2], y = k[i & 3];
+          s[i] = ffma(x.x, y.x, ffma(x.y, y.y, ffma(x.z, y.z, fmul(x.w, y.w))));
+        }
+#pragma unroll
+        for (int h = 8; h > 0; h >>= 1) {  // lanes 2 h apart trade halves
+          const bool up = lane & (2 * h);
+#pragma unroll
+          for (int i = 0; i < h; i++) {
+            const float give = up ? s[i] : s[i + h], own = up ? s[i + h] : s[i];
+            s[i] = fadd(own, __shfl_xor_sync(0xffffffffu, give, 2 * h));
+          }
+        }
+        float x = fadd(s[0], __shfl_xor_sync(0xffffffffu, s[0], 1));
+        const int own = key + ((lane >> 1) & 3);
+        if (own >= to || own >= row_hi || (own < row_lo && own >= row_sk)) x = -INFINITY;
+        float top = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+        top = fmaxf(m, fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4)));
+        const float f = m == -INFINITY ? 0.0f : exp2_approx(fsub(m, top));
+        const float w = x == -INFINITY ? 0.0f : exp2_approx(fsub(x, top));
+        float sum = fadd(w, __shfl_xor_sync(0xffffffffu, w, 2));
+        sum = fadd(sum, __shfl_xor_sync(0xffffffffu, sum, 4));
+        l = ffma(l, f, sum);
+        m = top;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float g = __shfl_sync(0xffffffffu, f, 8 * i);
+          o[i] = make_float4(fmul(o[i].x, g), fmul(o[i].y, g), fmul(o[i].z, g), fmul(o[i].w, g));
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float e = __shfl_sync(0xffffffffu, w, 8 * i + 2 * j);
+            if (e != 0.0f)
+              o[i] = make_float4(ffma(e, v[j].x, o[i].x), ffma(e, v[j].y, o[i].y),
+                                 ffma(e, v[j].z, o[i].z), ffma(e, v[j].w, o[i].w));
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float row_l = __shfl_sync(0xffffffffu, l, 8 * i);
+      const float inv = p.splits == 1 ? fdiv(1.0f, row_l) : 1.0f;
+      reinterpret_cast<float4*>(s_sum)[(16 * warp + i0 + i) * (KP_SUM_STRIDE / 4) + lane] =
+          make_float4(fmul(o[i].x, inv), fmul(o[i].y, inv), fmul(o[i].z, inv), fmul(o[i].w, inv));
+    }
+    if (p.splits > 1 && (lane & 7) == 0 && row0 + (lane >> 3) < p.rows) {
+      part_ml[(16 * warp + i0 + (lane >> 3)) * 2] = m;
+      part_ml[(16 * warp + i0 + (lane >> 3)) * 2 + 1] = l;
+    }
+  }
+}
+
 template <int KV, bool PAIR>
 static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvPromptArgs p) {
   // operand rows here (keys of K, output columns of V), stages of them, their bytes
@@ -213,8 +339,10 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
   __shared__ uint64_t s_bar[14];
   __shared__ uint32_t s_tmem;
   __shared__ int s_err, s_ok[2];
+  __shared__ int s_far[2];  // f16 parts do not do: found by the softmax warps, by the converters
   __shared__ float s_top[2][2][128];  // a row's maximum over either half, by tile parity
   __shared__ uint32_t s_dmax[2][4];   // converters: a warp's largest scale of K, V
+  __shared__ uint32_t s_dmin[4];      // 4-bit: its smallest of V
   __shared__ float s_kscale[4];       // K tile's factor back, by tile % 4
   __shared__ int s_vexp[4];           // V tile's exponent
   uint8_t* base = kp_raw + ((1024u - (smem_u32(kp_raw) & 1023u)) & 1023u);
@@ -243,7 +371,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
     mbar_init(q_full, PAIR ? 16 : 256);
     mbar_init(drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    s_err = 0;
+    s_err = s_far[0] = s_far[1] = 0;
   }
   if (warp == 12) kp_alloc<PAIR>(&s_tmem);
   tc_fence_before();
@@ -315,9 +443,11 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       kp_bar(2, 256);
       const float top = fmul(s_top[0][0][r], k);
       const int biased = (int)(__float_as_uint(top) >> 23);
-      const int e = biased == 0 ? 0 : max(-100, min(100, biased - 127 - 13));
+      const int e = max(-100, min(100, biased - 127 - 13));
+      if (biased - 127 - 13 > 100) *(volatile int*)&s_far[0] = 1;
       const float scale = live ? __uint_as_float((uint32_t)(127 - e) << 23) : 0.0f;
       unscale = __uint_as_float((uint32_t)(127 + e) << 23);
+      if (!SCALED && unscale > KP_MAX_UNIT_FP8) *(volatile int*)&s_far[0] = 1;
 #pragma unroll
       for (int b = 0; b < 2; b++) {  // 32 dimensions: one block
         const int w0 = 32 * half + 16 * b;
@@ -353,6 +483,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       for (int i = 0; i < 2; i++) kp_ld32(S + 64 * half + 32 * i, s + 32 * i);
       // not 0, which times a masked score is NaN; below 2^-126 a score is 0 anyway
       const float f = SCALED ? fmaxf(fmul(unscale, s_kscale[t & 3]), 0x1p-126f) : unscale;
+      if (SCALED && f > KP_MAX_UNIT) *(volatile int*)&s_far[0] = 1;
       const int ve = SCALED ? s_vexp[t & 3] : 0;
       const int key0 = key_of(t);
       const bool sink = t0 + t < sink_tiles;
@@ -377,12 +508,12 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
       kp_bar(2, 256);
       ok = s_ok[t & 1];  // one thread's look, so that all leave the loop together
       top = fmaxf(top, s_top[t & 1][half ^ 1][r]);
-      const bool grow = __any_sync(0xffffffffu, top > fadd(m, 8.0f) || ve > vexp);
+      const bool grow = __any_sync(0xffffffffu, top > fadd(m, 4.0f) || ve > vexp);
       const bool flush = t > 0 && t % KP_FLUSH == 0;
       float go = 1.0f;  // the outputs so far, in the new units
       if (grow) {
         const float mn = fmaxf(m, top);
-        const float nb = mn == -INFINITY ? 0.0f : fsub(mn, 6.0f);
+        const float nb = mn == -INFINITY ? 0.0f : fsub(mn, 10.0f);
         const float g = m == -INFINITY ? 0.0f : exp2_approx(fsub(base_, nb));
         const int ne = max(vexp, ve);
         l = fmul(l, g);
@@ -452,7 +583,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
     // after it has a barrier of its own, so that its parity says which
     for (int t = max(n - 2, 0); t < n; t++)
       if (ok && !mbar_wait(v_empty + (t & 1), (t >> 1) & 1, &s_err)) fail();
-    kp_bar(2, 256);  // s_top is read, every wait decided
+    kp_bar(3, 384);  // s_top is read, every wait decided, the converters are done
     s_top[0][half][r] = l;
     kp_bar(2, 256);
     ok = *(volatile int*)&s_err == 0;
@@ -462,6 +593,15 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
                    " ld.volatile.shared::cluster.s32 %0, [a];\n}\n"
                    : "=r"(other) : "r"(smem_u32(&s_err)), "r"(rank ^ 1) : "memory");
       ok = ok && other == 0;
+    }
+    // behind the last outputs every converter of the pair has said what it found
+    bool far = *(volatile int*)&s_far[0] || *(volatile int*)&s_far[1];
+    if (PAIR && WIDE) {
+      int other;
+      asm volatile("{\n .reg .b32 a;\n fence.acq_rel.cluster;\n mapa.shared::cluster.u32 a, %1, %2;\n"
+                   " ld.volatile.shared::cluster.s32 %0, [a];\n}\n"
+                   : "=r"(other) : "r"(smem_u32(&s_far[1])), "r"(rank ^ 1) : "memory");
+      far = far || other != 0;
     }
     l = fadd(s_top[0][0][r], s_top[0][1][r]);
     tc_fence_after();
@@ -488,11 +628,10 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
     const float mul = fmul(ok ? (n > 0 ? pow2f(max(vexp, -120)) : 0.0f) : NAN,
                            p.splits == 1 ? fdiv(1.0f, l) : 1.0f);
     const size_t part_row = (((size_t)head * gridDim.x + tile) * p.splits + z) * KP_ROWS;
+    float* part_ml = p.part + (size_t)gridDim.z * gridDim.x * p.splits * KP_ROWS * KV_HD + part_row * 2;
     if (live && half == 0 && p.splits > 1) {
-      float* ml = p.part + (size_t)gridDim.z * gridDim.x * p.splits * KP_ROWS * KV_HD +
-                  (part_row + r) * 2;
-      ml[0] = l > 0.0f ? base_ : -INFINITY;
-      ml[1] = l;
+      part_ml[2 * r] = l > 0.0f ? base_ : -INFINITY;
+      part_ml[2 * r + 1] = l;
     }
     kp_bar(2, 256);  // the sums are read
     // columns 64 half .. hold the dimensions 64 half .. (4-bit), 16 i + 8 half .. (e4m3)
@@ -504,6 +643,10 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
                       fmul(o[kp_vcol<KV>(d + 2)], mul), fmul(o[kp_vcol<KV>(d + 3)], mul));
     }
     kp_bar(2, 256);
+    if (__all_sync(0xffffffffu, far && ok)) {
+      kp_exact_rows<KV>(p, tile, head, pos, lo, hi, sk, t0, t1, s_sum, part_ml);
+      __syncwarp();
+    }
 #pragma unroll 4
     for (int i = 0; i < 16; i++) {
       const int rr = tile * KP_ROWS + 16 * warp + i;
@@ -598,7 +741,13 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         return __ldg(reinterpret_cast<const float4*>(row + 4 * d));
       }
     };
-    int vrun = -1000;  // the largest exponent of a V tile so far
+    int vrun = -1000;  // the largest exponent of a V tile so far, and the smallest
+    int vlow = 1000;
+    auto found_far = [&]() {
+      if (*(volatile int*)&s_far[1]) return;
+      *(volatile int*)&s_far[1] = 1;
+      if (PAIR) asm volatile("fence.acq_rel.cluster;" ::: "memory");  // ahead of the arrival
+    };
     // A tile's scales times 2^e lie below 2^10, so a value (below 2^13) keeps
     // its lo part; e as far as f16 can hold 2^e.
     uint32_t knorm = 0, vnorm = 0;  // f16 pairs 2^e of the K and the V tile last looked at
@@ -639,6 +788,8 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         const int ek = exponent(mk);
         // a tile of far smaller values than an earlier one need not fill f16
         vrun = max(vrun, -exponent(mv));
+        if (mv) vlow = min(vlow, -exponent(mv));
+        if (vrun - vlow > KR_SPREAD || mv >= 0x7F800000u) found_far();
         const int ev = -max(-exponent(mv), vrun - 30);
         knorm = __float_as_uint(pow2f(ek));
         vnorm = __float_as_uint(pow2f(ev));
@@ -648,25 +799,36 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         }
         return;
       }
-      auto top = [](__half2 h, uint2 d) {
-        return __hmax2(h, __hmax2(__habs2(as_h2(d.x)), __habs2(as_h2(d.y))));
+      // magnitudes order as their bits do
+      auto top = [](uint2 d) {
+        const uint32_t h = __vmaxu2(d.x & 0x7FFF7FFFu, d.y & 0x7FFF7FFFu);
+        return __reduce_max_sync(0xffffffffu, max(h & 0xFFFFu, h >> 16));
       };
-      auto bits = [](__half2 h) { return (uint32_t)__half_as_ushort(__hmax(__low2half(h), __high2half(h))); };
-      const __half2 zero = __float2half2_rn(0.0f);
-      const uint32_t bk = __reduce_max_sync(0xffffffffu, bits(top(zero, k_any)));
-      const uint32_t bv = __reduce_max_sync(0xffffffffu, bits(top(zero, v_any)));
+      // the smallest of the values' scales but 0 (less 1, so that 0 is the largest)
+      const uint32_t small2 = __viaddmin_u16x2(v_any.x & 0x7FFF7FFFu, 0xFFFFFFFFu,
+                              __vadd2(v_any.y & 0x7FFF7FFFu, 0xFFFFFFFFu));
+      const uint32_t small = __reduce_min_sync(0xffffffffu, min(small2 & 0xFFFFu, small2 >> 16));
+      const uint32_t bk = top(k_any), bv = top(v_any);
       if (lane == 0) {
         s_dmax[0][cw] = bk;
         s_dmax[1][cw] = bv;
+        s_dmin[cw] = small;
       }
       kp_bar(1, 128);
-      uint32_t mk = 0, mv = 0;
+      uint32_t mk = 0, mv = 0, mn = 0xFFFFu;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         mk = max(mk, s_dmax[0][i]);
         mv = max(mv, s_dmax[1][i]);
+        mn = min(mn, s_dmin[i]);
       }
       kp_bar(1, 128);  // read before the next tile's are written
+      if (mn != 0xFFFFu) {  // exponents of the largest and of the smallest scale
+        auto exponent = [](uint32_t b) { return b < 0x400u ? 22 - __clz((int)b) : (int)(b >> 10); };
+        vrun = max(vrun, exponent(mv));
+        vlow = min(vlow, exponent(mn + 1));
+      }
+      if (vrun - vlow > KR_SPREAD || max(mk, mv) >= 0x7C00u) found_far();
       // magnitude below 2^(exponent field - 14)
       const int ek = min(15, 10 - min((int)(mk >> 10) - 14, 16)), ev = min(15, 10 - min((int)(mv >> 10) - 14, 16));
       // f16 pair 2^e: e in -6 .. 15
@@ -733,6 +895,8 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         int from, to;
         range(t, from, to);
         const float f = __uint_as_float(norm);
+        // a thread's elements below KP_SMALL, zeros among them
+        __half2 small = __float2half2_rn(0.0f);
 #pragma unroll
         for (int i = 0; i < 4 / NB; i++) {  // dimensions 16 vn + 8 rank + 4 i ..
           float4 x[8];
@@ -746,11 +910,28 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
           for (int e = 0; e < 4; e++) {
             uint32_t h[4], l[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) split_f16(at(2 * j, e), at(2 * j + 1, e), h[j], l[j]);
+            for (int j = 0; j < 4; j++) {
+              split_f16(at(2 * j, e), at(2 * j + 1, e), h[j], l[j]);
+              small = __hadd2(small, __hlt2(__habs2(as_h2(h[j])), __float2half2_rn(KP_SMALL)));
+            }
             const uint32_t off = kp_off<OR>(8 * (4 * i + e) + vn, kg);
             *reinterpret_cast<uint4*>(oh + off) = make_uint4(h[0], h[1], h[2], h[3]);
             if (LO) *reinterpret_cast<uint4*>(ol + off) = make_uint4(l[0], l[1], l[2], l[3]);
           }
+        }
+        const int few = KP_FEW / NB, first = key_of(t) + 8 * kg;
+        const int in = min(8, max(0, to - first)) - min(8, max(0, from - first));  // keys of the range
+        auto over = [&](int n) { return (int)__reduce_add_sync(0xffffffffu, (uint32_t)n) > few; };
+        if (over((int)__low2float(small) + (int)__high2float(small) - (8 - in) * (16 / NB))) {  // again, without the zeros
+          int n = 0;
+#pragma unroll 1
+          for (int i = 0; i < 32 / NB; i++) {
+            const float4 x = wide4(vb, first + (i & 7), from, to,
+                                   16 * vn + 8 * rank + 4 * (i >> 3));
+            auto is = [&](float y) { return y != 0.0f && fabsf(fmul(y, f)) < KP_SMALL; };
+            n += is(x.x) + is(x.y) + is(x.z) + is(x.w);
+          }
+          if (over(n)) found_far();
         }
       } else if constexpr (Q4) {
 #pragma unroll
@@ -798,6 +979,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         fail();
         ok = false;
       }
+      ok = __all_sync(0xffffffffu, ok);  // put_v adds up over the warp
     };
     // K(t + 1), then V(t); raw bytes are loaded as soon as the last tile's are
     // used up.  A failed wait skips the writes but keeps the barriers' counts.
@@ -827,6 +1009,8 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
         load_v(t + 1);
       }
     }
+    __syncwarp();
+    asm volatile("bar.arrive 3, 384;" ::: "memory");
   } else {
     // ============================================================= products
     if (warp == 12 && lane == 0 && rank == 0) {

@@ -128,9 +128,128 @@ MANY = (40, 300)
 WIDE = ("f32", "bf16")
 
 
+def late(n, nq):
+    """A key that the first three quarters of the queries do not see."""
+    return n - nq // 4
+
+
+@pytest.mark.parametrize("dtype,ratio", [(d, 2.0 ** e) for d in WIDE for e in (8, 13, 20, 30, 90)]
+                         + [("q4", 2.0 ** e) for e in (8, 13, 17)])
+@pytest.mark.parametrize("nq", (8,) + MANY)
+def test_large_values_that_some_queries_do_not_see(torch, dev, nq, dtype, ratio):  # noqa: F811
+    k, v, q = rows(20, N, NKV), rows(21, N, NKV), rows(22, nq, HEADS)
+    v[late(N, nq)] *= ratio
+    check(torch, dev, dtype, q, k, v, N - nq)
+
+
+@pytest.mark.parametrize("dtype,ratio", [(d, 2.0 ** e) for d in WIDE for e in (8, 13, 20, 30, 90)]
+                         + [("q4", 2.0 ** e) for e in (8, 13, 27)])
+@pytest.mark.parametrize("nq", (8,) + MANY)
+@pytest.mark.parametrize("at", [0, 3, 333])
+def test_large_values_of_no_weight(torch, dev, nq, at, dtype, ratio):  # noqa: F811
+    k, v, q = rows(23, N, NKV, 0.3), rows(24, N, NKV, 1e-3), few(25, nq)
+    v[at] *= ratio
+    far_score(q, k, at, 100.0)
+    check(torch, dev, dtype, q, k, v, N - nq)
+
+
+@pytest.mark.parametrize("dtype,ratio", [(d, 2.0 ** e) for d in WIDE for e in (8, 13, 20, 30, 90)]
+                         + [("q4", 2.0 ** e) for e in (8, 13, 17)])
+@pytest.mark.parametrize("nq", (8,) + MANY)
+@pytest.mark.parametrize("what", ["block", "column", "half of the keys", "one small key"])
+def test_values_of_two_sizes(torch, dev, nq, what, dtype, ratio):  # noqa: F811
+    """From position 0: the first queries see few keys."""
+    n = max(nq, 200)
+    k, v, q = rows(26, n, NKV), rows(27, n, NKV), rows(28, nq, HEADS)
+    if what == "block":
+        v[:, :, 32:64] *= ratio
+    elif what == "column":
+        v[:, :, 5] *= ratio
+    elif what == "half of the keys":
+        v[nq // 2:] *= ratio
+    else:
+        v[1:] *= ratio
+    check(torch, dev, dtype, q, k[:nq], v[:nq], 0)
+
+
+@pytest.mark.parametrize("dtype", WIDE)
+@pytest.mark.parametrize("ratio", [2.0 ** e for e in (8, 13, 20, 30, 90)])
+@pytest.mark.parametrize("nq", (8,) + MANY)
+def test_large_keys_that_some_queries_do_not_see(torch, dev, nq, ratio, dtype):  # noqa: F811
+    """Where one is seen it has all the weight, or none (scores further apart than
+    f32's exponents)."""
+    k, v, q = rows(29, N, NKV), rows(30, N, NKV), rows(31, nq, HEADS)
+    at = late(N, nq)
+    k[at] *= ratio
+    s = np.einsum("qhd,khd->qhk", q.astype(np.float64), np.repeat(stored(torch, k, dtype), 2, 1))
+    far = np.abs(s[:, :, at]).min() / np.sqrt(HD)
+    if far < 200 and ratio > 2 ** 8:   # not by chance: push the others off
+        k[at] = ratio * np.sign(q.mean((0, 1)) + 1e-9)
+    check(torch, dev, dtype, q[: 3 * nq // 4], k, v, N - nq)
+
+
+@pytest.mark.parametrize("dtype", WIDE)
+@pytest.mark.parametrize("ratio", [2.0 ** e for e in (8, 13, 20, 30, 90)])
+@pytest.mark.parametrize("nq", (8,) + MANY)
+def test_large_keys_in_dimensions_that_queries_leave_out(torch, dev, nq, ratio, dtype):  # noqa: F811
+    k, v, q = rows(32, N, NKV), rows(33, N, NKV), rows(34, nq, HEADS)
+    k[:, :, 77] *= ratio
+    q[:, :, 77] = 0.0
+    check(torch, dev, dtype, q, k, v, N - nq)
+
+
+@pytest.mark.parametrize("dtype", WIDE + ("fp8", "q4"))
+@pytest.mark.parametrize("scale", [1e-36, 1e-20, 1e-5, 1e4, 1e30, 1e37])
+@pytest.mark.parametrize("nq", (8,) + MANY)
+def test_queries_of_any_size(torch, dev, nq, scale, dtype):  # noqa: F811
+    """Against keys that make up for it as far as their type goes; a query of 0."""
+    low, high = dict(f32=(1e-30, 1e30), bf16=(1e-30, 1e30), fp8=(0.05, 100.0), q4=(1e-3, 1e3))[dtype]
+    by = np.float32(min(max(1.0 / scale, low), high))
+    if scale * by > 10.0:   # scores past where f32 can tell keys apart
+        scale = 10.0 / by
+    k, v, q = rows(35, N, NKV, by), rows(36, N, NKV), rows(37, nq, HEADS, np.float32(scale))
+    q[nq // 2, 1] = 0.0
+    check(torch, dev, dtype, q, k, v, N - nq)
+
+
 @pytest.mark.parametrize("dtype", WIDE + ("fp8", "q4"))
 @pytest.mark.parametrize("scale", [0.0, 1e-30, 1e-7, 1.0])
 @pytest.mark.parametrize("nq", (1, 8) + MANY)
 def test_keys_of_zero_see_the_mean(torch, dev, nq, scale, dtype):  # noqa: F811
     k, v, q = np.zeros((N, NKV, HD), np.float32), rows(38, N, NKV), rows(39, nq, HEADS, scale)
     check(torch, dev, dtype, q, k, v, N - nq, window=90, sinks=3)
+
+
+@pytest.mark.parametrize("dtype", WIDE)
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("nq", MANY)
+def test_what_is_not_finite_stays_with_the_queries_that_see_it(torch, dev, nq, bad, dtype):  # noqa: F811
+    at = late(N, nq)
+    seen = at - (N - nq)   # the first query that does
+    for which in "kv":
+        k, v, q = rows(40, N, NKV), rows(41, N, NKV), rows(42, nq, HEADS)
+        x = dict(k=k, v=v)
+        x[which][at, :, 9] = bad
+        cache = filled(torch, dev, dtype, k, v, 704, garbage=True)
+        out = torch.full(q.shape, 7.0, device="cuda")
+        cache.attention(torch.from_numpy(q).cuda(), N - nq, out)
+        got = out.cpu().numpy().astype(np.float64)
+        want, mag = reference(q[:seen], kept(torch, k[:at], dtype), kept(torch, v[:at], dtype),
+                              N - nq, 0, 0)
+        err = np.linalg.norm(got[:seen] - want, axis=-1) / np.linalg.norm(mag, axis=-1)
+        assert err.max() < 1e-5
+        if which == "v" and np.isnan(bad):
+            assert np.isnan(got[seen:, :, 9]).all()
+
+
+@pytest.mark.parametrize("dtype", ("f32", "bf16", "q4"))
+def test_many_keys_of_two_sizes_in_splits(torch, dev, dtype):  # noqa: F811
+    """One tile of rows, many key splits, of which some have outliers."""
+    n, nq = 5000, 50
+    k, v, q = rows(43, n, NKV), rows(44, n, NKV), rows(45, nq, HEADS)
+    v[700] *= 2.0 ** 16
+    v[3000:3100, :, 40:50] *= 2.0 ** 10
+    k[700] = 0
+    far_score(q, k, 700, 0.0)
+    check(torch, dev, dtype, q, k, v, n - nq)
+    check(torch, dev, dtype, q, k, v, n - nq, window=2500, sinks=720)
