@@ -363,7 +363,8 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
       const int biased = (int)(__float_as_uint(top) >> 23);
-      const int e = biased == 0 ? 0 : max(-100, min(100, biased - 127 - 13));
+      // (up to f32's largest, whose exponent here is 114)
+      const int e = biased == 0 ? 0 : max(-100, min(114, biased - 127 - 13));
       const float scale = __uint_as_float((uint32_t)(127 - e) << 23);
       if (Q4) {  // pairs two apart: bytes 0 and 2, 1 and 3 of a code word
         const float y = x.y;

@@ -253,3 +253,27 @@ def test_many_keys_of_two_sizes_in_splits(torch, dev, dtype):  # noqa: F811
     far_score(q, k, 700, 0.0)
     check(torch, dev, dtype, q, k, v, n - nq)
     check(torch, dev, dtype, q, k, v, n - nq, window=2500, sinks=720)
+
+
+@pytest.mark.parametrize("dtype,scale", [("fp8", 1e36), ("q4", 1e36), ("fp8", 1e34), ("q4", 1e33),
+                                         ("f32", 1e36), ("bf16", 1e36)])
+@pytest.mark.parametrize("nq", (1, 8) + MANY)
+def test_queries_near_the_largest_number(torch, dev, nq, dtype, scale):  # noqa: F811
+    """Scores so far apart that one key has all the weight, by a margin of 1e-3 of
+    them (f32's own error is 1e-6 of the terms'), on any cache."""
+    k, v, q = rows(46, N, NKV, 0.05), rows(47, N, NKV), rows(48, nq, HEADS)
+    q /= np.abs(q).max()
+    q *= np.float32(scale)
+    ks = np.repeat(kept(torch, k, dtype), 2, 1)
+    s = np.einsum("qhd,khd->qhk", q.astype(np.float64), ks)
+    for i in range(nq):
+        s[i, :, N - nq + i + 1:] = -np.inf
+    best = np.sort(s, -1)
+    sure = (best[..., -1] - best[..., -2]) / best[..., -1] > 1e-3
+    cache = filled(torch, dev, dtype, k, v, 704, garbage=True)
+    out = torch.full(q.shape, float("nan"), device="cuda")
+    cache.attention(torch.from_numpy(q).cuda(), N - nq, out)
+    got, vs = out.cpu().numpy(), kept(torch, v, dtype)
+    assert np.isfinite(got).all() and sure.mean() > 0.8
+    for i, h in zip(*np.nonzero(sure)):
+        np.testing.assert_allclose(got[i, h], vs[s[i, h].argmax(), h // 2], rtol=1e-5, atol=1e-6)
