@@ -41,7 +41,7 @@
 namespace flock {
 
 constexpr int KR_GROUP = 16;  // keys per warp step
-constexpr int KR_SPREAD = 12;  // 4-bit value scales a warp takes in f16: 2^12 apart
+constexpr int KR_SPREAD = 14;  // 4-bit value scales a warp takes in f16: 2^14 apart
 constexpr int KR_MAX_ITEMS = 4096;  // (row tile, kv head) pairs that may be split: arrival counters
 constexpr size_t KR_PART_OFFSET = KR_MAX_ITEMS * 4;
 
@@ -400,8 +400,8 @@ static __global__ void __launch_bounds__(KrLayout<KV, NT>::THREADS, 1)
   // Weights are 2^(s - base), base = m - 10, m a running maximum that may lag by
   // 2^4: at most 2^14, inside f16, and a lo part loses nothing above 2^-35 of
   // the largest.  Value scales are divided by 2^dexp, a bound on those so far,
-  // which the outputs get back at the end; those down to 2^-12 of it leave the
-  // largest weight's products at 2^-2 and up, 2^23 of a lo part's last bit.
+  // which the outputs get back at the end; those down to 2^-14 of it leave the
+  // largest weight's products at 2^-4 and up, where a lo part's error is 2^-21.
   constexpr float HEADROOM = F16 ? 10.0f : 0.0f, LAG = F16 ? 4.0f : 8.0f;
   float m[RL], l[RL], base[RL];
   int dexp = -14;
