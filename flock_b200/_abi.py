@@ -104,6 +104,7 @@ SIGNATURES = {
     "flock_op_embed": [_vp, _vp, _i32p, _i, _fp],
     "flock_op_argmax": [_vp, _fp, _i64, _i64p, _fp],
     "flock_argmax_noalloc": [_vp, _i64, _vp, _vp, _vp],
+    "flock_pointer_device": [_vp],
     "flock_kv_create": [_vp, _i, _i, _i, _i64, _vp, _vp, _vp, _vp, _vp, _pp],
     "flock_kv_free": [_vp],
     "flock_kv_append": [_vp, _vp, _vp, _i64, _i64, _i, _vp],

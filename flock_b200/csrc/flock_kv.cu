@@ -207,6 +207,15 @@ int flock::kv_attention_enqueue(int sm_count, int kv_dtype, const KvAttnArgs& a,
 
 extern "C" {
 
+int flock_pointer_device(const void* p) {
+  cudaPointerAttributes at = {};
+  if (!p || cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
+  return at.type == cudaMemoryTypeDevice ? at.device : -1;
+}
+
 int flock_kv_create(flock_dev* dev, int kv_dtype, int n_kv_heads, int head_dim, int64_t capacity,
                     void* k, void* v, void* k_scales, void* v_scales, void* workspace,
                     flock_kv** out) {

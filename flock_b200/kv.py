@@ -56,7 +56,7 @@ def _array(a, dtype: str, ordinal: int, what: str):
     try:
         t, p = a.dtype, a.data_ptr()
     except AttributeError:
-        return _interface(a, dtype, what)
+        return _interface(a, dtype, ordinal, what)
     if (_torch_types.get(t) or _torch_type(t)) != dtype:
         raise ValueError(f"{what} is {t}, want torch.{_TYPES[dtype][1]}")
     if a.get_device() != ordinal:  # -1 on the host
@@ -64,14 +64,24 @@ def _array(a, dtype: str, ordinal: int, what: str):
     return p, a.shape, None if a.is_contiguous() else a.stride()
 
 
-def _interface(a, dtype: str, what: str):
+def _interface(a, dtype: str, ordinal: int, what: str):
     i = getattr(a, "__cuda_array_interface__", None)
     if i is None:
         raise ValueError(f"{what} is a {type(a).__name__}, not a device array")
     if i["typestr"] != _TYPES[dtype][0]:
         raise ValueError(f"{what} has type {i['typestr']}, want {_TYPES[dtype][0]}")
-    size, strides = int(i["typestr"][2:]), i.get("strides")
-    return i["data"][0], tuple(i["shape"]), strides and tuple(s // size for s in strides)
+    at, shape, strides = i["data"][0], tuple(i["shape"]), i.get("strides")
+    on = _abi.lib().flock_pointer_device(at or None)
+    if on >= 0 and on != ordinal:
+        raise ValueError(f"{what} is on cuda:{on}, the cache's device is cuda:{ordinal}")
+    if strides is None:
+        return at, shape, None
+    size = int(i["typestr"][2:])
+    if any(n > 1 and s % size for n, s in zip(shape, strides)):
+        raise ValueError(f"{what} has strides of {tuple(strides)} bytes, not of whole elements")
+    strides = tuple(s // size for s in strides)
+    dense = all(n == 1 or s == math.prod(shape[d + 1:]) for d, (n, s) in enumerate(zip(shape, strides)))
+    return at, shape, None if dense or 0 in shape else strides
 
 
 def _stream_of(a) -> int:

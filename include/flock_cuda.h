@@ -289,6 +289,9 @@ FLOCK_API int flock_argmax_noalloc(const float* x, int64_t n, int32_t* index_out
  * the row in k and at 8 (i / 2) + 2 b + i % 2 in v. */
 #define FLOCK_WORKSPACE_BYTES 8388608 /* of a flock_kv or flock_verify_draft workspace */
 
+/* The device whose memory p is, -1 for host memory or where the runtime does not
+ * know it. */
+FLOCK_API int flock_pointer_device(const void* p);
 /* A cache of `capacity` keys over the caller's planes (NULL: the handle
  * allocates them, zero-filled).  workspace: FLOCK_WORKSPACE_BYTES of device
  * memory that were zero-filled once and that nothing else writes (NULL: the

@@ -111,6 +111,8 @@ export const symbols = {
   flock_op_argmax: { parameters: ["pointer", "buffer", "i64", "buffer", "buffer"], result: "i32" },
   // (x, n, index_out, value_out, stream)
   flock_argmax_noalloc: { parameters: ["buffer", "i64", "buffer", "buffer", "buffer"], result: "i32" },
+  // (p)
+  flock_pointer_device: { parameters: ["buffer"], result: "i32" },
   // (dev, kv_dtype, n_kv_heads, head_dim, capacity, k, v, k_scales, v_scales, workspace, out)
   flock_kv_create: { parameters: ["pointer", "i32", "i32", "i32", "i64", "buffer", "buffer", "buffer", "buffer", "buffer", "buffer"], result: "i32" },
   // (c)

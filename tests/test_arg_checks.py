@@ -163,3 +163,47 @@ def test_the_stream_that_an_array_names():
 def test_wait_stream_wants_a_model():
     assert _abi.lib().flock_model_wait_stream(None, None) == _abi.FLOCK_E_ARG
     assert "wait_stream" in _abi.lib().flock_last_error().decode()
+
+
+# ------------------------------------------------------- __cuda_array_interface__
+class Array:
+    def __init__(self, shape, strides, typestr="<f4"):
+        self.__cuda_array_interface__ = dict(shape=shape, typestr=typestr, strides=strides,
+                                             data=(4096, False), version=3)
+
+
+def test_an_array_of_another_device_is_refused(monkeypatch):
+    a = Array((2, 2, 128), None)
+    assert kv._array(a, "f32", 0, "x") == (4096, (2, 2, 128), None)
+    for on in (0, 1, 5, -1):   # -1: the runtime does not know the address
+        monkeypatch.setattr(_abi, "lib", lambda: types.SimpleNamespace(flock_pointer_device=lambda p: on))
+        if on in (0, -1):
+            assert kv._array(a, "f32", 0, "x")[0] == 4096
+        else:
+            with pytest.raises(ValueError, match=f"x is on cuda:{on}"):
+                kv._array(a, "f32", 0, "x")
+
+
+def test_dense_strides_are_dense():
+    for shape, strides in [((2, 3, 128), (1536, 512, 4)), ((1, 3, 128), (99, 512, 4)),
+                           ((0, 3, 128), (0, 0, 4)), ((5,), (4,))]:
+        assert kv._array(Array(shape, strides), "f32", 0, "x")[2] is None
+    assert kv._array(Array((2, 3, 128), (2048, 512, 4)), "f32", 0, "x")[2] == (512, 128, 1)
+    assert kv._dense(Array((2, 3), (12, 4)), "f32", 0, "x", (2, 3)) == 4096
+
+
+def test_strides_of_parts_of_elements_are_refused():
+    with pytest.raises(ValueError, match="whole elements"):
+        kv._array(Array((2, 3), (18, 6)), "f32", 0, "x")
+
+
+@pytest.mark.gpu
+def test_the_device_of_a_pointer():
+    import torch
+    f = _abi.lib().flock_pointer_device
+    x = torch.zeros(4, device="cuda")
+    assert f(x.data_ptr()) == 0 and f(x.data_ptr() + 4) == 0
+    assert f(torch.zeros(4).data_ptr()) == -1 and f(torch.zeros(4).pin_memory().data_ptr()) == -1
+    assert f(None) == -1 and f(4096) == -1
+    x.add_(1)   # no error is left behind
+    torch.cuda.synchronize()
