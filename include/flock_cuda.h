@@ -507,8 +507,10 @@ FLOCK_API int flock_model_set_window(flock_model* m, int window, int sinks);
 /* One step of several greedy or sampled tokens (no counterpart in the
  * reference): ids[0] is the token to consume, ids[1 .. n-1] drafts of what
  * follows it (a small model's, or a lookup's).  All n run in one multi-token
- * step, flock_verify_draft decides on the logits after each, and the caches go
- * back to what is certain: pos has grown by *n_tokens = kept drafts + 1, tokens
+ * step, flock_verify_draft decides on the logits after each (at temperature 0: the
+ * tokens of greedy decoding, but that FLOCK_PREFILL_TENSOR gives a step of several
+ * tokens f16 GEMM operands, and so logits other than a single token's), and the
+ * caches go back to what is certain: pos has grown by *n_tokens = kept drafts + 1, tokens
  * [n] holds the kept drafts and the token after them (then -1), which is also
  * the one the next device-fed decode step consumes.  draft: device logits
  * [n - 1][vocab] the drafts were drawn from, or NULL; u: n uniform numbers
