@@ -80,7 +80,9 @@ constexpr int KP_OPND = 128 * 128 * 2;  // bytes of one 128 x 128 f16 operand
 // to 2^-12 moves a score by 2^-15.4, typically 2^-20.  e4m3 keys are exact, up to 448:
 // 2^-9.2 of q's unit, typically 2^-13.
 constexpr float KP_MAX_UNIT = 0x1p-12f, KP_MAX_UNIT_FP8 = 0x1p-6f;
-// Values: elements of a warp's 32 keys below 2^-15 of the tile's largest (2^-2 as scaled).
+// Values: elements of a warp's 32 keys below 2^-15 of the tile's largest (2^-2 as
+// scaled), of which a column has 32 and a key 64 or 128.  Half of the elements are
+// looked at, half of each key's and of each column's.
 constexpr float KP_SMALL = 0.25f;
 constexpr int KP_FEW = 24;
 
@@ -912,17 +914,19 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
 #pragma unroll
             for (int j = 0; j < 4; j++) {
               split_f16(at(2 * j, e), at(2 * j + 1, e), h[j], l[j]);
-              small = __hadd2(small, __hlt2(__habs2(as_h2(h[j])), __float2half2_rn(KP_SMALL)));
+              if ((e + j) % 2 == 0)
+                small = __hadd2(small, __hlt2(__habs2(as_h2(h[j])), __float2half2_rn(KP_SMALL)));
             }
             const uint32_t off = kp_off<OR>(8 * (4 * i + e) + vn, kg);
             *reinterpret_cast<uint4*>(oh + off) = make_uint4(h[0], h[1], h[2], h[3]);
             if (LO) *reinterpret_cast<uint4*>(ol + off) = make_uint4(l[0], l[1], l[2], l[3]);
           }
         }
-        const int few = KP_FEW / NB, first = key_of(t) + 8 * kg;
+        const int first = key_of(t) + 8 * kg;
         const int in = min(8, max(0, to - first)) - min(8, max(0, from - first));  // keys of the range
-        auto over = [&](int n) { return (int)__reduce_add_sync(0xffffffffu, (uint32_t)n) > few; };
-        if (over((int)__low2float(small) + (int)__high2float(small) - (8 - in) * (16 / NB))) {  // again, without the zeros
+        auto warp_sum = [](int n) { return (int)__reduce_add_sync(0xffffffffu, (uint32_t)n); };
+        const int n2 = (int)__low2float(small) + (int)__high2float(small) - (8 - in) * (8 / NB);
+        if (warp_sum(n2) > KP_FEW / 2) {  // again, all of them but the zeros
           int n = 0;
 #pragma unroll 1
           for (int i = 0; i < 32 / NB; i++) {
@@ -931,7 +935,7 @@ static __global__ void __launch_bounds__(KP_THREADS, 1) k_kv_prompt(const KvProm
             auto is = [&](float y) { return y != 0.0f && fabsf(fmul(y, f)) < KP_SMALL; };
             n += is(x.x) + is(x.y) + is(x.z) + is(x.w);
           }
-          if (over(n)) found_far();
+          if (warp_sum(n) > KP_FEW) found_far();
         }
       } else if constexpr (Q4) {
 #pragma unroll
