@@ -103,10 +103,10 @@ int64_t visible_keys(const KvAttnArgs& a) {
 // k_kv_rows or k_kv_prompt.  The first's time grows with rows times keys, the
 // second's starts at 12 to 25 us and grows with the keys of 128 rows.  us, first
 // against second, 8 kv heads, rows @ keys:
-//   4-bit  32 @ 32000 59 / 67   48 @ 32000 75 / 68    48 @ 8169 26 / 32    64 @ 8169 35 / 32
-//   e4m3   24 @ 32000 43 / 51   32 @ 32000 60 / 51    48 @ 8169 26 / 27    64 @ 8169 34 / 27
-//   bf16   32 @ 32000 139 / 193 48 @ 32000 266 / 194  128 @ 1000 26 / 27   48 @ 8169 74 / 56
-//   f32    16 @ 32000 208 / 227 24 @ 32000 272 / 226  32 @ 1000 21 / 31    48 @ 1000 32 / 31
+//   4-bit  32 @ 32000 60 / 69   48 @ 32000 76 / 69    48 @ 8169 28 / 33    64 @ 8169 36 / 33
+//   e4m3   24 @ 32000 43 / 51   32 @ 32000 59 / 51    48 @ 8169 26 / 27    64 @ 8169 35 / 27
+//   bf16   32 @ 32000 139 / 204 48 @ 32000 265 / 205  128 @ 1000 25 / 30   48 @ 8169 74 / 59
+//   f32    16 @ 32000 211 / 243 24 @ 32000 275 / 244  32 @ 1000 22 / 33    48 @ 1000 33 / 33
 template <int KV>
 bool few_rows(int64_t rows, int64_t keys, int64_t n_kv_heads) {
   constexpr int always = KV == FLOCK_KV_F32 ? 16 : KV == FLOCK_KV_FP8 ? 24 : 32;
@@ -152,8 +152,8 @@ int launch_prompt(uint8_t* workspace, const KvAttnArgs& a, cudaStream_t st) {
   int tiles = (p.rows + KP_ROWS - 1) / KP_ROWS;
   if (PAIR) tiles = (tiles + 1) & ~1;
   const int64_t items = (int64_t)tiles * a.c.n_kv_heads;
-  // key splits of a tile until the GPU is about full, at least two key tiles
-  // each; the workspace holds 125 tiles' partial outputs
+  // key splits of a tile, at least two key tiles each, as many for every tile as the
+  // workspace's 125 partial outputs allow: none from 63 (tile, kv head) items on
   const int64_t want = (visible_keys(a) + 2 * KP_KEYS - 1) / (2 * KP_KEYS);
   constexpr int64_t most = (FLOCK_WORKSPACE_BYTES - KR_PART_OFFSET) / (KP_ROWS * (KV_HD + 2) * 4);
   const int64_t room = most / items;
@@ -190,10 +190,10 @@ int flock::kv_attention_enqueue(int sm_count, int kv_dtype, const KvAttnArgs& a,
     constexpr int KV = decltype(kv)::value;
     if (!few_rows<KV>(rows, visible_keys(a), a.c.n_kv_heads)) {
       // Two tiles as a pair of CTAs where the operands are widened at a cost: 1024
-      // queries at 3000 keys of 16 / 8 heads 99 us against 114 (4-bit), 221
-      // against 276 (bf16); e4m3 gains 3% and loses 15% in a window.  A tile
-      // without a partner costs one: three tiles at 4000 keys 45 us against 36,
-      // thirteen in a window of 1500 keys 51 against 56.
+      // queries at 3000 keys of 16 / 8 heads 100 us against 120 (4-bit), 228
+      // against 292 (bf16); e4m3 gains 1 to 3% and loses 15% in a window.  A tile
+      // without a partner costs one: three tiles at 4000 keys 46 us against 38,
+      // thirteen in a window of 1500 keys 54 against 59.
       const int64_t tiles = (rows + KP_ROWS - 1) / KP_ROWS;
       if constexpr (KV != FLOCK_KV_FP8)
         if (tiles % 2 == 0 || tiles > 8) return launch_prompt<KV, true>(workspace, a, st);
