@@ -316,15 +316,19 @@ FLOCK_API int flock_kv_read(flock_kv* c, int64_t pos, int n, float* k, float* v,
  * kv heads in order (n_heads a multiple of n_kv_heads).  Keys no query sees
  * are not read into the result, whatever they hold; a NaN or infinity in a
  * key or value that only some queries of the call see makes the others'
- * outputs undefined.  Numbers: the matrix instructions take cached values
- * exactly in calls of few rows, and queries and weights to 2^-22 of themselves
- * (f32 and bf16 caches: 2^-24; an element of a query below 2^-16 of its largest
- * to 2^-38 of that, a weight below 2^-13 of its largest to 2^-35).  Calls of many
- * rows take f32 values to 2^-22 too, and where a tile's keys, values or queries lie
- * too far apart for that the rows are worked out in f32, which is 20 to 60 times
- * slower (about: elements 2^15 above the others of a tile of values, a product of
- * the largest |q| and |k| above 130000, over e4m3 keys a |q| above 2000).  At most 2^30 rows (queries times heads a kv head).  The waits
- * inside the many-row kernel are bounded (2 s); one that ran out, which nothing
+ * outputs undefined.  At most 2^30 rows (queries times heads a kv head).
+ *
+ * Numbers.  The matrix instructions take cached values exactly in calls of few
+ * rows, and queries and weights to 2^-22 of themselves (f32 and bf16 caches:
+ * 2^-24; an element of a query below 2^-16 of its largest to 2^-38 of that, a
+ * weight below 2^-13 of its row's largest to 2^-35 of that).  Calls of many rows
+ * take f32 values and every query and weight to 2^-22; where a tile's keys, values
+ * or queries lie too far apart for that its rows are worked out in f32, 16 to 60
+ * times slower (about: most elements of a tile of values 2^15 below the largest, a
+ * product of the largest |q| and |k| above 130000, over e4m3 keys a |q| above
+ * 2000).
+ *
+ * The waits inside the many-row kernel are bounded (2 s); one that ran out, which nothing
  * but a lost kernel of the device can cause, leaves NaN in its rows. */
 FLOCK_API int flock_kv_attention(flock_kv* c, const float* q, int64_t q_stride, int n_heads,
                                  int n_queries, int64_t pos, int window, int sinks, float* out,
